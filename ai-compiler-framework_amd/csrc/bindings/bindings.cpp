@@ -7,7 +7,7 @@
 //   graph_launch / graph_reset / graph_stream.
 // Every call goes through the C-ABI of libaicf_hip (include/aicf_hip.h); this
 // file holds no HIP code.  Differences: bf16 tensors are accepted
-// (DType::kBF16 = 3), HIP errors read "[HIP] ...", and graph_launch replays
+// (DType::kBF16 = 3) and 8-bit float ones, HIP errors read "[HIP] ...", and graph_launch replays
 // on torch's current stream (ordered after the work already queued there and
 // before the work queued there afterwards).
 #include <c10/hip/HIPStream.h>
@@ -61,6 +61,10 @@ enum class OpKind : int {
   AdamWMulti = AICF_OP_ADAMW_MULTI,
   MseColsum = AICF_OP_MSE_COLSUM,
   ColsumAdamW = AICF_OP_COLSUM_ADAMW,
+  QuantFp8 = AICF_OP_QUANT_FP8,
+  GemmFp8 = AICF_OP_GEMM_FP8,
+  DistillTopk = AICF_OP_DISTILL_TOPK,
+  SampleRow = AICF_OP_SAMPLE_ROW,
 };
 
 std::string tensor_brief(const torch::Tensor& t) {
@@ -80,18 +84,22 @@ uint8_t to_dtype(const torch::Tensor& t) {
     case at::kFloat: return AICF_DTYPE_F32;
     case at::kInt: return AICF_DTYPE_I32;
     case at::kBFloat16: return AICF_DTYPE_BF16;
+    case at::kFloat8_e4m3fn: return AICF_DTYPE_F8E4M3;
+    case at::kFloat8_e5m2: return AICF_DTYPE_F8E5M2;
     default: break;
   }
   TORCH_CHECK(false, "unsupported dtype. got: ", tensor_brief(t));
 }
 
-// bindings.cpp:92-104 of the reference, plus bf16.
+// bindings.cpp:92-104 of the reference, plus bf16 and the 8-bit floats.
 void check_tensor(const torch::Tensor& t, const char* what) {
   TORCH_CHECK(t.defined(), what, ": undefined tensor");
   TORCH_CHECK(t.is_cuda(), what, ": must be CUDA tensor. got: ", tensor_brief(t));
   const auto st = t.scalar_type();
-  TORCH_CHECK(st == at::kHalf || st == at::kFloat || st == at::kInt || st == at::kBFloat16, what,
-              ": dtype must be float16/bfloat16/float32/int32. got: ", tensor_brief(t));
+  TORCH_CHECK(st == at::kHalf || st == at::kFloat || st == at::kInt || st == at::kBFloat16 ||
+                  st == at::kFloat8_e4m3fn || st == at::kFloat8_e5m2,
+              what, ": dtype must be float16/bfloat16/float32/int32 or float8_e4m3fn/float8_e5m2. got: ",
+              tensor_brief(t));
   TORCH_CHECK(t.dim() >= 0 && t.dim() <= AICF_MAX_RANK, what, ": rank out of range. got rank=",
               t.dim(), " (kMaxRank=", AICF_MAX_RANK, ")");
 }
@@ -156,9 +164,22 @@ struct Call {
   }
 };
 
+// The appended ops from QuantFp8 on launch on the current device only.
+void check_device(int kind, const py::sequence& seq, const char* what) {
+  if (kind < AICF_OP_QUANT_FP8) return;
+  const int cur = c10::hip::getCurrentHIPStream().device_index();
+  for (auto h : seq) {
+    torch::Tensor t = py::cast<torch::Tensor>(h);
+    TORCH_CHECK(t.get_device() == cur, what, ": on another device than the current one (", cur,
+                "). got: cuda:", t.get_device(), " ", tensor_brief(t));
+  }
+}
+
 void op_call_impl(int kind, const py::sequence& inputs, const py::sequence& outputs,
                   uint32_t schema_id, const py::bytes& attrs_bytes, uint64_t stream_u64) {
   Call c(inputs, outputs, schema_id, attrs_bytes, stream_u64);
+  check_device(kind, inputs, "inputs");
+  check_device(kind, outputs, "outputs");
   {
     std::lock_guard<std::mutex> lock(g_mu);
     if (g_trace_enabled) g_trace.emplace_back(aicf_opkind_name(kind));
@@ -176,6 +197,8 @@ void launch_by_id_impl(const std::string& kid, int kind, const py::sequence& inp
                        const py::sequence& outputs, uint32_t schema_id,
                        const py::bytes& attrs_bytes, uint64_t stream_u64) {
   Call c(inputs, outputs, schema_id, attrs_bytes, stream_u64);
+  check_device(kind, inputs, "inputs");
+  check_device(kind, outputs, "outputs");
   {
     std::lock_guard<std::mutex> lock(g_mu);
     if (g_trace_enabled)
@@ -239,6 +262,10 @@ PYBIND11_MODULE(_C, m) {
       .value("AdamWMulti", OpKind::AdamWMulti)
       .value("MseColsum", OpKind::MseColsum)
       .value("ColsumAdamW", OpKind::ColsumAdamW)
+      .value("QuantFp8", OpKind::QuantFp8)
+      .value("GemmFp8", OpKind::GemmFp8)
+      .value("DistillTopk", OpKind::DistillTopk)
+      .value("SampleRow", OpKind::SampleRow)
       .export_values();
 
   m.def(

@@ -57,12 +57,17 @@ inline bool is_contig_2d_rowmajor(const TensorDesc& t) {
 
 inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
+inline int elem_bytes(DType d) {
+  if (d == DType::kF32 || d == DType::kI32) return 4;
+  return d == DType::kF8E4M3 || d == DType::kF8E5M2 ? 1 : 2;
+}
+
 // Byte range [lo, hi) that a view with non-negative strides can touch.
 struct Span {
   uintptr_t lo, hi;
 };
 inline Span span_of(const TensorDesc& t) {
-  const int64_t es = dt(t) == DType::kF32 || dt(t) == DType::kI32 ? 4 : 2;
+  const int64_t es = elem_bytes(dt(t));
   int64_t last = 0;
   for (int i = 0; i < t.rank && i < AICF_MAX_RANK; ++i) {
     if (t.shape[i] <= 0) return {0, 0};  // touches nothing

@@ -36,6 +36,8 @@ enum class DType : uint8_t {
   kF16 = AICF_DTYPE_F16,
   kBF16 = AICF_DTYPE_BF16,
   kI32 = AICF_DTYPE_I32,
+  kF8E4M3 = AICF_DTYPE_F8E4M3,
+  kF8E5M2 = AICF_DTYPE_F8E5M2,
 };
 
 enum class OpKind : int {
@@ -69,6 +71,10 @@ enum class OpKind : int {
   AdamWMulti = AICF_OP_ADAMW_MULTI,
   MseColsum = AICF_OP_MSE_COLSUM,
   ColsumAdamW = AICF_OP_COLSUM_ADAMW,
+  QuantFp8 = AICF_OP_QUANT_FP8,
+  GemmFp8 = AICF_OP_GEMM_FP8,
+  DistillTopk = AICF_OP_DISTILL_TOPK,
+  SampleRow = AICF_OP_SAMPLE_ROW,
   _Count = AICF_OP_COUNT,
 };
 

@@ -1,0 +1,361 @@
+// Matrix product in 8-bit floating point with a f32 scale for each block of
+// 128 along K, on the MFMA matrix cores.
+//
+//   C[m,n] = sum_b SA[m,b] SB[n,b] ( sum over k in block b of A[m,k] B[n,k] ) + bias[n]
+//
+// A [M, K] and B [N, K] are e4m3 or e5m2 each, K-contiguous; their scales are
+// by rows ([M, ceil(K/128)]) or by blocks ([ceil(M/128), ceil(K/128)]).
+//
+// A K-step is one scale block, 128 bytes a row: its products start from zero,
+// and the four results a lane are added to the f32 accumulators with one
+// multiply-add each by SA SB.
+//
+// 16-bit outputs: one v_mfma_f32_16x16x128_f8f6f4 a block.  That instruction
+// (and every other 8-bit one) adds the products of 8 consecutive K after
+// aligning them to the largest, and keeps 13 bits below its exponent; the groups
+// of 8 are added in f32.  On normally distributed codes the result is off by
+// 1.5e-5 in the 2-norm, where an output of 16 bits is off by 2e-4 (f16) or 1.7e-3
+// (bf16) through its own rounding.
+// f32 outputs: the codes become bf16, which holds both 8-bit types exactly, and
+// four v_mfma_f32_16x16x32_bf16 make the block's products and f32 sums (off by
+// 1e-8), at half the rate.
+//
+// The B rows are the MFMA's first operand, so a lane holds 4 consecutive
+// columns of one output row.  Which 32 of the 128 K a lane's 8 registers hold
+// does not matter as long as it is the same for both operands: the two 16-byte
+// chunks g and g + 4 of a row for the lane group g = lane / 16.
+//
+// No counterpart in the reference.
+#include "../common/head_util.hpp"
+
+namespace aicf::hip {
+
+namespace {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+struct Fp8Gemm {
+  const uint8_t* A;
+  const uint8_t* B;
+  const float* SA;
+  const float* SB;
+  const float* bias;
+  void* C;
+  int64_t lda, ldb, ldc;
+  int64_t sa_r, sa_c, sb_r, sb_c;  // scale strides
+  int M, N, K;
+  int sa_sh, sb_sh;  // row -> scale row: 0 by rows, 7 by blocks
+  int out;           // ElemKind
+  int tiles_m, tiles_n;
+};
+
+// A lane's 32 codes of a row: as they are, or as bf16.  F: 0 e4m3, 1 e5m2.
+template <int F, bool EXACT>
+struct Frag {
+  i32x8 w;
+  __device__ __forceinline__ void set(const u32x4_t& lo, const u32x4_t& hi) {
+    w = i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+  }
+};
+template <int F>
+struct Frag<F, true> {
+  u32x4_t w[4];
+  __device__ __forceinline__ void set(const u32x4_t& lo, const u32x4_t& hi) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t x = e < 4 ? lo[e] : hi[e - 4];
+      bf16x2_t p, q;
+      if constexpr (F == 0) {
+        p = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, false);
+        q = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, true);
+      } else {
+        p = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(x, 1.0f, false);
+        q = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(x, 1.0f, true);
+      }
+      w[e >> 1][(e & 1) * 2] = __builtin_bit_cast(uint32_t, p);
+      w[e >> 1][(e & 1) * 2 + 1] = __builtin_bit_cast(uint32_t, q);
+    }
+  }
+};
+
+// The products of 16 rows of B and 16 of A over one block of K.
+template <int AF, int BF>
+__device__ __forceinline__ f32x4 mfma_block(const Frag<BF, false>& b, const Frag<AF, false>& a) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b.w, a.w, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, BF, AF, 0, 0, 0,
+                                                          0);
+}
+template <int AF, int BF>
+__device__ __forceinline__ f32x4 mfma_block(const Frag<BF, true>& b, const Frag<AF, true>& a) {
+  typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+  f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, b.w[q]),
+                                                __builtin_bit_cast(bf16x8_t, a.w[q]), d, 0, 0, 0);
+  return d;
+}
+
+// 4 consecutive outputs of a row, n of them inside.
+__device__ __forceinline__ void store_out4(void* C, int out, int64_t at, const f32x4& v, int n) {
+  typedef uint32_t u32x2_a2 __attribute__((ext_vector_type(2), aligned(2)));
+  if (out == EL_F32) {
+    float* p = static_cast<float*>(C) + at;
+    if (n >= 4) {
+      *reinterpret_cast<f32x4_a4*>(p) = v;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 3; ++e)
+        if (e < n) p[e] = v[e];
+    }
+    return;
+  }
+  uint16_t* p = static_cast<uint16_t*>(C) + at;
+  uint32_t w0, w1;
+  if (out == EL_BF16) {
+    w0 = f32x2_to_bf16x2(v[0], v[1]);
+    w1 = f32x2_to_bf16x2(v[2], v[3]);
+  } else {
+    w0 = f32_to_f16(v[0]) | (uint32_t)f32_to_f16(v[1]) << 16;
+    w1 = f32_to_f16(v[2]) | (uint32_t)f32_to_f16(v[3]) << 16;
+  }
+  if (n >= 4) {
+    *reinterpret_cast<u32x2_a2*>(p) = u32x2_a2{w0, w1};
+  } else {
+    if (n > 0) p[0] = (uint16_t)w0;
+    if (n > 1) p[1] = (uint16_t)(w0 >> 16);
+    if (n > 2) p[2] = (uint16_t)w1;
+  }
+}
+
+// 16 bytes of a row from K position k on, zero from K on, at any alignment.
+__device__ __forceinline__ u32x4_t load_chunk(const uint8_t* row, int k, int K) {
+  u32x4_t w = {0, 0, 0, 0};
+  if (k + 16 <= K) {
+    w = *reinterpret_cast<const u32x4_a1*>(row + k);
+  } else if (k < K) {
+#pragma unroll
+    for (int e = 0; e < 15; ++e)
+      if (k + e < K) w[e >> 2] |= (uint32_t)row[k + e] << (8 * (e & 3));
+  }
+  return w;
+}
+
+// Byte of chunk c of a row in a stage of 128-byte rows: 16 rows' equal chunks
+// fall on 16 different 16-byte slots of the 256 bytes of all banks.
+__device__ __forceinline__ int stage_byte(int row, int c) { return row * 128 + ((c ^ ((row >> 1) & 7)) << 4); }
+
+template <int F, bool EXACT>
+__device__ __forceinline__ Frag<F, EXACT> read_frag(const uint8_t* st, int row, int g) {
+  Frag<F, EXACT> f;
+  f.set(*reinterpret_cast<const u32x4_t*>(st + stage_byte(row, g)),
+        *reinterpret_cast<const u32x4_t*>(st + stage_byte(row, g + 4)));
+  return f;
+}
+
+// ---------------------------------------------------------------------------
+// Any sizes, strides and alignments: tiles go through registers into one of
+// two LDS stages; the loads of the next block are in flight during this one's
+// products.  Rows past M or N read the last row again (not stored), K past the
+// end is zero in both operands.
+// ---------------------------------------------------------------------------
+template <int BM, int BN, int WM, int WN, int AF, int BF, bool BROW, bool EXACT>
+__global__ __launch_bounds__(64 * WM * WN) void gemm_fp8_kernel(Fp8Gemm p) {
+  constexpr int T = 64 * WM * WN;
+  constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
+  constexpr int CA = BM * 8 / T, CB = BN * 8 / T;  // 16-byte chunks a thread
+  static_assert(CA * T == BM * 8 && CB * T == BN * 8, "chunks split evenly");
+  __shared__ __attribute__((aligned(16))) uint8_t smem[2][(BM + BN) * 128];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int wm = wave / WN, wn = wave % WN, r = lane & 15, g = lane >> 4;
+  const int tile_m = blockIdx.x % p.tiles_m, tile_n = blockIdx.x / p.tiles_m;
+  const int m0 = tile_m * BM, n0 = tile_n * BN;
+  const int nkb = (p.K + 127) / 128;
+
+  const uint8_t* pa[CA];
+  const uint8_t* pb[CB];
+#pragma unroll
+  for (int i = 0; i < CA; ++i) pa[i] = p.A + (int64_t)min(m0 + (t >> 3) + i * (T / 8), p.M - 1) * p.lda;
+#pragma unroll
+  for (int i = 0; i < CB; ++i) pb[i] = p.B + (int64_t)min(n0 + (t >> 3) + i * (T / 8), p.N - 1) * p.ldb;
+  const int c = t & 7;
+  const int put = stage_byte(t >> 3, c);  // T/8 is a multiple of 16 rows: the same swizzle for every i
+  static_assert((T / 8) % 16 == 0, "swizzle period");
+
+  const float* sa[TM];
+  const float* sb[BROW ? TN * 4 : TN];
+#pragma unroll
+  for (int j = 0; j < TM; ++j)
+    sa[j] = p.SA + (int64_t)(min(m0 + (wm * TM + j) * 16 + r, p.M - 1) >> p.sa_sh) * p.sa_r;
+#pragma unroll
+  for (int i = 0; i < TN; ++i) {
+    const int n = n0 + (wn * TN + i) * 16;
+    if constexpr (BROW) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sb[i * 4 + e] = p.SB + (int64_t)min(n + 4 * g + e, p.N - 1) * p.sb_r;
+    } else {
+      sb[i] = p.SB + (int64_t)(min(n, p.N - 1) >> 7) * p.sb_r;
+    }
+  }
+
+  f32x4 acc[TM][TN];
+#pragma unroll
+  for (int j = 0; j < TM; ++j)
+#pragma unroll
+    for (int i = 0; i < TN; ++i) acc[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  u32x4_t ra[CA], rb[CB];
+  auto load = [&](int kb) {
+#pragma unroll
+    for (int i = 0; i < CA; ++i) ra[i] = load_chunk(pa[i], kb * 128 + c * 16, p.K);
+#pragma unroll
+    for (int i = 0; i < CB; ++i) rb[i] = load_chunk(pb[i], kb * 128 + c * 16, p.K);
+  };
+  auto store = [&](uint8_t* st) {
+#pragma unroll
+    for (int i = 0; i < CA; ++i) *reinterpret_cast<u32x4_t*>(st + put + i * T * 16) = ra[i];
+#pragma unroll
+    for (int i = 0; i < CB; ++i) *reinterpret_cast<u32x4_t*>(st + BM * 128 + put + i * T * 16) = rb[i];
+  };
+  load(0);
+  store(smem[0]);
+  __syncthreads();
+  for (int kb = 0; kb < nkb; ++kb) {
+    const uint8_t* st = smem[kb & 1];
+    if (kb + 1 < nkb) load(kb + 1);
+    float fa[TM], fb[BROW ? TN * 4 : TN];
+#pragma unroll
+    for (int j = 0; j < TM; ++j) fa[j] = sa[j][kb * p.sa_c];
+#pragma unroll
+    for (int i = 0; i < (BROW ? TN * 4 : TN); ++i) fb[i] = sb[i][kb * p.sb_c];
+    Frag<BF, EXACT> b[TN];
+#pragma unroll
+    for (int i = 0; i < TN; ++i) b[i] = read_frag<BF, EXACT>(st + BM * 128, (wn * TN + i) * 16 + r, g);
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+      const Frag<AF, EXACT> a = read_frag<AF, EXACT>(st, (wm * TM + j) * 16 + r, g);
+#pragma unroll
+      for (int i = 0; i < TN; ++i) {
+        const f32x4 d = mfma_block<AF, BF>(b[i], a);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[j][i][e] = fmaf(d[e], fa[j] * fb[BROW ? i * 4 + e : i], acc[j][i][e]);
+      }
+    }
+    if (kb + 1 < nkb) store(smem[(kb + 1) & 1]);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < TN; ++i) {
+    const int n = n0 + (wn * TN + i) * 16 + 4 * g, left = p.N - n;
+    f32x4 bv = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (p.bias) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < left) bv[e] = p.bias[n + e];
+    }
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+      const int m = m0 + (wm * TM + j) * 16 + r;
+      if (m < p.M) store_out4(p.C, p.out, (int64_t)m * p.ldc + n, acc[j][i] + bv, left);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+// Scales of a [rows, cols] operand: by rows or by blocks, any strides.
+bool scale_in(const TensorDesc& t, int64_t rows, int64_t cols, int* sh) {
+  if (dt(t) != DType::kF32 || t.rank != 2 || t.shape[1] != (cols + 127) / 128) return false;
+  if (t.stride[0] < 0 || t.stride[1] < 0) return false;
+  if (t.shape[0] == rows) *sh = 0;
+  else if (t.shape[0] == (rows + 127) / 128) *sh = 7;
+  else return false;
+  return true;
+}
+
+bool gemm_fp8_sup(const TensorDesc* in, int ni, const TensorDesc* out, int no, const void*) {
+  if (!in || !out || (ni != 4 && ni != 5) || no != 1) return false;
+  int64_t lda, ldb, ldc;
+  int sh, ek;
+  if (!is_fp8(in[0]) || !is_fp8(in[2]) || !matrix_ld(in[0], false, &lda) || !matrix_ld(in[2], false, &ldb))
+    return false;
+  const int64_t M = in[0].shape[0], K = in[0].shape[1], N = in[2].shape[0];
+  constexpr int64_t kMax = (int64_t{1} << 31) - 512;
+  if (K < 1 || in[2].shape[1] != K || M > kMax || N > kMax || K > kMax) return false;
+  if (!scale_in(in[1], M, K, &sh) || !scale_in(in[3], N, K, &sh)) return false;
+  if (ni == 5 && !vector_of(in[4], DType::kF32, N)) return false;
+  if (!elem_kind(out[0], &ek) || !matrix_ld(out[0], true, &ldc)) return false;
+  if (out[0].shape[0] != M || out[0].shape[1] != N) return false;
+  return !any_overlap(in, ni, out, no);
+}
+
+template <int BM, int BN, int WM, int WN, int AF, int BF>
+Status run_tiles(Fp8Gemm& p, hipStream_t s) {
+  p.tiles_m = (p.M + BM - 1) / BM;
+  p.tiles_n = (p.N + BN - 1) / BN;
+  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+  if (tiles * 64 * WM * WN > UINT32_MAX) return Status::InvalidArgument;  // a grid's lanes are counted in 32 bits
+  const unsigned g = (unsigned)tiles;
+  constexpr int T = 64 * WM * WN;
+  if (p.out == EL_F32) {
+    if (p.sb_sh == 0) gemm_fp8_kernel<BM, BN, WM, WN, AF, BF, true, true><<<g, T, 0, s>>>(p);
+    else gemm_fp8_kernel<BM, BN, WM, WN, AF, BF, false, true><<<g, T, 0, s>>>(p);
+  } else {
+    if (p.sb_sh == 0) gemm_fp8_kernel<BM, BN, WM, WN, AF, BF, true, false><<<g, T, 0, s>>>(p);
+    else gemm_fp8_kernel<BM, BN, WM, WN, AF, BF, false, false><<<g, T, 0, s>>>(p);
+  }
+  return launch_status("gemm_fp8");
+}
+
+template <int AF, int BF>
+Status gemm_fp8_run(Fp8Gemm& p, hipStream_t s) {
+  return run_tiles<128, 128, 2, 2, AF, BF>(p, s);
+}
+
+Status gemm_fp8_launch(const TensorDesc* in, int ni, TensorDesc* out, int no, const void* at, void*, size_t,
+                       void* stream) {
+  if (!gemm_fp8_sup(in, ni, out, no, at)) return Status::InvalidArgument;
+  if (numel_of(out[0]) == 0) return Status::Ok;
+  for (int k = 0; k < ni; ++k)
+    if (no_memory(in[k])) return Status::InvalidArgument;
+  if (no_memory(out[0])) return Status::InvalidArgument;
+  Fp8Gemm p{};
+  p.A = (const uint8_t*)in[0].data;
+  p.SA = (const float*)in[1].data;
+  p.B = (const uint8_t*)in[2].data;
+  p.SB = (const float*)in[3].data;
+  p.bias = ni == 5 ? (const float*)in[4].data : nullptr;
+  p.C = out[0].data;
+  matrix_ld(in[0], false, &p.lda);
+  matrix_ld(in[2], false, &p.ldb);
+  matrix_ld(out[0], true, &p.ldc);
+  p.sa_r = in[1].stride[0];
+  p.sa_c = in[1].stride[1];
+  p.sb_r = in[3].stride[0];
+  p.sb_c = in[3].stride[1];
+  p.M = (int)in[0].shape[0];
+  p.K = (int)in[0].shape[1];
+  p.N = (int)in[2].shape[0];
+  scale_in(in[1], p.M, p.K, &p.sa_sh);
+  scale_in(in[3], p.N, p.K, &p.sb_sh);
+  elem_kind(out[0], &p.out);
+  hipStream_t s = as_stream(stream);
+  const bool a5 = dt(in[0]) == DType::kF8E5M2, b5 = dt(in[2]) == DType::kF8E5M2;
+  if (a5) return b5 ? gemm_fp8_run<1, 1>(p, s) : gemm_fp8_run<1, 0>(p, s);
+  return b5 ? gemm_fp8_run<0, 1>(p, s) : gemm_fp8_run<0, 0>(p, s);
+}
+
+size_t no_workspace(const TensorDesc*, int, const void*) { return 0; }
+
+}  // namespace
+
+KernelVariant make_gemm_fp8_variant() {
+  KernelVariant v;
+  v.name = "gemm_fp8";
+  v.launch = gemm_fp8_launch;
+  v.supported = gemm_fp8_sup;
+  v.query_workspace = no_workspace;
+  return v;
+}
+
+}  // namespace aicf::hip

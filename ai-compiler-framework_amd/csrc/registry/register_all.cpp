@@ -77,6 +77,11 @@ KernelVariant make_adamw_multi_f32_variant();
 // eltwise.hip / optim.hip (step tail)
 KernelVariant make_mse_colsum_variant();
 KernelVariant make_colsum_adamw_f32_variant();
+// quant_fp8.hip, gemm_fp8.hip, distill.hip, sample.hip
+KernelVariant make_quant_fp8_variant();
+KernelVariant make_gemm_fp8_variant();
+KernelVariant make_distill_topk_variant();
+KernelVariant make_sample_row_variant();
 
 void register_all_kernels_into(KernelRegistry& R) {
   if (std::getenv("AICF_VERBOSE")) std::fprintf(stderr, "[aicf] register_all: gfx950 backend\n");
@@ -182,6 +187,10 @@ void register_all_kernels_into(KernelRegistry& R) {
   reg(OpKind::AdamWMulti, make_adamw_multi_f32_variant(), 0, "adamw_multi_f32_v0");
   reg(OpKind::MseColsum, make_mse_colsum_variant(), 0, "mse_colsum_v0");
   reg(OpKind::ColsumAdamW, make_colsum_adamw_f32_variant(), 0, "colsum_adamw_f32_v0");
+  reg(OpKind::QuantFp8, make_quant_fp8_variant(), 0, "quant_fp8_v0");
+  reg(OpKind::GemmFp8, make_gemm_fp8_variant(), 0, "gemm_fp8_mfma_v0");
+  reg(OpKind::DistillTopk, make_distill_topk_variant(), 0, "distill_topk_v0");
+  reg(OpKind::SampleRow, make_sample_row_variant(), 0, "sample_row_v0");
 }
 
 }  // namespace aicf::hip

@@ -163,6 +163,10 @@ const char* opkind_name(OpKind k) {
     case OpKind::AdamWMulti: return "adamw_multi";
     case OpKind::MseColsum: return "mse_colsum";
     case OpKind::ColsumAdamW: return "colsum_adamw";
+    case OpKind::QuantFp8: return "quant_fp8";
+    case OpKind::GemmFp8: return "gemm_fp8";
+    case OpKind::DistillTopk: return "distill_topk";
+    case OpKind::SampleRow: return "sample_row";
     case OpKind::_Count: break;
   }
   return "unknown";

@@ -12,6 +12,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libaicf_hip.so"
 
 MAX_RANK = 4
 DTYPE_UNKNOWN, DTYPE_F32, DTYPE_F16, DTYPE_BF16, DTYPE_I32 = 0, 1, 2, 3, 4
+DTYPE_F8E4M3, DTYPE_F8E5M2 = 5, 6
 STATUS_OK, STATUS_INVALID_ARGUMENT, STATUS_NOT_IMPLEMENTED, STATUS_INTERNAL = 0, 1, 2, 3
 
 

@@ -93,7 +93,8 @@ def build_binding_plan(ir: IRGraph, *, opts: Optional[PlanOptions] = None) -> Bi
 def torch_dtype(ds: str) -> torch.dtype:
     for key, dt in (("bfloat16", torch.bfloat16), ("float16", torch.float16),
                     ("float32", torch.float32), ("float64", torch.float64),
-                    ("int64", torch.int64), ("int32", torch.int32)):
+                    ("int64", torch.int64), ("int32", torch.int32),
+                    ("float8_e4m3fn", torch.float8_e4m3fn), ("float8_e5m2", torch.float8_e5m2)):
         if key in str(ds):
             return dt
     return torch.float32

@@ -34,6 +34,9 @@ extern "C" {
 #define AICF_DTYPE_F16 2
 #define AICF_DTYPE_BF16 3
 #define AICF_DTYPE_I32 4
+/* appended (no counterpart in the reference): the OCP 8-bit float types */
+#define AICF_DTYPE_F8E4M3 5 /* largest value 448, no infinities */
+#define AICF_DTYPE_F8E5M2 6 /* largest finite value 57344 */
 
 /* Replaces registry/status.hpp:6-11 (enum class Status : int32_t); same values. */
 #define AICF_STATUS_OK 0
@@ -85,7 +88,15 @@ extern "C" {
                                     column sums over P row blocks, the step counter (schema MSCS) */
 #define AICF_OP_COLSUM_ADAMW 29  /* T column-partial tensors [R_t, N_t], P, M, V, step -> G, P, M, V, Wb:
                                     G = the column sums (concatenated), AdamW on P with it (schema CADW) */
-#define AICF_OP_COUNT 30
+#define AICF_OP_QUANT_FP8 30     /* X[M,K] -> Q, S [, Q of X^T, its S]: 8-bit floats with a f32 scale for each
+                                    1 x 128 or 128 x 128 block (schema QFP8; see below) */
+#define AICF_OP_GEMM_FP8 31      /* A, SA, B, SB [, bias] -> C = (SA A)(SB B)^T + bias (see below) */
+#define AICF_OP_DISTILL_TOPK 32  /* logits, teacher logits, their classes [, labels] [, row weights] -> loss,
+                                    [dlogits,] row loss [, scratch]: distillation from a teacher's top K
+                                    logits, forward and backward (schema DTOP; see below) */
+#define AICF_OP_SAMPLE_ROW 33    /* logits, u, temperature, top_k, top_p, min_p -> token [, log-probability
+                                    [, scratch]]: one draw a row from given random numbers (see below) */
+#define AICF_OP_COUNT 34
 
 /*
  * Attribute schema ids (numeric ABI).  The reference mixes big-endian fourccs
@@ -117,6 +128,67 @@ extern "C" {
 #define AICF_SCHEMA_XHST 0x54534858u /* appended: b"XHST" little-endian, <i> step += i (0 or 1), optionally
                                        <fff> lr, b1, b2: an 8th output (2 f32) receives the advanced
                                        step's AdamW bias corrections {lr/bc1, 1/bc2} */
+
+#define AICF_SCHEMA_QFP8 0x38504651u /* appended: b"QFP8" little-endian, <i> flags: bit 0 = scales are powers of two */
+#define AICF_SCHEMA_DTOP 0x504F5444u /* appended: b"DTOP" little-endian, <ff> temperature, weight of the labels' loss */
+
+/*
+ * The 8-bit and vocabulary-head ops (appended kinds 30..33, no counterpart in
+ * the reference).  All tensors have rank 1 or 2 as given, a last stride of 1
+ * where nothing else is said, any row stride that keeps rows apart and any
+ * element alignment.  Outputs must not overlap inputs or one another (except
+ * dlogits, which may be the logits themselves: same data and strides).
+ *
+ * QUANT_FP8: X [M, K] f32/f16/bf16 -> Q [M, K] f8 and S f32, [M, ceil(K/128)]
+ *   (a scale for each 128 columns of a row) or [ceil(M/128), ceil(K/128)] (for
+ *   each 128 x 128 block); optionally also QT [K, M] and ST, the same of X^T:
+ *   [K, ceil(M/128)] or [ceil(K/128), ceil(M/128)], both by rows or both by
+ *   blocks.  S is stored row-major or column-major.
+ *     s = max(amax / FMAX, 2^-126), FMAX the type's largest finite value;
+ *     bit 0 of the flags: s rounded up to a power of two;  q = x * (1 / s)
+ *   in f32, rounded to nearest even.  A block with a NaN has a NaN scale and
+ *   NaN codes; one with an infinity has an infinite scale, zeros, and NaN at
+ *   the infinity.  M = 0 writes nothing.
+ *
+ * GEMM_FP8: A [M, K] f8, SA, B [N, K] f8, SB, bias [N] f32 (optional) ->
+ *   C [M, N] f32/f16/bf16; the scales as QUANT_FP8 writes them, each by rows
+ *   or by blocks, with any strides; the f8 types of A and B may differ.
+ *     C[m,n] = sum_b SA[m,b] SB[n,b] (sum over k in block b of A[m,k] B[n,k]) + bias[n]
+ *   in f32, rounded once.  K >= 1; M = 0 or N = 0 writes nothing.
+ *
+ * DISTILL_TOPK: logits Z [R, V] f32/f16/bf16; teacher logits T [R, K] f32/f16/
+ *   bf16 and their classes I [R, K] i32, 1 <= K <= 1024; labels [R] i32 and row
+ *   weights w [R] f32, each optional (without weights: 1/R).  tau > 0 is the
+ *   temperature, a in [0, 1] the weight of the labels' loss.
+ *     p = softmax over the entries with 0 <= I < V of T / tau
+ *     row loss = (1 - a) tau^2 KL(p || softmax(Z / tau)) + a CE(Z, label)
+ *     loss [1] = sum_r w_r row_loss_r;   dlogits = d loss / d Z, in Z's type
+ *   A class outside [0, V) is left out of its row; a row without any has no
+ *   first term, one whose label is outside [0, V) no second.  The same class
+ *   twice counts with the sum of its probabilities.  A row of weight 0 is not
+ *   read: its row loss and dlogits are 0.  A logit of -inf has probability 0;
+ *   a row of nothing else gives NaN.  Outputs (loss, dlogits, row loss) or, for
+ *   the loss alone, (loss, row loss); a last f32 output [R, P, 4], P >= 2, is
+ *   scratch that lets P workgroups share a row where there are few rows.
+ *
+ * SAMPLE_ROW: logits Z [R, V] f32/f16/bf16, V <= 2^24; u, temperature, top_p,
+ *   min_p [R] f32, top_k [R] i32 -> token [R] i32, optionally its
+ *   log-probability [R] f32 among the kept classes.  Classes are ordered by
+ *   falling logit, equal ones by rising index; w = exp((z - max) / temperature):
+ *     top-k keeps the first k classes (k <= 0: all);
+ *     top-p of those the ones whose predecessors' w add up to less than top_p
+ *     of the kept sum (top_p >= 1 or NaN: all; the first class always);
+ *     min-p of those the ones with w >= min_p (min_p <= 0 or NaN: all);
+ *     token = the lowest class i with sum over kept j <= i of w_j > u * (sum of
+ *     all kept w).
+ *   Sums are exact in units of w far below the rounding of any 32-bit sum, so
+ *   the token does not depend on how a row was divided.  A temperature that is
+ *   not > 0 takes the first class in the order (log-probability 0).  u is
+ *   clamped to [0, 1 - 2^-24] (NaN: 0).  -inf and NaN logits are never drawn;
+ *   a row of nothing else gives token -1 and log-probability -inf.  A third
+ *   output, i32 [R, S] with S >= 8192, is scratch that lets several workgroups
+ *   share a row where there are few rows.
+ */
 
 /* GEPI epilogue kinds.  0..2 are the values core_v2/exec.py:223-252 packs;
  * 3..7 are appended (no counterpart in the reference). */

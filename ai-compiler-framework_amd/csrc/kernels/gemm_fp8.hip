@@ -26,13 +26,19 @@
 // chunks g and g + 4 of a row for the lane group g = lane / 16.
 //
 // No counterpart in the reference.
+#include "../common/gemm_types.hpp"
 #include "../common/head_util.hpp"
+#include "../common/lds_load.hpp"
+
+#include <type_traits>
 
 namespace aicf::hip {
 
 namespace {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef uint64_t u64x2_t __attribute__((ext_vector_type(2)));
+typedef uint64_t u64x2_a1 __attribute__((ext_vector_type(2), aligned(1)));
 
 struct Fp8Gemm {
   const uint8_t* A;
@@ -127,17 +133,22 @@ __device__ __forceinline__ void store_out4(void* C, int out, int64_t at, const f
   }
 }
 
-// 16 bytes of a row from K position k on, zero from K on, at any alignment.
+// 16 bytes of a row from K position k on, zero from K on, at any alignment.  A
+// chunk that would pass K is moved back to end there and shifted into place.
 __device__ __forceinline__ u32x4_t load_chunk(const uint8_t* row, int k, int K) {
-  u32x4_t w = {0, 0, 0, 0};
-  if (k + 16 <= K) {
-    w = *reinterpret_cast<const u32x4_a1*>(row + k);
-  } else if (k < K) {
-#pragma unroll
-    for (int e = 0; e < 15; ++e)
-      if (k + e < K) w[e >> 2] |= (uint32_t)row[k + e] << (8 * (e & 3));
+  u64x2_t w = {0, 0};
+  if (k < K) {
+    if (K >= 16) {
+      const int at = min(k, K - 16), s = (k - at) * 8;
+      w = *reinterpret_cast<const u64x2_a1*>(row + at);
+      if (s >= 64) w = u64x2_t{w[1] >> (s - 64), 0};
+      else if (s > 0) w = u64x2_t{(w[0] >> s) | (w[1] << (64 - s)), w[1] >> s};
+    } else {
+#pragma unroll 1
+      for (int e = K - 1; e >= k; --e) w = u64x2_t{(w[0] << 8) | row[e], (w[1] << 8) | (w[0] >> 56)};
+    }
   }
-  return w;
+  return __builtin_bit_cast(u32x4_t, w);
 }
 
 // Byte of chunk c of a row in a stage of 128-byte rows: 16 rows' equal chunks
@@ -261,6 +272,189 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_fp8_kernel(Fp8Gemm p) {
 }
 
 // ---------------------------------------------------------------------------
+// Operands whose rows are 16-byte aligned: tiles go straight into LDS (a lane's
+// 16 bytes at the place its swizzled chunk has), two stages, one barrier a
+// block of K.  The barrier stands before the block's last row of fragments:
+// there the wave has read all it needs of the stage, the next stage has landed,
+// the loads of the one after it go out into the freed stage, and the next
+// fragments are read under the remaining products.  A block's results are
+// added to the accumulators one row of fragments late, so that no multiply-add
+// waits for its MFMA.  The scales of a block come through registers into LDS,
+// one a thread, two blocks ahead.  A last, partial block goes through registers
+// with zeros behind K.
+// ---------------------------------------------------------------------------
+template <int BM, int BN, int WM, int WN, int AF, int BF, bool BROW, bool EXACT>
+__global__ __launch_bounds__(64 * WM * WN, 2) void gemm_fp8_lds_kernel(Fp8Gemm p) {
+  constexpr int T = 64 * WM * WN, NW = WM * WN;
+  constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
+  constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW;  // 1 KB loads a wave and stage
+  constexpr int STAGE = (BM + BN) * 128;
+  static_assert(BM + BN <= T && PA * NW * 8 == BM && PB * NW * 8 == BN, "a scale a thread; whole loads a wave");
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * STAGE];
+  __shared__ __attribute__((aligned(16))) float scales[2][BM + BN];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int wm = wave / WN, wn = wave % WN, r = lane & 15, g = lane >> 4;
+  int tile_m, tile_n;
+  tile_coords_of(blockIdx.x, p.tiles_m, p.tiles_n, tile_m, tile_n);
+  const int m0 = tile_m * BM, n0 = tile_n * BN;
+  const int nfull = p.K >> 7;
+
+  // loads: wave w fills the blocks of 8 rows w, w + NW, ... of each operand
+  const int last_a = min(p.M - m0, BM) - 1, last_b = min(p.N - n0, BN) - 1;
+  const i32x4_t rsrc_a = buffer_rsrc(p.A + (int64_t)m0 * p.lda, (uint32_t)(last_a * p.lda + p.K));
+  const i32x4_t rsrc_b = buffer_rsrc(p.B + (int64_t)n0 * p.ldb, (uint32_t)(last_b * p.ldb + p.K));
+  int va[PA], vb[PB];
+#pragma unroll
+  for (int i = 0; i < PA; ++i) {
+    const int row = (wave + i * NW) * 8 + (lane >> 3);
+    va[i] = min(row, last_a) * (int)p.lda + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
+  }
+#pragma unroll
+  for (int i = 0; i < PB; ++i) {
+    const int row = (wave + i * NW) * 8 + (lane >> 3);
+    vb[i] = min(row, last_b) * (int)p.ldb + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
+  }
+  typedef __attribute__((address_space(3))) unsigned lds_u32;
+  auto issue = [&](int kb) {
+    uint8_t* st = smem + (kb & 1) * STAGE;
+#pragma unroll
+    for (int i = 0; i < PA; ++i)
+      raw_buffer_load_lds(rsrc_a, (lds_u32*)(st + (wave + i * NW) * 1024), 16, va[i], kb * 128, 0, 0);
+#pragma unroll
+    for (int i = 0; i < PB; ++i)
+      raw_buffer_load_lds(rsrc_b, (lds_u32*)(st + BM * 128 + (wave + i * NW) * 1024), 16, vb[i], kb * 128, 0, 0);
+  };
+  // the thread's scale
+  const float* sp = p.SA;
+  int64_t sc = p.sa_c;
+  if (t < BM) {
+    sp += (int64_t)(min(m0 + t, p.M - 1) >> p.sa_sh) * p.sa_r;
+  } else {
+    sp = p.SB + (int64_t)(min(n0 + min(t - BM, BN - 1), p.N - 1) >> p.sb_sh) * p.sb_r;
+    sc = p.sb_c;
+  }
+  auto put_scale = [&](int kb, float v) {
+    if (BM + BN == T || t < BM + BN) scales[kb & 1][t] = v;
+  };
+
+  f32x4 acc[TM][TN];
+#pragma unroll
+  for (int j = 0; j < TM; ++j)
+#pragma unroll
+    for (int i = 0; i < TN; ++i) acc[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  Frag<BF, EXACT> b[TN];
+  Frag<AF, EXACT> a;
+  const int row_a = wm * TM * 16 + r, row_b = wn * TN * 16 + r;
+  auto read_a = [&](const uint8_t* st, int j) { return read_frag<AF, EXACT>(st, row_a + j * 16, g); };
+  auto read_b = [&](const uint8_t* st, int i) { return read_frag<BF, EXACT>(st + BM * 128, row_b + i * 16, g); };
+
+  // One block.  MODE 0: the last one; 1: the next stage is read on into; 2: and
+  // the loads of the stage after that go out.
+  auto block = [&](int kb, auto mode, float coming) {
+    constexpr bool NEXT = decltype(mode)::value > 0;
+    const uint8_t* st = smem + (kb & 1) * STAGE;
+    const float* sl = scales[kb & 1];
+    float fb[BROW ? TN * 4 : TN];
+#pragma unroll
+    for (int i = 0; i < TN; ++i) {
+      const float* q = sl + BM + (wn * TN + i) * 16;
+      if constexpr (BROW) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(q + 4 * g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) fb[i * 4 + e] = v[e];
+      } else {
+        fb[i] = q[0];
+      }
+    }
+    f32x4 d[2][TN];
+    float fa[2];
+    auto add = [&](int j) {
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          acc[j][i][e] = fmaf(d[j & 1][i][e], fa[j & 1] * fb[BROW ? i * 4 + e : i], acc[j][i][e]);
+    };
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+      fa[j & 1] = sl[row_a + j * 16];
+      Frag<AF, EXACT> an;
+      if (j + 1 < TM) {
+        an = read_a(st, j + 1);
+      } else if constexpr (NEXT) {
+        wait_vm_lgkm0<0>();
+        barrier_keep_loads();
+        if constexpr (decltype(mode)::value == 2) {
+          issue(kb + 2);
+          put_scale(kb + 2, coming);  // no wave reads this block's scales any more
+        }
+        an = read_a(smem + ((kb + 1) & 1) * STAGE, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < TN; ++i) d[j & 1][i] = mfma_block<AF, BF>(b[i], a);
+      if (j > 0) add(j - 1);
+      if (j + 1 == TM) {
+        if constexpr (NEXT) {
+#pragma unroll
+          for (int i = 0; i < TN; ++i) b[i] = read_b(smem + ((kb + 1) & 1) * STAGE, i);
+        }
+      }
+      if (j + 1 < TM || NEXT) a = an;
+      __builtin_amdgcn_sched_barrier(0);  // a row of fragments at a time: more at once would spill
+    }
+    add(TM - 1);
+  };
+
+  issue(0);  // nfull >= 2
+  put_scale(0, sp[0]);
+  put_scale(1, sp[sc]);
+  wait_vm_lgkm0<0>();
+  __syncthreads();
+  issue(1);
+#pragma unroll
+  for (int i = 0; i < TN; ++i) b[i] = read_b(smem, i);
+  a = read_a(smem, 0);
+  int kb = 0;
+  for (; kb + 2 < nfull; ++kb) block(kb, std::integral_constant<int, 2>{}, sp[(kb + 2) * sc]);
+  block(kb, std::integral_constant<int, 1>{}, 0.0f);
+  block(kb + 1, std::integral_constant<int, 0>{}, 0.0f);
+  if (p.K & 127) {
+    __syncthreads();
+    uint8_t* st = smem + (nfull & 1) * STAGE;
+    const int c = t & 7;
+#pragma unroll 1
+    for (int row = t >> 3; row < BM; row += T / 8)
+      *reinterpret_cast<u32x4_t*>(st + stage_byte(row, c)) =
+          load_chunk(p.A + (int64_t)min(m0 + row, p.M - 1) * p.lda, nfull * 128 + c * 16, p.K);
+#pragma unroll 1
+    for (int row = t >> 3; row < BN; row += T / 8)
+      *reinterpret_cast<u32x4_t*>(st + BM * 128 + stage_byte(row, c)) =
+          load_chunk(p.B + (int64_t)min(n0 + row, p.N - 1) * p.ldb, nfull * 128 + c * 16, p.K);
+    put_scale(nfull, sp[nfull * sc]);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < TN; ++i) b[i] = read_b(st, i);
+    a = read_a(st, 0);
+    block(nfull, std::integral_constant<int, 0>{}, 0.0f);
+  }
+#pragma unroll
+  for (int i = 0; i < TN; ++i) {
+    const int n = n0 + (wn * TN + i) * 16 + 4 * g, left = p.N - n;
+    f32x4 bv = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (p.bias) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < left) bv[e] = p.bias[n + e];
+    }
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+      const int m = m0 + (wm * TM + j) * 16 + r;
+      if (m < p.M) store_out4(p.C, p.out, (int64_t)m * p.ldc + n, acc[j][i] + bv, left);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
 // Scales of a [rows, cols] operand: by rows or by blocks, any strides.
@@ -289,27 +483,38 @@ bool gemm_fp8_sup(const TensorDesc* in, int ni, const TensorDesc* out, int no, c
   return !any_overlap(in, ni, out, no);
 }
 
-template <int BM, int BN, int WM, int WN, int AF, int BF>
+// LDS: the kernel that loads straight into LDS.
+template <bool LDS, int BM, int BN, int WM, int WN, int AF, int BF>
 Status run_tiles(Fp8Gemm& p, hipStream_t s) {
   p.tiles_m = (p.M + BM - 1) / BM;
   p.tiles_n = (p.N + BN - 1) / BN;
-  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-  if (tiles * 64 * WM * WN > UINT32_MAX) return Status::InvalidArgument;  // a grid's lanes are counted in 32 bits
-  const unsigned g = (unsigned)tiles;
   constexpr int T = 64 * WM * WN;
+  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+  if (tiles * T > UINT32_MAX) return Status::InvalidArgument;  // a grid's lanes are counted in 32 bits
+  const unsigned g = (unsigned)tiles;
+  auto go = [&](auto brow, auto exact) {
+    constexpr bool R = decltype(brow)::value, E = decltype(exact)::value;
+    if constexpr (LDS) gemm_fp8_lds_kernel<BM, BN, WM, WN, AF, BF, R, E><<<g, T, 0, s>>>(p);
+    else gemm_fp8_kernel<BM, BN, WM, WN, AF, BF, R, E><<<g, T, 0, s>>>(p);
+  };
   if (p.out == EL_F32) {
-    if (p.sb_sh == 0) gemm_fp8_kernel<BM, BN, WM, WN, AF, BF, true, true><<<g, T, 0, s>>>(p);
-    else gemm_fp8_kernel<BM, BN, WM, WN, AF, BF, false, true><<<g, T, 0, s>>>(p);
+    if (p.sb_sh == 0) go(std::true_type{}, std::true_type{});
+    else go(std::false_type{}, std::true_type{});
   } else {
-    if (p.sb_sh == 0) gemm_fp8_kernel<BM, BN, WM, WN, AF, BF, true, false><<<g, T, 0, s>>>(p);
-    else gemm_fp8_kernel<BM, BN, WM, WN, AF, BF, false, false><<<g, T, 0, s>>>(p);
+    if (p.sb_sh == 0) go(std::true_type{}, std::false_type{});
+    else go(std::false_type{}, std::false_type{});
   }
   return launch_status("gemm_fp8");
 }
 
 template <int AF, int BF>
 Status gemm_fp8_run(Fp8Gemm& p, hipStream_t s) {
-  return run_tiles<128, 128, 2, 2, AF, BF>(p, s);
+  // straight into LDS: 16-byte aligned rows, a tile's bytes within 32-bit offsets
+  const bool lds = aligned(p.A, 16) && aligned(p.B, 16) && p.lda % 16 == 0 && p.ldb % 16 == 0 &&
+                   p.lda < (1 << 22) && p.ldb < (1 << 22) && p.K >= 256;
+  if (!lds) return run_tiles<false, 128, 128, 2, 2, AF, BF>(p, s);
+  if (p.out == EL_F32) return run_tiles<true, 128, 128, 2, 2, AF, BF>(p, s);
+  return run_tiles<true, 256, 256, 2, 4, AF, BF>(p, s);
 }
 
 Status gemm_fp8_launch(const TensorDesc* in, int ni, TensorDesc* out, int no, const void* at, void*, size_t,

@@ -314,15 +314,24 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_fp8_lds_kernel(Fp8Gemm p
     const int row = (wave + i * NW) * 8 + (lane >> 3);
     vb[i] = min(row, last_b) * (int)p.ldb + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
   }
-  typedef __attribute__((address_space(3))) unsigned lds_u32;
-  auto issue = [&](int kb) {
-    uint8_t* st = smem + (kb & 1) * STAGE;
+  // (inline asm: the compiler would wait for all loads in flight before every
+  // LDS read that follows one)
+  auto issue = [&](int kb, auto pad) {
+    const uint32_t st = (uint32_t)(uintptr_t)(smem + (kb & 1) * STAGE);
 #pragma unroll
     for (int i = 0; i < PA; ++i)
-      raw_buffer_load_lds(rsrc_a, (lds_u32*)(st + (wave + i * NW) * 1024), 16, va[i], kb * 128, 0, 0);
+      asm_buffer_load_lds<decltype(pad)::value>(rsrc_a, st + (wave + i * NW) * 1024, va[i], kb * 128);
 #pragma unroll
     for (int i = 0; i < PB; ++i)
-      raw_buffer_load_lds(rsrc_b, (lds_u32*)(st + BM * 128 + (wave + i * NW) * 1024), 16, vb[i], kb * 128, 0, 0);
+      asm_buffer_load_lds<decltype(pad)::value>(rsrc_b, st + BM * 128 + (wave + i * NW) * 1024, vb[i], kb * 128);
+  };
+  // Waits for the wave's loads; their offsets stay in their registers until then.
+  auto landed = [&] {
+    wait_vm_lgkm0<0>();
+#pragma unroll
+    for (int i = 0; i < PA; ++i) asm volatile("" ::"v"(va[i]));
+#pragma unroll
+    for (int i = 0; i < PB; ++i) asm volatile("" ::"v"(vb[i]));
   };
   // the thread's scale
   const float* sp = p.SA;
@@ -382,10 +391,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_fp8_lds_kernel(Fp8Gemm p
       if (j + 1 < TM) {
         an = read_a(st, j + 1);
       } else if constexpr (NEXT) {
-        wait_vm_lgkm0<0>();
+        landed();
         barrier_keep_loads();
         if constexpr (decltype(mode)::value == 2) {
-          issue(kb + 2);
+          issue(kb + 2, std::false_type{});
           put_scale(kb + 2, coming);  // no wave reads this block's scales any more
         }
         an = read_a(smem + ((kb + 1) & 1) * STAGE, 0);
@@ -400,17 +409,25 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_fp8_lds_kernel(Fp8Gemm p
         }
       }
       if (j + 1 < TM || NEXT) a = an;
+      if (!EXACT && j > 0 && j + 1 < TM) {  // the multiply-adds of row j - 1 between the MFMAs of row j
+        __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+#pragma unroll
+        for (int i = 0; i < TN; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, BROW ? 8 : 5, 0);
+        }
+      }
       __builtin_amdgcn_sched_barrier(0);  // a row of fragments at a time: more at once would spill
     }
     add(TM - 1);
   };
 
-  issue(0);  // nfull >= 2
+  issue(0, std::true_type{});  // nfull >= 2
   put_scale(0, sp[0]);
   put_scale(1, sp[sc]);
-  wait_vm_lgkm0<0>();
+  landed();
   __syncthreads();
-  issue(1);
+  issue(1, std::true_type{});
 #pragma unroll
   for (int i = 0; i < TN; ++i) b[i] = read_b(smem, i);
   a = read_a(smem, 0);

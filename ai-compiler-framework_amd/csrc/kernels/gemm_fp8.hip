@@ -101,6 +101,13 @@ __device__ __forceinline__ f32x4 mfma_block(const Frag<BF, true>& b, const Frag<
   return d;
 }
 
+// 4 outputs of a 16-bit type.
+__device__ __forceinline__ uint2 pack_out4(int out, const f32x4& v) {
+  if (out == EL_BF16) return uint2{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3])};
+  return uint2{f32_to_f16(v[0]) | (uint32_t)f32_to_f16(v[1]) << 16,
+               f32_to_f16(v[2]) | (uint32_t)f32_to_f16(v[3]) << 16};
+}
+
 // 4 consecutive outputs of a row, n of them inside.
 __device__ __forceinline__ void store_out4(void* C, int out, int64_t at, const f32x4& v, int n) {
   typedef uint32_t u32x2_a2 __attribute__((ext_vector_type(2), aligned(2)));
@@ -116,20 +123,13 @@ __device__ __forceinline__ void store_out4(void* C, int out, int64_t at, const f
     return;
   }
   uint16_t* p = static_cast<uint16_t*>(C) + at;
-  uint32_t w0, w1;
-  if (out == EL_BF16) {
-    w0 = f32x2_to_bf16x2(v[0], v[1]);
-    w1 = f32x2_to_bf16x2(v[2], v[3]);
-  } else {
-    w0 = f32_to_f16(v[0]) | (uint32_t)f32_to_f16(v[1]) << 16;
-    w1 = f32_to_f16(v[2]) | (uint32_t)f32_to_f16(v[3]) << 16;
-  }
+  const uint2 w = pack_out4(out, v);
   if (n >= 4) {
-    *reinterpret_cast<u32x2_a2*>(p) = u32x2_a2{w0, w1};
+    *reinterpret_cast<u32x2_a2*>(p) = u32x2_a2{w.x, w.y};
   } else {
-    if (n > 0) p[0] = (uint16_t)w0;
-    if (n > 1) p[1] = (uint16_t)(w0 >> 16);
-    if (n > 2) p[2] = (uint16_t)w1;
+    if (n > 0) p[0] = (uint16_t)w.x;
+    if (n > 1) p[1] = (uint16_t)(w.x >> 16);
+    if (n > 2) p[2] = (uint16_t)w.y;
   }
 }
 
@@ -363,17 +363,19 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_fp8_lds_kernel(Fp8Gemm p
     constexpr bool NEXT = decltype(mode)::value > 0;
     const uint8_t* st = smem + (kb & 1) * STAGE;
     const float* sl = scales[kb & 1];
-    float fb[BROW ? TN * 4 : TN];
+    // by blocks, the wave's columns (at most 128, and no block's end among
+    // them) share one scale
+    static_assert(128 % (TN * 16) == 0, "a wave's columns lie in one block");
+    float fb[BROW ? TN * 4 : 1];
+    if constexpr (BROW) {
 #pragma unroll
-    for (int i = 0; i < TN; ++i) {
-      const float* q = sl + BM + (wn * TN + i) * 16;
-      if constexpr (BROW) {
-        const f32x4 v = *reinterpret_cast<const f32x4*>(q + 4 * g);
+      for (int i = 0; i < TN; ++i) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(sl + BM + (wn * TN + i) * 16 + 4 * g);
 #pragma unroll
         for (int e = 0; e < 4; ++e) fb[i * 4 + e] = v[e];
-      } else {
-        fb[i] = q[0];
       }
+    } else {
+      fb[0] = sl[BM + wn * TN * 16];
     }
     f32x4 d[2][TN];
     float fa[2];
@@ -382,7 +384,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_fp8_lds_kernel(Fp8Gemm p
       for (int i = 0; i < TN; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          acc[j][i][e] = fmaf(d[j & 1][i][e], fa[j & 1] * fb[BROW ? i * 4 + e : i], acc[j][i][e]);
+          acc[j][i][e] = fmaf(d[j & 1][i][e], fa[j & 1] * fb[BROW ? i * 4 + e : 0], acc[j][i][e]);
     };
 #pragma unroll
     for (int j = 0; j < TM; ++j) {
@@ -454,19 +456,46 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_fp8_lds_kernel(Fp8Gemm p
     a = read_a(st, 0);
     block(nfull, std::integral_constant<int, 0>{}, 0.0f);
   }
+
+  // The tile goes through LDS, so that whole rows are stored, 16 bytes a lane:
+  // chunk c of a row at c ^ (row mod the row's chunks).
+  constexpr int OB = EXACT ? 4 : 2, ROWB = BN * OB, CPR = ROWB / 16, EPC = 16 / OB;
+  static_assert(BM * ROWB <= 2 * STAGE && BM * CPR % T == 0, "the tile fits the stages");
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < TN; ++i) {
-    const int n = n0 + (wn * TN + i) * 16 + 4 * g, left = p.N - n;
+    const int nl = (wn * TN + i) * 16 + 4 * g, left = p.N - n0 - nl;
     f32x4 bv = {0.0f, 0.0f, 0.0f, 0.0f};
     if (p.bias) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (e < left) bv[e] = p.bias[n + e];
+        if (e < left) bv[e] = p.bias[n0 + nl + e];
     }
 #pragma unroll
     for (int j = 0; j < TM; ++j) {
-      const int m = m0 + (wm * TM + j) * 16 + r;
-      if (m < p.M) store_out4(p.C, p.out, (int64_t)m * p.ldc + n, acc[j][i] + bv, left);
+      const int row = row_a + j * 16;
+      const f32x4 v = acc[j][i] + bv;
+      uint8_t* at = smem + row * ROWB + (((nl / EPC) ^ (row & (CPR - 1))) << 4);
+      if constexpr (EXACT) *reinterpret_cast<f32x4*>(at) = v;
+      else *reinterpret_cast<uint2*>(at + (nl & 4) * 2) = pack_out4(p.out, v);
+    }
+  }
+  __syncthreads();
+#pragma unroll 4
+  for (int q = t; q < BM * CPR; q += T) {
+    const int row = q / CPR, c = q % CPR, n = n0 + c * EPC;
+    const u32x4_t v = *reinterpret_cast<const u32x4_t*>(smem + row * ROWB + ((c ^ (row & (CPR - 1))) << 4));
+    if (m0 + row >= p.M || n >= p.N) continue;
+    uint8_t* dst = static_cast<uint8_t*>(p.C) + ((int64_t)(m0 + row) * p.ldc + n) * OB;
+    if (n + EPC <= p.N) {
+      *reinterpret_cast<u32x4_a1*>(dst) = v;
+    } else {
+#pragma unroll
+      for (int e = 0; e < EPC - 1; ++e)
+        if (n + e < p.N) {
+          if constexpr (EXACT) reinterpret_cast<uint32_t*>(dst)[e] = v[e];
+          else reinterpret_cast<uint16_t*>(dst)[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+        }
     }
   }
 }
@@ -500,8 +529,8 @@ bool gemm_fp8_sup(const TensorDesc* in, int ni, const TensorDesc* out, int no, c
   return !any_overlap(in, ni, out, no);
 }
 
-// LDS: the kernel that loads straight into LDS.
-template <bool LDS, int BM, int BN, int WM, int WN, int AF, int BF>
+// LDS: the kernel that loads straight into LDS.  EXACT: f32 outputs.
+template <bool LDS, bool EXACT, int BM, int BN, int WM, int WN, int AF, int BF>
 Status run_tiles(Fp8Gemm& p, hipStream_t s) {
   p.tiles_m = (p.M + BM - 1) / BM;
   p.tiles_n = (p.N + BN - 1) / BN;
@@ -509,18 +538,13 @@ Status run_tiles(Fp8Gemm& p, hipStream_t s) {
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
   if (tiles * T > UINT32_MAX) return Status::InvalidArgument;  // a grid's lanes are counted in 32 bits
   const unsigned g = (unsigned)tiles;
-  auto go = [&](auto brow, auto exact) {
-    constexpr bool R = decltype(brow)::value, E = decltype(exact)::value;
-    if constexpr (LDS) gemm_fp8_lds_kernel<BM, BN, WM, WN, AF, BF, R, E><<<g, T, 0, s>>>(p);
-    else gemm_fp8_kernel<BM, BN, WM, WN, AF, BF, R, E><<<g, T, 0, s>>>(p);
+  auto go = [&](auto brow) {
+    constexpr bool R = decltype(brow)::value;
+    if constexpr (LDS) gemm_fp8_lds_kernel<BM, BN, WM, WN, AF, BF, R, EXACT><<<g, T, 0, s>>>(p);
+    else gemm_fp8_kernel<BM, BN, WM, WN, AF, BF, R, EXACT><<<g, T, 0, s>>>(p);
   };
-  if (p.out == EL_F32) {
-    if (p.sb_sh == 0) go(std::true_type{}, std::true_type{});
-    else go(std::false_type{}, std::true_type{});
-  } else {
-    if (p.sb_sh == 0) go(std::true_type{}, std::false_type{});
-    else go(std::false_type{}, std::false_type{});
-  }
+  if (p.sb_sh == 0) go(std::true_type{});
+  else go(std::false_type{});
   return launch_status("gemm_fp8");
 }
 
@@ -529,9 +553,12 @@ Status gemm_fp8_run(Fp8Gemm& p, hipStream_t s) {
   // straight into LDS: 16-byte aligned rows, a tile's bytes within 32-bit offsets
   const bool lds = aligned(p.A, 16) && aligned(p.B, 16) && p.lda % 16 == 0 && p.ldb % 16 == 0 &&
                    p.lda < (1 << 22) && p.ldb < (1 << 22) && p.K >= 256;
-  if (!lds) return run_tiles<false, 128, 128, 2, 2, AF, BF>(p, s);
-  if (p.out == EL_F32) return run_tiles<true, 128, 128, 2, 2, AF, BF>(p, s);
-  return run_tiles<true, 256, 256, 2, 4, AF, BF>(p, s);
+  if (p.out == EL_F32) {
+    if (!lds) return run_tiles<false, true, 128, 128, 2, 2, AF, BF>(p, s);
+    return run_tiles<true, true, 128, 128, 2, 2, AF, BF>(p, s);
+  }
+  if (!lds) return run_tiles<false, false, 128, 128, 2, 2, AF, BF>(p, s);
+  return run_tiles<true, false, 256, 256, 2, 4, AF, BF>(p, s);
 }
 
 Status gemm_fp8_launch(const TensorDesc* in, int ni, TensorDesc* out, int no, const void* at, void*, size_t,

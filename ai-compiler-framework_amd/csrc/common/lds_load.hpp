@@ -48,6 +48,20 @@ __device__ __forceinline__ void asm_buffer_load_lds(i32x4_t rsrc, uint32_t lds_a
                  : "v"(voffset), "s"(rsrc), "s"(soffset), "{m0}"(lds_addr)
                  : "memory");
 }
+// The same for 4 bytes a lane: lane i's land at the LDS address + 4 i.
+template <bool PAD>
+__device__ __forceinline__ void asm_buffer_load_lds4(i32x4_t rsrc, uint32_t lds_addr, int voffset, int soffset) {
+  if constexpr (PAD)
+    asm volatile("s_nop 4\n\tbuffer_load_dword %0, %1, %2 offen lds"
+                 :
+                 : "v"(voffset), "s"(rsrc), "s"(soffset), "{m0}"(lds_addr)
+                 : "memory");
+  else
+    asm volatile("s_nop 0\n\tbuffer_load_dword %0, %1, %2 offen lds"
+                 :
+                 : "v"(voffset), "s"(rsrc), "s"(soffset), "{m0}"(lds_addr)
+                 : "memory");
+}
 __device__ __forceinline__ i32x4_t buffer_rsrc(const void* base, uint32_t bytes) {
   struct __attribute__((packed)) Rsrc {
     const void* ptr;

@@ -59,14 +59,14 @@ struct Fp8Gemm {
 template <int F, bool EXACT>
 struct Frag {
   i32x8 w;
-  __device__ __forceinline__ void set(const u32x4_t& lo, const u32x4_t& hi) {
+  __device__ __forceinline__ void set(u32x4_t lo, u32x4_t hi) {
     w = i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
   }
 };
 template <int F>
 struct Frag<F, true> {
   u32x4_t w[4];
-  __device__ __forceinline__ void set(const u32x4_t& lo, const u32x4_t& hi) {
+  __device__ __forceinline__ void set(u32x4_t lo, u32x4_t hi) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const uint32_t x = e < 4 ? lo[e] : hi[e - 4];
@@ -273,25 +273,30 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_fp8_kernel(Fp8Gemm p) {
 
 // ---------------------------------------------------------------------------
 // Operands whose rows are 16-byte aligned: tiles go straight into LDS (a lane's
-// 16 bytes at the place its swizzled chunk has), two stages, one barrier a
-// block of K.  The barrier stands before the block's last row of fragments:
-// there the wave has read all it needs of the stage, the next stage has landed,
-// the loads of the one after it go out into the freed stage, and the next
-// fragments are read under the remaining products.  A block's results are
-// added to the accumulators one row of fragments late, so that no multiply-add
-// waits for its MFMA.  The scales of a block come through registers into LDS,
-// one a thread, two blocks ahead.  A last, partial block goes through registers
-// with zeros behind K.
+// 16 bytes at the place its swizzled chunk has), and so do the block's scales,
+// one a lane; S stages, one barrier a block of K.  The barrier stands before the
+// block's last row of fragments: there the wave has read all it needs of the
+// stage, the next stage has landed, the loads of block kb + S go out into the
+// freed stage, and the next fragments are read under the remaining products.  A
+// block's results are added to the accumulators one row of fragments late, so
+// that no multiply-add waits for its MFMA.  A last, partial block goes through
+// registers with zeros behind K.
 // ---------------------------------------------------------------------------
-template <int BM, int BN, int WM, int WN, int AF, int BF, bool BROW, bool EXACT>
+template <int BM, int BN, int WM, int WN, int S, int AF, int BF, bool BROW, bool EXACT>
 __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_fp8_lds_kernel(Fp8Gemm p) {
   constexpr int T = 64 * WM * WN, NW = WM * WN;
   constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
   constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW;  // 1 KB loads a wave and stage
   constexpr int STAGE = (BM + BN) * 128;
-  static_assert(BM + BN <= T && PA * NW * 8 == BM && PB * NW * 8 == BN, "a scale a thread; whole loads a wave");
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * STAGE];
-  __shared__ __attribute__((aligned(16))) float scales[2][BM + BN];
+  // scales: wave w fetches those of rows 64 w .. of the tile's A rows and then B
+  // rows; waves beyond them repeat the last ones, so that every wave has the
+  // same loads in flight
+  constexpr int SW = (BM + BN) / 64, NVM = PA + PB + 1;
+  static_assert(BM + BN <= T && BM % 64 == 0 && BN % 64 == 0 && PA * NW * 8 == BM && PB * NW * 8 == BN,
+                "whole loads a wave");
+  static_assert(S >= 2 && (S - 1) * NVM < 64, "loads in flight are counted in 6 bits");
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[S * STAGE];
+  __shared__ __attribute__((aligned(16))) float scales[S][64 * (SW < NW ? SW + 1 : SW)];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int wm = wave / WN, wn = wave % WN, r = lane & 15, g = lane >> 4;
   int tile_m, tile_n;
@@ -314,37 +319,42 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_fp8_lds_kernel(Fp8Gemm p
     const int row = (wave + i * NW) * 8 + (lane >> 3);
     vb[i] = min(row, last_b) * (int)p.ldb + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
   }
+  const bool of_a = wave < BM / 64;
+  const int srow = (of_a ? wave : min(wave - BM / 64, BN / 64 - 1)) * 64 + lane;
+  const int64_t s_first = of_a ? (int64_t)(m0 >> p.sa_sh) * p.sa_r : (int64_t)(n0 >> p.sb_sh) * p.sb_r;
+  const i32x4_t rsrc_s = buffer_rsrc((of_a ? p.SA : p.SB) + s_first, 0x7fffffffu);
+  const int s_step = of_a ? (int)p.sa_c * 4 : (int)p.sb_c * 4;
+  const int vs = of_a ? (((m0 + min(srow, last_a)) >> p.sa_sh) - (m0 >> p.sa_sh)) * (int)p.sa_r * 4
+                      : (((n0 + min(srow, last_b)) >> p.sb_sh) - (n0 >> p.sb_sh)) * (int)p.sb_r * 4;
+
   // (inline asm: the compiler would wait for all loads in flight before every
   // LDS read that follows one)
   auto issue = [&](int kb, auto pad) {
-    const uint32_t st = (uint32_t)(uintptr_t)(smem + (kb & 1) * STAGE);
+    constexpr bool PAD = decltype(pad)::value;
+    const int slot = S == 2 ? kb & 1 : kb % S;
+    const uint32_t st = (uint32_t)(uintptr_t)(smem + slot * STAGE);
 #pragma unroll
-    for (int i = 0; i < PA; ++i)
-      asm_buffer_load_lds<decltype(pad)::value>(rsrc_a, st + (wave + i * NW) * 1024, va[i], kb * 128);
+    for (int i = 0; i < PA; ++i) asm_buffer_load_lds<PAD>(rsrc_a, st + (wave + i * NW) * 1024, va[i], kb * 128);
 #pragma unroll
     for (int i = 0; i < PB; ++i)
-      asm_buffer_load_lds<decltype(pad)::value>(rsrc_b, st + BM * 128 + (wave + i * NW) * 1024, vb[i], kb * 128);
+      asm_buffer_load_lds<PAD>(rsrc_b, st + BM * 128 + (wave + i * NW) * 1024, vb[i], kb * 128);
+    asm_buffer_load_lds4<PAD>(rsrc_s, (uint32_t)(uintptr_t)(scales[slot] + min(wave, SW) * 64), vs, kb * s_step);
   };
-  // Waits for the wave's loads; their offsets stay in their registers until then.
-  auto landed = [&] {
+  // Waits for all but the last n blocks' loads of the wave, n < S - 1.
+  auto wait_blocks = [&](int n) {
+    if constexpr (S > 3)
+      if (n >= 2) return wait_vm_lgkm0<2 * NVM>();
+    if constexpr (S > 2)
+      if (n == 1) return wait_vm_lgkm0<NVM>();
     wait_vm_lgkm0<0>();
+    // the loads' offsets stay in their registers until the last load has landed
 #pragma unroll
     for (int i = 0; i < PA; ++i) asm volatile("" ::"v"(va[i]));
 #pragma unroll
     for (int i = 0; i < PB; ++i) asm volatile("" ::"v"(vb[i]));
+    asm volatile("" ::"v"(vs));
   };
-  // the thread's scale
-  const float* sp = p.SA;
-  int64_t sc = p.sa_c;
-  if (t < BM) {
-    sp += (int64_t)(min(m0 + t, p.M - 1) >> p.sa_sh) * p.sa_r;
-  } else {
-    sp = p.SB + (int64_t)(min(n0 + min(t - BM, BN - 1), p.N - 1) >> p.sb_sh) * p.sb_r;
-    sc = p.sb_c;
-  }
-  auto put_scale = [&](int kb, float v) {
-    if (BM + BN == T || t < BM + BN) scales[kb & 1][t] = v;
-  };
+  static_assert(S <= 4, "wait_blocks");
 
   f32x4 acc[TM][TN];
 #pragma unroll
@@ -357,12 +367,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_fp8_lds_kernel(Fp8Gemm p
   auto read_a = [&](const uint8_t* st, int j) { return read_frag<AF, EXACT>(st, row_a + j * 16, g); };
   auto read_b = [&](const uint8_t* st, int i) { return read_frag<BF, EXACT>(st + BM * 128, row_b + i * 16, g); };
 
+  auto stage_of = [&](int kb) { return S == 2 ? kb & 1 : kb % S; };
   // One block.  MODE 0: the last one; 1: the next stage is read on into; 2: and
-  // the loads of the stage after that go out.
-  auto block = [&](int kb, auto mode, float coming) {
-    constexpr bool NEXT = decltype(mode)::value > 0;
-    const uint8_t* st = smem + (kb & 1) * STAGE;
-    const float* sl = scales[kb & 1];
+  // the loads of block kb + S go out.
+  auto block = [&](int kb, auto mode) {
+    constexpr int MODE = decltype(mode)::value;
+    constexpr bool NEXT = MODE > 0;
+    const uint8_t* st = smem + stage_of(kb) * STAGE;
+    const float* sl = scales[stage_of(kb)];
     // by blocks, the wave's columns (at most 128, and no block's end among
     // them) share one scale
     static_assert(128 % (TN * 16) == 0, "a wave's columns lie in one block");
@@ -393,13 +405,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_fp8_lds_kernel(Fp8Gemm p
       if (j + 1 < TM) {
         an = read_a(st, j + 1);
       } else if constexpr (NEXT) {
-        landed();
+        if constexpr (MODE == 2) wait_vm_lgkm0<(S - 2) * NVM>();
+        else wait_blocks(nfull - 2 - kb);
         barrier_keep_loads();
-        if constexpr (decltype(mode)::value == 2) {
-          issue(kb + 2, std::false_type{});
-          put_scale(kb + 2, coming);  // no wave reads this block's scales any more
-        }
-        an = read_a(smem + ((kb + 1) & 1) * STAGE, 0);
+        if constexpr (MODE == 2) issue(kb + S, std::false_type{});
+        an = read_a(smem + stage_of(kb + 1) * STAGE, 0);
       }
 #pragma unroll
       for (int i = 0; i < TN; ++i) d[j & 1][i] = mfma_block<AF, BF>(b[i], a);
@@ -407,7 +417,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_fp8_lds_kernel(Fp8Gemm p
       if (j + 1 == TM) {
         if constexpr (NEXT) {
 #pragma unroll
-          for (int i = 0; i < TN; ++i) b[i] = read_b(smem + ((kb + 1) & 1) * STAGE, i);
+          for (int i = 0; i < TN; ++i) b[i] = read_b(smem + stage_of(kb + 1) * STAGE, i);
         }
       }
       if (j + 1 < TM || NEXT) a = an;
@@ -424,22 +434,26 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_fp8_lds_kernel(Fp8Gemm p
     add(TM - 1);
   };
 
-  issue(0, std::true_type{});  // nfull >= 2
-  put_scale(0, sp[0]);
-  put_scale(1, sp[sc]);
-  landed();
-  __syncthreads();
-  issue(1, std::true_type{});
+  // nfull >= 2
+  issue(0, std::true_type{});
+  if constexpr (S > 2) {
+    for (int q = 1; q < S - 1 && q < nfull; ++q) issue(q, std::true_type{});
+    wait_blocks(min(nfull - 1, S - 2));
+  } else {
+    wait_blocks(0);
+  }
+  barrier_keep_loads();
+  if (S == 2 || S - 1 < nfull) issue(S - 1, std::true_type{});
 #pragma unroll
   for (int i = 0; i < TN; ++i) b[i] = read_b(smem, i);
   a = read_a(smem, 0);
   int kb = 0;
-  for (; kb + 2 < nfull; ++kb) block(kb, std::integral_constant<int, 2>{}, sp[(kb + 2) * sc]);
-  block(kb, std::integral_constant<int, 1>{}, 0.0f);
-  block(kb + 1, std::integral_constant<int, 0>{}, 0.0f);
+  for (; kb + S < nfull; ++kb) block(kb, std::integral_constant<int, 2>{});
+  for (; kb + 1 < nfull; ++kb) block(kb, std::integral_constant<int, 1>{});
+  block(kb, std::integral_constant<int, 0>{});
   if (p.K & 127) {
     __syncthreads();
-    uint8_t* st = smem + (nfull & 1) * STAGE;
+    uint8_t* st = smem + stage_of(nfull) * STAGE;
     const int c = t & 7;
 #pragma unroll 1
     for (int row = t >> 3; row < BM; row += T / 8)
@@ -449,18 +463,23 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_fp8_lds_kernel(Fp8Gemm p
     for (int row = t >> 3; row < BN; row += T / 8)
       *reinterpret_cast<u32x4_t*>(st + BM * 128 + stage_byte(row, c)) =
           load_chunk(p.B + (int64_t)min(n0 + row, p.N - 1) * p.ldb, nfull * 128 + c * 16, p.K);
-    put_scale(nfull, sp[nfull * sc]);
+    if (t < BM + BN) {
+      const bool ra = t < BM;
+      scales[stage_of(nfull)][t] =
+          ra ? p.SA[(int64_t)((m0 + min(t, last_a)) >> p.sa_sh) * p.sa_r + nfull * p.sa_c]
+             : p.SB[(int64_t)((n0 + min(t - BM, last_b)) >> p.sb_sh) * p.sb_r + nfull * p.sb_c];
+    }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < TN; ++i) b[i] = read_b(st, i);
     a = read_a(st, 0);
-    block(nfull, std::integral_constant<int, 0>{}, 0.0f);
+    block(nfull, std::integral_constant<int, 0>{});
   }
 
   // The tile goes through LDS, so that whole rows are stored, 16 bytes a lane:
   // chunk c of a row at c ^ (row mod the row's chunks).
   constexpr int OB = EXACT ? 4 : 2, ROWB = BN * OB, CPR = ROWB / 16, EPC = 16 / OB;
-  static_assert(BM * ROWB <= 2 * STAGE && BM * CPR % T == 0, "the tile fits the stages");
+  static_assert(BM * ROWB <= S * STAGE && BM * CPR % T == 0, "the tile fits the stages");
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < TN; ++i) {
@@ -501,6 +520,120 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_fp8_lds_kernel(Fp8Gemm p
 }
 
 // ---------------------------------------------------------------------------
+// At most 16 TM rows of A: the bytes of B are what counts.  A wave takes 16
+// rows of B over a share of K, straight into registers (a row's 128 bytes of a
+// block are one cache line), the KW waves of a workgroup share K and add up
+// through LDS in a fixed order.  Any alignment.  Products and sums in f32, as
+// for f32 outputs above: the matrix cores have nothing else to do.
+// ---------------------------------------------------------------------------
+template <int TM, int KW, int AF, int BF, bool BROW>
+__global__ __launch_bounds__(64 * KW) void gemm_fp8_rows_kernel(Fp8Gemm p) {
+  constexpr int U = TM == 1 ? 4 : 2;  // blocks in flight
+  __shared__ __attribute__((aligned(16))) f32x4 part[KW][TM][64];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * 16;
+  const int nkb = (p.K + 127) >> 7;
+  const int k0 = (int)((int64_t)nkb * wave / KW), k1 = (int)((int64_t)nkb * (wave + 1) / KW);
+  const uint8_t* pb = p.B + (int64_t)min(n0 + r, p.N - 1) * p.ldb;
+  const uint8_t* pa[TM];
+  const float* sa[TM];
+#pragma unroll
+  for (int j = 0; j < TM; ++j) {
+    const int m = min(j * 16 + r, p.M - 1);
+    pa[j] = p.A + (int64_t)m * p.lda;
+    sa[j] = p.SA + (int64_t)(m >> p.sa_sh) * p.sa_r;
+  }
+  const float* sb[BROW ? 4 : 1];
+#pragma unroll
+  for (int e = 0; e < (BROW ? 4 : 1); ++e)
+    sb[e] = p.SB + (int64_t)(min(n0 + (BROW ? 4 * g + e : 0), p.N - 1) >> p.sb_sh) * p.sb_r;
+
+  f32x4 acc[TM];
+#pragma unroll
+  for (int j = 0; j < TM; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  auto add = [&](int kb, const Frag<BF, true>& b, const Frag<AF, true>& a, int j, const float (&fb)[BROW ? 4 : 1],
+                 float fa) {
+    const f32x4 d = mfma_block<AF, BF>(b, a);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[j][e] = fmaf(d[e], fa * fb[BROW ? e : 0], acc[j][e]);
+  };
+  // 32 bytes a lane of a row: whole (WHOLE) or up to K
+  auto frag = [&](auto& f, const uint8_t* row, int kb, auto whole) {
+    const int k = kb * 128 + g * 16;
+    if constexpr (decltype(whole)::value)
+      f.set(*reinterpret_cast<const u32x4_a1*>(row + k), *reinterpret_cast<const u32x4_a1*>(row + k + 64));
+    else
+      f.set(load_chunk(row, k, p.K), load_chunk(row, k + 64, p.K));
+  };
+  auto one = [&](int kb, auto whole) {
+    Frag<BF, true> b;
+    frag(b, pb, kb, whole);
+    float fb[BROW ? 4 : 1];
+#pragma unroll
+    for (int e = 0; e < (BROW ? 4 : 1); ++e) fb[e] = sb[e][kb * p.sb_c];
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+      Frag<AF, true> a;
+      frag(a, pa[j], kb, whole);
+      add(kb, b, a, j, fb, sa[j][kb * p.sa_c]);
+    }
+  };
+  const int kw = min(k1, p.K >> 7);  // whole blocks
+  int kb = k0;
+  for (; kb + U <= kw; kb += U) {
+    u32x4_t wb[U][2], wa[U][TM][2];
+    float fb[U][BROW ? 4 : 1], fa[U][TM];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = (kb + u) * 128 + g * 16;
+      wb[u][0] = *reinterpret_cast<const u32x4_a1*>(pb + k);
+      wb[u][1] = *reinterpret_cast<const u32x4_a1*>(pb + k + 64);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = (kb + u) * 128 + g * 16;
+#pragma unroll
+      for (int j = 0; j < TM; ++j) {
+        wa[u][j][0] = *reinterpret_cast<const u32x4_a1*>(pa[j] + k);
+        wa[u][j][1] = *reinterpret_cast<const u32x4_a1*>(pa[j] + k + 64);
+        fa[u][j] = sa[j][(kb + u) * p.sa_c];
+      }
+#pragma unroll
+      for (int e = 0; e < (BROW ? 4 : 1); ++e) fb[u][e] = sb[e][(kb + u) * p.sb_c];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      Frag<BF, true> b;
+      b.set(wb[u][0], wb[u][1]);
+#pragma unroll
+      for (int j = 0; j < TM; ++j) {
+        Frag<AF, true> a;
+        a.set(wa[u][j][0], wa[u][j][1]);
+        add(kb + u, b, a, j, fb[u], fa[u][j]);
+      }
+    }
+  }
+  for (; kb < kw; ++kb) one(kb, std::true_type{});
+  if (kb < k1) one(kb, std::false_type{});  // the last, partial block
+
+#pragma unroll
+  for (int j = 0; j < TM; ++j) part[wave][j][lane] = acc[j];
+  __syncthreads();
+  if (wave < TM) {  // wave j adds up and stores the j-th 16 rows
+    f32x4 v = part[0][wave][lane];
+#pragma unroll
+    for (int w = 1; w < KW; ++w) v = v + part[w][wave][lane];
+    const int m = wave * 16 + r, n = n0 + 4 * g, left = p.N - n;
+    if (p.bias) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < left) v[e] += p.bias[n + e];
+    }
+    if (m < p.M) store_out4(p.C, p.out, (int64_t)m * p.ldc + n, v, left);
+  }
+}
+
+// ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
 // Scales of a [rows, cols] operand: by rows or by blocks, any strides.
@@ -529,8 +662,9 @@ bool gemm_fp8_sup(const TensorDesc* in, int ni, const TensorDesc* out, int no, c
   return !any_overlap(in, ni, out, no);
 }
 
-// LDS: the kernel that loads straight into LDS.  EXACT: f32 outputs.
-template <bool LDS, bool EXACT, int BM, int BN, int WM, int WN, int AF, int BF>
+// S: stages of the kernel that loads straight into LDS; 0: the one of any
+// alignment.  EXACT: f32 outputs.
+template <int S, bool EXACT, int BM, int BN, int WM, int WN, int AF, int BF>
 Status run_tiles(Fp8Gemm& p, hipStream_t s) {
   p.tiles_m = (p.M + BM - 1) / BM;
   p.tiles_n = (p.N + BN - 1) / BN;
@@ -540,7 +674,7 @@ Status run_tiles(Fp8Gemm& p, hipStream_t s) {
   const unsigned g = (unsigned)tiles;
   auto go = [&](auto brow) {
     constexpr bool R = decltype(brow)::value;
-    if constexpr (LDS) gemm_fp8_lds_kernel<BM, BN, WM, WN, AF, BF, R, EXACT><<<g, T, 0, s>>>(p);
+    if constexpr (S > 0) gemm_fp8_lds_kernel<BM, BN, WM, WN, S, AF, BF, R, EXACT><<<g, T, 0, s>>>(p);
     else gemm_fp8_kernel<BM, BN, WM, WN, AF, BF, R, EXACT><<<g, T, 0, s>>>(p);
   };
   if (p.sb_sh == 0) go(std::true_type{});
@@ -550,15 +684,34 @@ Status run_tiles(Fp8Gemm& p, hipStream_t s) {
 
 template <int AF, int BF>
 Status gemm_fp8_run(Fp8Gemm& p, hipStream_t s) {
-  // straight into LDS: 16-byte aligned rows, a tile's bytes within 32-bit offsets
-  const bool lds = aligned(p.A, 16) && aligned(p.B, 16) && p.lda % 16 == 0 && p.ldb % 16 == 0 &&
-                   p.lda < (1 << 22) && p.ldb < (1 << 22) && p.K >= 256;
-  if (p.out == EL_F32) {
-    if (!lds) return run_tiles<false, true, 128, 128, 2, 2, AF, BF>(p, s);
-    return run_tiles<true, true, 128, 128, 2, 2, AF, BF>(p, s);
+  if (p.M <= 32) {
+    const unsigned g = (unsigned)(((int64_t)p.N + 15) / 16);
+    auto go = [&](auto tm) {
+      constexpr int TM = decltype(tm)::value;
+      if (p.sb_sh == 0) gemm_fp8_rows_kernel<TM, 8, AF, BF, true><<<g, 512, 0, s>>>(p);
+      else gemm_fp8_rows_kernel<TM, 8, AF, BF, false><<<g, 512, 0, s>>>(p);
+    };
+    if ((int64_t)g * 512 > UINT32_MAX) return Status::InvalidArgument;
+    if (p.M <= 16) go(std::integral_constant<int, 1>{});
+    else go(std::integral_constant<int, 2>{});
+    return launch_status("gemm_fp8");
   }
-  if (!lds) return run_tiles<false, false, 128, 128, 2, 2, AF, BF>(p, s);
-  return run_tiles<true, false, 256, 256, 2, 4, AF, BF>(p, s);
+  // straight into LDS: 16-byte aligned rows, a tile's bytes and scales within
+  // 32-bit offsets, two blocks of K at least
+  const int64_t nkb = (p.K + 127) / 128, lim = 1 << 22;
+  const bool lds = aligned(p.A, 16) && aligned(p.B, 16) && p.lda % 16 == 0 && p.ldb % 16 == 0 && p.lda < lim &&
+                   p.ldb < lim && p.sa_r < (lim >> 2) && p.sb_r < (lim >> 2) && nkb * p.sa_c < (1 << 26) &&
+                   nkb * p.sb_c < (1 << 26) && p.K >= 256;
+  auto tiles = [&](int64_t b) { return ((p.M + b - 1) / b) * ((p.N + b - 1) / b); };
+  if (p.out == EL_F32) {
+    if (!lds) return run_tiles<0, true, 128, 128, 2, 2, AF, BF>(p, s);
+    if (tiles(128) < 256) return run_tiles<4, true, 64, 64, 2, 2, AF, BF>(p, s);
+    return run_tiles<2, true, 128, 128, 2, 2, AF, BF>(p, s);
+  }
+  if (!lds) return run_tiles<0, false, 128, 128, 2, 2, AF, BF>(p, s);
+  if (tiles(128) < 256) return run_tiles<4, false, 64, 64, 2, 2, AF, BF>(p, s);
+  if (tiles(256) < 256) return run_tiles<2, false, 128, 128, 2, 2, AF, BF>(p, s);
+  return run_tiles<2, false, 256, 256, 2, 4, AF, BF>(p, s);
 }
 
 Status gemm_fp8_launch(const TensorDesc* in, int ni, TensorDesc* out, int no, const void* at, void*, size_t,

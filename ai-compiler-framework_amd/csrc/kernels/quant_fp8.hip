@@ -18,6 +18,8 @@
 // No counterpart in the reference.
 #include "../common/head_util.hpp"
 
+#include <type_traits>
+
 namespace aicf::hip {
 
 namespace {
@@ -100,116 +102,140 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs a) {
 
 // ---------------------------------------------------------------------------
 // A 128 x 128 tile a workgroup, in registers: thread (tr, tc) holds rows
-// 8 tr .. +7 and columns 8 tc .. +7.  The transposed codes go through LDS in
-// pieces of 8 (one column's 8 rows), piece tr of column c at tr ^ (c >> 3).
+// 8 tr .. +7 and columns 8 tc .. +7.  Row maxima are taken over the 16 lanes of
+// a row's threads, column maxima through LDS; then each thread makes one of the
+// 256 scales (two IEEE divisions: 8 + 8 of them in every thread were half of
+// this kernel's time).  The transposed codes go through LDS in pieces of 8 (one
+// column's 8 rows), piece tr of column c at tr ^ (c >> 3).
 // ---------------------------------------------------------------------------
-template <int EK, int F>
-__global__ __launch_bounds__(256) void quant_tile_kernel(QuantArgs a) {
-  __shared__ uint32_t cmax[4][kB];
+// max over the 16 lanes of a DPP row
+__device__ __forceinline__ uint32_t row16_max(uint32_t v) {
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, false));  // row_ror:8
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x122, 0xf, 0xf, false));
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xf, 0xf, false));
+}
+
+// EDGE: M or K has a last block that is not full.  ROWS: scales by rows (with a
+// transpose).  TRANS: with a transpose.
+template <int EK, int F, bool EDGE, bool ROWS, bool TRANS>
+__global__ __launch_bounds__(256, 3) void quant_tile_kernel(QuantArgs a) {
+  typedef uint32_t u32x4v __attribute__((ext_vector_type(4)));
+  __shared__ __attribute__((aligned(16))) uint32_t cmax[16][kB];  // [tr][column]
+  __shared__ __attribute__((aligned(16))) uint32_t rmax[kB];
+  __shared__ __attribute__((aligned(16))) float inv_c[kB], inv_r[kB];
   __shared__ __attribute__((aligned(16))) uint8_t tile[kB * kB];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int tr = t >> 4, tc = t & 15;
-  const int64_t tiles_k = (a.K + kB - 1) / kB, tiles = tiles_k * ((a.M + kB - 1) / kB);
-  for (int64_t id = blockIdx.x; id < tiles; id += gridDim.x) {
-    const int64_t tm = id / tiles_k, tk = id % tiles_k;
-    const int64_t r0 = tm * kB + tr * 8, c0 = tk * kB + tc * 8;
-    const int64_t nc = a.K - c0, nr = a.M - r0;
-    float v[8][8];
+  const uint32_t tiles_k = (uint32_t)((a.K + kB - 1) / kB);
+  const int64_t tm = blockIdx.x / tiles_k, tk = blockIdx.x % tiles_k;
+  const int64_t r0 = tm * kB + tr * 8, c0 = tk * kB + tc * 8;
+  const int64_t nc = a.K - c0, nr = a.M - r0;
+  const bool whole = !EDGE || (tm * kB + kB <= a.M && tk * kB + kB <= a.K);  // uniform
+  float v[8][8];
+  if (whole) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) load8<EK>(v[i], a.x, (r0 + i) * a.ldx + c0, i < nr ? nc : 0);
-
-    uint32_t rm[8], cm[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) rm[e] = cm[e] = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t b = abs_bits(v[i][j]);
-        rm[i] = max(rm[i], b);
-        cm[j] = max(cm[j], b);
-      }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      cm[j] = max(cm[j], (uint32_t)__shfl_xor((int)cm[j], 16, 64));
-      cm[j] = max(cm[j], (uint32_t)__shfl_xor((int)cm[j], 32, 64));
-    }
-    float inv_r[8], inv_c[8];
-    if (!a.by_rows) {
-      uint32_t b = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) b = max(b, cm[j]);
-#pragma unroll
-      for (int off = 8; off > 0; off >>= 1) b = max(b, (uint32_t)__shfl_xor((int)b, off, 64));
-      if (lane == 0) cmax[wave][0] = b;
-      __syncthreads();
-      b = max(max(cmax[0][0], cmax[1][0]), max(cmax[2][0], cmax[3][0]));
-      const float s = block_scale<F>(b, a.pow2), inv = 1.0f / s;
-      if (t == 0) {
-        a.s[tm * a.s_r + tk * a.s_c] = s;
-        if (a.qt) a.st[tk * a.st_r + tm * a.st_c] = s;
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) inv_r[e] = inv_c[e] = inv;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-#pragma unroll
-        for (int off = 8; off > 0; off >>= 1) rm[i] = max(rm[i], (uint32_t)__shfl_xor((int)rm[i], off, 64));
-        const float s = block_scale<F>(rm[i], a.pow2);
-        inv_r[i] = 1.0f / s;
-        if (tc == 0 && i < nr) a.s[(r0 + i) * a.s_r + tk * a.s_c] = s;
-      }
-      if (a.qt) {
-        if (lane < 16) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) cmax[wave][tc * 8 + j] = cm[j];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int c = tc * 8 + j;
-          const float s =
-              block_scale<F>(max(max(cmax[0][c], cmax[1][c]), max(cmax[2][c], cmax[3][c])), a.pow2);
-          inv_c[j] = 1.0f / s;
-          if (tr == 0 && j < nc) a.st[(c0 + j) * a.st_r + tm * a.st_c] = s;
-        }
-      }
-    }
+    for (int i = 0; i < 8; ++i) load8<EK>(v[i], a.x, (r0 + i) * a.ldx + c0, 8);
+  } else {  // past an edge: the last row or column again, and zeros in its place
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float r = inv_r[i];
-      const uint2 w{pack4<F>(v[i][0] * r, v[i][1] * r, v[i][2] * r, v[i][3] * r),
-                    pack4<F>(v[i][4] * r, v[i][5] * r, v[i][6] * r, v[i][7] * r)};
-      if (i < nr) store8(a.q + (r0 + i) * a.ldq + c0, w, nc);
-    }
-    if (a.qt) {
+      const int64_t at = (i < nr ? r0 + i : a.M - 1) * a.ldx;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float r = inv_c[j];
-        const uint2 w{pack4<F>(v[0][j] * r, v[1][j] * r, v[2][j] * r, v[3][j] * r),
-                      pack4<F>(v[4][j] * r, v[5][j] * r, v[6][j] * r, v[7][j] * r)};
-        *reinterpret_cast<uint2*>(tile + (tc * 8 + j) * kB + ((tr ^ tc) * 8)) = w;
+        const float x = elem_f32<EK>(a.x, at + (j < nc ? c0 + j : a.K - 1));
+        v[i][j] = i < nr && j < nc ? x : 0.0f;
       }
-      __syncthreads();
+      __builtin_amdgcn_sched_barrier(0);  // a row's addresses at a time
+    }
+  }
+
+  uint32_t rm[8], cm[8];
 #pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        const int c = p * 32 + (t >> 3), piece = (t & 7) * 2, f = c >> 3;
-        const uint2 lo = *reinterpret_cast<const uint2*>(tile + c * kB + ((piece ^ f) * 8));
-        const uint2 hi = *reinterpret_cast<const uint2*>(tile + c * kB + (((piece + 1) ^ f) * 8));
-        const int64_t k = tk * kB + c, m = tm * kB + piece * 8, n = a.M - m;
-        if (k < a.K) {
-          uint8_t* dst = a.qt + k * a.ldqt + m;
-          if (n >= 16) {
-            *reinterpret_cast<u32x4_a1*>(dst) = u32x4_a1{lo.x, lo.y, hi.x, hi.y};
-          } else {
-            store8(dst, lo, n);
-            store8(dst + 8, hi, n - 8);
-          }
+  for (int e = 0; e < 8; ++e) rm[e] = cm[e] = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t b = abs_bits(v[i][j]);
+      rm[i] = max(rm[i], b);
+      cm[j] = max(cm[j], b);
+    }
+  if constexpr (!ROWS) {
+    uint32_t b = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b = max(b, cm[j]);
+    b = row16_max(b);
+    b = max(b, (uint32_t)__shfl_xor((int)b, 16, 64));
+    b = max(b, (uint32_t)__shfl_xor((int)b, 32, 64));
+    if (lane == 0) rmax[wave] = b;
+    __syncthreads();
+    const float s = block_scale<F>(max(max(rmax[0], rmax[1]), max(rmax[2], rmax[3])), a.pow2);
+    if (t < kB) inv_r[t] = 1.0f / s;
+    else inv_c[t - kB] = 1.0f / s;
+    if (t == 0) {
+      a.s[tm * a.s_r + tk * a.s_c] = s;
+      if (TRANS) a.st[tk * a.st_r + tm * a.st_c] = s;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) rm[i] = row16_max(rm[i]);
+    if (tc == 0) {
+      *reinterpret_cast<u32x4v*>(&rmax[tr * 8]) = u32x4v{rm[0], rm[1], rm[2], rm[3]};
+      *reinterpret_cast<u32x4v*>(&rmax[tr * 8 + 4]) = u32x4v{rm[4], rm[5], rm[6], rm[7]};
+    }
+    if constexpr (TRANS) {
+      *reinterpret_cast<u32x4v*>(&cmax[tr][tc * 8]) = u32x4v{cm[0], cm[1], cm[2], cm[3]};
+      *reinterpret_cast<u32x4v*>(&cmax[tr][tc * 8 + 4]) = u32x4v{cm[4], cm[5], cm[6], cm[7]};
+    }
+    __syncthreads();
+    if (t < kB) {
+      const float s = block_scale<F>(rmax[t], a.pow2);
+      inv_r[t] = 1.0f / s;
+      if (tm * kB + t < a.M) a.s[(tm * kB + t) * a.s_r + tk * a.s_c] = s;
+    } else {
+      const int c = t - kB;
+      uint32_t b = 0;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) b = max(b, cmax[i][c]);
+      const float s = block_scale<F>(b, a.pow2);
+      inv_c[c] = 1.0f / s;
+      if (tk * kB + c < a.K) a.st[(tk * kB + c) * a.st_r + tm * a.st_c] = s;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float r = inv_r[tr * 8 + i];
+    const uint2 w{pack4<F>(v[i][0] * r, v[i][1] * r, v[i][2] * r, v[i][3] * r),
+                  pack4<F>(v[i][4] * r, v[i][5] * r, v[i][6] * r, v[i][7] * r)};
+    if (whole) store8(a.q + (r0 + i) * a.ldq + c0, w, 8);
+    else if (i < nr) store8(a.q + (r0 + i) * a.ldq + c0, w, nc);
+  }
+  if constexpr (TRANS) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float r = inv_c[tc * 8 + j];
+      const uint2 w{pack4<F>(v[0][j] * r, v[1][j] * r, v[2][j] * r, v[3][j] * r),
+                    pack4<F>(v[4][j] * r, v[5][j] * r, v[6][j] * r, v[7][j] * r)};
+      *reinterpret_cast<uint2*>(tile + (tc * 8 + j) * kB + ((tr ^ tc) * 8)) = w;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const int c = p * 32 + (t >> 3), piece = (t & 7) * 2, f = c >> 3;
+      const uint2 lo = *reinterpret_cast<const uint2*>(tile + c * kB + ((piece ^ f) * 8));
+      const uint2 hi = *reinterpret_cast<const uint2*>(tile + c * kB + (((piece + 1) ^ f) * 8));
+      const int64_t k = tk * kB + c, m = tm * kB + piece * 8, n = a.M - m;
+      if (k < a.K) {
+        uint8_t* dst = a.qt + k * a.ldqt + m;
+        if (n >= 16) {
+          *reinterpret_cast<u32x4_a1*>(dst) = u32x4_a1{lo.x, lo.y, hi.x, hi.y};
+        } else {
+          store8(dst, lo, n);
+          store8(dst + 8, hi, n - 8);
         }
       }
     }
-    __syncthreads();  // cmax and the tile are free for the next tile
   }
 }
 
@@ -237,7 +263,7 @@ bool quant_sup(const TensorDesc* in, int ni, const TensorDesc* out, int no, cons
   int64_t ld, r, c;
   if (!elem_kind(in[0], &ek) || !matrix_ld(in[0], false, &ld)) return false;
   const int64_t M = in[0].shape[0], K = in[0].shape[1];
-  if (K < 1) return false;
+  if (K < 1 || blocks_of(M) * blocks_of(K) >= 1 << 24) return false;  // a grid's lanes are counted in 32 bits
   bool may_rows = true, may_blocks = true;
   for (int k = 0; k < no; k += 2) {
     const int64_t R = k ? K : M, C = k ? M : K;
@@ -256,7 +282,15 @@ Status quant_run(const QuantArgs& a, hipStream_t s) {
     const int64_t waves = a.M * ((a.K + 511) / 512);
     quant_rows_kernel<EK, F><<<grid_1d(waves, 4, 1 << 20), 256, 0, s>>>(a);
   } else {
-    quant_tile_kernel<EK, F><<<grid_1d(blocks_of(a.M) * blocks_of(a.K), 1, 1 << 20), 256, 0, s>>>(a);
+    const unsigned g = (unsigned)(blocks_of(a.M) * blocks_of(a.K));
+    auto go = [&](auto rows, auto trans) {
+      constexpr bool R = decltype(rows)::value, T = decltype(trans)::value;
+      if (a.M % kB || a.K % kB) quant_tile_kernel<EK, F, true, R, T><<<g, 256, 0, s>>>(a);
+      else quant_tile_kernel<EK, F, false, R, T><<<g, 256, 0, s>>>(a);
+    };
+    if (a.by_rows) go(std::true_type{}, std::true_type{});
+    else if (a.qt) go(std::false_type{}, std::true_type{});
+    else go(std::false_type{}, std::false_type{});
   }
   return launch_status("quant_fp8");
 }

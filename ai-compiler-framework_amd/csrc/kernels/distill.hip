@@ -15,6 +15,8 @@
 // No counterpart in the reference.
 #include "../common/head_util.hpp"
 
+#include <type_traits>
+
 namespace aicf::hip {
 
 namespace {
@@ -34,64 +36,38 @@ struct DistillArgs {
   float tau, alpha, w0;  // w0: the weight of every row where w is absent
 };
 
-constexpr float kLog2e = 1.4426950408889634f;
+typedef int i32x4_d __attribute__((ext_vector_type(4)));
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// Maximum of a row segment, and the sums of exp((z - m) / tau) and exp(z - m).
-struct Soft {
-  float m, s, s1;
-};
 __device__ __forceinline__ float safe_ref(float m) { return m == -INFINITY ? 0.0f : m; }
-template <bool DUAL>
-__device__ __forceinline__ void soft_merge(Soft& a, const Soft& b, float c) {
-  const float M = fmaxf(a.m, b.m), ref = safe_ref(M);
-  a.s = a.s * __builtin_amdgcn_exp2f((a.m - ref) * c) + b.s * __builtin_amdgcn_exp2f((b.m - ref) * c);
-  if constexpr (DUAL)
-    a.s1 = a.s1 * __builtin_amdgcn_exp2f((a.m - ref) * kLog2e) + b.s1 * __builtin_amdgcn_exp2f((b.m - ref) * kLog2e);
-  a.m = M;
-}
-template <bool DUAL>
-__device__ __forceinline__ void soft_add8(Soft& a, const float (&v)[8], int n, float c) {
-  float m = a.m;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) m = e < n ? fmaxf(m, v[e]) : m;
-  const float ref = safe_ref(m);
-  float s = 0.0f, s1 = 0.0f;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float d = e < n ? v[e] - ref : -INFINITY;
-    s += __builtin_amdgcn_exp2f(d * c);
-    if constexpr (DUAL) s1 += __builtin_amdgcn_exp2f(d * kLog2e);
-  }
-  if (m != a.m) {
-    a.s *= __builtin_amdgcn_exp2f((a.m - ref) * c);
-    if constexpr (DUAL) a.s1 *= __builtin_amdgcn_exp2f((a.m - ref) * kLog2e);
-    a.m = m;
-  }
-  a.s += s;
-  if constexpr (DUAL) a.s1 += s1;
+// 2^(z c - mc).  mc = m c is rounded once for the whole row, so its error is a
+// common factor of every exponential and of their sum.
+__device__ __forceinline__ float exp_of(float z, float c, float mc) {
+  return __builtin_amdgcn_exp2f(fmaf(z, c, -mc));
 }
 
-template <int NT>
-__device__ __forceinline__ float block_max(float v, float* red) {
-  v = wave_max(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = red[0];
+// Up to three values over the workgroup at once, in a fixed order (lds: 4
+// floats a wave).  OP 0: maxima, 1: sums.
+template <int OP, int N>
+__device__ __forceinline__ void block_reduce(float (&v)[N], float* lds) {
+  const int nw = blockDim.x >> 6;
 #pragma unroll
-  for (int k = 1; k < NT / 64; ++k) v = fmaxf(v, red[k]);
-  return v;
-}
-template <int NT>
-__device__ __forceinline__ float block_sum(float v, float* red) {
-  v = wave_sum(v);
+  for (int i = 0; i < N; ++i) v[i] = OP == 0 ? wave_max(v[i]) : wave_sum(v[i]);
+  if (nw == 1) {
+    __syncthreads();  // (what the callers left in LDS)
+    return;
+  }
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = red[0];
+  if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-  for (int k = 1; k < NT / 64; ++k) v += red[k];
-  return v;
+    for (int i = 0; i < N; ++i) lds[(threadIdx.x >> 6) * 4 + i] = v[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = lds[i];
+  for (int k = 1; k < nw; ++k)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = OP == 0 ? fmaxf(v[i], lds[k * 4 + i]) : v[i] + lds[k * 4 + i];
 }
 
 template <int EK>
@@ -133,115 +109,409 @@ __device__ __forceinline__ float elem_any(const void* p, int64_t i, int ek) {
   return ek == EL_F16 ? elem_f32<EL_F16>(p, i) : elem_f32<EL_BF16>(p, i);
 }
 
+// 8 logits as they are stored.
+template <int EK>
+struct Vec8 {
+  typedef uint16_t u16x8v __attribute__((ext_vector_type(8)));
+  static constexpr uint16_t NONE = EK == EL_F16 ? 0xfc00 : 0xff80;  // -inf
+  u16x8v h;
+  // elements i .. i + 7 of the columns at p
+  __device__ __forceinline__ void load(const uint8_t* p, int i) {
+    h = *reinterpret_cast<const u16x8_a2*>(p + (uint32_t)i * 2u);
+  }
+  __device__ __forceinline__ void load_first(const uint8_t* p, int n) {  // n < 8 of them
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = e < n ? reinterpret_cast<const uint16_t*>(p)[e] : NONE;
+  }
+  __device__ __forceinline__ void drop(int n) {  // the first n become -inf
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = e < n ? NONE : h[e];
+  }
+  // What a pass made of the values is not kept for the next one.
+  __device__ __forceinline__ void forget() { asm volatile("" : "+v"(h)); }
+  __device__ __forceinline__ float operator[](int e) const { return EK == EL_F16 ? f16_to_f32(h[e]) : bf16_to_f32(h[e]); }
+};
+template <>
+struct Vec8<EL_F32> {
+  f32x4 a, b;
+  __device__ __forceinline__ void load(const uint8_t* p, int i) {
+    a = *reinterpret_cast<const f32x4_a4*>(p + (uint32_t)i * 4u);
+    b = *reinterpret_cast<const f32x4_a4*>(p + (uint32_t)i * 4u + 16u);
+  }
+  __device__ __forceinline__ void load_first(const uint8_t* p, int n) {
+    const float* q = reinterpret_cast<const float*>(p);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      a[e] = e < n ? q[e] : -INFINITY;
+      b[e] = e + 4 < n ? q[e + 4] : -INFINITY;
+    }
+  }
+  __device__ __forceinline__ void drop(int n) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      a[e] = e < n ? -INFINITY : a[e];
+      b[e] = e + 4 < n ? -INFINITY : b[e];
+    }
+  }
+  __device__ __forceinline__ void forget() { asm volatile("" : "+v"(a), "+v"(b)); }
+  __device__ __forceinline__ float operator[](int e) const { return e < 4 ? a[e] : b[e - 4]; }
+};
+
+// A workgroup's columns of a row, n of them: in registers (VPT vectors of 8 a
+// thread; with WHOLE the first half of them lies inside), or (VPT 0) read again
+// in each pass.  A vector that would pass the end is moved back to end there;
+// its elements that an earlier vector holds become -inf, which adds nothing to a
+// maximum or a sum, and are not stored.
+template <int NT, int EK, int VPT, bool WHOLE>
+struct Part {
+  const uint8_t* z;  // the first column
+  int n;
+  Vec8<EK> v[VPT > 0 ? VPT : 1];
+  __device__ __forceinline__ int first(int k) const { return (k * NT + (int)threadIdx.x) * 8; }
+  __device__ __forceinline__ static bool inner(int k) { return WHOLE && k < VPT / 2; }
+  __device__ __forceinline__ bool beyond(int k) const { return !inner(k) && k > 0 && k * NT * 8 >= n; }  // uniform
+  __device__ __forceinline__ int col(int k) const { return inner(k) ? first(k) : n >= 8 ? min(first(k), n - 8) : 0; }
+  // the elements [lo, hi) of vector k are its own
+  __device__ __forceinline__ int lo(int k) const { return inner(k) ? 0 : min(first(k) - col(k), 8); }
+  __device__ __forceinline__ int hi() const { return n >= 8 ? 8 : (n > 0 ? n : 0); }
+  __device__ __forceinline__ void fetch(Vec8<EK>& x, int k) const {
+    if (inner(k) || n >= 8) {
+      x.load(z, col(k));
+      if (!inner(k) && (k + 1) * NT * 8 > n) x.drop(lo(k));  // (uniform)
+    } else {
+      x.load_first(z, first(k) == 0 ? n : 0);
+    }
+  }
+  __device__ __forceinline__ void open(const void* base, int64_t row, int c0, int c1) {
+    z = static_cast<const uint8_t*>(base) + (row + c0) * (EK == EL_F32 ? 4 : 2);
+    n = c1 - c0;
+    if constexpr (VPT > 0) {
+#pragma unroll
+      for (int k = 0; k < VPT; ++k)
+        if (!beyond(k)) fetch(v[k], k);
+    }
+  }
+  // f(vector, its column, lo)
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    if constexpr (VPT > 0) {
+#pragma unroll
+      for (int k = 0; k < VPT; ++k) {
+        if (!beyond(k)) f(v[k], col(k), lo(k));
+        __builtin_amdgcn_sched_barrier(0);  // a vector at a time: the row's registers leave little else
+      }
+    } else {
+      for (int k = 0; first(k) < n; ++k) {
+        Vec8<EK> x;
+        fetch(x, k);
+        f(x, col(k), lo(k));
+      }
+    }
+  }
+  // Between two passes over registers: the compiler would keep the first one's
+  // conversions and exponentials, several registers for each that holds the row.
+  __device__ __forceinline__ void forget() {
+    if constexpr (VPT > 0) {
+#pragma unroll
+      for (int k = 0; k < VPT; ++k) v[k].forget();
+    }
+  }
+  __device__ __forceinline__ float top() const {
+    float m = -INFINITY;
+    each([&](const Vec8<EK>& x, int, int) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m = fmaxf(m, x[e]);
+    });
+    return m;
+  }
+  // sums of exp((z - m) / tau) and, DUAL, of exp(z - m)
+  template <bool DUAL>
+  __device__ __forceinline__ void sums(float c, float mc, float mc1, float& s, float& s1) const {
+    s = s1 = 0.0f;
+    each([&](const Vec8<EK>& x, int, int) {
+      float p[2] = {0.0f, 0.0f}, p1[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        p[e & 1] += exp_of(x[e], c, mc);
+        if constexpr (DUAL) p1[e & 1] += exp_of(x[e], kLog2e, mc1);
+      }
+      s += p[0] + p[1];
+      if constexpr (DUAL) s1 += p1[0] + p1[1];
+    });
+  }
+};
+
+// A row's special classes in LDS: the teacher's, and the label at K (-1: none),
+// and -1 behind up to a multiple of 4.
+struct Special {
+  int* cls;
+  float* z;  // their logits
+  float* e;  // the teacher's logit / tau; then what the gradient has less there
+  int n;     // K + 1, rounded up
+};
+__device__ __forceinline__ Special special_lds(int K) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t dyn[];
+  const int n = (K + 4) & ~3;
+  return Special{reinterpret_cast<int*>(dyn), reinterpret_cast<float*>(dyn) + n, reinterpret_cast<float*>(dyn) + 2 * n,
+                 n};
+}
+inline unsigned special_bytes(int K) { return (unsigned)((K + 4) & ~3) * 12; }
+
+// Fills cls, z, e of a row; the thread's largest teacher logit / tau.
+template <int EK>
+__device__ __forceinline__ float gather_special(const DistillArgs& a, int tk, int64_t row, const Special& sp) {
+  float tm = -INFINITY;
+  const int V = (int)a.V;
+  for (int j = threadIdx.x; j < sp.n; j += blockDim.x) {
+    int id = -1;
+    if (j < a.K) id = a.ids[row * a.ldi + j];
+    else if (j == a.K && a.labels && a.alpha != 0.0f) id = a.labels[row];
+    const bool ok = id >= 0 && id < V;
+    sp.cls[j] = ok ? id : -1;
+    sp.z[j] = ok ? elem_f32<EK>(a.z, row * a.ldz + id) : 0.0f;
+    if (j < a.K) {
+      const float x = ok ? elem_any(a.t, row * a.ldt + j, tk) / a.tau : -INFINITY;
+      sp.e[j] = x;
+      tm = fmaxf(tm, x);
+    } else if (j > a.K) {
+      sp.e[j] = 0.0f;
+    }
+  }
+  return tm;
+}
+
+// Writes columns [c0, c1) of a row of dz: k2 exp((z - m) / tau) (+ k1 exp(z -
+// m)), and the special classes among them with w e less.
+template <int EK, bool DUAL, typename P>
+__device__ __forceinline__ void write_gradient(const DistillArgs& a, int64_t row, int c0, int c1,
+                                               const P& part, const Special& sp, float c2, float mc,
+                                               float mc1, float k2, float k1, float w) {
+  auto dense = [&](float z) {
+    float g = k2 * exp_of(z, c2, mc);
+    if constexpr (DUAL) g = fmaf(k1, exp_of(z, kLog2e, mc1), g);
+    return g;
+  };
+  const int hi = part.hi();
+  part.each([&](const Vec8<EK>& x, int c, int lo) {
+    float g[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) g[e] = dense(x[e]);
+    const int64_t at = row * a.lddz + c0 + c;
+    if (lo == 0 && hi == 8) {
+      put8<EK>(a.dz, at, g, 8);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e >= lo && e < hi) put_elem<EK>(a.dz, at + e, g[e]);
+    }
+  });
+  __syncthreads();  // the special classes' dense values are stored
+  for (int j = threadIdx.x; j <= a.K; j += blockDim.x) {
+    const int id = sp.cls[j];
+    if (id < c0 || id >= c1) continue;
+    // the same class again: the first of them writes the sum, in the entries' order
+    float e = 0.0f;
+    bool first = true;
+    for (int i = 0; i < sp.n; i += 4) {
+      const i32x4_d q = *reinterpret_cast<const i32x4_d*>(sp.cls + i);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (q[u] == id) {
+          e += sp.e[i + u];
+          first = first && i + u >= j;
+        }
+    }
+    if (first) put_elem<EK>(a.dz, row * a.lddz + id, dense(sp.z[j]) - w * e);
+  }
+}
+
+template <int EK>
+__device__ __forceinline__ void write_zeros(const DistillArgs& a, int64_t row, int c0, int c1) {
+  const float zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  for (int c = c0 + threadIdx.x * 8; c < c1; c += blockDim.x * 8) put8<EK>(a.dz, row * a.lddz + c, zero, c1 - c);
+}
+
 // One workgroup a row.
-template <int NT, int EK, bool DUAL>
-__global__ __launch_bounds__(NT) void distill_row_kernel(DistillArgs a, int tk) {
-  __shared__ int cls[kMaxK + 1];    // the row's special classes: the teacher's, the label (-1: none)
-  __shared__ float zs[kMaxK + 1];   // their logits
-  __shared__ float es[kMaxK + 1];   // what the gradient has less there: (1 - a) tau p, a
-  __shared__ float red[NT / 64];
-  __shared__ Soft part[NT / 64];
-  const int t = threadIdx.x;
+// Where the row takes at most 32 registers a thread, 8 waves fit a SIMD: a row's
+// chain of loads and reductions hides behind other rows'.
+template <int NT, int EK, int VPT, bool DUAL>
+__global__ __launch_bounds__(NT, VPT * (EK == EL_F32 ? 8 : 4) <= 32 ? 8 : 4) void distill_row_kernel(DistillArgs a, int tk) {
+  const Special sp = special_lds(a.K);
+  __shared__ float red[16 * 4];
+  const int t = threadIdx.x, V = (int)a.V;
   const int64_t row = blockIdx.x;
   const float w = a.w ? a.w[row] : a.w0;
-  const int V = (int)a.V;
   if (w == 0.0f) {  // left out: not read
-    if (a.dz) {
-      const float zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-      for (int c = t * 8; c < V; c += NT * 8) put8<EK>(a.dz, row * a.lddz + c, zero, V - c);
-    }
+    if (a.dz) write_zeros<EK>(a, row, 0, V);
     if (t == 0) a.row_loss[row] = 0.0f;
     return;
   }
   const float c2 = kLog2e / a.tau;
-  const int64_t zrow = row * a.ldz;
+  Part<NT, EK, VPT, true> part;
+  part.open(a.z, row * a.ldz, 0, V);
+  float mx[2] = {0.0f, gather_special<EK>(a, tk, row, sp)};
+  mx[0] = part.top();
+  part.forget();
+  block_reduce<0>(mx, red);
+  const float m = safe_ref(mx[0]), tm = safe_ref(mx[1]), mc = m * c2, mc1 = m * kLog2e;
+  float sm[3];
+  part.template sums<DUAL>(c2, mc, mc1, sm[0], sm[1]);
+  part.forget();
+  sm[2] = 0.0f;
+  for (int j = t; j < a.K; j += blockDim.x) sm[2] += __expf(sp.e[j] - tm);
+  block_reduce<1>(sm, red);
+  const bool none = mx[0] == -INFINITY;  // no class has any probability
+  const float S = none ? __builtin_nanf("") : sm[0], S1 = none ? S : DUAL ? sm[1] : sm[0], ts = sm[2];
 
-  // the special classes
-  float tm = -INFINITY;
-  for (int j = t; j < a.K; j += NT) {
-    const int id = a.ids[row * a.ldi + j];
-    const bool ok = id >= 0 && id < V;
-    cls[j] = ok ? id : -1;
-    zs[j] = ok ? elem_f32<EK>(a.z, zrow + id) : 0.0f;
-    const float x = ok ? elem_any(a.t, row * a.ldt + j, tk) / a.tau : -INFINITY;
-    es[j] = x;
-    tm = fmaxf(tm, x);
-  }
-  if (t == 0) {
-    const int lab = a.labels && a.alpha != 0.0f ? a.labels[row] : -1;
-    const bool ok = lab >= 0 && lab < V;
-    cls[a.K] = ok ? lab : -1;
-    zs[a.K] = ok ? elem_f32<EK>(a.z, zrow + lab) : 0.0f;
-  }
-  tm = safe_ref(block_max<NT>(tm, red));
-
-  // the row's statistics
-  Soft st{-INFINITY, 0.0f, 0.0f};
-  for (int c = t * 8; c < V; c += NT * 8) {
-    float v[8];
-    load8<EK>(v, a.z, zrow + c, V - c);
-    soft_add8<DUAL>(st, v, V - c, c2);
-  }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1)
-    soft_merge<DUAL>(st, Soft{__shfl_xor(st.m, off, 64), __shfl_xor(st.s, off, 64), __shfl_xor(st.s1, off, 64)}, c2);
-  if ((t & 63) == 0) part[t >> 6] = st;
-  float ts = 0.0f;
-  for (int j = t; j < a.K; j += NT) ts += __expf(es[j] - tm);
-  ts = block_sum<NT>(ts, red);  // (its barriers order `part` too)
-  st = part[0];
-#pragma unroll
-  for (int k = 1; k < NT / 64; ++k) soft_merge<DUAL>(st, part[k], c2);
-  if (!DUAL) st.s1 = st.s;  // tau = 1, or no labels' loss
-  if (st.m == -INFINITY) st.s = st.s1 = __builtin_nanf("");  // no class has any probability
-
-  const bool some = ts > 0.0f || ts != ts;
-  const bool has = cls[a.K] >= 0;
+  const bool some = !(ts <= 0.0f), has = sp.cls[a.K] >= 0;
   const float soft_w = some ? (1.0f - a.alpha) * a.tau : 0.0f, hard_w = has ? a.alpha : 0.0f;
-  const float lnS = logf(st.s), lnT = logf(ts), inv_t = some ? 1.0f / ts : 0.0f;
-  float l = 0.0f;
-  for (int j = t; j < a.K; j += NT) {
-    const float x = es[j] - tm, p = cls[j] >= 0 ? __expf(x) * inv_t : 0.0f;
-    if (p != 0.0f) l += p * ((x - lnT) - ((zs[j] - st.m) / a.tau - lnS));
-    es[j] = soft_w * p;
+  const float lgS = log2f(S), lnT = logf(ts), inv_t = some ? 1.0f / ts : 0.0f;
+  float l[1] = {0.0f};
+  for (int j = t; j < a.K; j += blockDim.x) {
+    const float x = sp.e[j] - tm, p = sp.cls[j] >= 0 ? __expf(x) * inv_t : 0.0f;
+    if (p != 0.0f) l[0] += p * ((x - lnT) - (fmaf(sp.z[j], c2, -mc) - lgS) * kLn2);
+    sp.e[j] = soft_w * p;
   }
-  if (t == 0) es[a.K] = hard_w;
-  l = block_sum<NT>(l, red);
+  if (t == 0) sp.e[a.K] = hard_w;
+  block_reduce<1>(l, red);
   if (t == 0) {
-    float rl = (1.0f - a.alpha) * a.tau * a.tau * l;
-    if (has) rl -= a.alpha * ((zs[a.K] - st.m) - logf(st.s1));
+    float rl = (1.0f - a.alpha) * a.tau * a.tau * l[0];
+    if (has) rl -= a.alpha * ((fmaf(sp.z[a.K], kLog2e, -mc1) - log2f(S1)) * kLn2);
     a.row_loss[row] = rl;
   }
   if (!a.dz) return;
+  const float k1 = w * hard_w / S1, k2 = w * soft_w / S + (DUAL ? 0.0f : k1);
+  write_gradient<EK, DUAL>(a, row, 0, V, part, sp, c2, mc, mc1, k2, k1, w);
+}
 
-  // the dense part
-  const float k1 = w * hard_w / st.s1, k2 = w * soft_w / st.s + (DUAL ? 0.0f : k1);
-  auto dense = [&](float z) {
-    const float d = z - st.m;
-    float g = k2 * __builtin_amdgcn_exp2f(d * c2);
-    if constexpr (DUAL) g = fmaf(k1, __builtin_amdgcn_exp2f(d * kLog2e), g);
-    return g;
-  };
-  for (int c = t * 8; c < V; c += NT * 8) {
-    float v[8];
-    load8<EK>(v, a.z, zrow + c, V - c);
+// Few rows: P workgroups a row, in two launches.  Each leaves its columns'
+// maximum and sums in scratch [R, P, 4]; the first also what the loss takes
+// from the teacher and the label (the second launch may write over the logits)
+// in the fourth floats: sum p (log p - (z - z0) / tau) in f64, the label's logit,
+// and z0, a class's logit, so that nothing large cancels.
+constexpr int kPartNT = 256;
+__device__ __forceinline__ void part_columns(int V, int P, int* c0, int* c1) {
+  const int len = ((V + P - 1) / P + 7) & ~7;
+  *c0 = min((int)blockIdx.x * len, V);
+  *c1 = min(*c0 + len, V);
+}
+
+template <int EK, int VPT, bool DUAL>
+__global__ __launch_bounds__(kPartNT) void distill_stats_kernel(DistillArgs a, int tk, float* scratch, int P, int ldp) {
+  const Special sp = special_lds(a.K);
+  __shared__ float red[kPartNT / 64 * 4];
+  __shared__ double red64[kPartNT / 64];
+  __shared__ float z0s;
+  const int64_t row = blockIdx.y;
+  const float w = a.w ? a.w[row] : a.w0;
+  if (w == 0.0f) return;
+  int c0, c1;
+  part_columns((int)a.V, P, &c0, &c1);
+  const float c2 = kLog2e / a.tau;
+  Part<kPartNT, EK, VPT, false> part;
+  part.open(a.z, row * a.ldz, c0, c1);
+  float mx[1] = {part.top()};
+  block_reduce<0>(mx, red);
+  const float m = safe_ref(mx[0]);
+  float sm[2];
+  part.template sums<DUAL>(c2, m * c2, m * kLog2e, sm[0], sm[1]);
+  block_reduce<1>(sm, red);
+  float* out = scratch + (row * ldp + blockIdx.x) * 4;
+  if (threadIdx.x == 0) {
+    out[0] = mx[0];
+    out[1] = sm[0];
+    out[2] = sm[1];
+  }
+  if (blockIdx.x != 0) return;
+  float tm[1] = {gather_special<EK>(a, tk, row, sp)};
+  block_reduce<0>(tm, red);
+  tm[0] = safe_ref(tm[0]);
+  if (threadIdx.x == 0) {
+    int j = 0;
+    while (j < a.K && sp.cls[j] < 0) ++j;
+    const float z = j < a.K ? sp.z[j] : 0.0f;
+    z0s = fabsf(z) < INFINITY ? z : 0.0f;
+  }
+  float ts[1] = {0.0f};
+  for (int j = threadIdx.x; j < a.K; j += blockDim.x) ts[0] += __expf(sp.e[j] - tm[0]);
+  block_reduce<1>(ts, red);
+  const double c2e = (double)c2 * 0.6931471805599453;  // as the sums' exponentials have it
+  const float lnT = logf(ts[0]), inv_t = !(ts[0] <= 0.0f) ? 1.0f / ts[0] : 0.0f;
+  double l = 0.0;
+  for (int j = threadIdx.x; j < a.K; j += blockDim.x) {
+    const float x = sp.e[j] - tm[0], p = sp.cls[j] >= 0 ? __expf(x) * inv_t : 0.0f;
+    if (p != 0.0f) l += (double)p * ((double)(x - lnT) - ((double)sp.z[j] - (double)z0s) * c2e);
+  }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = dense(v[e]);
-    put8<EK>(a.dz, row * a.lddz + c, v, V - c);
+  for (int off = 32; off > 0; off >>= 1) l += __shfl_xor(l, off, 64);
+  if ((threadIdx.x & 63) == 0) red64[threadIdx.x >> 6] = l;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    l = (red64[0] + red64[1]) + (red64[2] + red64[3]);
+    const uint64_t bits = (uint64_t)__double_as_longlong(l);
+    out[3] = __uint_as_float((uint32_t)bits);
+    out[7] = __uint_as_float((uint32_t)(bits >> 32));
+    out[11] = sp.z[a.K];
+    out[15] = z0s;
   }
-  __syncthreads();  // the special classes' dense values are stored
-  for (int j = t; j <= a.K; j += NT) {
-    const int id = cls[j];
-    float e = 0.0f;
-    bool first = id >= 0;
-    for (int i = 0; i <= a.K; ++i) {
-      if (cls[i] == id) {
-        e += es[i];
-        first = first && i >= j;
-      }
-    }
-    if (first) put_elem<EK>(a.dz, row * a.lddz + id, dense(zs[j]) - w * e);
+}
+
+template <int EK, int VPT, bool DUAL>
+__global__ __launch_bounds__(kPartNT) void distill_grad_kernel(DistillArgs a, int tk, const float* scratch, int P,
+                                                               int ldp) {
+  const Special sp = special_lds(a.K);
+  __shared__ float red[kPartNT / 64 * 4];
+  const int64_t row = blockIdx.y;
+  const int t = threadIdx.x;
+  const float w = a.w ? a.w[row] : a.w0;
+  int c0, c1;
+  part_columns((int)a.V, P, &c0, &c1);
+  if (w == 0.0f) {
+    if (a.dz) write_zeros<EK>(a, row, c0, c1);
+    if (t == 0 && blockIdx.x == 0) a.row_loss[row] = 0.0f;
+    return;
   }
+  const float c2 = kLog2e / a.tau;
+  Part<kPartNT, EK, VPT, false> part;
+  if (a.dz) part.open(a.z, row * a.ldz, c0, c1);
+  // the row's statistics, and the special classes: those of other
+  // workgroups' columns only for their probabilities, as their logits may be written over by now
+  const float* in = scratch + row * ldp * 4;
+  f32x4 own = {-INFINITY, 0.0f, 0.0f, 0.0f};  // P <= 64: one a lane, the same in every wave
+  if ((t & 63) < P) own = *reinterpret_cast<const f32x4_a4*>(in + (t & 63) * 4);
+  const float mx = wave_max(own[0]), m = safe_ref(mx), mc = m * c2, mc1 = m * kLog2e, mq = safe_ref(own[0]);
+  float S = wave_sum(own[1] * __builtin_amdgcn_exp2f(mq * c2 - mc));
+  float S1 = DUAL ? wave_sum(own[2] * __builtin_amdgcn_exp2f(mq * kLog2e - mc1)) : S;
+  if (mx == -INFINITY) S = S1 = __builtin_nanf("");
+  float tm[1] = {gather_special<EK>(a, tk, row, sp)};
+  block_reduce<0>(tm, red);
+  tm[0] = safe_ref(tm[0]);
+  float ts[1] = {0.0f};
+  for (int j = t; j < a.K; j += blockDim.x) ts[0] += __expf(sp.e[j] - tm[0]);
+  block_reduce<1>(ts, red);
+  const bool some = !(ts[0] <= 0.0f), has = sp.cls[a.K] >= 0;
+  const float soft_w = some ? (1.0f - a.alpha) * a.tau : 0.0f, hard_w = has ? a.alpha : 0.0f;
+  const float inv_t = some ? 1.0f / ts[0] : 0.0f;
+  float pr[1] = {0.0f};  // the sum of the probabilities: 1, or 0 without a teacher, or NaN
+  for (int j = t; j < a.K; j += blockDim.x) {
+    const float p = sp.cls[j] >= 0 ? __expf(sp.e[j] - tm[0]) * inv_t : 0.0f;
+    pr[0] += p;
+    sp.e[j] = soft_w * p;
+  }
+  if (t == 0) sp.e[a.K] = hard_w;
+  block_reduce<1>(pr, red);
+  if (t == 0 && blockIdx.x == 0) {
+    const double l = __longlong_as_double((long long)((uint64_t)__float_as_uint(in[3]) |
+                                                      (uint64_t)__float_as_uint(in[7]) << 32));
+    // sum p (log p - (z - z0) / tau) + sum p (log sum exp(z / tau) - z0 / tau)
+    const double lse = ((double)mc + (double)log2f(S) - (double)in[15] * (double)c2) * 0.6931471805599453;
+    float rl = some ? (1.0f - a.alpha) * a.tau * a.tau * (float)(l + (double)pr[0] * lse) : 0.0f;
+    if (has) rl -= a.alpha * ((fmaf(in[11], kLog2e, -mc1) - log2f(S1)) * kLn2);
+    a.row_loss[row] = rl;
+  }
+  if (!a.dz) return;
+  const float k1 = w * hard_w / S1, k2 = w * soft_w / S + (DUAL ? 0.0f : k1);
+  write_gradient<EK, DUAL>(a, row, c0, c1, part, sp, c2, mc, mc1, k2, k1, w);
 }
 
 // loss = sum of w_r row_loss_r, f64 in a fixed order (one workgroup).
@@ -333,24 +603,63 @@ bool distill_sup(const TensorDesc* in, int ni, const TensorDesc* out, int no, co
   return true;
 }
 
+// Row r of the tensors becomes the first.
+template <int EK>
+DistillArgs from_row(const DistillArgs& a, int tk, int64_t r, int64_t rows) {
+  const int64_t es = EK == EL_F32 ? 4 : 2, et = tk == EL_F32 ? 4 : 2;
+  DistillArgs p = a;
+  p.R = rows;
+  p.z = (const uint8_t*)a.z + r * a.ldz * es;
+  p.t = (const uint8_t*)a.t + r * a.ldt * et;
+  p.ids = a.ids + r * a.ldi;
+  if (a.labels) p.labels = a.labels + r;
+  if (a.w) p.w = a.w + r;
+  if (a.dz) p.dz = (uint8_t*)a.dz + r * a.lddz * es;
+  p.row_loss = a.row_loss + r;
+  return p;
+}
+
 template <int EK, bool DUAL>
-Status distill_rows(const DistillArgs& a, int tk, hipStream_t s) {
-  // a grid's lanes are counted in 32 bits
-  const int nt = a.V > 8192 ? 1024 : 256;
-  const int64_t step = (int64_t{1} << 31) / nt;
-  for (int64_t r = 0; r < a.R; r += step) {
-    DistillArgs p = a;
-    p.R = a.R - r < step ? a.R - r : step;
-    const int64_t es = EK == EL_F32 ? 4 : 2, et = tk == EL_F32 ? 4 : 2;
-    p.z = (const uint8_t*)a.z + r * a.ldz * es;
-    p.t = (const uint8_t*)a.t + r * a.ldt * et;
-    p.ids = a.ids + r * a.ldi;
-    if (a.labels) p.labels = a.labels + r;
-    if (a.w) p.w = a.w + r;
-    if (a.dz) p.dz = (uint8_t*)a.dz + r * a.lddz * es;
-    p.row_loss = a.row_loss + r;
-    if (nt == 1024) distill_row_kernel<1024, EK, DUAL><<<(unsigned)p.R, 1024, 0, s>>>(p, tk);
-    else distill_row_kernel<256, EK, DUAL><<<(unsigned)p.R, 256, 0, s>>>(p, tk);
+Status distill_rows(const DistillArgs& a, int tk, float* scratch, int ldp, hipStream_t s) {
+  // Few rows share the chip: parts of 2048 columns or more, about two
+  // workgroups a CU.
+  const unsigned lds = special_bytes(a.K);
+  int64_t P = (512 + a.R - 1) / a.R;
+  if (P > a.V / 2048) P = a.V / 2048;
+  if (P > ldp) P = ldp;
+  if (P > 64) P = 64;
+  if (scratch && a.R < 256 && P >= 4) {
+    const dim3 grid((unsigned)P, (unsigned)a.R);
+    const int64_t len = (a.V + P - 1) / P + 7;
+    auto go = [&](auto vpt) {
+      constexpr int VPT = decltype(vpt)::value;
+      distill_stats_kernel<EK, VPT, DUAL><<<grid, kPartNT, lds, s>>>(a, tk, scratch, (int)P, ldp);
+      distill_grad_kernel<EK, VPT, DUAL><<<grid, kPartNT, lds, s>>>(a, tk, scratch, (int)P, ldp);
+    };
+    if (len <= kPartNT * 8 * 2) go(std::integral_constant<int, 2>{});
+    else go(std::integral_constant<int, 0>{});
+    return launch_status("distill_topk");
+  }
+  // The row in the registers of the fewest threads that hold it: up to 64
+  // columns a thread in 16 bits and 56 in f32 (128 in 16 bits for the longest);
+  // beyond 2^17 or 57344 columns it is read in each pass.
+  const int64_t kStep = 1 << 21;  // rows a launch: a grid's lanes are counted in 32 bits
+  for (int64_t r = 0; r < a.R; r += kStep) {
+    const DistillArgs p = from_row<EK>(a, tk, r, a.R - r < kStep ? a.R - r : kStep);
+    const unsigned g = (unsigned)p.R;
+    constexpr int L = EK == EL_F32 ? 7 : 8, XL = EK == EL_F32 ? 0 : 16;
+#define DISTILL_ROW(NT, VPT) distill_row_kernel<NT, EK, VPT, DUAL><<<g, NT, lds, s>>>(p, tk)
+    if (a.V <= 512) DISTILL_ROW(64, 1);
+    else if (a.V <= 1024) DISTILL_ROW(64, 2);
+    else if (a.V <= 2048) DISTILL_ROW(64, 4);
+    else if (a.V <= 4096) DISTILL_ROW(128, 4);
+    else if (a.V <= 8192) DISTILL_ROW(256, 4);
+    else if (a.V <= 16384) DISTILL_ROW(512, 4);
+    else if (a.V <= 512 * 8 * L) DISTILL_ROW(512, L);
+    else if (a.V <= 1024 * 8 * L) DISTILL_ROW(1024, L);
+    else if (XL && a.V <= 131072) DISTILL_ROW(1024, XL);
+    else DISTILL_ROW(1024, 0);
+#undef DISTILL_ROW
     const Status st = launch_status("distill_topk");
     if (st != Status::Ok) return st;
   }
@@ -389,10 +698,15 @@ Status distill_launch(const TensorDesc* in, int ni, TensorDesc* out, int no, con
   elem_kind(*c.t, &tk);
   hipStream_t s = as_stream(stream);
   const bool dual = a.labels && a.alpha != 0.0f && a.tau != 1.0f;
+  float* sc = c.scratch ? (float*)c.scratch->data : nullptr;
+  const int ldp = c.scratch ? (int)c.scratch->shape[1] : 0;
   Status st;
-  if (ek == EL_F32) st = dual ? distill_rows<EL_F32, true>(a, tk, s) : distill_rows<EL_F32, false>(a, tk, s);
-  else if (ek == EL_F16) st = dual ? distill_rows<EL_F16, true>(a, tk, s) : distill_rows<EL_F16, false>(a, tk, s);
-  else st = dual ? distill_rows<EL_BF16, true>(a, tk, s) : distill_rows<EL_BF16, false>(a, tk, s);
+  if (ek == EL_F32)
+    st = dual ? distill_rows<EL_F32, true>(a, tk, sc, ldp, s) : distill_rows<EL_F32, false>(a, tk, sc, ldp, s);
+  else if (ek == EL_F16)
+    st = dual ? distill_rows<EL_F16, true>(a, tk, sc, ldp, s) : distill_rows<EL_F16, false>(a, tk, sc, ldp, s);
+  else
+    st = dual ? distill_rows<EL_BF16, true>(a, tk, sc, ldp, s) : distill_rows<EL_BF16, false>(a, tk, sc, ldp, s);
   if (st != Status::Ok) return st;
   distill_loss_kernel<<<1, 256, 0, s>>>(a.row_loss, a.w, a.w0, a.R, (float*)c.loss->data);
   return launch_status("distill_loss");

@@ -75,13 +75,27 @@ __device__ __forceinline__ void put_elem(void* p, int64_t i, float v) {
   if constexpr (EK == EL_F32) static_cast<float*>(p)[i] = v;
   else static_cast<uint16_t*>(p)[i] = EK == EL_F16 ? f32_to_f16(v) : f32_to_bf16(v);
 }
-template <int EK>
+// STREAM: loads and stores of a row with the nontemporal hint.  It pays where
+// rows start on 128-byte lines (4096 x 32000 bf16 132 -> 115 us, 16384 x 8000
+// 163 -> 130): nothing here is read again.  Elsewhere a line is shared by two
+// vectors and would be fetched twice (4096 x 50021 f32 362 -> 491 us).
+template <bool STREAM, typename V>
+__device__ __forceinline__ V vec_load(const V* p) {
+  if constexpr (STREAM) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+template <bool STREAM, typename V>
+__device__ __forceinline__ void vec_store(V* p, V v) {
+  if constexpr (STREAM) __builtin_nontemporal_store(v, p);
+  else *p = v;
+}
+template <int EK, bool STREAM = false>
 __device__ __forceinline__ void put8(void* p, int64_t i, const float (&v)[8], int n) {
   if (n >= 8) {
     if constexpr (EK == EL_F32) {
       float* q = static_cast<float*>(p) + i;
-      *reinterpret_cast<f32x4_a4*>(q) = f32x4_a4{v[0], v[1], v[2], v[3]};
-      *reinterpret_cast<f32x4_a4*>(q + 4) = f32x4_a4{v[4], v[5], v[6], v[7]};
+      vec_store<STREAM>(reinterpret_cast<f32x4_a4*>(q), f32x4_a4{v[0], v[1], v[2], v[3]});
+      vec_store<STREAM>(reinterpret_cast<f32x4_a4*>(q + 4), f32x4_a4{v[4], v[5], v[6], v[7]});
     } else {
       u16x8_a2 o;
 #pragma unroll
@@ -95,7 +109,7 @@ __device__ __forceinline__ void put8(void* p, int64_t i, const float (&v)[8], in
           o[e + 1] = f32_to_f16(v[e + 1]);
         }
       }
-      *reinterpret_cast<u16x8_a2*>(static_cast<uint16_t*>(p) + i) = o;
+      vec_store<STREAM>(reinterpret_cast<u16x8_a2*>(static_cast<uint16_t*>(p) + i), o);
     }
   } else {
 #pragma unroll
@@ -116,8 +130,9 @@ struct Vec8 {
   static constexpr uint16_t NONE = EK == EL_F16 ? 0xfc00 : 0xff80;  // -inf
   u16x8v h;
   // elements i .. i + 7 of the columns at p
+  template <bool STREAM>
   __device__ __forceinline__ void load(const uint8_t* p, int i) {
-    h = *reinterpret_cast<const u16x8_a2*>(p + (uint32_t)i * 2u);
+    h = vec_load<STREAM>(reinterpret_cast<const u16x8_a2*>(p + (uint32_t)i * 2u));
   }
   __device__ __forceinline__ void load_first(const uint8_t* p, int n) {  // n < 8 of them
 #pragma unroll
@@ -134,9 +149,10 @@ struct Vec8 {
 template <>
 struct Vec8<EL_F32> {
   f32x4 a, b;
+  template <bool STREAM>
   __device__ __forceinline__ void load(const uint8_t* p, int i) {
-    a = *reinterpret_cast<const f32x4_a4*>(p + (uint32_t)i * 4u);
-    b = *reinterpret_cast<const f32x4_a4*>(p + (uint32_t)i * 4u + 16u);
+    a = vec_load<STREAM>(reinterpret_cast<const f32x4_a4*>(p + (uint32_t)i * 4u));
+    b = vec_load<STREAM>(reinterpret_cast<const f32x4_a4*>(p + (uint32_t)i * 4u + 16u));
   }
   __device__ __forceinline__ void load_first(const uint8_t* p, int n) {
     const float* q = reinterpret_cast<const float*>(p);
@@ -162,8 +178,9 @@ struct Vec8<EL_F32> {
 // in each pass.  A vector that would pass the end is moved back to end there;
 // its elements that an earlier vector holds become -inf, which adds nothing to a
 // maximum or a sum, and are not stored.
-template <int NT, int EK, int VPT, bool WHOLE>
+template <int NT, int EK, int VPT, bool WHOLE, bool STREAM_>
 struct Part {
+  static constexpr bool STREAM = STREAM_;
   const uint8_t* z;  // the first column
   int n;
   Vec8<EK> v[VPT > 0 ? VPT : 1];
@@ -176,7 +193,7 @@ struct Part {
   __device__ __forceinline__ int hi() const { return n >= 8 ? 8 : (n > 0 ? n : 0); }
   __device__ __forceinline__ void fetch(Vec8<EK>& x, int k) const {
     if (inner(k) || n >= 8) {
-      x.load(z, col(k));
+      x.template load<STREAM>(z, col(k));
       if (!inner(k) && (k + 1) * NT * 8 > n) x.drop(lo(k));  // (uniform)
     } else {
       x.load_first(z, first(k) == 0 ? n : 0);
@@ -298,7 +315,7 @@ __device__ __forceinline__ void write_gradient(const DistillArgs& a, int64_t row
     for (int e = 0; e < 8; ++e) g[e] = dense(x[e]);
     const int64_t at = row * a.lddz + c0 + c;
     if (lo == 0 && hi == 8) {
-      put8<EK>(a.dz, at, g, 8);
+      put8<EK, P::STREAM>(a.dz, at, g, 8);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -325,16 +342,16 @@ __device__ __forceinline__ void write_gradient(const DistillArgs& a, int64_t row
   }
 }
 
-template <int EK>
+template <int EK, bool STREAM>
 __device__ __forceinline__ void write_zeros(const DistillArgs& a, int64_t row, int c0, int c1) {
   const float zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  for (int c = c0 + threadIdx.x * 8; c < c1; c += blockDim.x * 8) put8<EK>(a.dz, row * a.lddz + c, zero, c1 - c);
+  for (int c = c0 + threadIdx.x * 8; c < c1; c += blockDim.x * 8) put8<EK, STREAM>(a.dz, row * a.lddz + c, zero, c1 - c);
 }
 
 // One workgroup a row.
 // Where the row takes at most 32 registers a thread, 8 waves fit a SIMD: a row's
 // chain of loads and reductions hides behind other rows'.
-template <int NT, int EK, int VPT, bool DUAL>
+template <int NT, int EK, int VPT, bool DUAL, bool STREAM>
 __global__ __launch_bounds__(NT, VPT * (EK == EL_F32 ? 8 : 4) <= 32 ? 8 : 4) void distill_row_kernel(DistillArgs a, int tk) {
   const Special sp = special_lds(a.K);
   __shared__ float red[16 * 4];
@@ -342,12 +359,12 @@ __global__ __launch_bounds__(NT, VPT * (EK == EL_F32 ? 8 : 4) <= 32 ? 8 : 4) voi
   const int64_t row = blockIdx.x;
   const float w = a.w ? a.w[row] : a.w0;
   if (w == 0.0f) {  // left out: not read
-    if (a.dz) write_zeros<EK>(a, row, 0, V);
+    if (a.dz) write_zeros<EK, STREAM>(a, row, 0, V);
     if (t == 0) a.row_loss[row] = 0.0f;
     return;
   }
   const float c2 = kLog2e / a.tau;
-  Part<NT, EK, VPT, true> part;
+  Part<NT, EK, VPT, true, STREAM> part;
   part.open(a.z, row * a.ldz, 0, V);
   float mx[2] = {0.0f, gather_special<EK>(a, tk, row, sp)};
   mx[0] = part.top();
@@ -408,7 +425,7 @@ __global__ __launch_bounds__(kPartNT) void distill_stats_kernel(DistillArgs a, i
   int c0, c1;
   part_columns((int)a.V, P, &c0, &c1);
   const float c2 = kLog2e / a.tau;
-  Part<kPartNT, EK, VPT, false> part;
+  Part<kPartNT, EK, VPT, false, false> part;
   part.open(a.z, row * a.ldz, c0, c1);
   float mx[1] = {part.top()};
   block_reduce<0>(mx, red);
@@ -467,12 +484,12 @@ __global__ __launch_bounds__(kPartNT) void distill_grad_kernel(DistillArgs a, in
   int c0, c1;
   part_columns((int)a.V, P, &c0, &c1);
   if (w == 0.0f) {
-    if (a.dz) write_zeros<EK>(a, row, c0, c1);
+    if (a.dz) write_zeros<EK, false>(a, row, c0, c1);
     if (t == 0 && blockIdx.x == 0) a.row_loss[row] = 0.0f;
     return;
   }
   const float c2 = kLog2e / a.tau;
-  Part<kPartNT, EK, VPT, false> part;
+  Part<kPartNT, EK, VPT, false, false> part;
   if (a.dz) part.open(a.z, row * a.ldz, c0, c1);
   // the row's statistics, and the special classes: those of other
   // workgroups' columns only for their probabilities, as their logits may be written over by now
@@ -643,12 +660,18 @@ Status distill_rows(const DistillArgs& a, int tk, float* scratch, int ldp, hipSt
   // The row in the registers of the fewest threads that hold it: up to 64
   // columns a thread in 16 bits and 56 in f32 (128 in 16 bits for the longest);
   // beyond 2^17 or 57344 columns it is read in each pass.
+  const int64_t es = EK == EL_F32 ? 4 : 2;
+  const bool stream = aligned(a.z, 128) && a.ldz * es % 128 == 0 && aligned(a.dz, 128) && a.lddz * es % 128 == 0;
   const int64_t kStep = 1 << 21;  // rows a launch: a grid's lanes are counted in 32 bits
   for (int64_t r = 0; r < a.R; r += kStep) {
     const DistillArgs p = from_row<EK>(a, tk, r, a.R - r < kStep ? a.R - r : kStep);
     const unsigned g = (unsigned)p.R;
     constexpr int L = EK == EL_F32 ? 7 : 8, XL = EK == EL_F32 ? 0 : 16;
-#define DISTILL_ROW(NT, VPT) distill_row_kernel<NT, EK, VPT, DUAL><<<g, NT, lds, s>>>(p, tk)
+#define DISTILL_ROW(NT, VPT)                                                                  \
+  do {                                                                                        \
+    if (stream) distill_row_kernel<NT, EK, VPT, DUAL, true><<<g, NT, lds, s>>>(p, tk);        \
+    else distill_row_kernel<NT, EK, VPT, DUAL, false><<<g, NT, lds, s>>>(p, tk);              \
+  } while (0)
     if (a.V <= 512) DISTILL_ROW(64, 1);
     else if (a.V <= 1024) DISTILL_ROW(64, 2);
     else if (a.V <= 2048) DISTILL_ROW(64, 4);
@@ -658,7 +681,7 @@ Status distill_rows(const DistillArgs& a, int tk, float* scratch, int ldp, hipSt
     else if (a.V <= 512 * 8 * L) DISTILL_ROW(512, L);
     else if (a.V <= 1024 * 8 * L) DISTILL_ROW(1024, L);
     else if (XL && a.V <= 131072) DISTILL_ROW(1024, XL);
-    else DISTILL_ROW(1024, 0);
+    else distill_row_kernel<1024, EK, 0, DUAL, false><<<g, 1024, lds, s>>>(p, tk);
 #undef DISTILL_ROW
     const Status st = launch_status("distill_topk");
     if (st != Status::Ok) return st;

@@ -31,6 +31,7 @@ namespace aicf::hip {
 namespace {
 
 typedef unsigned long long u64;
+typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
 
 struct SampleArgs {
   const void* z;
@@ -48,25 +49,27 @@ struct SampleArgs {
 constexpr int kBins = 1536;  // of 1 + distance / T: 256 an octave, 6 octaves; the last takes all beyond
 constexpr int kList = 2048;  // members a limit is sorted out of
 
-// exp(-y) 2^S for y >= 0, to the nearest integer: 2^t = 2^n 2^f with |f| <=
-// 1/2, the series of 2^f to f^11 (1e-14 relative).
-__device__ __forceinline__ u64 weight_of(double y, int S) {
-  y = fmin(y, 800.0);
-  const double t = -y * 1.4426950408889634, n = rint(t), f = (t - n) * 0.6931471805599453;
-  double p = 1.0 / 39916800.0;
-  p = fma(p, f, 1.0 / 3628800.0);
-  p = fma(p, f, 1.0 / 362880.0);
-  p = fma(p, f, 1.0 / 40320.0);
-  p = fma(p, f, 1.0 / 5040.0);
-  p = fma(p, f, 1.0 / 720.0);
-  p = fma(p, f, 1.0 / 120.0);
-  p = fma(p, f, 1.0 / 24.0);
-  p = fma(p, f, 1.0 / 6.0);
-  p = fma(p, f, 0.5);
-  p = fma(p, f, 1.0);
+// 2^(S - t) for t >= 0, to the nearest integer: 2^n 2^f with |f| <= 1/2, the
+// series of 2^f to f^10 (at most 2.2e-13 off, relative).
+__device__ __forceinline__ u64 weight_of(double t, int S) {
+  t = fmin(t, 1100.0);
+  const double n = rint(t), f = n - t;
+  constexpr double L = 0.6931471805599453;
+  constexpr double L2 = L * L, L3 = L2 * L, L4 = L3 * L, L5 = L4 * L, L6 = L5 * L, L7 = L6 * L, L8 = L7 * L,
+                   L9 = L8 * L, L10 = L9 * L;
+  double p = L10 / 3628800.0;
+  p = fma(p, f, L9 / 362880.0);
+  p = fma(p, f, L8 / 40320.0);
+  p = fma(p, f, L7 / 5040.0);
+  p = fma(p, f, L6 / 720.0);
+  p = fma(p, f, L5 / 120.0);
+  p = fma(p, f, L4 / 24.0);
+  p = fma(p, f, L3 / 6.0);
+  p = fma(p, f, L2 / 2.0);
+  p = fma(p, f, L);
   p = fma(p, f, 1.0);
   // adding 2^52 leaves the integer in the low bits
-  const double r = ldexp(p, (int)n + S) + 4503599627370496.0;
+  const double r = ldexp(p, S - (int)n) + 4503599627370496.0;
   return (u64)__double_as_longlong(r) - 0x4330000000000000ull;
 }
 
@@ -74,13 +77,9 @@ __device__ __forceinline__ uint32_t key_of(float z) {
   const uint32_t b = __float_as_uint(z);
   return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
-constexpr uint32_t kKeyNone = 0x007fffffu;  // the key of -inf
 __device__ __forceinline__ float z_of_key(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
-// A logit as the order sees it: NaN is -inf, -0 is 0.
-__device__ __forceinline__ float clean(float z) { return z == z ? z + 0.0f : -INFINITY; }
-
 __device__ __forceinline__ u64 shfl_xor64(u64 v, int off) { return (u64)__shfl_xor((long long)v, off, 64); }
 __device__ __forceinline__ u64 shfl_up64(u64 v, int off) { return (u64)__shfl_up((long long)v, off, 64); }
 __device__ __forceinline__ u64 wave_sum64(u64 v) {
@@ -98,10 +97,17 @@ __device__ __forceinline__ u64 wave_scan64(u64 v) {  // inclusive
   return v;
 }
 
+constexpr int kSegs = 1024;  // segments of a row whose kept sums are held
+
 template <int NT>
 struct SampleLds {
-  uint32_t cnt[kBins];
-  u64 mass[kBins];
+  union {
+    struct {
+      uint32_t cnt[kBins];
+      u64 mass[kBins];
+    };
+    u64 seg[kSegs];
+  };
   u64 list[kList];
   u64 wred[NT / 64 + 1], wred2[NT / 64 + 1];
   u64 b64[4];
@@ -117,33 +123,83 @@ struct SampleRow {
   const uint8_t* z;  // the row
   int nvec;          // vectors of 8 a thread
   float zmax;
-  double inv_t;
+  double c2;         // log2(e) / T
   float inv_tf;
+  // what is kept: logits above z_t, and at z_t the classes up to c_t
+  float z_t = -INFINITY;
+  int c_t = -1;
 
   // The thread's vector k: classes (k NT + t) 8 .. +7; past the row: -inf.
   __device__ __forceinline__ int first(int k) const { return (k * NT + (int)threadIdx.x) * 8; }
-  __device__ __forceinline__ void get(int k, float (&v)[8]) const {
+  struct Raw {
+    u32x4_t w[EK == EL_F32 ? 2 : 1];
+  };
+  __device__ __forceinline__ void fetch(Raw& x, int k) const {
+    constexpr int ES = EK == EL_F32 ? 4 : 2;
     const int c = first(k), n = a.V - c;
-    load8<EK>(v, z, c, n);
+    if (n >= 8) {
+      const uint8_t* p = z + (uint32_t)c * (uint32_t)ES;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = e < n ? clean(v[e]) : -INFINITY;
-  }
-  // f(z, class) for every element of the thread
-  template <typename F>
-  __device__ __forceinline__ void each(F f) const {
-    for (int k = 0; k < nvec; ++k) {
-      float v[8];
-      get(k, v);
+      for (int i = 0; i < (EK == EL_F32 ? 2 : 1); ++i) x.w[i] = *reinterpret_cast<const u32x4_a2*>(p + i * 16);
+    } else if constexpr (EK == EL_F32) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f(v[e], first(k) + e);
+      for (int e = 0; e < 8; ++e)
+        x.w[e >> 2][e & 3] = e < n ? reinterpret_cast<const uint32_t*>(z)[c + e] : 0xff800000u;
+    } else {
+      constexpr uint32_t NONE = EK == EL_F16 ? 0xfc00u : 0xff80u;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t lo = 2 * e < n ? reinterpret_cast<const uint16_t*>(z)[c + 2 * e] : NONE;
+        const uint32_t hi = 2 * e + 1 < n ? reinterpret_cast<const uint16_t*>(z)[c + 2 * e + 1] : NONE;
+        x.w[0][e] = lo | hi << 16;
+      }
     }
+  }
+  __device__ __forceinline__ static float at(const Raw& x, int e) {
+    if constexpr (EK == EL_F32) return __uint_as_float(x.w[e >> 2][e & 3]);
+    const uint16_t h = (uint16_t)(x.w[0][(e & 7) >> 1] >> (16 * (e & 1)));
+    return EK == EL_F16 ? f16_to_f32(h) : bf16_to_f32(h);
+  }
+  // f(k, v) for every vector of the thread, v as they are stored (the maximum
+  // and comparisons leave NaN out); the next vector is on its way meanwhile.
+  template <typename F>
+  __device__ __forceinline__ void each_vec(F f) const {
+    Raw x;
+    fetch(x, 0);
+#pragma unroll 1
+    for (int k = 0; k < nvec; ++k) {
+      Raw y = x;
+      if (k + 1 < nvec) fetch(y, k + 1);
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = at(x, e);
+      f(k, v);
+      x = y;
+    }
+  }
+  // f(v, class) for every element that may be drawn and is no worse than v0.
+  template <typename F>
+  __device__ __forceinline__ void each_from(float v0, F f) const {
+    each_vec([&](int k, const float (&v)[8]) {
+      float m = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m = fmaxf(m, v[e]);
+      if (!__any(m >= v0 && m > -INFINITY)) return;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+      {
+        if (v[e] >= v0 && v[e] > -INFINITY) f(v[e], first(k) + e);
+        __builtin_amdgcn_sched_barrier(0);  // one element's work at a time: 64-bit weights take many registers
+      }
+    });
   }
 
   __device__ __forceinline__ u64 weight(float v) const {
     if (v == zmax) return 1ull << a.shift;
-    return weight_of(((double)zmax - (double)v) * inv_t, a.shift);
+    return weight_of(((double)zmax - (double)v) * c2, a.shift);
   }
-  __device__ __forceinline__ static u64 comp(float v, int c) { return ((u64)(~key_of(v)) << 32) | (uint32_t)c; }
+  __device__ __forceinline__ static u64 comp(float v, int c) { return ((u64)(~key_of(v + 0.0f)) << 32) | (uint32_t)c; }
+  __device__ __forceinline__ bool kept(float v, int c) const { return v > z_t || (v == z_t && c <= c_t); }
   __device__ __forceinline__ int bin_of(float v) const {
     // rounding is monotone: a lower logit never has a lower bin
     const float y = v == zmax ? 1.0f : fmaf(zmax - v, inv_tf, 1.0f);
@@ -287,13 +343,13 @@ struct SampleRow {
     return s.bi[2];
   }
 
-  // Fills list with the composites of the elements f accepts.
+  // Fills list with the composites of the elements from v0 on that f accepts; how many those are.
   template <typename F>
-  __device__ __forceinline__ int compact(F f) {
+  __device__ __forceinline__ int compact(float v0, F f) {
     __syncthreads();
     if (threadIdx.x == 0) s.bi[3] = 0;
     __syncthreads();
-    each([&](float v, int c) {
+    each_from(v0, [&](float v, int c) {
       if (f(v, c)) {
         const int at = atomicAdd(&s.bi[3], 1);
         if (at < kList) s.list[at] = comp(v, c);
@@ -303,49 +359,62 @@ struct SampleRow {
     return s.bi[3];
   }
 
-  // Among the elements with composite <= limit: the composite of the target-th
-  // (by count), or of the last one before which the masses add up to less than
-  // target.  `cut` is the bin of bin_of that holds it.
-  __device__ u64 refine(u64 limit, bool by_mass, u64 target, Cut cut) {
-    // the bin's members span composites [lo, hi]
-    u64 lo = ~0ull, hi_inv = ~0ull;
-    const int b0 = cut.bin;
-    each([&](float v, int c) {
-      const u64 q = comp(v, c);
-      if (key_of(v) > kKeyNone && q <= limit && bin_of(v) == b0) {
-        lo = q < lo ? q : lo;
-        hi_inv = ~q < hi_inv ? ~q : hi_inv;
-      }
+  // Histogram of what is kept over bin_of.
+  __device__ __forceinline__ void histogram(bool by_mass) {
+    clear_hist(kBins);
+    each_from(z_t, [&](float v, int c) {
+      if (!kept(v, c)) return;
+      const int b = bin_of(v);
+      atomicAdd(&s.cnt[b], 1u);
+      if (by_mass) atomicAdd(&s.mass[b], weight(v));
     });
-    lo = block_min64(lo);
-    u64 hi = ~block_min64(hi_inv);
+  }
+
+  // Of what is kept, the target-th element (by count), or the last one before
+  // which the masses add up to less than target, becomes the last one kept;
+  // `cut` is the bin of bin_of that holds it.
+  __device__ __forceinline__ void refine(bool by_mass, u64 target, Cut cut) {
     u64 cnt_before = cut.cnt_before, mass_before = cut.mass_before;
-    u64 n = cut.n;
-    while (n > kList) {
-      // 1024 bins over [lo, hi]
-      int shift = 64 - __clzll((long long)(hi - lo)) - 10;
-      shift = shift < 0 ? 0 : shift;
-      clear_hist(1024);
-      each([&](float v, int c) {
+    int m;
+    if (cut.n <= kList) {
+      m = compact(z_t, [&](float v, int c) { return bin_of(v) == cut.bin && kept(v, c); });
+    } else {
+      // the bin's members span composites [lo, hi]: 1024 bins over those, until one holds little
+      u64 lo = ~0ull, hi_inv = ~0ull;
+      each_from(z_t, [&](float v, int c) {
         const u64 q = comp(v, c);
-        if (q >= lo && q <= hi) {
-          const int b = (int)((q - lo) >> shift);
-          atomicAdd(&s.cnt[b], 1u);
-          if (by_mass) atomicAdd(&s.mass[b], weight(v));
+        if (bin_of(v) == cut.bin && kept(v, c)) {
+          lo = q < lo ? q : lo;
+          hi_inv = ~q < hi_inv ? ~q : hi_inv;
         }
       });
-      const Cut k = find_bin(1024, by_mass, target - (by_mass ? mass_before : cnt_before));
-      cnt_before += k.cnt_before;
-      mass_before += k.mass_before;
-      n = k.n;
-      const u64 base = lo + ((u64)k.bin << shift), top = base + ((1ull << shift) - 1);
-      lo = base;
-      hi = top < hi ? top : hi;
+      lo = block_min64(lo);
+      u64 hi = ~block_min64(hi_inv), n = cut.n;
+      while (n > kList) {
+        int shift = 64 - __clzll((long long)(hi - lo)) - 10;
+        shift = shift < 0 ? 0 : shift;
+        clear_hist(1024);
+        each_from(z_t, [&](float v, int c) {
+          const u64 q = comp(v, c);
+          if (q >= lo && q <= hi) {
+            const int b = (int)((q - lo) >> shift);
+            atomicAdd(&s.cnt[b], 1u);
+            if (by_mass) atomicAdd(&s.mass[b], weight(v));
+          }
+        });
+        const Cut k = find_bin(1024, by_mass, target - (by_mass ? mass_before : cnt_before));
+        cnt_before += k.cnt_before;
+        mass_before += k.mass_before;
+        n = k.n;
+        const u64 base = lo + ((u64)k.bin << shift), top = base + ((1ull << shift) - 1);
+        lo = base;
+        hi = top < hi ? top : hi;
+      }
+      m = compact(z_t, [&](float v, int c) {
+        const u64 q = comp(v, c);
+        return q >= lo && q <= hi;
+      });
     }
-    const int m = compact([&](float v, int c) {
-      const u64 q = comp(v, c);
-      return q >= lo && q <= hi;
-    });
     sort_list(m);
     int at;
     if (by_mass) {
@@ -355,8 +424,9 @@ struct SampleRow {
       at = at < m ? at : m - 1;
     }
     const u64 q = s.list[at];
+    z_t = z_of_key(~(uint32_t)(q >> 32));
+    c_t = (int)(uint32_t)q;
     __syncthreads();
-    return q;
   }
 
   __device__ __forceinline__ void write(int token, float lp) const {
@@ -366,7 +436,7 @@ struct SampleRow {
     }
   }
   __device__ __forceinline__ float log_of(float v, u64 total) const {
-    const double d = v == zmax ? 0.0 : ((double)zmax - (double)v) * inv_t;
+    const double d = v == zmax ? 0.0 : ((double)zmax - (double)v) * c2 * 0.6931471805599453;
     return (float)(-d - log(ldexp((double)total, -a.shift)));
   }
   __device__ __forceinline__ u64 draw_at(u64 total) const {
@@ -376,7 +446,7 @@ struct SampleRow {
   }
 
   // The draw where everything kept is in list[0 .. m), sorted by composite.
-  __device__ void draw_small(int m) {
+  __device__ __forceinline__ void draw_small(int m) {
     // into the order of the classes, the key in the low half
     for (int i = threadIdx.x; i < m; i += NT) s.list[i] = (s.list[i] << 32) | (s.list[i] >> 32);
     sort_list(m);
@@ -408,80 +478,219 @@ struct SampleRow {
     }
   }
 
-  // The draw over the row: kept are composites <= limit with weight >= least.
-  __device__ void draw_row(u64 limit, u64 least) {
-    auto kept = [&](float v, int c) -> u64 {
-      if (key_of(v) <= kKeyNone || comp(v, c) > limit) return 0;
+  // The draw over the row, of what is kept with weight >= least.  The kept sums
+  // of segments of 512 classes (a vector of a wave; of as many vectors as leave
+  // at most kSegs segments) are held, so one segment is gone through again.
+  __device__ __forceinline__ void draw_row(u64 least) {
+    const int per = (nvec * NW + kSegs - 1) / kSegs;  // vectors a segment
+    auto own = [&](float v, int c) -> u64 {
+      if (!kept(v, c)) return 0;
       const u64 w = weight(v);
       return w >= least ? w : 0;
     };
-    u64 own = 0;
-    each([&](float v, int c) { own += kept(v, c); });
-    const u64 total = block_sum64(own), at = draw_at(total);
-    // segments of 512 classes (a vector of a wave) in the order of the classes
-    u64 before = 0;
-    for (int k = 0; k < nvec; ++k) {
-      float v[8];
-      get(k, v);
-      u64 w[8], sum = 0;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int nseg = (nvec + per - 1) / per * NW;
+    __syncthreads();
+    u64 sum = 0;
+    each_vec([&](int k, const float (&v)[8]) {
+      float m = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        w[e] = kept(v[e], first(k) + e);
-        sum += w[e];
+      for (int e = 0; e < 8; ++e) m = fmaxf(m, v[e]);
+      if (__any(m >= z_t)) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          sum += own(v[e], first(k) + e);
+          if (e & 1) __builtin_amdgcn_sched_barrier(0);
+        }
       }
-      const u64 incl = wave_scan64(sum);
+      // with per > 1 a segment's vectors lie NT 8 classes apart: all waves' share of `per` vectors is one
+      // stretch of classes, gone through in order below
+      if ((k + 1) % per == 0 || k + 1 == nvec) {
+        const u64 w = wave_sum64(sum);
+        if (lane == 0) s.seg[k / per * NW + wave] = w;
+        sum = 0;
+      }
+    });
+    __syncthreads();
+    // the stretch of classes (one vector of every wave where per is 1) that holds the target
+    u64 total = 0, before = 0, w = 0;
+    const int t = threadIdx.x;
+    constexpr int PER = kSegs / NT;
+    u64 mine[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      mine[i] = t * PER + i < nseg ? s.seg[t * PER + i] : 0;
+      w += mine[i];
+    }
+    u64 run = wave_scan64(w) - w;
+    if (lane == 63) s.wred[wave] = run + w;
+    if (t == 0) s.bi[0] = 0;
+    __syncthreads();
+    for (int k = 0; k < NW; ++k) {
+      if (k < wave) run += s.wred[k];
+      total += s.wred[k];
+    }
+    const u64 target = draw_at(total);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (run <= target && target < run + mine[i]) {
+        s.bi[0] = t * PER + i;
+        s.b64[0] = run;
+      }
+      run += mine[i];
+    }
+    __syncthreads();
+    const int seg = s.bi[0];
+    before = s.b64[0];
+    if (per == 1) {
+      if (wave != seg % NW) return;
+      Raw x;
+      fetch(x, seg / NW);
+      pick(x, seg / NW, before, target, total, own);
+      return;
+    }
+    // the sums before the segment's first vector: those of the stretch's earlier waves are interleaved with it
+    for (int q = seg / NW * NW; q < seg; ++q) before -= s.seg[q];
+    for (int k = seg / NW * per; k < (seg / NW + 1) * per && k < nvec; ++k) {
+      Raw x;
+      fetch(x, k);
+      u64 sum = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += own(at(x, e), first(k) + e);
+      sum = wave_sum64(sum);
       __syncthreads();
-      if ((threadIdx.x & 63) == 63) s.wred[threadIdx.x >> 6] = incl;
+      if (lane == 0) s.wred[wave] = sum;
       __syncthreads();
-      u64 run = before + incl - sum;
+      u64 at_wave = before;
       for (int q = 0; q < NW; ++q) {
-        if (q < (int)(threadIdx.x >> 6)) run += s.wred[q];
+        if (q < wave) at_wave += s.wred[q];
         before += s.wred[q];
       }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (run <= at && at < run + w[e]) {
-          a.token[blockIdx.x] = first(k) + e;
-          if (a.logprob) a.logprob[blockIdx.x] = log_of(v[e], total);
-        }
-        run += w[e];
-      }
-      if (before > at) return;
+      pick(x, k, at_wave, target, total, own);
+      if (before > target) return;
     }
   }
 
-  __device__ void run() {
+  // Writes the class of the wave's vector k at which the sum passes target, if
+  // it is there; `run` is the sum before the wave's first.
+  template <typename F>
+  __device__ __forceinline__ void pick(const Raw& x, int k, u64 run, u64 target, u64 total, F own) {
+    u64 w[8], sum = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      w[e] = own(at(x, e), first(k) + e);
+      sum += w[e];
+    }
+    run += wave_scan64(sum) - sum;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (run <= target && target < run + w[e]) {
+        a.token[blockIdx.x] = first(k) + e;
+        if (a.logprob) a.logprob[blockIdx.x] = log_of(at(x, e), total);
+      }
+      run += w[e];
+    }
+  }
+
+  // The sorted list[0 .. m) holds all that may be kept: its last cuts and the draw.
+  __device__ __forceinline__ void finish_list(int m, bool by_k, int top_k, bool by_p, float top_p, u64 least) {
+    if (by_k) m = top_k < m ? top_k : m;
+    if (by_p) {
+      constexpr int PER = kList / NT;
+      u64 own = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int j = threadIdx.x * PER + i;
+        if (j < m) own += weight(z_of_key(~(uint32_t)(s.list[j] >> 32)));
+      }
+      const u64 total = block_sum64(own);
+      __syncthreads();
+      m = last_below(m, 0, (u64)ceil((double)top_p * (double)total)) + 1;
+    }
+    cut_min_p(m, least);
+  }
+  __device__ __forceinline__ void cut_min_p(int m, u64 least) {
+    if (least) {  // the weights fall along the order
+      int n = 0;
+      for (int j = threadIdx.x; j < m; j += NT)
+        if (weight(z_of_key(~(uint32_t)(s.list[j] >> 32))) >= least) ++n;
+      m = (int)block_sum64((u64)n);
+    }
+    __syncthreads();
+    draw_small(m);
+  }
+
+  // A logit that at least n elements reach: the least, over the waves, of the
+  // ceil(n / NW)-th largest of their lanes' maxima.  n <= NT.
+  __device__ __forceinline__ float reached_by(int n, float lane_max) {
+    float v = lane_max;
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int k = 2; k <= 64; k <<= 1)
+#pragma unroll
+      for (int j = k >> 1; j > 0; j >>= 1) {  // falling over the lanes
+        const float o = __shfl_xor(v, j, 64);
+        const bool low = (lane & j) == 0, down = (lane & k) == 0;
+        v = low == down ? fmaxf(v, o) : fminf(v, o);
+      }
+    const float w = __shfl(v, (n + NW - 1) / NW - 1, 64);
+    __syncthreads();
+    float* red = reinterpret_cast<float*>(s.wred);
+    if (lane == 0) red[threadIdx.x >> 6] = w;
+    __syncthreads();
+    float t = red[0];
+#pragma unroll
+    for (int k = 1; k < NW; ++k) t = fminf(t, red[k]);
+    __syncthreads();
+    return t;
+  }
+
+  __device__ __forceinline__ void run() {
     const int row = blockIdx.x;
     const float T = a.temperature[row], top_p = a.top_p[row], min_p = a.min_p[row];
     const int top_k = a.top_k[row];
     nvec = (a.V + NT * 8 - 1) / (NT * 8);
-    u64 best = ~0ull;
-    each([&](float v, int c) {
-      const u64 q = comp(v, c);
-      best = q < best ? q : best;
+    float own_max = -INFINITY;
+    each_vec([&](int, const float (&v)[8]) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) own_max = fmaxf(own_max, v[e]);
     });
-    best = block_min64(best);
-    zmax = z_of_key(~(uint32_t)(best >> 32));
+    {
+      const float w = wave_max(own_max);
+      float* red = reinterpret_cast<float*>(s.wred);
+      if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = w;
+      __syncthreads();
+      zmax = red[0];
+#pragma unroll
+      for (int k = 1; k < NW; ++k) zmax = fmaxf(zmax, red[k]);
+      __syncthreads();
+    }
     if (zmax == -INFINITY) return write(-1, -INFINITY);
-    if (!(T > 0.0f) || top_k == 1 || top_p <= 0.0f) return write((int)(uint32_t)best, 0.0f);
-    inv_t = 1.0 / (double)T;
+    if (!(T > 0.0f) || top_k == 1 || top_p <= 0.0f) {
+      u64 best = ~0ull;
+      each_from(zmax, [&](float, int c) { best = (u64)c < best ? (u64)c : best; });
+      return write((int)block_min64(best), 0.0f);
+    }
+    const double inv_t = 1.0 / (double)T;
+    c2 = 1.4426950408889634 * inv_t;
     inv_tf = (float)inv_t;
     u64 least = 0;
     // w >= min_p: on the rounded weights, the least whole number that min_p admits
     if (min_p > 0.0f) least = (u64)ceil(ldexp((double)fminf(min_p, 1.0f), a.shift));
     const bool by_k = top_k > 0 && top_k < a.V, by_p = top_p < 1.0f;
-    u64 limit = ~0ull;
+    if (by_k && top_k <= NT) {
+      // the k largest are among what reaches a logit that k lanes' maxima reach
+      const float t = reached_by(top_k, own_max);
+      const int m = compact(t, [](float, int) { return true; });
+      if (m <= kList) {
+        sort_list(m);
+        return finish_list(m, true, top_k, by_p, top_p, least);
+      }
+    }
     for (int pass = 0; pass < 2; ++pass) {
       const bool by_mass = pass == 1;
       if (!(by_mass ? by_p : by_k)) continue;
-      clear_hist(kBins);
-      each([&](float v, int c) {
-        if (key_of(v) > kKeyNone && comp(v, c) <= limit) {
-          const int b = bin_of(v);
-          atomicAdd(&s.cnt[b], 1u);
-          if (by_mass) atomicAdd(&s.mass[b], weight(v));
-        }
-      });
+      histogram(by_mass);
       u64 target = (u64)top_k;
       if (by_mass) {
         u64 own = 0;
@@ -492,39 +701,15 @@ struct SampleRow {
       const Cut cut = find_bin(kBins, by_mass, target);
       if (cut.cnt_before + cut.n <= kList) {
         // little lies up to the cut: all of it, sorted
-        int m = compact([&](float v, int c) {
-          return key_of(v) > kKeyNone && comp(v, c) <= limit && bin_of(v) <= cut.bin;
-        });
+        int m = compact(z_t, [&](float v, int c) { return bin_of(v) <= cut.bin && kept(v, c); });
         sort_list(m);
-        if (!by_mass) {
-          m = top_k < m ? top_k : m;
-          if (by_p) {
-            constexpr int PER = kList / NT > 0 ? kList / NT : 1;
-            u64 own = 0;
-#pragma unroll
-            for (int i = 0; i < PER; ++i) {
-              const int j = threadIdx.x * PER + i;
-              if (j < m) own += weight(z_of_key(~(uint32_t)(s.list[j] >> 32)));
-            }
-            const u64 total = block_sum64(own);
-            __syncthreads();
-            m = last_below(m, 0, (u64)ceil((double)top_p * (double)total)) + 1;
-          }
-        } else {
-          m = last_below(m, 0, target) + 1;
-        }
-        if (least) {  // the weights fall along the order
-          int n = 0;
-          for (int j = threadIdx.x; j < m; j += NT)
-            if (weight(z_of_key(~(uint32_t)(s.list[j] >> 32))) >= least) ++n;
-          m = (int)block_sum64((u64)n);
-        }
-        __syncthreads();
-        return draw_small(m);
+        if (!by_mass) return finish_list(m, true, top_k, by_p, top_p, least);
+        m = last_below(m, 0, target) + 1;
+        return cut_min_p(m, least);
       }
-      limit = refine(limit, by_mass, target, cut);
+      refine(by_mass, target, cut);
     }
-    draw_row(limit, least);
+    draw_row(least);
   }
 };
 

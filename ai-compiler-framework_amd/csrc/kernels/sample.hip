@@ -50,27 +50,41 @@ constexpr int kBins = 1536;  // of 1 + distance / T: 256 an octave, 6 octaves; t
 constexpr int kList = 2048;  // members a limit is sorted out of
 
 // 2^(S - t) for t >= 0, to the nearest integer: 2^n 2^f with |f| <= 1/2, the
-// series of 2^f to f^10 (at most 2.2e-13 off, relative).
-__device__ __forceinline__ u64 weight_of(double t, int S) {
-  t = fmin(t, 1100.0);
-  const double n = rint(t), f = n - t;
-  constexpr double L = 0.6931471805599453;
-  constexpr double L2 = L * L, L3 = L2 * L, L4 = L3 * L, L5 = L4 * L, L6 = L5 * L, L7 = L6 * L, L8 = L7 * L,
-                   L9 = L8 * L, L10 = L9 * L;
-  double p = L10 / 3628800.0;
-  p = fma(p, f, L9 / 362880.0);
-  p = fma(p, f, L8 / 40320.0);
-  p = fma(p, f, L7 / 5040.0);
-  p = fma(p, f, L6 / 720.0);
-  p = fma(p, f, L5 / 120.0);
-  p = fma(p, f, L4 / 24.0);
-  p = fma(p, f, L3 / 6.0);
-  p = fma(p, f, L2 / 2.0);
-  p = fma(p, f, L);
-  p = fma(p, f, 1.0);
-  // adding 2^52 leaves the integer in the low bits
-  const double r = ldexp(p, S - (int)n) + 4503599627370496.0;
-  return (u64)__double_as_longlong(r) - 0x4330000000000000ull;
+// series of 2^f to f^10 (at most 2.2e-13 off, relative).  Adding 1.5 2^52 rounds
+// t to an integer in the sum's low bits, adding to the exponent field scales,
+// adding 2^52 leaves the rounded result in the low bits: conversions and ldexp
+// issue at a quarter of the rate of f64 additions.
+// The series' coefficients stay in scalar registers: as literals each would be
+// moved to a vector register for every term.
+struct Exp2Series {
+  double k[11];
+  __device__ __forceinline__ Exp2Series() {
+    constexpr double L = 0.6931471805599453;
+    double c = 1.0;
+#pragma unroll
+    for (int i = 0; i < 11; ++i) {
+      k[i] = c;
+      asm volatile("" : "+s"(k[i]));
+      c *= L / (i + 1);
+    }
+  }
+};
+__device__ __forceinline__ u64 weight_of(const Exp2Series& x, double t, int S) {
+  t = fmin(t, 900.0);
+  const double r = t + 6755399441055744.0;  // 1.5 2^52
+  const int n = (int)(uint32_t)__double_as_longlong(r);
+  const double f = (r - 6755399441055744.0) - t;
+  double p = x.k[10];
+#pragma unroll
+  for (int i = 9; i >= 0; --i) p = fma(p, f, x.k[i]);
+  p = __hiloint2double(__double2hiint(p) + ((S - n) << 20), __double2loint(p));  // stays normal: n <= 900
+  return (u64)__double_as_longlong(p + 4503599627370496.0) - 0x4330000000000000ull;
+}
+// f32 -> f64 by the bits; 0 and the subnormals become up to 2^-126, which
+// changes no difference of logits.
+__device__ __forceinline__ double wide(float z) {
+  const uint32_t u = __float_as_uint(z);
+  return __hiloint2double((int)(((u & 0x7fffffffu) >> 3) + (896u << 20) | (u & 0x80000000u)), (int)(u << 29));
 }
 
 __device__ __forceinline__ uint32_t key_of(float z) {
@@ -123,11 +137,17 @@ struct SampleRow {
   const uint8_t* z;  // the row
   int nvec;          // vectors of 8 a thread
   float zmax;
+  double zmax_w;
   double c2;         // log2(e) / T
   float inv_tf;
+  Exp2Series series;
   // what is kept: logits above z_t, and at z_t the classes up to c_t
   float z_t = -INFINITY;
   int c_t = -1;
+
+  __device__ __forceinline__ SampleRow(const SampleArgs& a_, SampleLds<NT>& s_) : a(a_), s(s_) {
+    z = static_cast<const uint8_t*>(a.z) + (int64_t)blockIdx.x * a.ldz * (EK == EL_F32 ? 4 : 2);
+  }
 
   // The thread's vector k: classes (k NT + t) 8 .. +7; past the row: -inf.
   __device__ __forceinline__ int first(int k) const { return (k * NT + (int)threadIdx.x) * 8; }
@@ -195,8 +215,8 @@ struct SampleRow {
   }
 
   __device__ __forceinline__ u64 weight(float v) const {
-    if (v == zmax) return 1ull << a.shift;
-    return weight_of(((double)zmax - (double)v) * c2, a.shift);
+    const u64 w = weight_of(series, (zmax_w - wide(v)) * c2, a.shift);
+    return v == zmax ? 1ull << a.shift : w;
   }
   __device__ __forceinline__ static u64 comp(float v, int c) { return ((u64)(~key_of(v + 0.0f)) << 32) | (uint32_t)c; }
   __device__ __forceinline__ bool kept(float v, int c) const { return v > z_t || (v == z_t && c <= c_t); }
@@ -362,11 +382,27 @@ struct SampleRow {
   // Histogram of what is kept over bin_of.
   __device__ __forceinline__ void histogram(bool by_mass) {
     clear_hist(kBins);
-    each_from(z_t, [&](float v, int c) {
-      if (!kept(v, c)) return;
-      const int b = bin_of(v);
-      atomicAdd(&s.cnt[b], 1u);
-      if (by_mass) atomicAdd(&s.mass[b], weight(v));
+    if (!by_mass) {
+      each_from(z_t, [&](float v, int c) {
+        if (kept(v, c)) atomicAdd(&s.cnt[bin_of(v)], 1u);
+      });
+      return;
+    }
+    each_vec([&](int k, const float (&v)[8]) {
+      float m = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m = fmaxf(m, v[e]);
+      if (!__any(m >= z_t && m > -INFINITY)) return;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const u64 w = weight(v[e]);
+        if (kept(v[e], first(k) + e)) {
+          const int b = bin_of(v[e]);
+          atomicAdd(&s.cnt[b], 1u);
+          atomicAdd(&s.mass[b], w);
+        }
+        if (e & 1) __builtin_amdgcn_sched_barrier(0);
+      }
     });
   }
 
@@ -484,9 +520,8 @@ struct SampleRow {
   __device__ __forceinline__ void draw_row(u64 least) {
     const int per = (nvec * NW + kSegs - 1) / kSegs;  // vectors a segment
     auto own = [&](float v, int c) -> u64 {
-      if (!kept(v, c)) return 0;
       const u64 w = weight(v);
-      return w >= least ? w : 0;
+      return kept(v, c) && w >= least ? w : 0;
     };
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int nseg = (nvec + per - 1) / per * NW;
@@ -592,6 +627,87 @@ struct SampleRow {
     }
   }
 
+  // LDS between the steps of one wave: its operations are in order, the
+  // compiler's are kept so.
+  __device__ __forceinline__ static void wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+  // Sorts list[0 .. n), n <= 256, in one wave.
+  __device__ __forceinline__ void wave_sort(int n) {
+    const int lane = threadIdx.x & 63;
+    int m = 64;
+    while (m < n) m <<= 1;
+    for (int i = n + lane; i < m; i += 64) s.list[i] = ~0ull;
+    for (int k = 2; k <= m; k <<= 1)
+      for (int j = k >> 1; j > 0; j >>= 1) {
+        wave_order();
+        for (int q = lane; q < m / 2; q += 64) {
+          const int i = (q & ~(j - 1)) * 2 + (q & (j - 1)), o = i + j;
+          const u64 x = s.list[i], y = s.list[o];
+          if ((x > y) == ((i & k) == 0)) {
+            s.list[i] = y;
+            s.list[o] = x;
+          }
+        }
+      }
+    wave_order();
+  }
+  // The same as finish_list for m <= 256 (not sorted yet), in the first wave
+  // alone: 4 entries a lane, no barrier of the workgroup.
+  __device__ __forceinline__ void finish_wave(int m, bool by_k, int top_k, bool by_p, float top_p, u64 mass_target,
+                                              u64 least) {
+    if (threadIdx.x >= 64) return;
+    const int lane = threadIdx.x;
+    wave_sort(m);
+    if (by_k && top_k < m) m = top_k;
+    u64 q[4], w[4], own = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      q[i] = lane * 4 + i < m ? s.list[lane * 4 + i] : ~0ull;
+      w[i] = lane * 4 + i < m ? weight(z_of_key(~(uint32_t)(q[i] >> 32))) : 0;
+      own += w[i];
+    }
+    const u64 incl = wave_scan64(own), total = (u64)__shfl((long long)incl, 63, 64);
+    u64 run = incl - own;
+    const u64 target = by_p ? (mass_target ? mass_target : (u64)ceil((double)top_p * (double)total)) : ~0ull;
+    int n = 0;  // kept of this lane: a prefix of the order
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool first = lane * 4 + i == 0;
+      if (lane * 4 + i < m && (first || (run < target && w[i] >= least))) ++n;
+      run += w[i];
+    }
+    m = n;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) m += __shfl_xor(m, off, 64);
+    // into the order of the classes, the key in the low half
+    wave_order();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) s.list[lane * 4 + i] = (q[i] << 32) | (q[i] >> 32);
+    wave_order();
+    wave_sort(m);
+    own = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      q[i] = lane * 4 + i < m ? s.list[lane * 4 + i] : 0;
+      w[i] = lane * 4 + i < m ? weight(z_of_key(~(uint32_t)q[i])) : 0;
+      own += w[i];
+    }
+    const u64 sum = wave_scan64(own), all = (u64)__shfl((long long)sum, 63, 64);
+    run = sum - own;
+    const u64 at = draw_at(all);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (run <= at && at < run + w[i]) {
+        a.token[blockIdx.x] = (int)(q[i] >> 32);
+        if (a.logprob) a.logprob[blockIdx.x] = log_of(z_of_key(~(uint32_t)q[i]), all);
+      }
+      run += w[i];
+    }
+  }
+
   // The sorted list[0 .. m) holds all that may be kept: its last cuts and the draw.
   __device__ __forceinline__ void finish_list(int m, bool by_k, int top_k, bool by_p, float top_p, u64 least) {
     if (by_k) m = top_k < m ? top_k : m;
@@ -673,6 +789,7 @@ struct SampleRow {
     }
     const double inv_t = 1.0 / (double)T;
     c2 = 1.4426950408889634 * inv_t;
+    zmax_w = fabsf(zmax) < INFINITY ? wide(zmax) : (double)zmax;
     inv_tf = (float)inv_t;
     u64 least = 0;
     // w >= min_p: on the rounded weights, the least whole number that min_p admits
@@ -682,6 +799,7 @@ struct SampleRow {
       // the k largest are among what reaches a logit that k lanes' maxima reach
       const float t = reached_by(top_k, own_max);
       const int m = compact(t, [](float, int) { return true; });
+      if (m <= 256) return finish_wave(m, true, top_k, by_p, top_p, 0, least);
       if (m <= kList) {
         sort_list(m);
         return finish_list(m, true, top_k, by_p, top_p, least);
@@ -702,6 +820,7 @@ struct SampleRow {
       if (cut.cnt_before + cut.n <= kList) {
         // little lies up to the cut: all of it, sorted
         int m = compact(z_t, [&](float v, int c) { return bin_of(v) <= cut.bin && kept(v, c); });
+        if (m <= 256) return finish_wave(m, !by_mass, top_k, by_p, top_p, by_mass ? target : 0, least);
         sort_list(m);
         if (!by_mass) return finish_list(m, true, top_k, by_p, top_p, least);
         m = last_below(m, 0, target) + 1;
@@ -716,8 +835,7 @@ struct SampleRow {
 template <int EK, int NT>
 __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
   __shared__ SampleLds<NT> lds;
-  SampleRow<EK, NT> row{a, lds,
-                             static_cast<const uint8_t*>(a.z) + (int64_t)blockIdx.x * a.ldz * (EK == EL_F32 ? 4 : 2)};
+  SampleRow<EK, NT> row(a, lds);
   row.run();
 }
 

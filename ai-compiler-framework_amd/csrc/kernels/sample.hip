@@ -123,7 +123,7 @@ struct SampleLds {
     u64 seg[kSegs];
   };
   u64 list[kList];
-  u64 wred[NT / 64 + 1], wred2[NT / 64 + 1];
+  u64 wred[NT / 64 + 1], wred2[NT / 64 + 1];  // (reached_by: two words a wave)
   u64 b64[4];
   int bi[4];
 };
@@ -134,7 +134,9 @@ struct SampleRow {
 
   const SampleArgs& a;
   SampleLds<NT>& s;
-  const uint8_t* z;  // the row
+  int row;
+  const uint8_t* z;  // the row's classes from `base` on, len of them
+  int base, len;
   int nvec;          // vectors of 8 a thread
   float zmax;
   double zmax_w;
@@ -145,18 +147,21 @@ struct SampleRow {
   float z_t = -INFINITY;
   int c_t = -1;
 
-  __device__ __forceinline__ SampleRow(const SampleArgs& a_, SampleLds<NT>& s_) : a(a_), s(s_) {
-    z = static_cast<const uint8_t*>(a.z) + (int64_t)blockIdx.x * a.ldz * (EK == EL_F32 ? 4 : 2);
+  __device__ __forceinline__ SampleRow(const SampleArgs& a_, SampleLds<NT>& s_, int row_, int c0, int c1)
+      : a(a_), s(s_), row(row_), base(c0), len(c1 - c0) {
+    z = static_cast<const uint8_t*>(a.z) + ((int64_t)row * a.ldz + c0) * (EK == EL_F32 ? 4 : 2);
+    nvec = (len + NT * 8 - 1) / (NT * 8);
   }
 
-  // The thread's vector k: classes (k NT + t) 8 .. +7; past the row: -inf.
+  // The thread's vector k: classes base + (k NT + t) 8 .. +7; past the end: -inf.
   __device__ __forceinline__ int first(int k) const { return (k * NT + (int)threadIdx.x) * 8; }
+  __device__ __forceinline__ int cls(int k) const { return base + first(k); }
   struct Raw {
     u32x4_t w[EK == EL_F32 ? 2 : 1];
   };
   __device__ __forceinline__ void fetch(Raw& x, int k) const {
     constexpr int ES = EK == EL_F32 ? 4 : 2;
-    const int c = first(k), n = a.V - c;
+    const int c = first(k), n = len - c;
     if (n >= 8) {
       const uint8_t* p = z + (uint32_t)c * (uint32_t)ES;
 #pragma unroll
@@ -208,7 +213,7 @@ struct SampleRow {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
       {
-        if (v[e] >= v0 && v[e] > -INFINITY) f(v[e], first(k) + e);
+        if (v[e] >= v0 && v[e] > -INFINITY) f(v[e], cls(k) + e);
         __builtin_amdgcn_sched_barrier(0);  // one element's work at a time: 64-bit weights take many registers
       }
     });
@@ -396,7 +401,7 @@ struct SampleRow {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const u64 w = weight(v[e]);
-        if (kept(v[e], first(k) + e)) {
+        if (kept(v[e], cls(k) + e)) {
           const int b = bin_of(v[e]);
           atomicAdd(&s.cnt[b], 1u);
           atomicAdd(&s.mass[b], w);
@@ -467,8 +472,8 @@ struct SampleRow {
 
   __device__ __forceinline__ void write(int token, float lp) const {
     if (threadIdx.x == 0) {
-      a.token[blockIdx.x] = token;
-      if (a.logprob) a.logprob[blockIdx.x] = lp;
+      a.token[row] = token;
+      if (a.logprob) a.logprob[row] = lp;
     }
   }
   __device__ __forceinline__ float log_of(float v, u64 total) const {
@@ -476,7 +481,7 @@ struct SampleRow {
     return (float)(-d - log(ldexp((double)total, -a.shift)));
   }
   __device__ __forceinline__ u64 draw_at(u64 total) const {
-    float u = a.u[blockIdx.x];
+    float u = a.u[row];
     u = u > 0.0f ? fminf(u, 0.99999994f) : 0.0f;
     return (u64)((double)u * (double)total);  // the sum has to pass this
   }
@@ -507,24 +512,22 @@ struct SampleRow {
     for (int i = 0; i < PER; ++i) {
       if (run <= at && at < run + w[i]) {
         const u64 q = s.list[threadIdx.x * PER + i];
-        a.token[blockIdx.x] = (int)(q >> 32);
-        if (a.logprob) a.logprob[blockIdx.x] = log_of(z_of_key(~(uint32_t)q), total);
+        a.token[row] = (int)(q >> 32);
+        if (a.logprob) a.logprob[row] = log_of(z_of_key(~(uint32_t)q), total);
       }
       run += w[i];
     }
   }
 
-  // The draw over the row, of what is kept with weight >= least.  The kept sums
-  // of segments of 512 classes (a vector of a wave; of as many vectors as leave
-  // at most kSegs segments) are held, so one segment is gone through again.
-  __device__ __forceinline__ void draw_row(u64 least) {
-    const int per = (nvec * NW + kSegs - 1) / kSegs;  // vectors a segment
-    auto own = [&](float v, int c) -> u64 {
-      const u64 w = weight(v);
-      return kept(v, c) && w >= least ? w : 0;
-    };
+  __device__ __forceinline__ u64 kept_weight(float v, int c, u64 least) const {
+    const u64 w = weight(v);
+    return kept(v, c) && w >= least ? w : 0;
+  }
+
+  // The sums of what is kept with weight >= least, by segments: the classes of
+  // `per` vectors of a wave, 512 each.  Segment (k / per) NW + wave.
+  __device__ __forceinline__ void segment_sums(u64 least, int per) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int nseg = (nvec + per - 1) / per * NW;
     __syncthreads();
     u64 sum = 0;
     each_vec([&](int k, const float (&v)[8]) {
@@ -534,12 +537,10 @@ struct SampleRow {
       if (__any(m >= z_t)) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          sum += own(v[e], first(k) + e);
+          sum += kept_weight(v[e], cls(k) + e, least);
           if (e & 1) __builtin_amdgcn_sched_barrier(0);
         }
       }
-      // with per > 1 a segment's vectors lie NT 8 classes apart: all waves' share of `per` vectors is one
-      // stretch of classes, gone through in order below
       if ((k + 1) % per == 0 || k + 1 == nvec) {
         const u64 w = wave_sum64(sum);
         if (lane == 0) s.seg[k / per * NW + wave] = w;
@@ -547,17 +548,22 @@ struct SampleRow {
       }
     });
     __syncthreads();
-    // the stretch of classes (one vector of every wave where per is 1) that holds the target
-    u64 total = 0, before = 0, w = 0;
-    const int t = threadIdx.x;
+  }
+
+  // The draw where seg[0 .. nseg) holds those sums of the whole row: the
+  // segment that the target falls into is gone through again.  With per > 1 the
+  // waves' vectors of a stretch of `per` alternate, so the stretch is.
+  __device__ __forceinline__ void draw_segments(u64 least, int per, int nseg) {
+    const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
+    auto own = [&](float v, int c) { return kept_weight(v, c, least); };
     constexpr int PER = kSegs / NT;
-    u64 mine[PER];
+    u64 mine[PER], w = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       mine[i] = t * PER + i < nseg ? s.seg[t * PER + i] : 0;
       w += mine[i];
     }
-    u64 run = wave_scan64(w) - w;
+    u64 run = wave_scan64(w) - w, total = 0;
     if (lane == 63) s.wred[wave] = run + w;
     if (t == 0) s.bi[0] = 0;
     __syncthreads();
@@ -576,7 +582,7 @@ struct SampleRow {
     }
     __syncthreads();
     const int seg = s.bi[0];
-    before = s.b64[0];
+    u64 before = s.b64[0];
     if (per == 1) {
       if (wave != seg % NW) return;
       Raw x;
@@ -584,14 +590,13 @@ struct SampleRow {
       pick(x, seg / NW, before, target, total, own);
       return;
     }
-    // the sums before the segment's first vector: those of the stretch's earlier waves are interleaved with it
-    for (int q = seg / NW * NW; q < seg; ++q) before -= s.seg[q];
+    for (int q = seg / NW * NW; q < seg; ++q) before -= s.seg[q];  // the stretch's start
     for (int k = seg / NW * per; k < (seg / NW + 1) * per && k < nvec; ++k) {
       Raw x;
       fetch(x, k);
       u64 sum = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum += own(at(x, e), first(k) + e);
+      for (int e = 0; e < 8; ++e) sum += own(at(x, e), cls(k) + e);
       sum = wave_sum64(sum);
       __syncthreads();
       if (lane == 0) s.wred[wave] = sum;
@@ -606,6 +611,13 @@ struct SampleRow {
     }
   }
 
+  // The draw over the row, of what is kept with weight >= least.
+  __device__ __forceinline__ void draw_row(u64 least) {
+    const int per = (nvec * NW + kSegs - 1) / kSegs;  // vectors a segment
+    segment_sums(least, per);
+    draw_segments(least, per, (nvec + per - 1) / per * NW);
+  }
+
   // Writes the class of the wave's vector k at which the sum passes target, if
   // it is there; `run` is the sum before the wave's first.
   template <typename F>
@@ -613,15 +625,15 @@ struct SampleRow {
     u64 w[8], sum = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      w[e] = own(at(x, e), first(k) + e);
+      w[e] = own(at(x, e), cls(k) + e);
       sum += w[e];
     }
     run += wave_scan64(sum) - sum;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       if (run <= target && target < run + w[e]) {
-        a.token[blockIdx.x] = first(k) + e;
-        if (a.logprob) a.logprob[blockIdx.x] = log_of(at(x, e), total);
+        a.token[row] = cls(k) + e;
+        if (a.logprob) a.logprob[row] = log_of(at(x, e), total);
       }
       run += w[e];
     }
@@ -701,8 +713,8 @@ struct SampleRow {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (run <= at && at < run + w[i]) {
-        a.token[blockIdx.x] = (int)(q[i] >> 32);
-        if (a.logprob) a.logprob[blockIdx.x] = log_of(z_of_key(~(uint32_t)q[i]), all);
+        a.token[row] = (int)(q[i] >> 32);
+        if (a.logprob) a.logprob[row] = log_of(z_of_key(~(uint32_t)q[i]), all);
       }
       run += w[i];
     }
@@ -736,107 +748,298 @@ struct SampleRow {
     draw_small(m);
   }
 
-  // A logit that at least n elements reach: the least, over the waves, of the
-  // ceil(n / NW)-th largest of their lanes' maxima.  n <= NT.
+  // A logit that at least n elements reach, and not many more lanes' maxima than
+  // n do: bisected on the keys.  1 <= n <= NT; -inf where fewer lanes have one.
   __device__ __forceinline__ float reached_by(int n, float lane_max) {
-    float v = lane_max;
-    const int lane = threadIdx.x & 63;
+    const uint32_t key = key_of(lane_max + 0.0f);
+    uint32_t* cnt = reinterpret_cast<uint32_t*>(s.wred);  // two sets of NW, in turn
+    uint32_t lo = key_of(-INFINITY), hi = 0xff800001u;  // reached by n or more; by fewer
+    __syncthreads();
+    for (int i = 0; hi - lo > 1; ++i) {
+      const uint32_t mid = lo + (hi - lo) / 2;
+      const uint32_t c = (uint32_t)__popcll(__ballot(key >= mid));
+      uint32_t* set = cnt + (i & 1) * NW;
+      if ((threadIdx.x & 63) == 0) set[threadIdx.x >> 6] = c;
+      __syncthreads();
+      uint32_t all = 0;
 #pragma unroll
-    for (int k = 2; k <= 64; k <<= 1)
-#pragma unroll
-      for (int j = k >> 1; j > 0; j >>= 1) {  // falling over the lanes
-        const float o = __shfl_xor(v, j, 64);
-        const bool low = (lane & j) == 0, down = (lane & k) == 0;
-        v = low == down ? fmaxf(v, o) : fminf(v, o);
+      for (int k = 0; k < NW; ++k) all += set[k];
+      if (all >= (uint32_t)n) {
+        lo = mid;
+        if (all <= (uint32_t)(n + n / 8)) break;
+      } else {
+        hi = mid;
       }
-    const float w = __shfl(v, (n + NW - 1) / NW - 1, 64);
+    }
     __syncthreads();
-    float* red = reinterpret_cast<float*>(s.wred);
-    if (lane == 0) red[threadIdx.x >> 6] = w;
-    __syncthreads();
-    float t = red[0];
-#pragma unroll
-    for (int k = 1; k < NW; ++k) t = fminf(t, red[k]);
-    __syncthreads();
-    return t;
+    return z_of_key(lo);
   }
 
-  __device__ __forceinline__ void run() {
-    const int row = blockIdx.x;
-    const float T = a.temperature[row], top_p = a.top_p[row], min_p = a.min_p[row];
-    const int top_k = a.top_k[row];
-    nvec = (a.V + NT * 8 - 1) / (NT * 8);
-    float own_max = -INFINITY;
+  // The row's settings.
+  struct Set {
+    float T, top_p, min_p;
+    int top_k;
+    bool greedy, by_k, by_p;
+    u64 least;
+  };
+  __device__ __forceinline__ static Set settings(const SampleArgs& a, int row) {
+    Set q;
+    q.T = a.temperature[row];
+    q.top_p = a.top_p[row];
+    q.min_p = a.min_p[row];
+    q.top_k = a.top_k[row];
+    q.greedy = !(q.T > 0.0f) || q.top_k == 1 || q.top_p <= 0.0f;
+    q.by_k = q.top_k > 0 && q.top_k < a.V;
+    q.by_p = q.top_p < 1.0f;
+    // w >= min_p: on the rounded weights, the least whole number that min_p admits
+    q.least = q.min_p > 0.0f ? (u64)ceil(ldexp((double)fminf(q.min_p, 1.0f), a.shift)) : 0;
+    return q;
+  }
+  __device__ __forceinline__ float lane_max() {
+    float m = -INFINITY;
     each_vec([&](int, const float (&v)[8]) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) own_max = fmaxf(own_max, v[e]);
+      for (int e = 0; e < 8; ++e) m = fmaxf(m, v[e]);
     });
-    {
-      const float w = wave_max(own_max);
-      float* red = reinterpret_cast<float*>(s.wred);
-      if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = w;
-      __syncthreads();
-      zmax = red[0];
+    return m;
+  }
+  __device__ __forceinline__ float block_maxf(float v) {
+    v = wave_max(v);
+    float* red = reinterpret_cast<float*>(s.wred);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = red[0];
 #pragma unroll
-      for (int k = 1; k < NW; ++k) zmax = fmaxf(zmax, red[k]);
-      __syncthreads();
-    }
-    if (zmax == -INFINITY) return write(-1, -INFINITY);
-    if (!(T > 0.0f) || top_k == 1 || top_p <= 0.0f) {
-      u64 best = ~0ull;
-      each_from(zmax, [&](float, int c) { best = (u64)c < best ? (u64)c : best; });
-      return write((int)block_min64(best), 0.0f);
-    }
+    for (int k = 1; k < NW; ++k) v = fmaxf(v, red[k]);
+    __syncthreads();
+    return v;
+  }
+  __device__ __forceinline__ int first_of_max() {
+    u64 best = ~0ull;
+    each_from(zmax, [&](float, int c) { best = (u64)c < best ? (u64)c : best; });
+    return (int)block_min64(best);
+  }
+  __device__ __forceinline__ void scale_by(float zm, float T) {
+    zmax = zm;
     const double inv_t = 1.0 / (double)T;
     c2 = 1.4426950408889634 * inv_t;
     zmax_w = fabsf(zmax) < INFINITY ? wide(zmax) : (double)zmax;
     inv_tf = (float)inv_t;
-    u64 least = 0;
-    // w >= min_p: on the rounded weights, the least whole number that min_p admits
-    if (min_p > 0.0f) least = (u64)ceil(ldexp((double)fminf(min_p, 1.0f), a.shift));
-    const bool by_k = top_k > 0 && top_k < a.V, by_p = top_p < 1.0f;
-    if (by_k && top_k <= NT) {
-      // the k largest are among what reaches a logit that k lanes' maxima reach
-      const float t = reached_by(top_k, own_max);
-      const int m = compact(t, [](float, int) { return true; });
-      if (m <= 256) return finish_wave(m, true, top_k, by_p, top_p, 0, least);
-      if (m <= kList) {
-        sort_list(m);
-        return finish_list(m, true, top_k, by_p, top_p, least);
-      }
-    }
+  }
+  // The draw from the list's m members, not sorted yet, which hold the top k.
+  __device__ __forceinline__ void finish_top_k(int m, const Set& q) {
+    if (m <= 256) return finish_wave(m, true, q.top_k, q.by_p, q.top_p, 0, q.least);
+    sort_list(m);
+    finish_list(m, true, q.top_k, q.by_p, q.top_p, q.least);
+  }
+  __device__ __forceinline__ u64 mass_target(float top_p) {
+    u64 own = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < kBins; i += NT) own += s.mass[i];
+    return (u64)ceil((double)top_p * (double)block_sum64(own));
+  }
+
+  // The whole row in this workgroup; `made`: the masses' histogram is there.
+  __device__ __forceinline__ void cut_and_draw(const Set& q, bool made) {
     for (int pass = 0; pass < 2; ++pass) {
       const bool by_mass = pass == 1;
-      if (!(by_mass ? by_p : by_k)) continue;
-      histogram(by_mass);
-      u64 target = (u64)top_k;
-      if (by_mass) {
-        u64 own = 0;
-        __syncthreads();
-        for (int i = threadIdx.x; i < kBins; i += NT) own += s.mass[i];
-        target = (u64)ceil((double)top_p * (double)block_sum64(own));
-      }
+      if (!(by_mass ? q.by_p : q.by_k)) continue;
+      if (!made) histogram(by_mass);
+      const u64 target = by_mass ? mass_target(q.top_p) : (u64)q.top_k;
       const Cut cut = find_bin(kBins, by_mass, target);
       if (cut.cnt_before + cut.n <= kList) {
         // little lies up to the cut: all of it, sorted
         int m = compact(z_t, [&](float v, int c) { return bin_of(v) <= cut.bin && kept(v, c); });
-        if (m <= 256) return finish_wave(m, !by_mass, top_k, by_p, top_p, by_mass ? target : 0, least);
+        if (!by_mass) return finish_top_k(m, q);
+        if (m <= 256) return finish_wave(m, false, 0, true, q.top_p, target, q.least);
         sort_list(m);
-        if (!by_mass) return finish_list(m, true, top_k, by_p, top_p, least);
         m = last_below(m, 0, target) + 1;
-        return cut_min_p(m, least);
+        return cut_min_p(m, q.least);
       }
       refine(by_mass, target, cut);
     }
-    draw_row(least);
+    draw_row(q.least);
+  }
+
+  __device__ __forceinline__ void run() {
+    const Set q = settings(a, row);
+    const float own_max = lane_max();
+    zmax = block_maxf(own_max);
+    if (zmax == -INFINITY) return write(-1, -INFINITY);
+    if (q.greedy) return write(first_of_max(), 0.0f);
+    scale_by(zmax, q.T);
+    if (q.by_k && q.top_k <= NT) {
+      // the k largest are among what reaches a logit that k lanes' maxima reach
+      const float t = reached_by(q.top_k, own_max);
+      const int m = compact(t, [](float, int) { return true; });
+      if (m <= kList) return finish_top_k(m, q);
+    }
+    cut_and_draw(q, false);
   }
 };
 
 template <int EK, int NT>
 __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
   __shared__ SampleLds<NT> lds;
-  SampleRow<EK, NT> row(a, lds);
+  SampleRow<EK, NT> row(a, lds, blockIdx.x, 0, a.V);
   row.run();
+}
+
+// ---------------------------------------------------------------------------
+// Few rows: P workgroups a row, in three launches.
+//   1  each takes its waves' maxima, and the first class that has the largest;
+//      clears the row's counters
+//   2  top-k: the classes that reach a logit which k of the waves' maxima reach,
+//      into the row's list; top-p alone: the row's histogram; neither: the
+//      segments' sums
+//   3  one workgroup a row: what is left of the cuts, and the draw (a list that
+//      overflowed, or a nucleus of many classes, as without scratch)
+// Scratch, in words: 0 the list's count; 16 + 8 q the q-th workgroup's (1: the
+// first class of its maximum, 4 ..: its waves' maxima); 2048 the list, the histogram's counts and masses, or the segments' sums.
+// ---------------------------------------------------------------------------
+constexpr int kPartNT = 256, kPartWords = 8, kPartAt = 16, kDataAt = 2048;
+static_assert(kDataAt + kBins * 3 <= 8192 && kDataAt + kList * 2 <= 8192 && kDataAt + kSegs * 2 <= 8192, "scratch");
+
+// Classes of a part: whole segments of 512.  Of ceil(V / part_len(V, P)) parts,
+// only the last may have fewer.
+__host__ __device__ inline int part_len(int V, int P) { return ((V + P - 1) / P + 511) & ~511; }
+__device__ __forceinline__ void part_classes(int V, int P, int q, int* c0, int* c1) {
+  const int len = part_len(V, P);
+  *c0 = q * len;
+  *c1 = min(*c0 + len, V);
+}
+template <int EK>
+__global__ __launch_bounds__(kPartNT) void sample_part_max_kernel(SampleArgs a, uint32_t* scratch, int64_t lds, int P) {
+  __shared__ SampleLds<kPartNT> sl;
+  typedef SampleRow<EK, kPartNT> Row;
+  const int r = blockIdx.y, q = blockIdx.x;
+  int c0, c1;
+  part_classes(a.V, P, q, &c0, &c1);
+  Row part(a, sl, r, c0, c1);
+  const typename Row::Set set = Row::settings(a, r);
+  uint32_t* row = scratch + (int64_t)r * lds;
+  if (q == 0 && threadIdx.x == 0) row[0] = 0;
+  if (set.by_p && !set.by_k)
+    for (int i = q * kPartNT + threadIdx.x; i < kBins * 3; i += P * kPartNT) row[kDataAt + i] = 0;
+  const float own = part.lane_max();
+  uint32_t* out = row + kPartAt + q * kPartWords;
+  const float w = wave_max(own);
+  if ((threadIdx.x & 63) == 0) out[4 + (threadIdx.x >> 6)] = __float_as_uint(w);
+  if (set.greedy) {
+    part.zmax = part.block_maxf(own);
+    const int at = part.zmax > -INFINITY ? part.first_of_max() : -1;
+    if (threadIdx.x == 0) out[1] = (uint32_t)at;
+  }
+}
+
+// The waves' maxima of a row's parts, those of part `lane` in each lane.
+__device__ __forceinline__ f32x4 parts_max(const uint32_t* row, int P) {
+  const int lane = threadIdx.x & 63;
+  if (lane >= P) return f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  return *reinterpret_cast<const f32x4_a4*>(row + kPartAt + lane * kPartWords + 4);
+}
+__device__ __forceinline__ float max4(const f32x4& m) { return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])); }
+// A logit that n of them reach (n <= 4 P; -inf where fewer are there), and not
+// many more: bisected on the keys, in each wave for itself.
+__device__ __forceinline__ float reached_by_parts(const f32x4& m, int n) {
+  uint32_t key[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) key[i] = key_of(m[i] + 0.0f);
+  uint32_t lo = key_of(-INFINITY), hi = 0xff800001u;
+  while (hi - lo > 1) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c += __popcll(__ballot(key[i] >= mid));
+    if (c >= n) {
+      lo = mid;
+      if (c <= n + n / 8) break;
+    } else {
+      hi = mid;
+    }
+  }
+  return z_of_key(lo);
+}
+
+template <int EK>
+__global__ __launch_bounds__(kPartNT) void sample_part_kernel(SampleArgs a, uint32_t* scratch, int64_t lds, int P) {
+  __shared__ SampleLds<kPartNT> sl;
+  typedef SampleRow<EK, kPartNT> Row;
+  const int r = blockIdx.y, q = blockIdx.x;
+  const typename Row::Set set = Row::settings(a, r);
+  uint32_t* row = scratch + (int64_t)r * lds;
+  const f32x4 maxima = parts_max(row, P);
+  const float zmax = wave_max(max4(maxima));
+  if (set.greedy || zmax == -INFINITY) return;
+  int c0, c1;
+  part_classes(a.V, P, q, &c0, &c1);
+  Row part(a, sl, r, c0, c1);
+  part.scale_by(zmax, set.T);
+  u64* data = reinterpret_cast<u64*>(row + kDataAt);
+  if (set.by_k) {
+    if (set.top_k > 4 * P) return;  // the third launch takes it whole
+    const float t = reached_by_parts(maxima, set.top_k);
+    const int m = part.compact(t, [](float, int) { return true; });
+    if (threadIdx.x == 0) sl.bi[0] = m > 0 ? (int)atomicAdd(row, (uint32_t)m) : 0;
+    __syncthreads();
+    const int at = sl.bi[0], n = min(m, kList);
+    for (int i = threadIdx.x; i < n && at + i < kList; i += kPartNT) data[at + i] = sl.list[i];
+  } else if (set.by_p) {
+    part.histogram(true);
+    __syncthreads();
+    uint32_t* cnt = reinterpret_cast<uint32_t*>(data + kBins);
+    for (int i = threadIdx.x; i < kBins; i += kPartNT)
+      if (sl.cnt[i]) {
+        atomicAdd(cnt + i, sl.cnt[i]);
+        atomicAdd(data + i, sl.mass[i]);
+      }
+  } else {
+    part.segment_sums(set.least, 1);
+    const int nseg = (c1 - c0 + 511) / 512;
+    for (int i = threadIdx.x; i < nseg; i += kPartNT) data[c0 / 512 + i] = sl.seg[i];
+  }
+}
+
+template <int EK>
+__global__ __launch_bounds__(1024) void sample_join_kernel(SampleArgs a, const uint32_t* scratch, int64_t lds, int P) {
+  constexpr int NT = 1024;
+  __shared__ SampleLds<NT> sl;
+  typedef SampleRow<EK, NT> Row;
+  const int r = blockIdx.x, lane = threadIdx.x & 63;
+  const uint32_t* row = scratch + (int64_t)r * lds;
+  Row whole(a, sl, r, 0, a.V);
+  const typename Row::Set set = Row::settings(a, r);
+  const float part_max = max4(parts_max(row, P)), zmax = wave_max(part_max);
+  if (zmax == -INFINITY) return whole.write(-1, -INFINITY);
+  if (set.greedy) {
+    uint32_t at = lane < P && part_max == zmax ? row[kPartAt + lane * kPartWords + 1] : 0xffffffffu;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) at = min(at, (uint32_t)__shfl_xor((int)at, off, 64));
+    return whole.write((int)at, 0.0f);
+  }
+  whole.scale_by(zmax, set.T);
+  const u64* data = reinterpret_cast<const u64*>(row + kDataAt);
+  if (set.by_k) {
+    const uint32_t m = row[0];
+    if (set.top_k > 4 * P || m > kList) return whole.run();
+    for (int i = threadIdx.x; i < (int)m; i += NT) sl.list[i] = data[i];
+    __syncthreads();
+    return whole.finish_top_k((int)m, set);
+  }
+  if (set.by_p) {
+    const uint32_t* cnt = reinterpret_cast<const uint32_t*>(data + kBins);
+    for (int i = threadIdx.x; i < kBins; i += NT) {
+      sl.cnt[i] = cnt[i];
+      sl.mass[i] = data[i];
+    }
+    __syncthreads();
+    return whole.cut_and_draw(set, true);
+  }
+  const int nseg = (a.V + 511) / 512;
+  for (int i = threadIdx.x; i < nseg; i += NT) sl.seg[i] = data[i];
+  __syncthreads();
+  whole.draw_segments(set.least, 1, nseg);
 }
 
 // ---------------------------------------------------------------------------
@@ -861,8 +1064,21 @@ bool sample_sup(const TensorDesc* in, int ni, const TensorDesc* out, int no, con
 }
 
 template <int EK>
-Status sample_run(const SampleArgs& a, hipStream_t s) {
+Status sample_run(const SampleArgs& a, uint32_t* scratch, int64_t lds, hipStream_t s) {
   const unsigned g = (unsigned)a.R;
+  // Few rows share the chip: parts of 2048 classes or more, about one workgroup
+  // a CU.
+  int P = 256 / a.R;
+  if (P > a.V / 2048) P = a.V / 2048;
+  if (P > 64) P = 64;
+  if (scratch && P >= 4 && a.V <= 512 * kSegs) {
+    P = (a.V + part_len(a.V, P) - 1) / part_len(a.V, P);
+    const dim3 grid((unsigned)P, g);
+    sample_part_max_kernel<EK><<<grid, kPartNT, 0, s>>>(a, scratch, lds, P);
+    sample_part_kernel<EK><<<grid, kPartNT, 0, s>>>(a, scratch, lds, P);
+    sample_join_kernel<EK><<<g, 1024, 0, s>>>(a, scratch, lds, P);
+    return launch_status("sample_row");
+  }
   if (a.V <= 8192) sample_kernel<EK, 256><<<g, 256, 0, s>>>(a);
   else sample_kernel<EK, 1024><<<g, 1024, 0, s>>>(a);
   return launch_status("sample_row");
@@ -894,8 +1110,10 @@ Status sample_launch(const TensorDesc* in, int ni, TensorDesc* out, int no, cons
   int ek;
   elem_kind(in[0], &ek);
   hipStream_t s = as_stream(stream);
-  if (ek == EL_F32) return sample_run<EL_F32>(a, s);
-  return ek == EL_F16 ? sample_run<EL_F16>(a, s) : sample_run<EL_BF16>(a, s);
+  uint32_t* scratch = no > 2 && aligned(out[2].data, 8) && out[2].shape[1] % 2 == 0 ? (uint32_t*)out[2].data : nullptr;
+  const int64_t lds = no > 2 ? out[2].shape[1] : 0;
+  if (ek == EL_F32) return sample_run<EL_F32>(a, scratch, lds, s);
+  return ek == EL_F16 ? sample_run<EL_F16>(a, scratch, lds, s) : sample_run<EL_BF16>(a, scratch, lds, s);
 }
 
 size_t no_workspace(const TensorDesc*, int, const void*) { return 0; }

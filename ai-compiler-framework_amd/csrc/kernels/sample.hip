@@ -111,6 +111,7 @@ __device__ __forceinline__ u64 wave_scan64(u64 v) {  // inclusive
   return v;
 }
 
+constexpr int kPairs = 256;   // entries that are ordered by counting; one a thread
 constexpr int kSegs = 1024;  // segments of a row whose kept sums are held
 
 template <int NT>
@@ -141,7 +142,7 @@ struct SampleRow {
   float zmax;
   double zmax_w;
   double c2;         // log2(e) / T
-  float inv_tf;
+  float inv_tf, u;
   Exp2Series series;
   // what is kept: logits above z_t, and at z_t the classes up to c_t
   float z_t = -INFINITY;
@@ -481,8 +482,6 @@ struct SampleRow {
     return (float)(-d - log(ldexp((double)total, -a.shift)));
   }
   __device__ __forceinline__ u64 draw_at(u64 total) const {
-    float u = a.u[row];
-    u = u > 0.0f ? fminf(u, 0.99999994f) : 0.0f;
     return (u64)((double)u * (double)total);  // the sum has to pass this
   }
 
@@ -639,84 +638,41 @@ struct SampleRow {
     }
   }
 
-  // LDS between the steps of one wave: its operations are in order, the
-  // compiler's are kept so.
-  __device__ __forceinline__ static void wave_order() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-  }
-  // Sorts list[0 .. n), n <= 256, in one wave.
-  __device__ __forceinline__ void wave_sort(int n) {
-    const int lane = threadIdx.x & 63;
-    int m = 64;
-    while (m < n) m <<= 1;
-    for (int i = n + lane; i < m; i += 64) s.list[i] = ~0ull;
-    for (int k = 2; k <= m; k <<= 1)
-      for (int j = k >> 1; j > 0; j >>= 1) {
-        wave_order();
-        for (int q = lane; q < m / 2; q += 64) {
-          const int i = (q & ~(j - 1)) * 2 + (q & (j - 1)), o = i + j;
-          const u64 x = s.list[i], y = s.list[o];
-          if ((x > y) == ((i & k) == 0)) {
-            s.list[i] = y;
-            s.list[o] = x;
-          }
-        }
-      }
-    wave_order();
-  }
-  // The same as finish_list for m <= 256 (not sorted yet), in the first wave
-  // alone: 4 entries a lane, no barrier of the workgroup.
-  __device__ __forceinline__ void finish_wave(int m, bool by_k, int top_k, bool by_p, float top_p, u64 mass_target,
-                                              u64 least) {
-    if (threadIdx.x >= 64) return;
-    const int lane = threadIdx.x;
-    wave_sort(m);
-    if (by_k && top_k < m) m = top_k;
-    u64 q[4], w[4], own = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      q[i] = lane * 4 + i < m ? s.list[lane * 4 + i] : ~0ull;
-      w[i] = lane * 4 + i < m ? weight(z_of_key(~(uint32_t)(q[i] >> 32))) : 0;
-      own += w[i];
+  // The same as finish_list for m <= kPairs (the list not sorted): an entry's place
+  // in either order, and the sum before it, are counted over all entries, which
+  // the lanes of a wave read from LDS together (the last launch of 1 x 131072, k 50:
+  // 10.8 us; with two sorts 11.9).
+  __device__ __forceinline__ void finish_pairs(int m, bool by_k, int top_k, bool by_p, float top_p, u64 mass_target,
+                                               u64 least) {
+    const int t = threadIdx.x, some = (t & ~63) < m ? m : 0;  // none for a wave without entries
+    u64* const w1 = s.list + kPairs;
+    u64* const w2 = w1 + kPairs;
+    const u64 q = t < m ? s.list[t] : ~0ull;
+    const u64 w = t < m ? weight(z_of_key(~(uint32_t)(q >> 32))) : 0;
+    if (t < m) w1[t] = w;
+    __syncthreads();
+    u64 run = 0;
+    int rank = 0;
+#pragma unroll 4
+    for (int j = 0; j < some; ++j) {
+      const bool before = s.list[j] < q;
+      rank += before;
+      run += before ? w1[j] : 0;
     }
-    const u64 incl = wave_scan64(own), total = (u64)__shfl((long long)incl, 63, 64);
-    u64 run = incl - own;
-    const u64 target = by_p ? (mass_target ? mass_target : (u64)ceil((double)top_p * (double)total)) : ~0ull;
-    int n = 0;  // kept of this lane: a prefix of the order
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const bool first = lane * 4 + i == 0;
-      if (lane * 4 + i < m && (first || (run < target && w[i] >= least))) ++n;
-      run += w[i];
-    }
-    m = n;
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) m += __shfl_xor(m, off, 64);
-    // into the order of the classes, the key in the low half
-    wave_order();
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < n) s.list[lane * 4 + i] = (q[i] << 32) | (q[i] >> 32);
-    wave_order();
-    wave_sort(m);
-    own = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      q[i] = lane * 4 + i < m ? s.list[lane * 4 + i] : 0;
-      w[i] = lane * 4 + i < m ? weight(z_of_key(~(uint32_t)q[i])) : 0;
-      own += w[i];
-    }
-    const u64 sum = wave_scan64(own), all = (u64)__shfl((long long)sum, 63, 64);
-    run = sum - own;
-    const u64 at = draw_at(all);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (run <= at && at < run + w[i]) {
-        a.token[row] = (int)(q[i] >> 32);
-        if (a.logprob) a.logprob[row] = log_of(z_of_key(~(uint32_t)q[i]), all);
-      }
-      run += w[i];
+    const bool in = t < m && (!by_k || rank < top_k);
+    u64 target = ~0ull;
+    if (by_p) target = mass_target ? mass_target : (u64)ceil((double)top_p * (double)block_sum64(in ? w : 0));
+    const bool keep = in && (rank == 0 || (run < target && w >= least));
+    const u64 own = keep ? w : 0;
+    if (t < m) w2[t] = own;
+    const u64 total = block_sum64(own);
+    run = 0;
+#pragma unroll 4
+    for (int j = 0; j < some; ++j) run += (uint32_t)s.list[j] < (uint32_t)q ? w2[j] : 0;
+    const u64 at = draw_at(total);
+    if (run <= at && at < run + own) {
+      a.token[row] = (int)(uint32_t)q;
+      if (a.logprob) a.logprob[row] = log_of(z_of_key(~(uint32_t)(q >> 32)), total);
     }
   }
 
@@ -753,8 +709,8 @@ struct SampleRow {
   __device__ __forceinline__ float reached_by(int n, float lane_max) {
     const uint32_t key = key_of(lane_max + 0.0f);
     uint32_t* cnt = reinterpret_cast<uint32_t*>(s.wred);  // two sets of NW, in turn
-    uint32_t lo = key_of(-INFINITY), hi = 0xff800001u;  // reached by n or more; by fewer
-    __syncthreads();
+    // reached by n or more (by all NT); by fewer
+    uint32_t lo = key_of(-block_maxf(-lane_max) + 0.0f), hi = key_of(zmax + 0.0f) + 1;
     for (int i = 0; hi - lo > 1; ++i) {
       const uint32_t mid = lo + (hi - lo) / 2;
       const uint32_t c = (uint32_t)__popcll(__ballot(key >= mid));
@@ -766,7 +722,7 @@ struct SampleRow {
       for (int k = 0; k < NW; ++k) all += set[k];
       if (all >= (uint32_t)n) {
         lo = mid;
-        if (all <= (uint32_t)(n + n / 8)) break;
+        if (all <= (uint32_t)(n + n / 16)) break;
       } else {
         hi = mid;
       }
@@ -777,7 +733,7 @@ struct SampleRow {
 
   // The row's settings.
   struct Set {
-    float T, top_p, min_p;
+    float T, top_p, min_p, u;
     int top_k;
     bool greedy, by_k, by_p;
     u64 least;
@@ -785,6 +741,7 @@ struct SampleRow {
   __device__ __forceinline__ static Set settings(const SampleArgs& a, int row) {
     Set q;
     q.T = a.temperature[row];
+    q.u = a.u[row];
     q.top_p = a.top_p[row];
     q.min_p = a.min_p[row];
     q.top_k = a.top_k[row];
@@ -820,16 +777,17 @@ struct SampleRow {
     each_from(zmax, [&](float, int c) { best = (u64)c < best ? (u64)c : best; });
     return (int)block_min64(best);
   }
-  __device__ __forceinline__ void scale_by(float zm, float T) {
+  __device__ __forceinline__ void scale_by(float zm, const Set& q) {
     zmax = zm;
-    const double inv_t = 1.0 / (double)T;
+    u = q.u > 0.0f ? fminf(q.u, 0.99999994f) : 0.0f;
+    const double inv_t = 1.0 / (double)q.T;
     c2 = 1.4426950408889634 * inv_t;
     zmax_w = fabsf(zmax) < INFINITY ? wide(zmax) : (double)zmax;
     inv_tf = (float)inv_t;
   }
   // The draw from the list's m members, not sorted yet, which hold the top k.
   __device__ __forceinline__ void finish_top_k(int m, const Set& q) {
-    if (m <= 256) return finish_wave(m, true, q.top_k, q.by_p, q.top_p, 0, q.least);
+    if (m <= kPairs) return finish_pairs(m, true, q.top_k, q.by_p, q.top_p, 0, q.least);
     sort_list(m);
     finish_list(m, true, q.top_k, q.by_p, q.top_p, q.least);
   }
@@ -852,7 +810,7 @@ struct SampleRow {
         // little lies up to the cut: all of it, sorted
         int m = compact(z_t, [&](float v, int c) { return bin_of(v) <= cut.bin && kept(v, c); });
         if (!by_mass) return finish_top_k(m, q);
-        if (m <= 256) return finish_wave(m, false, 0, true, q.top_p, target, q.least);
+        if (m <= kPairs) return finish_pairs(m, false, 0, true, q.top_p, target, q.least);
         sort_list(m);
         m = last_below(m, 0, target) + 1;
         return cut_min_p(m, q.least);
@@ -868,7 +826,7 @@ struct SampleRow {
     zmax = block_maxf(own_max);
     if (zmax == -INFINITY) return write(-1, -INFINITY);
     if (q.greedy) return write(first_of_max(), 0.0f);
-    scale_by(zmax, q.T);
+    scale_by(zmax, q);
     if (q.by_k && q.top_k <= NT) {
       // the k largest are among what reaches a logit that k lanes' maxima reach
       const float t = reached_by(q.top_k, own_max);
@@ -888,17 +846,19 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
 
 // ---------------------------------------------------------------------------
 // Few rows: P workgroups a row, in three launches.
-//   1  each takes its waves' maxima, and the first class that has the largest;
-//      clears the row's counters
-//   2  top-k: the classes that reach a logit which k of the waves' maxima reach,
-//      into the row's list; top-p alone: the row's histogram; neither: the
-//      segments' sums
+//   1  each takes the maxima of its 16 groups of 16 lanes, and the first class
+//      that has the largest; clears the row's counters
+//   2  top-k: the classes that reach a logit which k of those maxima reach, into
+//      the row's list; top-p alone: the row's histogram; neither: the segments'
+//      sums
 //   3  one workgroup a row: what is left of the cuts, and the draw (a list that
 //      overflowed, or a nucleus of many classes, as without scratch)
-// Scratch, in words: 0 the list's count; 16 + 8 q the q-th workgroup's (1: the
-// first class of its maximum, 4 ..: its waves' maxima); 2048 the list, the histogram's counts and masses, or the segments' sums.
+// Scratch, in words: 0 the list's count; 16 + 20 q the q-th workgroup's (0: the
+// first class of its maximum, 4 ..: the groups' maxima); 2048 the list, the
+// histogram's masses and counts, or the segments' sums.
 // ---------------------------------------------------------------------------
-constexpr int kPartNT = 256, kPartWords = 8, kPartAt = 16, kDataAt = 2048;
+constexpr int kPartNT = 256, kPartWords = 20, kPartAt = 16, kDataAt = 2048;
+static_assert(kPartAt + 64 * kPartWords <= kDataAt, "scratch");
 static_assert(kDataAt + kBins * 3 <= 8192 && kDataAt + kList * 2 <= 8192 && kDataAt + kSegs * 2 <= 8192, "scratch");
 
 // Classes of a part: whole segments of 512.  Of ceil(V / part_len(V, P)) parts,
@@ -924,37 +884,55 @@ __global__ __launch_bounds__(kPartNT) void sample_part_max_kernel(SampleArgs a, 
     for (int i = q * kPartNT + threadIdx.x; i < kBins * 3; i += P * kPartNT) row[kDataAt + i] = 0;
   const float own = part.lane_max();
   uint32_t* out = row + kPartAt + q * kPartWords;
-  const float w = wave_max(own);
-  if ((threadIdx.x & 63) == 0) out[4 + (threadIdx.x >> 6)] = __float_as_uint(w);
+  float w = own;
+#pragma unroll
+  for (int off = 8; off > 0; off >>= 1) w = fmaxf(w, __shfl_xor(w, off, 64));
+  if ((threadIdx.x & 15) == 0) out[4 + (threadIdx.x >> 4)] = __float_as_uint(w);
   if (set.greedy) {
     part.zmax = part.block_maxf(own);
     const int at = part.zmax > -INFINITY ? part.first_of_max() : -1;
-    if (threadIdx.x == 0) out[1] = (uint32_t)at;
+    if (threadIdx.x == 0) out[0] = (uint32_t)at;
   }
 }
 
-// The waves' maxima of a row's parts, those of part `lane` in each lane.
-__device__ __forceinline__ f32x4 parts_max(const uint32_t* row, int P) {
+// The groups' maxima of a row's parts, those of part `lane` in each lane.
+constexpr int kGroups = 16;
+__device__ __forceinline__ void parts_max(const uint32_t* row, int P, float (&m)[kGroups]) {
   const int lane = threadIdx.x & 63;
-  if (lane >= P) return f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-  return *reinterpret_cast<const f32x4_a4*>(row + kPartAt + lane * kPartWords + 4);
-}
-__device__ __forceinline__ float max4(const f32x4& m) { return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])); }
-// A logit that n of them reach (n <= 4 P; -inf where fewer are there), and not
-// many more: bisected on the keys, in each wave for itself.
-__device__ __forceinline__ float reached_by_parts(const f32x4& m, int n) {
-  uint32_t key[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) key[i] = key_of(m[i] + 0.0f);
-  uint32_t lo = key_of(-INFINITY), hi = 0xff800001u;
+  for (int i = 0; i < kGroups; i += 4) {
+    f32x4 v = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    if (lane < P) v = *reinterpret_cast<const f32x4_a4*>(row + kPartAt + lane * kPartWords + 4 + i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m[i + e] = v[e];
+  }
+}
+__device__ __forceinline__ float max_of(const float (&m)[kGroups]) {
+  float t = m[0];
+#pragma unroll
+  for (int i = 1; i < kGroups; ++i) t = fmaxf(t, m[i]);
+  return t;
+}
+// A logit that n of them reach (n <= 16 P; -inf where fewer are there), and not
+// many more: bisected on the keys, in each wave for itself.
+__device__ __forceinline__ float reached_by_parts(const float (&m)[kGroups], int P, float zmax, int n) {
+  uint32_t key[kGroups];
+#pragma unroll
+  for (int i = 0; i < kGroups; ++i) key[i] = key_of(m[i] + 0.0f);
+  // reached by all 16 P, or by n; by fewer
+  float low = INFINITY;
+#pragma unroll
+  for (int i = 0; i < kGroups; ++i) low = fminf(low, m[i]);
+  low = -wave_max((int)(threadIdx.x & 63) < P ? -low : -INFINITY);
+  uint32_t lo = key_of(low + 0.0f), hi = key_of(zmax + 0.0f) + 1;
   while (hi - lo > 1) {
     const uint32_t mid = lo + (hi - lo) / 2;
     int c = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c += __popcll(__ballot(key[i] >= mid));
+    for (int i = 0; i < kGroups; ++i) c += __popcll(__ballot(key[i] >= mid));
     if (c >= n) {
       lo = mid;
-      if (c <= n + n / 8) break;
+      if (c <= n + n / 16) break;
     } else {
       hi = mid;
     }
@@ -969,17 +947,18 @@ __global__ __launch_bounds__(kPartNT) void sample_part_kernel(SampleArgs a, uint
   const int r = blockIdx.y, q = blockIdx.x;
   const typename Row::Set set = Row::settings(a, r);
   uint32_t* row = scratch + (int64_t)r * lds;
-  const f32x4 maxima = parts_max(row, P);
-  const float zmax = wave_max(max4(maxima));
+  float maxima[kGroups];
+  parts_max(row, P, maxima);
+  const float zmax = wave_max(max_of(maxima));
   if (set.greedy || zmax == -INFINITY) return;
   int c0, c1;
   part_classes(a.V, P, q, &c0, &c1);
   Row part(a, sl, r, c0, c1);
-  part.scale_by(zmax, set.T);
+  part.scale_by(zmax, set);
   u64* data = reinterpret_cast<u64*>(row + kDataAt);
   if (set.by_k) {
-    if (set.top_k > 4 * P) return;  // the third launch takes it whole
-    const float t = reached_by_parts(maxima, set.top_k);
+    if (set.top_k > kGroups / 2 * P) return;  // the third launch takes it whole
+    const float t = reached_by_parts(maxima, P, zmax, set.top_k);
     const int m = part.compact(t, [](float, int) { return true; });
     if (threadIdx.x == 0) sl.bi[0] = m > 0 ? (int)atomicAdd(row, (uint32_t)m) : 0;
     __syncthreads();
@@ -1010,20 +989,25 @@ __global__ __launch_bounds__(1024) void sample_join_kernel(SampleArgs a, const u
   const uint32_t* row = scratch + (int64_t)r * lds;
   Row whole(a, sl, r, 0, a.V);
   const typename Row::Set set = Row::settings(a, r);
-  const float part_max = max4(parts_max(row, P)), zmax = wave_max(part_max);
+  // on their way with the settings, before it is known that there is a list
+  const u64* data = reinterpret_cast<const u64*>(row + kDataAt);
+  const uint32_t m = row[0];
+  const u64 entry = data[threadIdx.x];
+  float maxima[kGroups];
+  parts_max(row, P, maxima);
+  const float part_max = max_of(maxima), zmax = wave_max(part_max);
   if (zmax == -INFINITY) return whole.write(-1, -INFINITY);
   if (set.greedy) {
-    uint32_t at = lane < P && part_max == zmax ? row[kPartAt + lane * kPartWords + 1] : 0xffffffffu;
+    uint32_t at = lane < P && part_max == zmax ? row[kPartAt + lane * kPartWords] : 0xffffffffu;
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) at = min(at, (uint32_t)__shfl_xor((int)at, off, 64));
     return whole.write((int)at, 0.0f);
   }
-  whole.scale_by(zmax, set.T);
-  const u64* data = reinterpret_cast<const u64*>(row + kDataAt);
+  whole.scale_by(zmax, set);
   if (set.by_k) {
-    const uint32_t m = row[0];
-    if (set.top_k > 4 * P || m > kList) return whole.run();
-    for (int i = threadIdx.x; i < (int)m; i += NT) sl.list[i] = data[i];
+    if (set.top_k > kGroups / 2 * P || m > kList) return whole.run();
+    if (threadIdx.x < m) sl.list[threadIdx.x] = entry;
+    if (threadIdx.x + NT < m) sl.list[threadIdx.x + NT] = data[threadIdx.x + NT];
     __syncthreads();
     return whole.finish_top_k((int)m, set);
   }

@@ -6,7 +6,15 @@ compile-time rewrites of the reference pipeline:
     LinearBwd -> gemm dX = dY.W, gemm dW = dY^T.X, reduce_sum(axis 0) for db
     Save      -> copy_saved;  other ops map one to one
   and the ops this backend appends (GELU, softmax cross-entropy, fused MSE
-  loss, AdamW with in-kernel bias correction, row softmax / reduce).
+  loss, AdamW with in-kernel bias correction, row softmax / reduce, the
+  vocabulary head's distillation loss and sampling), and Linear layers in
+  8 bits (not in the reference):
+    LinearFp8    x, W [, b] -> y, xq, xs, wq, ws [, xqT, xsT [, wqT, wsT]]
+      quant_fp8 of x (rows) and of W (blocks; not with quant_w=False, for
+      weights that were quantised once) + gemm_fp8
+    LinearFp8Bwd dY, xqT, xsT [, wqT, wsT] -> dW, dyq, dys, dyqT, dysT [, db] [, dX]
+      quant_fp8 of dY both ways, gemm_fp8 dW = dY^T.X and (need_dx)
+      dX = dY.W, reduce_sum(axis 0) for db (bias)
 * StageC  fuse_gemm_epilogue    (reference rewrites/stageC_fuse_epilogue.py:5-76)
     gemm [-> bias_add in place] -> relu  ==> gemm_epilogue (bias_relu/relu)
   extended with gemm -> bias_add -> gelu (==> bias_gelu, keeping the
@@ -53,14 +61,17 @@ _PRIMITIVES = {
     "sgd_step", "gelu", "gelu_bwd", "softmax_xent", "row_softmax", "row_reduce", "mse_loss",
     "adamw_step", "layernorm_fwd", "layernorm_bwd", "batchnorm_fwd", "batchnorm_bwd",
     "transpose", "gemm_adamw", "xent_head", "grad_group", "adamw_multi", "mse_colsum",
-    "colsum_adamw", "grad_group_adamw", "gemm_epilogue_bcopy",
+    "colsum_adamw", "grad_group_adamw", "gemm_epilogue_bcopy", "quant_fp8", "gemm_fp8",
+    "distill_topk", "sample_row",
 }
 
 _ALIASES = {"adamstep": "adam_step", "stepinc": "step_inc", "biascorr": "bias_corr",
             "msegrad": "mse_grad", "relubwd": "relu_bwd", "sgdstep": "sgd_step",
             "linearbwd": "linear_bwd", "gelubwd": "gelu_bwd", "softmaxxent": "softmax_xent",
             "mseloss": "mse_loss", "adamwstep": "adamw_step", "rowsoftmax": "row_softmax",
-            "rowreduce": "row_reduce"}
+            "rowreduce": "row_reduce", "quantfp8": "quant_fp8", "gemmfp8": "gemm_fp8",
+            "distilltopk": "distill_topk", "samplerow": "sample_row", "linearfp8": "linear_fp8",
+            "linearfp8bwd": "linear_fp8_bwd"}
 
 
 EPILOGUE_KINDS = {"bias_relu": 0, "bias": 1, "relu": 2, "bias_gelu": 3, "gelu": 4, "dgelu": 5}
@@ -112,6 +123,26 @@ def lower_to_backend_ops(ir: IRGraph) -> Lowered:
             if attrs.get("bias", False) and len(outs) >= 3:
                 rs_outs = [outs[2]] + ([int(attrs["db_workspace"])] if "db_workspace" in attrs else [])
                 out.append(_item("reduce_sum", [dy], rs_outs, {"axis": 0, "keepdim": False}))
+        elif op == "linear_fp8":
+            bias = ins[2:]
+            qa = {"pow2": bool(attrs.get("pow2", False))}
+            if len(ins) != 2 + bool(attrs.get("bias", False)) or len(outs) not in (5, 7, 9):
+                raise RuntimeError(f"[lower] linear_fp8: {len(ins)} inputs and {len(outs)} outputs")
+            out.append(_item("quant_fp8", [ins[0]], outs[1:3] + outs[5:7], qa))
+            if attrs.get("quant_w", True):
+                out.append(_item("quant_fp8", [ins[1]], outs[3:5] + outs[7:9], qa))
+            out.append(_item("gemm_fp8", outs[1:5] + bias, [outs[0]]))
+        elif op == "linear_fp8_bwd":
+            need_dx, bias = bool(attrs.get("need_dx", True)), bool(attrs.get("bias", False))
+            if len(ins) < (5 if need_dx else 3) or len(outs) != 5 + bias + need_dx:
+                raise RuntimeError(f"[lower] linear_fp8_bwd: {len(ins)} inputs and {len(outs)} outputs")
+            out.append(_item("quant_fp8", [ins[0]], outs[1:5], {"pow2": bool(attrs.get("pow2", False))}))
+            if need_dx:
+                out.append(_item("gemm_fp8", outs[1:3] + ins[3:5], [outs[5 + bias]]))
+            out.append(_item("gemm_fp8", outs[3:5] + ins[1:3], [outs[0]]))
+            if bias:
+                rs_outs = [outs[5]] + ([int(attrs["db_workspace"])] if "db_workspace" in attrs else [])
+                out.append(_item("reduce_sum", [ins[0]], rs_outs, {"axis": 0, "keepdim": False}))
         elif op == "save":
             out.append(_item("copy_saved", [ins[0]], [outs[0]]))
         elif op in ("relu", "mse_grad", "relu_bwd", "sgd_step") or op in _PRIMITIVES:
@@ -394,6 +425,10 @@ def pick_kernel_id(ir: IRGraph, it: Dict[str, Any]) -> Optional[str]:
         return "mse_colsum_v0"
     if op == "colsum_adamw":
         return "colsum_adamw_f32_v0"
+    if op in ("quant_fp8", "distill_topk", "sample_row"):
+        return f"{op}_v0"
+    if op == "gemm_fp8":
+        return "gemm_fp8_mfma_v0"
     if op in ("layernorm_fwd", "layernorm_bwd"):
         return f"{op}_{'f16' if f16 else 'f32'}_v0"
     if op in ("batchnorm_fwd", "batchnorm_bwd"):

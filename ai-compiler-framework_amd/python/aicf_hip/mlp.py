@@ -8,8 +8,11 @@
   (bf16 shadow weights in a flat bf16 buffer), so the optimizer is one
   streaming AdamW launch over every parameter.  At batch 8192, 4 x 4096^2
   this is the hipGraph benchmark step.
+* build_mlp_distill: a 2-layer student with a vocabulary head, its products in
+  8 bits: logits, a token drawn a row, the distillation loss from a teacher's
+  top logits, both layers' gradients, AdamW on fp32 master weights.
 
-Both return (ir, lowered, plan) ready for PlannedExecutor, plus helpers to
+All return (ir, lowered, plan) ready for PlannedExecutor, plus helpers to
 initialise inputs/parameters from a seed.
 """
 from __future__ import annotations
@@ -205,6 +208,84 @@ def init_mlp_mse(B: int, D: int, L: int, seed: int = 0, device: str = "cuda:0"):
     x = torch.randn((B, D), device=device, dtype=torch.float32, generator=gen).to(torch.bfloat16)
     t = torch.randn((B, D), device=device, dtype=torch.float32, generator=gen)
     return {"x": x, "t": t}, {"flat.params": P}
+
+
+# ============================================================ 8-bit distillation MLP
+DISTILL_INPUTS = {"x", "t", "teacher", "teacher.ids", "u", "temperature", "top_k", "top_p", "min_p"}
+
+
+def build_mlp_distill(B: int, din: int, dh: int, V: int, K: int, *, tau: float = 1.0,
+                      label_weight: float = 0.0, pow2: bool = False, lr: float = 1e-3,
+                      beta1: float = 0.9, beta2: float = 0.999, eps: float = 1e-8,
+                      device: str = "cuda:0"):
+    """x [B, din] bf16 -> Linear -> GELU -> Linear -> logits [B, V] bf16, each
+    product of both layers and of their gradients over 8-bit codes: e4m3 for
+    activations and weights, e5m2 for gradients.  `teacher` [B, K] holds the
+    teacher's top logits (f32), `teacher.ids` their classes (i32), t the labels
+    (i32; outside [0, V): none).  `token` and `logprob` are the draw from the
+    logits before the step, with u and the row's settings."""
+    ir = IRGraph(name=f"mlp_distill_{B}x{din}x{dh}x{V}")
+    nv = lambda n, s, dt=F32: ir.new_value(name=n, shape=s, dtype=dt, device=device)  # noqa: E731
+    blocks = lambda n: -(-n // 128)  # noqa: E731
+    E4M3, E5M2 = "torch.float8_e4m3fn", "torch.float8_e5m2"
+
+    def codes(name, r, c, dt=E4M3, by_rows=True, both=True):
+        f = (lambda n: n) if by_rows else blocks
+        out = [nv(f"{name}.q", (r, c), dt), nv(f"{name}.s", (f(r), blocks(c)))]
+        return out + ([nv(f"{name}.qT", (c, r), dt), nv(f"{name}.sT", (f(c), blocks(r)))] if both else [])
+
+    x, t = nv("x", (B, din), BF16), nv("t", (B,), I32)
+    teacher, ids = nv("teacher", (B, K)), nv("teacher.ids", (B, K), I32)
+    u, temp, top_p, min_p = (nv(n, (B,)) for n in ("u", "temperature", "top_p", "min_p"))
+    top_k = nv("top_k", (B,), I32)
+    W1, b1, W2, b2 = nv("1.W", (dh, din)), nv("1.b", (dh,)), nv("2.W", (V, dh)), nv("2.b", (V,))
+    z, h, logits = nv("z1", (B, dh), BF16), nv("h1", (B, dh), BF16), nv("logits", (B, V), BF16)
+    token, logprob, draw_ws = nv("token", (B,), I32), nv("logprob", (B,)), nv("draw.ws", (B, 8192), I32)
+    loss, row_loss, loss_ws = nv("loss", (1,)), nv("row_loss", (B,)), nv("loss.ws", (B, 64, 4))
+    dY, dh_, dz = nv("dY", (B, V), BF16), nv("d_h1", (B, dh), BF16), nv("d_z1", (B, dh), BF16)
+    dW1, db1, dW2, db2 = (nv(f"d_{p.name}", p.shape) for p in (W1, b1, W2, b2))
+    step = nv("opt.step", (), I32)
+    xq, w1q = codes("x", B, din), codes("1.W8", dh, din, by_rows=False, both=False)
+    hq, w2q = codes("h1", B, dh), codes("2.W8", V, dh, by_rows=False)
+    yq, zq = codes("dY", B, V, E5M2), codes("d_z1", B, dh, E5M2)
+    lin = {"bias": True, "pow2": pow2}
+    ir.emit(op="LinearFp8", inputs=[x, W1, b1], outputs=[z] + xq[:2] + w1q + xq[2:], attrs=lin)
+    ir.emit(op="Gelu", inputs=[z], outputs=[h])
+    ir.emit(op="LinearFp8", inputs=[h, W2, b2], outputs=[logits] + hq[:2] + w2q[:2] + hq[2:] + w2q[2:], attrs=lin)
+    ir.emit(op="SampleRow", inputs=[logits, u, temp, top_k, top_p, min_p], outputs=[token, logprob, draw_ws])
+    ir.emit(op="DistillTopk", inputs=[logits, teacher, ids, t], outputs=[loss, dY, row_loss, loss_ws],
+            attrs={"temperature": tau, "label_weight": label_weight})
+    ir.emit(op="LinearFp8Bwd", inputs=[dY] + hq[2:] + w2q[2:], outputs=[dW2] + yq + [db2, dh_], attrs=lin)
+    ir.emit(op="GeluBwd", inputs=[dh_, z], outputs=[dz])
+    ir.emit(op="LinearFp8Bwd", inputs=[dz] + xq[2:], outputs=[dW1] + zq + [db1], attrs=dict(lin, need_dx=False))
+    ir.emit(op="StepInc", inputs=[step], outputs=[step])
+    hp = {"lr": lr, "beta1": beta1, "beta2": beta2, "eps": eps, "weight_decay": 0.0}
+    for p, g in ((W1, dW1), (b1, db1), (W2, dW2), (b2, db2)):
+        m, v = nv(f"opt.m.{p.name}", p.shape), nv(f"opt.v.{p.name}", p.shape)
+        ir.emit(op="AdamWStep", inputs=[p, g, m, v, step], outputs=[p, m, v], attrs=hp)
+    lowered = compile_lowered(ir)
+    plan = build_binding_plan(ir, opts=PlanOptions(input_names=set(DISTILL_INPUTS)))
+    return ir, lowered, plan
+
+
+def init_mlp_distill(B: int, din: int, dh: int, V: int, K: int, seed: int = 0, device: str = "cuda:0"):
+    """Synthetic rows, a random teacher's top K logits, settings that differ by
+    row; Kaiming-uniform weights, zero biases.  (inputs, params)."""
+    r = np.random.default_rng(seed)
+    t_logits = torch.from_numpy(2.0 * r.standard_normal((B, V)).astype(np.float32))
+    top, ids = t_logits.topk(K, -1)
+    rows = np.arange(B)
+    ins = {"x": torch.from_numpy(r.standard_normal((B, din)).astype(np.float32)).to(torch.bfloat16),
+           "t": torch.from_numpy(r.integers(0, V, B).astype(np.int32)),
+           "teacher": top, "teacher.ids": ids.to(torch.int32),
+           "u": torch.from_numpy(r.random(B, dtype=np.float32)),
+           "temperature": torch.from_numpy((0.5 * (rows % 4)).astype(np.float32)),
+           "top_k": torch.from_numpy((20 * (rows % 3)).astype(np.int32)),
+           "top_p": torch.from_numpy((1.0 - 0.1 * (rows % 2)).astype(np.float32)),
+           "min_p": torch.from_numpy((0.01 * (rows % 5)).astype(np.float32))}
+    params = {"1.W": torch.from_numpy(kaiming_uniform(r, dh, din)), "1.b": torch.zeros(dh),
+              "2.W": torch.from_numpy(kaiming_uniform(r, V, dh)), "2.b": torch.zeros(V)}
+    return {k: v.to(device) for k, v in ins.items()}, {k: v.to(device) for k, v in params.items()}
 
 
 def make_executor(ir, lowered, plan, device="cuda:0", require_kernel_id=True,

@@ -588,7 +588,7 @@ bool distill_sup(const TensorDesc* in, int ni, const TensorDesc* out, int no, co
   int64_t ld;
   if (!elem_kind(*c.z, &ek) || !matrix_ld(*c.z, false, &ld)) return false;
   const int64_t R = c.z->shape[0], V = c.z->shape[1];
-  if (R < 1 || V < 1 || R > INT32_MAX || V > INT32_MAX - (1 << 16)) return false;
+  if (R < 1 || V < 1 || R > INT32_MAX || V > (1 << 28)) return false;  // a row's byte offsets: 32 bits
   if (!elem_kind(*c.t, &tk) || !matrix_ld(*c.t, false, &ld)) return false;
   const int64_t K = c.t->shape[1];
   if (c.t->shape[0] != R || K < 1 || K > kMaxK) return false;

@@ -154,12 +154,14 @@ extern "C" {
  *   C [M, N] f32/f16/bf16; the scales as QUANT_FP8 writes them, each by rows
  *   or by blocks, with any strides; the f8 types of A and B may differ.
  *     C[m,n] = sum_b SA[m,b] SB[n,b] (sum over k in block b of A[m,k] B[n,k]) + bias[n]
- *   in f32, rounded once.  K >= 1; M = 0 or N = 0 writes nothing.
+ *   in f32, rounded once; for C of 16 bits the products of 8 consecutive K are
+ *   aligned to their largest and keep 13 bits below its exponent (the sum is off
+ *   by some 1e-5 of its terms' magnitude).  K >= 1; M = 0 or N = 0 writes nothing.
  *
- * DISTILL_TOPK: logits Z [R, V] f32/f16/bf16; teacher logits T [R, K] f32/f16/
- *   bf16 and their classes I [R, K] i32, 1 <= K <= 1024; labels [R] i32 and row
- *   weights w [R] f32, each optional (without weights: 1/R).  tau > 0 is the
- *   temperature, a in [0, 1] the weight of the labels' loss.
+ * DISTILL_TOPK: logits Z [R, V] f32/f16/bf16, R >= 1, V <= 2^28; teacher logits
+ *   T [R, K] f32/f16/bf16 and their classes I [R, K] i32, 1 <= K <= 1024; labels
+ *   [R] i32 and row weights w [R] f32, each optional (without weights: 1/R).
+ *   tau > 0 is the temperature, a in [0, 1] the weight of the labels' loss.
  *     p = softmax over the entries with 0 <= I < V of T / tau
  *     row loss = (1 - a) tau^2 KL(p || softmax(Z / tau)) + a CE(Z, label)
  *     loss [1] = sum_r w_r row_loss_r;   dlogits = d loss / d Z, in Z's type
@@ -169,7 +171,9 @@ extern "C" {
  *   read: its row loss and dlogits are 0.  A logit of -inf has probability 0;
  *   a row of nothing else gives NaN.  Outputs (loss, dlogits, row loss) or, for
  *   the loss alone, (loss, row loss); a last f32 output [R, P, 4], P >= 2, is
- *   scratch that lets P workgroups share a row where there are few rows.
+ *   scratch that lets P workgroups share a row where there are few rows.  What
+ *   scratch holds before and after a call means nothing; calls that may run at
+ *   the same time (two streams, two graphs) need scratch of their own.
  *
  * SAMPLE_ROW: logits Z [R, V] f32/f16/bf16, V <= 2^24; u, temperature, top_p,
  *   min_p [R] f32, top_k [R] i32 -> token [R] i32, optionally its
@@ -187,7 +191,8 @@ extern "C" {
  *   clamped to [0, 1 - 2^-24] (NaN: 0).  -inf and NaN logits are never drawn;
  *   a row of nothing else gives token -1 and log-probability -inf.  A third
  *   output, i32 [R, S] with S >= 8192, is scratch that lets several workgroups
- *   share a row where there are few rows.
+ *   share a row where there are few rows (used where S is even and its address a
+ *   multiple of 8).
  */
 
 /* GEPI epilogue kinds.  0..2 are the values core_v2/exec.py:223-252 packs;

@@ -11,9 +11,9 @@
 //           classes in their own order, passes u W
 //
 // Every cut is a prefix of the order, so what is kept is "composite <= limit"
-// (and w >= min_p).  A limit is found by a histogram of the row, its one bin
-// that holds the cut, and a sort of that bin's members (or of everything above
-// it, where that is little).
+// (and w >= min_p).  A limit is found by a histogram of the row, finer ones of
+// the bin that holds the cut, and the order of the last few by counting; where
+// little lies up to the cut, that alone is ordered and drawn from.
 //
 // A sum's rounding draws another token, so no sum is rounded: w is computed in
 // f64 and rounded once to a multiple of 2^-S, and the sums are 64-bit integers,
@@ -203,14 +203,14 @@ struct SampleRow {
       x = y;
     }
   }
-  // f(v, class) for every element that may be drawn and is no worse than v0.
-  template <typename F>
-  __device__ __forceinline__ void each_from(float v0, F f) const {
+  // f(v, class) for every element that may be drawn and is no worse than v0, until enough().
+  template <typename F, typename G>
+  __device__ __forceinline__ void each_from(float v0, F f, G enough) const {
     each_vec([&](int k, const float (&v)[8]) {
       float m = -INFINITY;
 #pragma unroll
       for (int e = 0; e < 8; ++e) m = fmaxf(m, v[e]);
-      if (!__any(m >= v0 && m > -INFINITY)) return;
+      if (!__any(m >= v0 && m > -INFINITY) || enough()) return;
 #pragma unroll
       for (int e = 0; e < 8; ++e)
       {
@@ -218,6 +218,11 @@ struct SampleRow {
         __builtin_amdgcn_sched_barrier(0);  // one element's work at a time: 64-bit weights take many registers
       }
     });
+  }
+
+  template <typename F>
+  __device__ __forceinline__ void each_from(float v0, F f) const {
+    each_from(v0, f, [] { return false; });
   }
 
   __device__ __forceinline__ u64 weight(float v) const {
@@ -369,9 +374,10 @@ struct SampleRow {
     return s.bi[2];
   }
 
-  // Fills list with the composites of the elements from v0 on that f accepts; how many those are.
+  // Fills list with the composites of the elements from v0 on that f accepts; how
+  // many those are, or more than most <= kList (and the rest is not looked at).
   template <typename F>
-  __device__ __forceinline__ int compact(float v0, F f) {
+  __device__ __forceinline__ int compact(float v0, F f, int most = kList) {
     __syncthreads();
     if (threadIdx.x == 0) s.bi[3] = 0;
     __syncthreads();
@@ -380,12 +386,12 @@ struct SampleRow {
         const int at = atomicAdd(&s.bi[3], 1);
         if (at < kList) s.list[at] = comp(v, c);
       }
-    });
+    }, [&] { return *const_cast<volatile int*>(&s.bi[3]) > most; });
     __syncthreads();
     return s.bi[3];
   }
 
-  // Histogram of what is kept over bin_of.
+  // Histogram of what is kept over bin_of: the counts or the masses.
   __device__ __forceinline__ void histogram(bool by_mass) {
     clear_hist(kBins);
     if (!by_mass) {
@@ -403,9 +409,7 @@ struct SampleRow {
       for (int e = 0; e < 8; ++e) {
         const u64 w = weight(v[e]);
         if (kept(v[e], cls(k) + e)) {
-          const int b = bin_of(v[e]);
-          atomicAdd(&s.cnt[b], 1u);
-          atomicAdd(&s.mass[b], w);
+          atomicAdd(&s.mass[bin_of(v[e])], w);
         }
         if (e & 1) __builtin_amdgcn_sched_barrier(0);
       }
@@ -417,10 +421,8 @@ struct SampleRow {
   // `cut` is the bin of bin_of that holds it.
   __device__ __forceinline__ void refine(bool by_mass, u64 target, Cut cut) {
     u64 cnt_before = cut.cnt_before, mass_before = cut.mass_before;
-    int m;
-    if (cut.n <= kList) {
-      m = compact(z_t, [&](float v, int c) { return bin_of(v) == cut.bin && kept(v, c); });
-    } else {
+    int m = compact(z_t, [&](float v, int c) { return bin_of(v) == cut.bin && kept(v, c); });
+    if (m > kList) {
       // the bin's members span composites [lo, hi]: 1024 bins over those, until one holds little
       u64 lo = ~0ull, hi_inv = ~0ull;
       each_from(z_t, [&](float v, int c) {
@@ -431,7 +433,7 @@ struct SampleRow {
         }
       });
       lo = block_min64(lo);
-      u64 hi = ~block_min64(hi_inv), n = cut.n;
+      u64 hi = ~block_min64(hi_inv), n = m;
       while (n > kList) {
         int shift = 64 - __clzll((long long)(hi - lo)) - 10;
         shift = shift < 0 ? 0 : shift;
@@ -448,8 +450,8 @@ struct SampleRow {
         cnt_before += k.cnt_before;
         mass_before += k.mass_before;
         n = k.n;
-        const u64 base = lo + ((u64)k.bin << shift), top = base + ((1ull << shift) - 1);
-        lo = base;
+        lo += (u64)k.bin << shift;
+        const u64 top = lo + ((1ull << shift) - 1);
         hi = top < hi ? top : hi;
       }
       m = compact(z_t, [&](float v, int c) {
@@ -457,17 +459,64 @@ struct SampleRow {
         return q >= lo && q <= hi;
       });
     }
-    sort_list(m);
-    int at;
-    if (by_mass) {
-      at = last_below(m, mass_before, target);
-    } else {
-      at = (int)(target - cnt_before) - 1;
-      at = at < m ? at : m - 1;
+    // of the list, what spans [lo, hi]: 1024 bins over those, until one holds few
+    u64 lo = ~0ull, hi_inv = ~0ull;
+    for (int i = threadIdx.x; i < m; i += NT) {
+      const u64 q = s.list[i];
+      lo = q < lo ? q : lo;
+      hi_inv = ~q < hi_inv ? ~q : hi_inv;
     }
-    const u64 q = s.list[at];
-    z_t = z_of_key(~(uint32_t)(q >> 32));
-    c_t = (int)(uint32_t)q;
+    lo = block_min64(lo);
+    u64 hi = ~block_min64(hi_inv);
+    for (int n = m; n > kPairs;) {
+      int shift = 64 - __clzll((long long)(hi - lo)) - 10;
+      shift = shift < 0 ? 0 : shift;
+      clear_hist(1024);
+      for (int i = threadIdx.x; i < m; i += NT) {
+        const u64 q = s.list[i];
+        if (q < lo || q > hi) continue;
+        const int b = (int)((q - lo) >> shift);
+        atomicAdd(&s.cnt[b], 1u);
+        if (by_mass) atomicAdd(&s.mass[b], weight(z_of_key(~(uint32_t)(q >> 32))));
+      }
+      const Cut k = find_bin(1024, by_mass, target - (by_mass ? mass_before : cnt_before));
+      cnt_before += k.cnt_before;
+      mass_before += k.mass_before;
+      n = k.n;
+      lo += (u64)k.bin << shift;
+      const u64 top = lo + ((1ull << shift) - 1);
+      hi = top < hi ? top : hi;
+    }
+    // those few, ordered by counting
+    __syncthreads();
+    u64* const few = s.seg;
+    u64* const w1 = s.seg + kPairs;
+    if (threadIdx.x == 0) s.bi[3] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < m; i += NT) {
+      const u64 q = s.list[i];
+      if (q < lo || q > hi) continue;
+      const int at = atomicAdd(&s.bi[3], 1);
+      few[at] = q;
+      w1[at] = by_mass ? weight(z_of_key(~(uint32_t)(q >> 32))) : 0;
+    }
+    __syncthreads();
+    const int n = s.bi[3], t = threadIdx.x, some = (t & ~63) < n ? n : 0;
+    const u64 q = t < n ? few[t] : ~0ull;
+    u64 run = mass_before;
+    int rank = 0;
+#pragma unroll 4
+    for (int j = 0; j < some; ++j) {
+      const bool before = few[j] < q;
+      rank += before;
+      run += before ? w1[j] : 0;
+    }
+    if (t < n && (by_mass ? run < target && (run + w1[t] >= target || rank == n - 1)
+                          : rank == (int)min((int64_t)(target - cnt_before), (int64_t)n) - 1))
+      s.b64[2] = q;
+    __syncthreads();
+    z_t = z_of_key(~(uint32_t)(s.b64[2] >> 32));
+    c_t = (int)(uint32_t)s.b64[2];
     __syncthreads();
   }
 
@@ -691,9 +740,6 @@ struct SampleRow {
       __syncthreads();
       m = last_below(m, 0, (u64)ceil((double)top_p * (double)total)) + 1;
     }
-    cut_min_p(m, least);
-  }
-  __device__ __forceinline__ void cut_min_p(int m, u64 least) {
     if (least) {  // the weights fall along the order
       int n = 0;
       for (int j = threadIdx.x; j < m; j += NT)
@@ -806,14 +852,12 @@ struct SampleRow {
       if (!made) histogram(by_mass);
       const u64 target = by_mass ? mass_target(q.top_p) : (u64)q.top_k;
       const Cut cut = find_bin(kBins, by_mass, target);
-      if (cut.cnt_before + cut.n <= kList) {
-        // little lies up to the cut: all of it, sorted
-        int m = compact(z_t, [&](float v, int c) { return bin_of(v) <= cut.bin && kept(v, c); });
-        if (!by_mass) return finish_top_k(m, q);
-        if (m <= kPairs) return finish_pairs(m, false, 0, true, q.top_p, target, q.least);
-        sort_list(m);
-        m = last_below(m, 0, target) + 1;
-        return cut_min_p(m, q.least);
+      // what lies up to the cut, if that is little
+      const int most = by_mass ? kPairs : kList;
+      if (by_mass || cut.cnt_before + cut.n <= kList) {
+        const int m = compact(z_t, [&](float v, int c) { return bin_of(v) <= cut.bin && kept(v, c); }, most);
+        if (m <= most)
+          return by_mass ? finish_pairs(m, false, 0, true, q.top_p, target, q.least) : finish_top_k(m, q);
       }
       refine(by_mass, target, cut);
     }
@@ -855,11 +899,11 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
 //      overflowed, or a nucleus of many classes, as without scratch)
 // Scratch, in words: 0 the list's count; 16 + 20 q the q-th workgroup's (0: the
 // first class of its maximum, 4 ..: the groups' maxima); 2048 the list, the
-// histogram's masses and counts, or the segments' sums.
+// histogram's masses, or the segments' sums.
 // ---------------------------------------------------------------------------
 constexpr int kPartNT = 256, kPartWords = 20, kPartAt = 16, kDataAt = 2048;
 static_assert(kPartAt + 64 * kPartWords <= kDataAt, "scratch");
-static_assert(kDataAt + kBins * 3 <= 8192 && kDataAt + kList * 2 <= 8192 && kDataAt + kSegs * 2 <= 8192, "scratch");
+static_assert(kDataAt + kBins * 2 <= 8192 && kDataAt + kList * 2 <= 8192 && kDataAt + kSegs * 2 <= 8192, "scratch");
 
 // Classes of a part: whole segments of 512.  Of ceil(V / part_len(V, P)) parts,
 // only the last may have fewer.
@@ -881,7 +925,7 @@ __global__ __launch_bounds__(kPartNT) void sample_part_max_kernel(SampleArgs a, 
   uint32_t* row = scratch + (int64_t)r * lds;
   if (q == 0 && threadIdx.x == 0) row[0] = 0;
   if (set.by_p && !set.by_k)
-    for (int i = q * kPartNT + threadIdx.x; i < kBins * 3; i += P * kPartNT) row[kDataAt + i] = 0;
+    for (int i = q * kPartNT + threadIdx.x; i < kBins * 2; i += P * kPartNT) row[kDataAt + i] = 0;
   const float own = part.lane_max();
   uint32_t* out = row + kPartAt + q * kPartWords;
   float w = own;
@@ -967,12 +1011,8 @@ __global__ __launch_bounds__(kPartNT) void sample_part_kernel(SampleArgs a, uint
   } else if (set.by_p) {
     part.histogram(true);
     __syncthreads();
-    uint32_t* cnt = reinterpret_cast<uint32_t*>(data + kBins);
     for (int i = threadIdx.x; i < kBins; i += kPartNT)
-      if (sl.cnt[i]) {
-        atomicAdd(cnt + i, sl.cnt[i]);
-        atomicAdd(data + i, sl.mass[i]);
-      }
+      if (sl.mass[i]) atomicAdd(data + i, sl.mass[i]);
   } else {
     part.segment_sums(set.least, 1);
     const int nseg = (c1 - c0 + 511) / 512;
@@ -1012,11 +1052,7 @@ __global__ __launch_bounds__(1024) void sample_join_kernel(SampleArgs a, const u
     return whole.finish_top_k((int)m, set);
   }
   if (set.by_p) {
-    const uint32_t* cnt = reinterpret_cast<const uint32_t*>(data + kBins);
-    for (int i = threadIdx.x; i < kBins; i += NT) {
-      sl.cnt[i] = cnt[i];
-      sl.mass[i] = data[i];
-    }
+    for (int i = threadIdx.x; i < kBins; i += NT) sl.mass[i] = data[i];
     __syncthreads();
     return whole.cut_and_draw(set, true);
   }

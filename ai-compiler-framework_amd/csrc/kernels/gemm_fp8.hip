@@ -291,8 +291,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_fp8_lds_kernel(Fp8Gemm p
   // scales: wave w fetches those of rows 64 w .. of the tile's A rows and then B
   // rows; waves beyond them repeat the last ones, so that every wave has the
   // same loads in flight
-  constexpr int SW = (BM + BN) / 64, NVM = PA + PB + 1;
-  static_assert(BM + BN <= T && BM % 64 == 0 && BN % 64 == 0 && PA * NW * 8 == BM && PB * NW * 8 == BN,
+  constexpr int SBM = (BM + 63) / 64 * 64;  // (a tile of 32 rows: as for 64)
+  constexpr int SW = (SBM + BN) / 64, NVM = PA + PB + 1;
+  static_assert(SBM + BN <= T && BN % 64 == 0 && PA * NW * 8 == BM && PB * NW * 8 == BN,
                 "whole loads a wave");
   static_assert(S >= 2 && (S - 1) * NVM < 64, "loads in flight are counted in 6 bits");
   __shared__ __attribute__((aligned(1024))) uint8_t smem[S * STAGE];
@@ -319,8 +320,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_fp8_lds_kernel(Fp8Gemm p
     const int row = (wave + i * NW) * 8 + (lane >> 3);
     vb[i] = min(row, last_b) * (int)p.ldb + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
   }
-  const bool of_a = wave < BM / 64;
-  const int srow = (of_a ? wave : min(wave - BM / 64, BN / 64 - 1)) * 64 + lane;
+  const bool of_a = wave < SBM / 64;
+  const int srow = (of_a ? wave : min(wave - SBM / 64, BN / 64 - 1)) * 64 + lane;
   const int64_t s_first = of_a ? (int64_t)(m0 >> p.sa_sh) * p.sa_r : (int64_t)(n0 >> p.sb_sh) * p.sb_r;
   const i32x4_t rsrc_s = buffer_rsrc((of_a ? p.SA : p.SB) + s_first, 0x7fffffffu);
   const int s_step = of_a ? (int)p.sa_c * 4 : (int)p.sb_c * 4;
@@ -382,12 +383,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_fp8_lds_kernel(Fp8Gemm p
     if constexpr (BROW) {
 #pragma unroll
       for (int i = 0; i < TN; ++i) {
-        const f32x4 v = *reinterpret_cast<const f32x4*>(sl + BM + (wn * TN + i) * 16 + 4 * g);
+        const f32x4 v = *reinterpret_cast<const f32x4*>(sl + SBM + (wn * TN + i) * 16 + 4 * g);
 #pragma unroll
         for (int e = 0; e < 4; ++e) fb[i * 4 + e] = v[e];
       }
     } else {
-      fb[0] = sl[BM + wn * TN * 16];
+      fb[0] = sl[SBM + wn * TN * 16];
     }
     f32x4 d[2][TN];
     float fa[2];
@@ -463,11 +464,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_fp8_lds_kernel(Fp8Gemm p
     for (int row = t >> 3; row < BN; row += T / 8)
       *reinterpret_cast<u32x4_t*>(st + BM * 128 + stage_byte(row, c)) =
           load_chunk(p.B + (int64_t)min(n0 + row, p.N - 1) * p.ldb, nfull * 128 + c * 16, p.K);
-    if (t < BM + BN) {
-      const bool ra = t < BM;
+    if (t < SBM + BN) {
+      const bool ra = t < SBM;
       scales[stage_of(nfull)][t] =
           ra ? p.SA[(int64_t)((m0 + min(t, last_a)) >> p.sa_sh) * p.sa_r + nfull * p.sa_c]
-             : p.SB[(int64_t)((n0 + min(t - BM, last_b)) >> p.sb_sh) * p.sb_r + nfull * p.sb_c];
+             : p.SB[(int64_t)((n0 + min(t - SBM, last_b)) >> p.sb_sh) * p.sb_r + nfull * p.sb_c];
     }
     __syncthreads();
 #pragma unroll
@@ -684,24 +685,38 @@ Status run_tiles(Fp8Gemm& p, hipStream_t s) {
 
 template <int AF, int BF>
 Status gemm_fp8_run(Fp8Gemm& p, hipStream_t s) {
-  if (p.M <= 32) {
-    const unsigned g = (unsigned)(((int64_t)p.N + 15) / 16);
-    auto go = [&](auto tm) {
-      constexpr int TM = decltype(tm)::value;
-      if (p.sb_sh == 0) gemm_fp8_rows_kernel<TM, 8, AF, BF, true><<<g, 512, 0, s>>>(p);
-      else gemm_fp8_rows_kernel<TM, 8, AF, BF, false><<<g, 512, 0, s>>>(p);
-    };
-    if ((int64_t)g * 512 > UINT32_MAX) return Status::InvalidArgument;
-    if (p.M <= 16) go(std::integral_constant<int, 1>{});
-    else go(std::integral_constant<int, 2>{});
-    return launch_status("gemm_fp8");
-  }
   // straight into LDS: 16-byte aligned rows, a tile's bytes and scales within
   // 32-bit offsets, two blocks of K at least
   const int64_t nkb = (p.K + 127) / 128, lim = 1 << 22;
   const bool lds = aligned(p.A, 16) && aligned(p.B, 16) && p.lda % 16 == 0 && p.ldb % 16 == 0 && p.lda < lim &&
                    p.ldb < lim && p.sa_r < (lim >> 2) && p.sb_r < (lim >> 2) && nkb * p.sa_c < (1 << 26) &&
                    nkb * p.sb_c < (1 << 26) && p.K >= 256;
+  if (p.M <= 32) {
+    // Few columns: workgroups of 16 (or where tiles do not go straight into LDS).
+    // From about two of those a CU on the tiles are the faster ones: 1 x 4096 x
+    // 4096 4.9 us (tiles 8.8), 32 x 4096 x 4096 f32 9.6 (11.7), 16 x 8192 x 4096
+    // f32 11.3 (11.6), 1 x 11008 x 4096 13.3 (9.0), 1 x 32000 x 4096 f32 32.1
+    // (21.3), 32 rows 58.8 (21.4).
+    const unsigned g = (unsigned)(((int64_t)p.N + 15) / 16);
+    const int64_t work = (int64_t)g * (p.M <= 16 ? 1 : 2);
+    if (lds && work > 512) {
+      if (p.out == EL_F32) return run_tiles<4, true, 32, 64, 2, 2, AF, BF>(p, s);
+      return run_tiles<4, false, 32, 64, 2, 2, AF, BF>(p, s);
+    }
+    if ((int64_t)g * 512 > UINT32_MAX) return Status::InvalidArgument;
+    auto go = [&](auto tm) {
+      constexpr int TM = decltype(tm)::value;
+      if (p.sb_sh == 0) gemm_fp8_rows_kernel<TM, 8, AF, BF, true><<<g, 512, 0, s>>>(p);
+      else gemm_fp8_rows_kernel<TM, 8, AF, BF, false><<<g, 512, 0, s>>>(p);
+    };
+    if (p.M <= 16) go(std::integral_constant<int, 1>{});
+    else go(std::integral_constant<int, 2>{});
+    return launch_status("gemm_fp8");
+  }
+  // Larger tiles where they fill the chip.  64 x 64 against 128 x 128: 256 x 4096
+  // x 4096 bf16 11.5 us (22.0), 512 19.9 (24.0), 1024 32.9 (26.9); 1001 x 1003 x
+  // 784 f16 6.6 (11.3).  128 x 128 against 256 x 256: 2048 x 4096 x 4096 40.2
+  // (53.6), 4096 78.1 (63.4).
   auto tiles = [&](int64_t b) { return ((p.M + b - 1) / b) * ((p.N + b - 1) / b); };
   if (p.out == EL_F32) {
     if (!lds) return run_tiles<0, true, 128, 128, 2, 2, AF, BF>(p, s);

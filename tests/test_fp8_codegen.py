@@ -51,8 +51,8 @@ def asm_loads(body):
 
 
 def test_every_form_is_there(bodies):
-    # 4 pairs of types, scales of B by rows or blocks; f32 outputs 2 tiles, 16-bit ones 3
-    assert len(bodies) == 4 * 2 * 5
+    # 4 pairs of types, scales of B by rows or blocks; f32 outputs 3 tiles, 16-bit ones 4
+    assert len(bodies) == 4 * 2 * 7
 
 
 def test_no_spills(bodies):

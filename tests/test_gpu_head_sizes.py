@@ -11,7 +11,7 @@ import torch
 
 import head_ref as ref
 from aicf_cuda import abi
-from test_gpu_fp8 import DT, QFP8, codes
+from test_gpu_fp8 import DT, QFP8, check_gemm, codes
 from test_gpu_head import check, distill, student
 from test_head_ops import DISTILL, I32, At, refused
 
@@ -99,6 +99,16 @@ def test_sample_shared_rows_of_equal_logits(C, dev):
         want = [ref.sample(z[i], u[i].item(), *as_f32(s))[0] for i in range(6)]
         for scratch in (0, 8192):
             assert draw(C, dev, z.to(dev), u, sets, scratch)[0].tolist() == want, s
+
+
+@gpu
+@pytest.mark.parametrize("m,n,k", [(1, 8192, 256), (1, 8208, 272), (16, 8209, 256), (17, 4096, 300), (17, 4112, 300),
+                                   (32, 4100, 1023), (32, 9001, 512), (33, 4100, 256), (5, 16384, 255)])
+def test_gemm_of_few_rows(C, dev, m, n, k):
+    """Workgroups of 16 columns, and tiles of 32 rows from some hundreds of those on."""
+    for out, b_by in (("f32", "rows"), ("bf16", "blocks"), ("f16", "rows")):
+        check_gemm(C, dev, m, n, k, b_by=b_by, out=out, bias=out != "f32", pad=-k % 16, cpad=1)
+    check_gemm(C, dev, m, n, k, "e5m2", a_by="blocks", out="f32", pad=-k % 16, s_t=True)
 
 
 FAR = 1_200_000_000  # elements between rows: the third starts beyond 2^31 of them

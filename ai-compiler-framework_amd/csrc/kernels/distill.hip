@@ -638,14 +638,16 @@ DistillArgs from_row(const DistillArgs& a, int tk, int64_t r, int64_t rows) {
 
 template <int EK, bool DUAL>
 Status distill_rows(const DistillArgs& a, int tk, float* scratch, int ldp, hipStream_t s) {
-  // Few rows share the chip: parts of 2048 columns or more, about two
-  // workgroups a CU.
+  // Few long rows share the chip: parts of 2048 columns or more, about two
+  // workgroups a CU.  A row a workgroup against this: 8 x 200000 bf16 34.3 us
+  // (15.2), 8 x 65536 15.4 (13.8), f32 20.2 (13.6), 48 x 131072 22.3 (21.3); the
+  // other way 8 x 32000 f32 12.8 (15.1), 128 x 131072 f32 47.1 (51.3).
   const unsigned lds = special_bytes(a.K);
   int64_t P = (512 + a.R - 1) / a.R;
   if (P > a.V / 2048) P = a.V / 2048;
   if (P > ldp) P = ldp;
   if (P > 64) P = 64;
-  if (scratch && a.R < 256 && P >= 4) {
+  if (scratch && a.R <= 48 && a.V >= 49152 && P >= 4) {  // (a row's last words are in the fourth part's floats)
     const dim3 grid((unsigned)P, (unsigned)a.R);
     const int64_t len = (a.V + P - 1) / P + 7;
     auto go = [&](auto vpt) {

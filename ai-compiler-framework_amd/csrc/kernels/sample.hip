@@ -1086,12 +1086,17 @@ bool sample_sup(const TensorDesc* in, int ni, const TensorDesc* out, int no, con
 template <int EK>
 Status sample_run(const SampleArgs& a, uint32_t* scratch, int64_t lds, hipStream_t s) {
   const unsigned g = (unsigned)a.R;
-  // Few rows share the chip: parts of 2048 classes or more, about one workgroup
-  // a CU.
+  // Few long rows share the chip: parts of 2048 classes or more, about one
+  // workgroup a CU.  A row a workgroup against this, bf16: plain draws 1 x 40000
+  // 23.9 us (15.2), 1 x 262144 93.1 (15.2), 32 x 65536 32.2 (17.8); top-p 0.9 1 x
+  // 262144 257.6 (180.5), 32 x 65536 87.5 (78.4); top-k 50 32 x 131072 27.3 (25.5),
+  // 1 x 40000 17.6 (23.3), 64 x 131072 27.8 (42.2).  The settings are on the
+  // device; below 32768 classes and beyond 32 rows top-k loses more than others
+  // gain.
   int P = 256 / a.R;
   if (P > a.V / 2048) P = a.V / 2048;
   if (P > 64) P = 64;
-  if (scratch && P >= 4 && a.V <= 512 * kSegs) {
+  if (scratch && a.R <= 32 && a.V >= 32768 && a.V <= 512 * kSegs) {
     P = (a.V + part_len(a.V, P) - 1) / part_len(a.V, P);
     const dim3 grid((unsigned)P, g);
     sample_part_max_kernel<EK><<<grid, kPartNT, 0, s>>>(a, scratch, lds, P);

@@ -240,8 +240,10 @@ def build_mlp_distill(B: int, din: int, dh: int, V: int, K: int, *, tau: float =
     top_k = nv("top_k", (B,), I32)
     W1, b1, W2, b2 = nv("1.W", (dh, din)), nv("1.b", (dh,)), nv("2.W", (V, dh)), nv("2.b", (V,))
     z, h, logits = nv("z1", (B, dh), BF16), nv("h1", (B, dh), BF16), nv("logits", (B, V), BF16)
-    token, logprob, draw_ws = nv("token", (B,), I32), nv("logprob", (B,)), nv("draw.ws", (B, 8192), I32)
-    loss, row_loss, loss_ws = nv("loss", (1,)), nv("row_loss", (B,)), nv("loss.ws", (B, 64, 4))
+    token, logprob, loss, row_loss = nv("token", (B,), I32), nv("logprob", (B,)), nv("loss", (1,)), nv("row_loss", (B,))
+    # few rows are shared by workgroups
+    draw_ws = [nv("draw.ws", (B, 8192), I32)] if B <= 32 else []
+    loss_ws = [nv("loss.ws", (B, 64, 4))] if B <= 48 else []
     dY, dh_, dz = nv("dY", (B, V), BF16), nv("d_h1", (B, dh), BF16), nv("d_z1", (B, dh), BF16)
     dW1, db1, dW2, db2 = (nv(f"d_{p.name}", p.shape) for p in (W1, b1, W2, b2))
     step = nv("opt.step", (), I32)
@@ -252,8 +254,8 @@ def build_mlp_distill(B: int, din: int, dh: int, V: int, K: int, *, tau: float =
     ir.emit(op="LinearFp8", inputs=[x, W1, b1], outputs=[z] + xq[:2] + w1q + xq[2:], attrs=lin)
     ir.emit(op="Gelu", inputs=[z], outputs=[h])
     ir.emit(op="LinearFp8", inputs=[h, W2, b2], outputs=[logits] + hq[:2] + w2q[:2] + hq[2:] + w2q[2:], attrs=lin)
-    ir.emit(op="SampleRow", inputs=[logits, u, temp, top_k, top_p, min_p], outputs=[token, logprob, draw_ws])
-    ir.emit(op="DistillTopk", inputs=[logits, teacher, ids, t], outputs=[loss, dY, row_loss, loss_ws],
+    ir.emit(op="SampleRow", inputs=[logits, u, temp, top_k, top_p, min_p], outputs=[token, logprob] + draw_ws)
+    ir.emit(op="DistillTopk", inputs=[logits, teacher, ids, t], outputs=[loss, dY, row_loss] + loss_ws,
             attrs={"temperature": tau, "label_weight": label_weight})
     ir.emit(op="LinearFp8Bwd", inputs=[dY] + hq[2:] + w2q[2:], outputs=[dW2] + yq + [db2, dh_], attrs=lin)
     ir.emit(op="GeluBwd", inputs=[dh_, z], outputs=[dz])

@@ -171,9 +171,9 @@ extern "C" {
  *   read: its row loss and dlogits are 0.  A logit of -inf has probability 0;
  *   a row of nothing else gives NaN.  Outputs (loss, dlogits, row loss) or, for
  *   the loss alone, (loss, row loss); a last f32 output [R, P, 4], P >= 2, is
- *   scratch that lets P workgroups share a row where there are few rows.  What
- *   scratch holds before and after a call means nothing; calls that may run at
- *   the same time (two streams, two graphs) need scratch of their own.
+ *   scratch that lets P workgroups (4 to 64) share a row where there are few long
+ *   rows.  What scratch holds before and after a call means nothing; calls that
+ *   may run at the same time (two streams, two graphs) need scratch of their own.
  *
  * SAMPLE_ROW: logits Z [R, V] f32/f16/bf16, V <= 2^24; u, temperature, top_p,
  *   min_p [R] f32, top_k [R] i32 -> token [R] i32, optionally its
@@ -191,8 +191,8 @@ extern "C" {
  *   clamped to [0, 1 - 2^-24] (NaN: 0).  -inf and NaN logits are never drawn;
  *   a row of nothing else gives token -1 and log-probability -inf.  A third
  *   output, i32 [R, S] with S >= 8192, is scratch that lets several workgroups
- *   share a row where there are few rows (used where S is even and its address a
- *   multiple of 8).
+ *   share a row where there are few long rows (used where S is even and its
+ *   address a multiple of 8).
  */
 
 /* GEPI epilogue kinds.  0..2 are the values core_v2/exec.py:223-252 packs;

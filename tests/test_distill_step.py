@@ -57,14 +57,16 @@ def gelu_grad(z):
 
 
 @pytest.mark.gpu
-def test_step_eager_and_replayed():
-    ir, low, plan = build_mlp_distill(**SIZES, tau=2.0, label_weight=0.25)
-    B, V = SIZES["B"], SIZES["V"]
+@pytest.mark.parametrize("sizes", [SIZES, dict(B=50, din=128, dh=96, V=300, K=4),
+                                   dict(B=5, din=64, dh=130, V=50021, K=33)])
+def test_step_eager_and_replayed(sizes):
+    ir, low, plan = build_mlp_distill(**sizes, tau=2.0, label_weight=0.25)
+    B = sizes["B"]
     outs = ("token", "logprob", "loss", "row_loss", "dY", "d_1.W", "d_2.W", "d_1.b", "d_2.b")
 
     def states(replayed):
         """The values of three steps and the parameters after them."""
-        ins, params = init_mlp_distill(**SIZES)
+        ins, params = init_mlp_distill(**sizes)
         first = {k: v.clone() for k, v in params.items()}
         ex = make_executor(ir, low, plan, own_graph=True)
         if replayed:

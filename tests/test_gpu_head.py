@@ -73,7 +73,7 @@ def test_distill_masks_and_repeats(C, dev):
     """Rows without a teacher, without a label, with neither; the same class
     twice, with a label among the teacher's; classes out of range; -inf
     logits; rows of weight 0, whose logits may be anything."""
-    for v, dtype in ((300, "f32"), (9001, "bf16")):
+    for v, dtype in ((300, "f32"), (9001, "bf16"), (50001, "bf16")):
         r, k = 8, 6
         z, t, ids, g = student(r, v, k, dtype, 11)
         labels = torch.tensor([0, 5, -1, v, v - 1, 3, 2, 1], dtype=torch.int32)
@@ -96,14 +96,15 @@ def test_distill_masks_and_repeats(C, dev):
 
 
 def test_distill_row_of_nothing_is_nan(C, dev):
-    z, t, ids, _ = student(3, 500, 4, "f32", 2)
-    z[1] = -math.inf
-    for scratch in (0, 8):
-        loss, dz, rl = distill(C, dev, z, t, ids, 1.0, 0.0, scratch=scratch)
-        assert dz[1].isnan().all() and rl[1].isnan() and not dz[[0, 2]].isnan().any()
+    for v in (500, 50000):
+        z, t, ids, _ = student(3, v, 4, "f32", 2)
+        z[1] = -math.inf
+        for scratch in (0, 8):
+            loss, dz, rl = distill(C, dev, z, t, ids, 1.0, 0.0, scratch=scratch)
+            assert dz[1].isnan().all() and rl[1].isnan() and not dz[[0, 2]].isnan().any()
 
 
-@pytest.mark.parametrize("v", [77, 4096, 12289])
+@pytest.mark.parametrize("v", [77, 4096, 12289, 50003])
 def test_distill_in_place_loss_alone_and_repeated(C, dev, v):
     z, t, ids, g = student(5, v, 33, "bf16", v)
     labels = torch.randint(0, v, (5,), generator=g, dtype=torch.int32)
@@ -140,9 +141,10 @@ def test_distill_gradient_against_differences(C, dev):
 
 
 def test_distill_captured(C, dev):
-    z, t, ids, g = student(6, 9000, 20, "f32", 4)
+    v = 50009
+    z, t, ids, g = student(6, v, 20, "f32", 4)
     zd, td, idd = z.to(dev), t.to(dev), ids.to(dev)
-    loss, dz, rl, sc = (torch.empty(s, device=dev) for s in ((1,), (6, 9000), (6,), (6, 16, 4)))
+    loss, dz, rl, sc = (torch.empty(s, device=dev) for s in ((1,), (6, v), (6,), (6, 16, 4)))
 
     def call(stream=0):
         C.op_call(C.OpKind.DistillTopk, [zd, td, idd], [loss, dz, rl, sc], DTOP, struct.pack("<ff", 1.0, 0.0), stream)
@@ -151,7 +153,7 @@ def test_distill_captured(C, dev):
     call(C.graph_begin_h(h))
     C.graph_end_h(h)
     for i in range(4):
-        zd.copy_(torch.randn((6, 9000), generator=g) * 2)
+        zd.copy_(torch.randn((6, v), generator=g) * 2)
         C.graph_launch_h(h)
         got = [x.clone() for x in (loss, dz, rl)]
         torch.cuda.synchronize()
@@ -219,7 +221,7 @@ def test_sample_ties_and_flat_rows(C, dev, v):
 
 def test_sample_not_finite_and_edges(C, dev):
     inf, nan = math.inf, math.nan
-    for v in (6, 10007):
+    for v in (6, 10007, 40009):
         base = torch.full((9, v), -inf)
         base[1, 3] = -50.0
         base[2, :] = nan
@@ -251,7 +253,7 @@ def test_sample_draws_every_class_at_its_share(C, dev):
 
 def test_sample_captured_and_without_log_probability(C, dev):
     g = torch.Generator().manual_seed(6)
-    r, v = 4, 30000
+    r, v = 4, 34000
     z = torch.empty((r, v), device=dev)
     u, temp, p, m = (torch.empty(r, device=dev) for _ in range(4))
     k = torch.full((r,), 20, device=dev, dtype=torch.int32)

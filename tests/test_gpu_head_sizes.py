@@ -35,10 +35,11 @@ def test_distill_row_forms(C, dev, v, dtype):
 
 
 @gpu
-@pytest.mark.parametrize("r,p", [(1, 2), (1, 64), (3, 5), (40, 64), (255, 64), (256, 64)])
-def test_distill_shared_rows(C, dev, r, p):
+@pytest.mark.parametrize("r,p,v", [(1, 2, 49152), (1, 64, 49151), (3, 5, 50021), (1, 64, 70000), (40, 64, 49153),
+                                   (48, 3, 49999), (49, 64, 49999)])
+def test_distill_shared_rows(C, dev, r, p, v):
     """A row shared by as many workgroups as the scratch and the rows allow."""
-    z, t, ids, _ = student(r, 9000, 4, "bf16", r)
+    z, t, ids, _ = student(r, v, 4, "bf16", r)
     check(distill(C, dev, z, t, ids, 1.0, 0.0, scratch=p), z, t, ids, 1.0, 0.0)
 
 
@@ -63,7 +64,8 @@ def as_f32(s):
 
 
 @gpu
-@pytest.mark.parametrize("v,dtype", [(8191, "f32"), (8192, "bf16"), (8193, "f32"), (32003, "f16"), (131072, "bf16"),
+@pytest.mark.parametrize("v,dtype", [(8191, "f32"), (8192, "bf16"), (8193, "f32"), (32003, "f16"), (32768, "f16"), (50021, "bf16"), (131072, "bf16"),
+
                                      (524288, "f32"), (524289, "bf16"), (1500001, "f32")])
 def test_sample_forms(C, dev, v, dtype):
     """Rows of all settings together, whole and shared by workgroups."""
@@ -109,6 +111,101 @@ def test_gemm_of_few_rows(C, dev, m, n, k):
     for out, b_by in (("f32", "rows"), ("bf16", "blocks"), ("f16", "rows")):
         check_gemm(C, dev, m, n, k, b_by=b_by, out=out, bias=out != "f32", pad=-k % 16, cpad=1)
     check_gemm(C, dev, m, n, k, "e5m2", a_by="blocks", out="f32", pad=-k % 16, s_t=True)
+
+
+@gpu
+def test_many_rows(C, dev):
+    """More rows than one launch takes, than a grid has workgroups for in one pass."""
+    g = torch.Generator(device=dev).manual_seed(5)
+    rnd = lambda *s: torch.randn(s, device=dev, generator=g)  # noqa: E731
+    r, v = (1 << 21) + 5, 4
+    z, t = rnd(r, v), rnd(r, 1)
+    ids = torch.randint(-1, v, (r, 1), device=dev, generator=g).to(torch.int32)
+    labels = torch.randint(-1, v + 1, (r,), device=dev, generator=g).to(torch.int32)
+    w = torch.rand(r, device=dev, generator=g)
+    loss, dz, rl = torch.empty(1, device=dev), torch.empty_like(z), torch.empty(r, device=dev)
+    C.op_call(C.OpKind.DistillTopk, [z, t, ids, labels, w], [loss, dz, rl], DTOP, struct.pack("<ff", 1.0, 0.25))
+    q = torch.log_softmax(z.double(), -1)
+    col = torch.arange(v, device=dev)
+    soft, hard = (ids >= 0), (labels >= 0)[:, None] & (labels < v)[:, None]
+    at_t, at_l = (col == ids).double(), (col == labels[:, None]).double()
+    want = w.double()[:, None] * (0.75 * soft * (q.exp() - at_t) + 0.25 * hard * (q.exp() - at_l))
+    rows = -0.75 * (q * at_t).sum(-1) - 0.25 * (q * at_l).sum(-1)
+    rows[w == 0] = 0  # (a row of weight 0 is left out: there is one)
+    # terms of at most 1, some ten roundings each; a row's loss: log q of at most 12, as many
+    assert ((dz.double() - want).abs() <= 16 * ref.U * w.double()[:, None]).all()
+    assert ((rl.double() - rows).abs() <= 16 * ref.U * (rows + 1)).all()
+    # the weighted rows are added in 64 bits
+    total = (w.double() * rows).sum()
+    assert abs(loss.item() - total) <= 16 * ref.U * (w.double() * (rows + 1)).sum() + ref.U * total
+
+    x = rnd(5_000_001, 3)
+    out, s = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev), torch.empty((x.shape[0], 1), device=dev)
+    C.op_call(C.OpKind.QuantFp8, [x], [out, s], QFP8, struct.pack("<i", 0))
+    for part in (slice(0, 1000), slice(4_999_001, None)):
+        wq, ws = ref.quant(x[part].cpu(), "e4m3", "rows", False)
+        assert torch.equal(out[part].cpu().view(torch.uint8), wq.view(torch.uint8)) and torch.equal(s[part].cpu(), ws)
+    assert ((out.float() * s - x).abs() <= 2.0 ** -4 * x.abs() * (1 + 8 * ref.U) + 2.0 ** -10 * s).all()
+
+    r = 100_003
+    z, u = rnd(r, 3), torch.rand(r, device=dev, generator=g)
+    one = torch.ones(r, device=dev)
+    tok = torch.empty(r, dtype=torch.int32, device=dev)
+    C.op_call(C.OpKind.SampleRow, [z, u, one, torch.zeros_like(tok), one, 0 * one], [tok])
+    cum = torch.softmax(z.double(), -1).cumsum(-1)
+    want = (cum[:, :2] <= u.double()[:, None]).sum(-1)
+    near = ((cum[:, :2] - u.double()[:, None]).abs() < 1e-12).any(-1)  # (64-bit sums either way there)
+    assert (near | (tok == want)).all()
+
+
+@gpu
+@pytest.mark.parametrize("m,n,k", [(70001, 1, 272), (1, 70001, 272), (33, 1, 256), (2, 1, 300)])
+def test_gemm_of_one_row_or_column(C, dev, m, n, k):
+    for out in ("f32", "bf16"):
+        check_gemm(C, dev, m, n, k, b_by="rows", out=out, bias=True, pad=-k % 16)
+
+
+@gpu
+def test_scales_of_any_strides(C, dev):
+    """One scale for all blocks, scales shared by rows, every second word; the same matrix as both operands."""
+    g = torch.Generator().manual_seed(4)
+    for m, k in ((9, 300), (200, 512)):
+        a, sa, ad, sad = codes(m, k, "e4m3", "rows", g, dev, -k % 16)
+        nb = ref.blocks(k)
+        wide = torch.rand((m, 2 * nb), generator=g).to(dev)
+        for s in (torch.full((1, 1), 0.5, device=dev).expand(m, nb), sad[:1].expand(m, nb), sad[:, :1].expand(m, nb),
+                  wide[:, ::2]):
+            c = torch.empty((m, m), device=dev)
+            C.op_call(C.OpKind.GemmFp8, [ad, s, ad, s], [c])
+            want, mag = ref.gemm(a, s.cpu(), a, s.cpu())
+            assert ((c.cpu().double() - want).abs() <= ref.gemm_bound(want, mag, k, torch.float32)).all()
+    for by in ("rows", "blocks"):  # scales written column by column, with a gap
+        x = torch.randn((130, 500), generator=g)
+        f = (lambda n: n) if by == "rows" else ref.blocks
+        q, qt = (torch.empty(s, dtype=torch.float8_e5m2, device=dev) for s in ((130, 500), (500, 130)))
+        s, st = (torch.full((b, r + 3), math.nan, device=dev).t()[:r] for b, r in ((4, f(130)), (2, f(500))))
+        for outs in ([q, s], [q, s, qt, st]):
+            C.op_call(C.OpKind.QuantFp8, [x.to(dev)], outs, QFP8, struct.pack("<i", 1))
+            for i, y in enumerate((x, x.t().contiguous())[:len(outs) // 2]):
+                wq, ws = ref.quant(y, "e5m2", by, True)
+                assert torch.equal(outs[2 * i].cpu().view(torch.uint8), wq.view(torch.uint8))
+                assert torch.equal(outs[2 * i + 1].cpu(), ws)
+                behind = torch.as_strided(outs[2 * i + 1], (3, ws.shape[1]), outs[2 * i + 1].stride(), ws.shape[0])
+                assert behind.isnan().all()
+
+
+@gpu
+def test_distill_of_rows_that_share_logits(C, dev):
+    """Logits, teacher and classes of one row for all (row stride 0)."""
+    for v in (700, 50001):
+        z, t, ids, g = student(1, v, 6, "f16", v)
+        r = 4
+        labels = torch.randint(0, v, (r,), generator=g, dtype=torch.int32)
+        loss, rl, dz = torch.empty(1, device=dev), torch.empty(r, device=dev), torch.empty((r, v), device=dev).half()
+        ins = [x.to(dev).expand(r, -1) for x in (z, t, ids)] + [labels.to(dev)]
+        C.op_call(C.OpKind.DistillTopk, ins, [loss, dz, rl, torch.empty((r, 8, 4), device=dev)], DTOP,
+                  struct.pack("<ff", 1.5, 0.5))
+        check((loss.cpu(), dz.cpu(), rl.cpu()), z.expand(r, -1), t.expand(r, -1), ids.expand(r, -1), 1.5, 0.5, labels)
 
 
 FAR = 1_200_000_000  # elements between rows: the third starts beyond 2^31 of them

@@ -348,7 +348,9 @@ __device__ __forceinline__ void write_zeros(const DistillArgs& a, int64_t row, i
   for (int c = c0 + threadIdx.x * 8; c < c1; c += blockDim.x * 8) put8<EK, STREAM>(a.dz, row * a.lddz + c, zero, c1 - c);
 }
 
-// One workgroup a row.
+// One workgroup a row: 4096 x 32000 bf16 101 us (5.2 TB/s, HBM), 1023 x 50021 f32
+// 110 (3.7: rows off the 128-byte lines), 1 x 9000 bf16 10 (its chain of loads and
+// reductions, and the loss).
 // Where the row takes at most 32 registers a thread, 8 waves fit a SIMD: a row's
 // chain of loads and reductions hides behind other rows'.
 template <int NT, int EK, int VPT, bool DUAL, bool STREAM>
@@ -405,7 +407,8 @@ __global__ __launch_bounds__(NT, VPT * (EK == EL_F32 ? 8 : 4) <= 32 ? 8 : 4) voi
 // maximum and sums in scratch [R, P, 4]; the first also what the loss takes
 // from the teacher and the label (the second launch may write over the logits)
 // in the fourth floats: sum p (log p - (z - z0) / tau) in f64, the label's logit,
-// and z0, a class's logit, so that nothing large cancels.
+// and z0, a class's logit, so that nothing large cancels.  8 x 131072 bf16: 5.2 +
+// 8.9 us, a load round trip and a few reductions each.
 constexpr int kPartNT = 256;
 __device__ __forceinline__ void part_columns(int V, int P, int* c0, int* c1) {
   const int len = ((V + P - 1) / P + 7) & ~7;

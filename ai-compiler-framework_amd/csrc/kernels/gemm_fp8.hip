@@ -168,9 +168,13 @@ __device__ __forceinline__ Frag<F, EXACT> read_frag(const uint8_t* st, int row, 
 // two LDS stages; the loads of the next block are in flight during this one's
 // products.  Rows past M or N read the last row again (not stored), K past the
 // end is zero in both operands.
+// 4096 x 4096 x 4095, rows at any byte: bf16 193 us, f32 258 (64 x 64 tiles 316
+// and 334, 128 x 64 278 and 274); 1001 x 1003 x 785 f16 9.4 on 64 x 64 (19.4 on 128
+// x 128).  Bound by the loads: a 16-byte load that crosses a line counts twice.
+// With all registers of a SIMD to one wave nothing spills, and it takes 263.
 // ---------------------------------------------------------------------------
 template <int BM, int BN, int WM, int WN, int AF, int BF, bool BROW, bool EXACT>
-__global__ __launch_bounds__(64 * WM * WN) void gemm_fp8_kernel(Fp8Gemm p) {
+__global__ __launch_bounds__(64 * WM * WN, 2) void gemm_fp8_kernel(Fp8Gemm p) {
   constexpr int T = 64 * WM * WN;
   constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
   constexpr int CA = BM * 8 / T, CB = BN * 8 / T;  // 16-byte chunks a thread
@@ -216,10 +220,18 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_fp8_kernel(Fp8Gemm p) {
 
   u32x4_t ra[CA], rb[CB];
   auto load = [&](int kb) {
+    const int k = kb * 128 + c * 16;
+    if (kb * 128 + 128 <= p.K) {
 #pragma unroll
-    for (int i = 0; i < CA; ++i) ra[i] = load_chunk(pa[i], kb * 128 + c * 16, p.K);
+      for (int i = 0; i < CA; ++i) ra[i] = *reinterpret_cast<const u32x4_a1*>(pa[i] + k);
 #pragma unroll
-    for (int i = 0; i < CB; ++i) rb[i] = load_chunk(pb[i], kb * 128 + c * 16, p.K);
+      for (int i = 0; i < CB; ++i) rb[i] = *reinterpret_cast<const u32x4_a1*>(pb[i] + k);
+    } else {
+#pragma unroll
+      for (int i = 0; i < CA; ++i) ra[i] = load_chunk(pa[i], k, p.K);
+#pragma unroll
+      for (int i = 0; i < CB; ++i) rb[i] = load_chunk(pb[i], k, p.K);
+    }
   };
   auto store = [&](uint8_t* st) {
 #pragma unroll
@@ -281,6 +293,13 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_fp8_kernel(Fp8Gemm p) {
 // block's results are added to the accumulators one row of fragments late, so
 // that no multiply-add waits for its MFMA.  A last, partial block goes through
 // registers with zeros behind K.
+// 8192 x 4096 x 4096 bf16 126-138 us (2.0-2.2 PFLOP/s; the library's 8-bit product
+// 2.8), 11008 x 4096 x 8192 f32 704 us (1.05; bf16 products 1.45).  Bound by the
+// matrix cores and the VALU beside them: an 8-bit MFMA alone issues every 35
+// cycles a SIMD, with the 5 multiply-adds of a block's results 39, with 8 (B's
+// scales by rows) 49; f32 outputs have 2 conversions and 2 multiply-adds beside
+// each bf16 MFMA (18 cycles alone, 24 with two).  Their 256 x 256 tiles would not
+// fit the LDS.  1 x 32000 x 4096 f32: 21-25 us, B at 5.2-6.1 TB/s.
 // ---------------------------------------------------------------------------
 template <int BM, int BN, int WM, int WN, int S, int AF, int BF, bool BROW, bool EXACT>
 __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_fp8_lds_kernel(Fp8Gemm p) {
@@ -525,7 +544,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_fp8_lds_kernel(Fp8Gemm p
 // rows of B over a share of K, straight into registers (a row's 128 bytes of a
 // block are one cache line), the KW waves of a workgroup share K and add up
 // through LDS in a fixed order.  Any alignment.  Products and sums in f32, as
-// for f32 outputs above: the matrix cores have nothing else to do.
+// for f32 outputs above: the matrix cores have nothing else to do.  1 x 4096 x
+// 4096 4.9 us, 16 rows 7.0: one round of loads and the sum over the waves; beyond
+// two workgroups a CU each repeats that, and A's rows (1 x 11008 x 4096 13.3).
 // ---------------------------------------------------------------------------
 template <int TM, int KW, int AF, int BF, bool BROW>
 __global__ __launch_bounds__(64 * KW) void gemm_fp8_rows_kernel(Fp8Gemm p) {
@@ -719,10 +740,12 @@ Status gemm_fp8_run(Fp8Gemm& p, hipStream_t s) {
   // (53.6), 4096 78.1 (63.4).
   auto tiles = [&](int64_t b) { return ((p.M + b - 1) / b) * ((p.N + b - 1) / b); };
   if (p.out == EL_F32) {
+    if (!lds && tiles(128) < 256) return run_tiles<0, true, 64, 64, 2, 2, AF, BF>(p, s);
     if (!lds) return run_tiles<0, true, 128, 128, 2, 2, AF, BF>(p, s);
     if (tiles(128) < 256) return run_tiles<4, true, 64, 64, 2, 2, AF, BF>(p, s);
     return run_tiles<2, true, 128, 128, 2, 2, AF, BF>(p, s);
   }
+  if (!lds && tiles(128) < 256) return run_tiles<0, false, 64, 64, 2, 2, AF, BF>(p, s);
   if (!lds) return run_tiles<0, false, 128, 128, 2, 2, AF, BF>(p, s);
   if (tiles(128) < 256) return run_tiles<4, false, 64, 64, 2, 2, AF, BF>(p, s);
   if (tiles(256) < 256) return run_tiles<2, false, 128, 128, 2, 2, AF, BF>(p, s);

@@ -75,7 +75,8 @@ __device__ __forceinline__ void store8(uint8_t* p, uint2 w, int64_t n) {
 
 // ---------------------------------------------------------------------------
 // By rows, no transpose: 16 lanes hold a block (8 elements each), a wave 512
-// columns of a row.  One read and one write of memory.
+// columns of a row.  One read and one write of memory: 8192 x 4096 bf16 20.8 us
+// (4.85 TB/s), f32 25.0 (6.7, from the cache), 16 x 4096 2.8.
 // ---------------------------------------------------------------------------
 template <int EK, int F>
 __global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs a) {
@@ -107,6 +108,8 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs a) {
 // 256 scales (two IEEE divisions: 8 + 8 of them in every thread were half of
 // this kernel's time).  The transposed codes go through LDS in pieces of 8 (one
 // column's 8 rows), piece tr of column c at tr ^ (c >> 3).
+// 8192 x 4096 bf16 by rows both ways 24.0 us (5.7 TB/s), 11008 x 4096 f32 by blocks
+// both ways 44.3 (6.1): HBM.
 // ---------------------------------------------------------------------------
 // max over the 16 lanes of a DPP row
 __device__ __forceinline__ uint32_t row16_max(uint32_t v) {

@@ -21,7 +21,10 @@
 // ceil(log2 V), at most 51: for 2^17 classes a term is off by at most 2^-46 of
 // the largest weight.
 //
-// A workgroup owns a row and reads it again, from the caches, in each pass.
+// A workgroup owns a row and reads it again, from the caches, in each pass.  256
+// x 65521 bf16: greedy 12-15 us, top-k 50 30, plain draws 41, top-p 0.9 100; the
+// f64 weights (half rate, some 20 operations each) and the histogram's 64-bit LDS
+// atomics bound them, not the 7 us of bytes.
 //
 // No counterpart in the reference.
 #include "../common/head_util.hpp"

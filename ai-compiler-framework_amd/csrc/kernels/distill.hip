@@ -70,32 +70,47 @@ __device__ __forceinline__ void block_reduce(float (&v)[N], float* lds) {
     for (int i = 0; i < N; ++i) v[i] = OP == 0 ? fmaxf(v[i], lds[k * 4 + i]) : v[i] + lds[k * 4 + i];
 }
 
+// Columns of a 16-byte vector.
+constexpr int width(int ek) { return ek == EL_F32 ? 4 : 8; }
+
 template <int EK>
 __device__ __forceinline__ void put_elem(void* p, int64_t i, float v) {
   if constexpr (EK == EL_F32) static_cast<float*>(p)[i] = v;
   else static_cast<uint16_t*>(p)[i] = EK == EL_F16 ? f32_to_f16(v) : f32_to_bf16(v);
 }
-// STREAM: loads and stores of a row with the nontemporal hint.  It pays where
-// rows start on 128-byte lines (4096 x 32000 bf16 132 -> 115 us, 16384 x 8000
-// 163 -> 130): nothing here is read again.  Elsewhere a line is shared by two
-// vectors and would be fetched twice (4096 x 50021 f32 362 -> 491 us).
-template <bool STREAM, typename V>
-__device__ __forceinline__ V vec_load(const V* p) {
+// STREAM: loads and stores of a row with the nontemporal hint, where it is held in
+// registers and nothing is read again (without it: 4096 x 32000 bf16 118.4 us,
+// with it 106.9; rows at odd addresses 128.8, 123.3; f32 1023 x 50021 99.4, 96.0,
+// 4096 x 50021 at odd addresses 334.6, 345.2, on 128-byte lines 326.9, 318.3).  A
+// wave's accesses have to cover their lines whole: with two 16-byte vectors a lane
+// in a row f32 took 461.
+// (Not templates of the vector's type: that would lose its alignment.)
+template <bool STREAM>
+__device__ __forceinline__ f32x4 vec_load(const f32x4_a4* p) {
   if constexpr (STREAM) return __builtin_nontemporal_load(p);
   else return *p;
 }
-template <bool STREAM, typename V>
-__device__ __forceinline__ void vec_store(V* p, V v) {
+template <bool STREAM>
+__device__ __forceinline__ u16x8_a2 vec_load(const u16x8_a2* p) {
+  if constexpr (STREAM) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+template <bool STREAM>
+__device__ __forceinline__ void vec_store(f32x4_a4* p, f32x4 v) {
+  if constexpr (STREAM) __builtin_nontemporal_store(v, p);
+  else *p = v;
+}
+template <bool STREAM>
+__device__ __forceinline__ void vec_store(u16x8_a2* p, u16x8_a2 v) {
   if constexpr (STREAM) __builtin_nontemporal_store(v, p);
   else *p = v;
 }
 template <int EK, bool STREAM = false>
-__device__ __forceinline__ void put8(void* p, int64_t i, const float (&v)[8], int n) {
-  if (n >= 8) {
+__device__ __forceinline__ void put_vec(void* p, int64_t i, const float (&v)[width(EK)], int n) {
+  constexpr int W = width(EK);
+  if (n >= W) {
     if constexpr (EK == EL_F32) {
-      float* q = static_cast<float*>(p) + i;
-      vec_store<STREAM>(reinterpret_cast<f32x4_a4*>(q), f32x4_a4{v[0], v[1], v[2], v[3]});
-      vec_store<STREAM>(reinterpret_cast<f32x4_a4*>(q + 4), f32x4_a4{v[4], v[5], v[6], v[7]});
+      vec_store<STREAM>(reinterpret_cast<f32x4_a4*>(static_cast<float*>(p) + i), f32x4_a4{v[0], v[1], v[2], v[3]});
     } else {
       u16x8_a2 o;
 #pragma unroll
@@ -113,7 +128,7 @@ __device__ __forceinline__ void put8(void* p, int64_t i, const float (&v)[8], in
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 7; ++e)
+    for (int e = 0; e < W - 1; ++e)
       if (e < n) put_elem<EK>(p, i + e, v[e]);
   }
 }
@@ -123,9 +138,9 @@ __device__ __forceinline__ float elem_any(const void* p, int64_t i, int ek) {
   return ek == EL_F16 ? elem_f32<EL_F16>(p, i) : elem_f32<EL_BF16>(p, i);
 }
 
-// 8 logits as they are stored.
+// 16 bytes of logits as they are stored.
 template <int EK>
-struct Vec8 {
+struct Vec {
   typedef uint16_t u16x8v __attribute__((ext_vector_type(8)));
   static constexpr uint16_t NONE = EK == EL_F16 ? 0xfc00 : 0xff80;  // -inf
   u16x8v h;
@@ -147,54 +162,47 @@ struct Vec8 {
   __device__ __forceinline__ float operator[](int e) const { return EK == EL_F16 ? f16_to_f32(h[e]) : bf16_to_f32(h[e]); }
 };
 template <>
-struct Vec8<EL_F32> {
-  f32x4 a, b;
+struct Vec<EL_F32> {
+  f32x4 a;
   template <bool STREAM>
   __device__ __forceinline__ void load(const uint8_t* p, int i) {
     a = vec_load<STREAM>(reinterpret_cast<const f32x4_a4*>(p + (uint32_t)i * 4u));
-    b = vec_load<STREAM>(reinterpret_cast<const f32x4_a4*>(p + (uint32_t)i * 4u + 16u));
   }
   __device__ __forceinline__ void load_first(const uint8_t* p, int n) {
-    const float* q = reinterpret_cast<const float*>(p);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      a[e] = e < n ? q[e] : -INFINITY;
-      b[e] = e + 4 < n ? q[e + 4] : -INFINITY;
-    }
+    for (int e = 0; e < 4; ++e) a[e] = e < n ? reinterpret_cast<const float*>(p)[e] : -INFINITY;
   }
   __device__ __forceinline__ void drop(int n) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      a[e] = e < n ? -INFINITY : a[e];
-      b[e] = e + 4 < n ? -INFINITY : b[e];
-    }
+    for (int e = 0; e < 4; ++e) a[e] = e < n ? -INFINITY : a[e];
   }
-  __device__ __forceinline__ void forget() { asm volatile("" : "+v"(a), "+v"(b)); }
-  __device__ __forceinline__ float operator[](int e) const { return e < 4 ? a[e] : b[e - 4]; }
+  __device__ __forceinline__ void forget() { asm volatile("" : "+v"(a)); }
+  __device__ __forceinline__ float operator[](int e) const { return a[e]; }
 };
 
-// A workgroup's columns of a row, n of them: in registers (VPT vectors of 8 a
-// thread; with WHOLE the first half of them lies inside), or (VPT 0) read again
+// A workgroup's columns of a row, n of them: in registers (VPT vectors a
+// thread; with WHOLE the first half of them, rounded down to 8 columns, lies inside), or (VPT 0) read again
 // in each pass.  A vector that would pass the end is moved back to end there;
 // its elements that an earlier vector holds become -inf, which adds nothing to a
 // maximum or a sum, and are not stored.
 template <int NT, int EK, int VPT, bool WHOLE, bool STREAM_>
 struct Part {
   static constexpr bool STREAM = STREAM_;
+  static constexpr int W = width(EK), INNER = WHOLE ? VPT * W / 8 / 2 * (8 / W) : 0;
   const uint8_t* z;  // the first column
   int n;
-  Vec8<EK> v[VPT > 0 ? VPT : 1];
-  __device__ __forceinline__ int first(int k) const { return (k * NT + (int)threadIdx.x) * 8; }
-  __device__ __forceinline__ static bool inner(int k) { return WHOLE && k < VPT / 2; }
-  __device__ __forceinline__ bool beyond(int k) const { return !inner(k) && k > 0 && k * NT * 8 >= n; }  // uniform
-  __device__ __forceinline__ int col(int k) const { return inner(k) ? first(k) : n >= 8 ? min(first(k), n - 8) : 0; }
+  Vec<EK> v[VPT > 0 ? VPT : 1];
+  __device__ __forceinline__ int first(int k) const { return (k * NT + (int)threadIdx.x) * W; }
+  __device__ __forceinline__ static bool inner(int k) { return k < INNER; }
+  __device__ __forceinline__ bool beyond(int k) const { return !inner(k) && k > 0 && k * NT * W >= n; }  // uniform
+  __device__ __forceinline__ int col(int k) const { return inner(k) ? first(k) : n >= W ? min(first(k), n - W) : 0; }
   // the elements [lo, hi) of vector k are its own
-  __device__ __forceinline__ int lo(int k) const { return inner(k) ? 0 : min(first(k) - col(k), 8); }
-  __device__ __forceinline__ int hi() const { return n >= 8 ? 8 : (n > 0 ? n : 0); }
-  __device__ __forceinline__ void fetch(Vec8<EK>& x, int k) const {
-    if (inner(k) || n >= 8) {
+  __device__ __forceinline__ int lo(int k) const { return inner(k) ? 0 : min(first(k) - col(k), W); }
+  __device__ __forceinline__ int hi() const { return n >= W ? W : (n > 0 ? n : 0); }
+  __device__ __forceinline__ void fetch(Vec<EK>& x, int k) const {
+    if (inner(k) || n >= W) {
       x.template load<STREAM>(z, col(k));
-      if (!inner(k) && (k + 1) * NT * 8 > n) x.drop(lo(k));  // (uniform)
+      if (!inner(k) && (k + 1) * NT * W > n) x.drop(lo(k));  // (uniform)
     } else {
       x.load_first(z, first(k) == 0 ? n : 0);
     }
@@ -218,10 +226,13 @@ struct Part {
         __builtin_amdgcn_sched_barrier(0);  // a vector at a time: the row's registers leave little else
       }
     } else {
-      for (int k = 0; first(k) < n; ++k) {
-        Vec8<EK> x;
+      for (int k = 0; first(k) < n; k += 2) {  // two vectors on their way
+        Vec<EK> x, y;
+        const bool two = first(k + 1) < n;
         fetch(x, k);
+        if (two) fetch(y, k + 1);
         f(x, col(k), lo(k));
+        if (two) f(y, col(k + 1), lo(k + 1));
       }
     }
   }
@@ -235,9 +246,9 @@ struct Part {
   }
   __device__ __forceinline__ float top() const {
     float m = -INFINITY;
-    each([&](const Vec8<EK>& x, int, int) {
+    each([&](const Vec<EK>& x, int, int) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) m = fmaxf(m, x[e]);
+      for (int e = 0; e < W; ++e) m = fmaxf(m, x[e]);
     });
     return m;
   }
@@ -245,10 +256,10 @@ struct Part {
   template <bool DUAL>
   __device__ __forceinline__ void sums(float c, float mc, float mc1, float& s, float& s1) const {
     s = s1 = 0.0f;
-    each([&](const Vec8<EK>& x, int, int) {
+    each([&](const Vec<EK>& x, int, int) {
       float p[2] = {0.0f, 0.0f}, p1[2] = {0.0f, 0.0f};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
+      for (int e = 0; e < W; ++e) {
         p[e & 1] += exp_of(x[e], c, mc);
         if constexpr (DUAL) p1[e & 1] += exp_of(x[e], kLog2e, mc1);
       }
@@ -309,16 +320,17 @@ __device__ __forceinline__ void write_gradient(const DistillArgs& a, int64_t row
     return g;
   };
   const int hi = part.hi();
-  part.each([&](const Vec8<EK>& x, int c, int lo) {
-    float g[8];
+  part.each([&](const Vec<EK>& x, int c, int lo) {
+    constexpr int W = width(EK);
+    float g[W];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) g[e] = dense(x[e]);
+    for (int e = 0; e < W; ++e) g[e] = dense(x[e]);
     const int64_t at = row * a.lddz + c0 + c;
-    if (lo == 0 && hi == 8) {
-      put8<EK, P::STREAM>(a.dz, at, g, 8);
+    if (lo == 0 && hi == W) {
+      put_vec<EK, P::STREAM>(a.dz, at, g, W);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
+      for (int e = 0; e < W; ++e)
         if (e >= lo && e < hi) put_elem<EK>(a.dz, at + e, g[e]);
     }
   });
@@ -344,19 +356,21 @@ __device__ __forceinline__ void write_gradient(const DistillArgs& a, int64_t row
 
 template <int EK, bool STREAM>
 __device__ __forceinline__ void write_zeros(const DistillArgs& a, int64_t row, int c0, int c1) {
-  const float zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  for (int c = c0 + threadIdx.x * 8; c < c1; c += blockDim.x * 8) put8<EK, STREAM>(a.dz, row * a.lddz + c, zero, c1 - c);
+  constexpr int W = width(EK);
+  const float zero[W] = {};
+  for (int c = c0 + threadIdx.x * W; c < c1; c += blockDim.x * W) put_vec<EK, STREAM>(a.dz, row * a.lddz + c, zero, c1 - c);
 }
 
 // One workgroup a row: 4096 x 32000 bf16 101 us (5.2 TB/s, HBM), 1023 x 50021 f32
-// 110 (3.7: rows off the 128-byte lines), 1 x 9000 bf16 10 (its chain of loads and
+// 96 (4.3: a CU holds one row at a time), 1 x 9000 bf16 10 (its chain of loads and
 // reductions, and the loss).
 // Where the row takes at most 32 registers a thread, 8 waves fit a SIMD: a row's
 // chain of loads and reductions hides behind other rows'.
-template <int NT, int EK, int VPT, bool DUAL, bool STREAM>
-__global__ __launch_bounds__(NT, VPT * (EK == EL_F32 ? 8 : 4) <= 32 ? 8 : 4) void distill_row_kernel(DistillArgs a, int tk) {
+template <int NT, int EK, int VPT, bool DUAL>
+__global__ __launch_bounds__(NT, VPT * 4 <= 32 && !(DUAL && EK == EL_F32) ? 8 : 4) void distill_row_kernel(DistillArgs a, int tk) {
   const Special sp = special_lds(a.K);
   __shared__ float red[16 * 4];
+  constexpr bool STREAM = VPT > 0;
   const int t = threadIdx.x, V = (int)a.V;
   const int64_t row = blockIdx.x;
   const float w = a.w ? a.w[row] : a.w0;
@@ -658,15 +672,13 @@ Status distill_rows(const DistillArgs& a, int tk, float* scratch, int ldp, hipSt
       distill_stats_kernel<EK, VPT, DUAL><<<grid, kPartNT, lds, s>>>(a, tk, scratch, (int)P, ldp);
       distill_grad_kernel<EK, VPT, DUAL><<<grid, kPartNT, lds, s>>>(a, tk, scratch, (int)P, ldp);
     };
-    if (len <= kPartNT * 8 * 2) go(std::integral_constant<int, 2>{});
+    if (len <= kPartNT * 8 * 2) go(std::integral_constant<int, 2 * 8 / width(EK)>{});
     else go(std::integral_constant<int, 0>{});
     return launch_status("distill_topk");
   }
   // The row in the registers of the fewest threads that hold it: up to 64
   // columns a thread in 16 bits and 56 in f32 (128 in 16 bits for the longest);
   // beyond 2^17 or 57344 columns it is read in each pass.
-  const int64_t es = EK == EL_F32 ? 4 : 2;
-  const bool stream = aligned(a.z, 128) && a.ldz * es % 128 == 0 && aligned(a.dz, 128) && a.lddz * es % 128 == 0;
   const int64_t kStep = 1 << 21;  // rows a launch: a grid's lanes are counted in 32 bits
   for (int64_t r = 0; r < a.R; r += kStep) {
     const DistillArgs p = from_row<EK>(a, tk, r, a.R - r < kStep ? a.R - r : kStep);
@@ -674,8 +686,8 @@ Status distill_rows(const DistillArgs& a, int tk, float* scratch, int ldp, hipSt
     constexpr int L = EK == EL_F32 ? 7 : 8, XL = EK == EL_F32 ? 0 : 16;
 #define DISTILL_ROW(NT, VPT)                                                                  \
   do {                                                                                        \
-    if (stream) distill_row_kernel<NT, EK, VPT, DUAL, true><<<g, NT, lds, s>>>(p, tk);        \
-    else distill_row_kernel<NT, EK, VPT, DUAL, false><<<g, NT, lds, s>>>(p, tk);              \
+    constexpr int N = (VPT) * 8 / width(EK);                                                  \
+    distill_row_kernel<NT, EK, N, DUAL><<<g, NT, lds, s>>>(p, tk);                            \
   } while (0)
     if (a.V <= 512) DISTILL_ROW(64, 1);
     else if (a.V <= 1024) DISTILL_ROW(64, 2);
@@ -686,7 +698,7 @@ Status distill_rows(const DistillArgs& a, int tk, float* scratch, int ldp, hipSt
     else if (a.V <= 512 * 8 * L) DISTILL_ROW(512, L);
     else if (a.V <= 1024 * 8 * L) DISTILL_ROW(1024, L);
     else if (XL && a.V <= 131072) DISTILL_ROW(1024, XL);
-    else distill_row_kernel<1024, EK, 0, DUAL, false><<<g, 1024, lds, s>>>(p, tk);
+    else distill_row_kernel<1024, EK, 0, DUAL><<<g, 1024, lds, s>>>(p, tk);
 #undef DISTILL_ROW
     const Status st = launch_status("distill_topk");
     if (st != Status::Ok) return st;

@@ -658,7 +658,7 @@ Status distill_rows(const DistillArgs& a, int tk, float* scratch, int ldp, hipSt
   // Few long rows share the chip: parts of 2048 columns or more, about two
   // workgroups a CU.  A row a workgroup against this: 8 x 200000 bf16 34.3 us
   // (15.2), 8 x 65536 15.4 (13.8), f32 20.2 (13.6), 48 x 131072 22.3 (21.3); the
-  // other way 8 x 32000 f32 12.8 (15.1), 128 x 131072 f32 47.1 (51.3).
+  // other way 8 x 32000 f32 12.8 (15.1), 128 x 131072 f32 45.8 (51.3).
   const unsigned lds = special_bytes(a.K);
   int64_t P = (512 + a.R - 1) / a.R;
   if (P > a.V / 2048) P = a.V / 2048;

@@ -1107,7 +1107,12 @@ Status sample_run(const SampleArgs& a, uint32_t* scratch, int64_t lds, hipStream
     sample_join_kernel<EK><<<g, 1024, 0, s>>>(a, scratch, lds, P);
     return launch_status("sample_row");
   }
-  if (a.V <= 8192) sample_kernel<EK, 256><<<g, 256, 0, s>>>(a);
+  // Short rows, and several rows a CU: 256 threads; else 1024.  256 against 1024,
+  // bf16, plain draws and top-p 0.9: 64 x 2000 7.7 us (15.3), 10.8 (19.2); 64 x
+  // 16384 16.1 (17.2), 33.4 (31.1); 2048 x 50021 161.5 (268.2), 325.7 (437.7); the
+  // other way 256 x 32000 28.3 (26.8), 83.6 (59.3).  At 512 x 131072 126.3 (124.1),
+  // 346.3 (313.5), top-k 50 61.5 (66.5).
+  if (a.V <= 16384 || a.R >= 512) sample_kernel<EK, 256><<<g, 256, 0, s>>>(a);
   else sample_kernel<EK, 1024><<<g, 1024, 0, s>>>(a);
   return launch_status("sample_row");
 }

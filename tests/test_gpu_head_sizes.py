@@ -84,6 +84,19 @@ def test_sample_forms(C, dev, v, dtype):
 
 
 @gpu
+def test_sample_of_many_long_rows(C, dev):
+    """Several rows a CU: 256 threads go through rows longer than 16384 classes too."""
+    for r, v in ((520, 20011), (513, 16385)):
+        g = torch.Generator().manual_seed(v)
+        z = (torch.randn((r, v), generator=g) * 2).bfloat16()
+        z[::7, : v // 2] = 0.0
+        u = torch.rand(r, generator=g)
+        sets = [SETTINGS[i % len(SETTINGS)] for i in range(r)]
+        tok, _ = draw(C, dev, z.to(dev), u, sets, 0)
+        assert tok.tolist() == [ref.sample(z[i], u[i].item(), *as_f32(s))[0] for i, s in enumerate(sets)]
+
+
+@gpu
 def test_sample_shared_rows_of_equal_logits(C, dev):
     """More classes at the cut than any list holds; few finite ones; one; none."""
     v = 40000

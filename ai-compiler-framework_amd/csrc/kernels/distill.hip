@@ -513,9 +513,11 @@ __global__ __launch_bounds__(kPartNT) void distill_grad_kernel(DistillArgs a, in
   const float* in = scratch + row * ldp * 4;
   f32x4 own = {-INFINITY, 0.0f, 0.0f, 0.0f};  // P <= 64: one a lane, the same in every wave
   if ((t & 63) < P) own = *reinterpret_cast<const f32x4_a4*>(in + (t & 63) * 4);
-  const float mx = wave_max(own[0]), m = safe_ref(mx), mc = m * c2, mc1 = m * kLog2e, mq = safe_ref(own[0]);
-  float S = wave_sum(own[1] * __builtin_amdgcn_exp2f(mq * c2 - mc));
-  float S1 = DUAL ? wave_sum(own[2] * __builtin_amdgcn_exp2f(mq * kLog2e - mc1)) : S;
+  // (a part without a class, and a lane without a part, has the maximum -inf and the factor 0: with 0 in the
+  // maximum's place the factor would overflow far below zero, and 0 inf is NaN)
+  const float mx = wave_max(own[0]), m = safe_ref(mx), mc = m * c2, mc1 = m * kLog2e;
+  float S = wave_sum(own[1] * __builtin_amdgcn_exp2f(own[0] * c2 - mc));
+  float S1 = DUAL ? wave_sum(own[2] * __builtin_amdgcn_exp2f(own[0] * kLog2e - mc1)) : S;
   if (mx == -INFINITY) S = S1 = __builtin_nanf("");
   float tm[1] = {gather_special<EK>(a, tk, row, sp)};
   block_reduce<0>(tm, red);

@@ -34,17 +34,20 @@ struct DistillArgs {
   int64_t R, V, ldz, ldt, ldi, lddz;
   int K;
   float tau, alpha, w0;  // w0: the weight of every row where w is absent
+  float c2;              // log2(e) / tau, rounded once
 };
 
 typedef int i32x4_d __attribute__((ext_vector_type(4)));
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ float safe_ref(float m) { return m == -INFINITY ? 0.0f : m; }
-// 2^(z c - mc).  mc = m c is rounded once for the whole row, so its error is a
-// common factor of every exponential and of their sum.
-__device__ __forceinline__ float exp_of(float z, float c, float mc) {
-  return __builtin_amdgcn_exp2f(fmaf(z, c, -mc));
-}
+// 2^((z - m) c).  The difference comes first, so that the exponent is off by
+// roundings of itself alone: z c - m c in one multiply-add is off by a rounding of
+// m c, which differs from part to part of a row (1e-4 near logits of 1000), and is
+// not a number where m c passes the type's range (rows masked with the lowest value).
+// The teacher's the same.  (One more operation a class and pass: 4096 x 32000 bf16
+// 105.8 -> 106.7 us, 1023 x 50021 f32 with labels 98.8 -> 100.3.)
+__device__ __forceinline__ float exp_of(float z, float c, float m) { return __builtin_amdgcn_exp2f((z - m) * c); }
 
 // Up to three values over the workgroup at once, in a fixed order (lds: 4
 // floats a wave).  OP 0: maxima, 1: sums.
@@ -254,14 +257,14 @@ struct Part {
   }
   // sums of exp((z - m) / tau) and, DUAL, of exp(z - m)
   template <bool DUAL>
-  __device__ __forceinline__ void sums(float c, float mc, float mc1, float& s, float& s1) const {
+  __device__ __forceinline__ void sums(float c, float m, float& s, float& s1) const {
     s = s1 = 0.0f;
     each([&](const Vec<EK>& x, int, int) {
       float p[2] = {0.0f, 0.0f}, p1[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int e = 0; e < W; ++e) {
-        p[e & 1] += exp_of(x[e], c, mc);
-        if constexpr (DUAL) p1[e & 1] += exp_of(x[e], kLog2e, mc1);
+        p[e & 1] += exp_of(x[e], c, m);
+        if constexpr (DUAL) p1[e & 1] += exp_of(x[e], kLog2e, m);
       }
       s += p[0] + p[1];
       if constexpr (DUAL) s1 += p1[0] + p1[1];
@@ -274,7 +277,7 @@ struct Part {
 struct Special {
   int* cls;
   float* z;  // their logits
-  float* e;  // the teacher's logit / tau; then what the gradient has less there
+  float* e;  // the teacher's logit; then what the gradient has less there
   int n;     // K + 1, rounded up
 };
 __device__ __forceinline__ Special special_lds(int K) {
@@ -285,7 +288,7 @@ __device__ __forceinline__ Special special_lds(int K) {
 }
 inline unsigned special_bytes(int K) { return (unsigned)((K + 4) & ~3) * 12; }
 
-// Fills cls, z, e of a row; the thread's largest teacher logit / tau.
+// Fills cls, z, e of a row; the thread's largest teacher logit.
 template <int EK>
 __device__ __forceinline__ float gather_special(const DistillArgs& a, int tk, int64_t row, const Special& sp) {
   float tm = -INFINITY;
@@ -298,7 +301,7 @@ __device__ __forceinline__ float gather_special(const DistillArgs& a, int tk, in
     sp.cls[j] = ok ? id : -1;
     sp.z[j] = ok ? elem_f32<EK>(a.z, row * a.ldz + id) : 0.0f;
     if (j < a.K) {
-      const float x = ok ? elem_any(a.t, row * a.ldt + j, tk) / a.tau : -INFINITY;
+      const float x = ok ? elem_any(a.t, row * a.ldt + j, tk) : -INFINITY;
       sp.e[j] = x;
       tm = fmaxf(tm, x);
     } else if (j > a.K) {
@@ -312,11 +315,11 @@ __device__ __forceinline__ float gather_special(const DistillArgs& a, int tk, in
 // m)), and the special classes among them with w e less.
 template <int EK, bool DUAL, typename P>
 __device__ __forceinline__ void write_gradient(const DistillArgs& a, int64_t row, int c0, int c1,
-                                               const P& part, const Special& sp, float c2, float mc,
-                                               float mc1, float k2, float k1, float w) {
+                                               const P& part, const Special& sp, float c2, float m, float k2,
+                                               float k1, float w) {
   auto dense = [&](float z) {
-    float g = k2 * exp_of(z, c2, mc);
-    if constexpr (DUAL) g = fmaf(k1, exp_of(z, kLog2e, mc1), g);
+    float g = k2 * exp_of(z, c2, m);
+    if constexpr (DUAL) g = fmaf(k1, exp_of(z, kLog2e, m), g);
     return g;
   };
   const int hi = part.hi();
@@ -379,19 +382,19 @@ __global__ __launch_bounds__(NT, VPT * 4 <= 32 && !(DUAL && EK == EL_F32) ? 8 : 
     if (t == 0) a.row_loss[row] = 0.0f;
     return;
   }
-  const float c2 = kLog2e / a.tau;
+  const float c2 = a.c2;
   Part<NT, EK, VPT, true, STREAM> part;
   part.open(a.z, row * a.ldz, 0, V);
   float mx[2] = {0.0f, gather_special<EK>(a, tk, row, sp)};
   mx[0] = part.top();
   part.forget();
   block_reduce<0>(mx, red);
-  const float m = safe_ref(mx[0]), tm = safe_ref(mx[1]), mc = m * c2, mc1 = m * kLog2e;
+  const float m = safe_ref(mx[0]), tm = safe_ref(mx[1]);
   float sm[3];
-  part.template sums<DUAL>(c2, mc, mc1, sm[0], sm[1]);
+  part.template sums<DUAL>(c2, m, sm[0], sm[1]);
   part.forget();
   sm[2] = 0.0f;
-  for (int j = t; j < a.K; j += blockDim.x) sm[2] += __expf(sp.e[j] - tm);
+  for (int j = t; j < a.K; j += blockDim.x) sm[2] += exp_of(sp.e[j], c2, tm);
   block_reduce<1>(sm, red);
   const bool none = mx[0] == -INFINITY;  // no class has any probability
   const float S = none ? __builtin_nanf("") : sm[0], S1 = none ? S : DUAL ? sm[1] : sm[0], ts = sm[2];
@@ -401,20 +404,20 @@ __global__ __launch_bounds__(NT, VPT * 4 <= 32 && !(DUAL && EK == EL_F32) ? 8 : 
   const float lgS = log2f(S), lnT = logf(ts), inv_t = some ? 1.0f / ts : 0.0f;
   float l[1] = {0.0f};
   for (int j = t; j < a.K; j += blockDim.x) {
-    const float x = sp.e[j] - tm, p = sp.cls[j] >= 0 ? __expf(x) * inv_t : 0.0f;
-    if (p != 0.0f) l[0] += p * ((x - lnT) - (fmaf(sp.z[j], c2, -mc) - lgS) * kLn2);
+    const float x = (sp.e[j] - tm) / a.tau, p = sp.cls[j] >= 0 ? exp_of(sp.e[j], c2, tm) * inv_t : 0.0f;
+    if (p != 0.0f) l[0] += p * ((x - lnT) - ((sp.z[j] - m) * c2 - lgS) * kLn2);
     sp.e[j] = soft_w * p;
   }
   if (t == 0) sp.e[a.K] = hard_w;
   block_reduce<1>(l, red);
   if (t == 0) {
     float rl = (1.0f - a.alpha) * a.tau * a.tau * l[0];
-    if (has) rl -= a.alpha * ((fmaf(sp.z[a.K], kLog2e, -mc1) - log2f(S1)) * kLn2);
+    if (has) rl -= a.alpha * ((sp.z[a.K] - m) - log2f(S1) * kLn2);
     a.row_loss[row] = rl;
   }
   if (!a.dz) return;
   const float k1 = w * hard_w / S1, k2 = w * soft_w / S + (DUAL ? 0.0f : k1);
-  write_gradient<EK, DUAL>(a, row, 0, V, part, sp, c2, mc, mc1, k2, k1, w);
+  write_gradient<EK, DUAL>(a, row, 0, V, part, sp, c2, m, k2, k1, w);
 }
 
 // Few rows: P workgroups a row, in two launches.  Each leaves its columns'
@@ -441,14 +444,13 @@ __global__ __launch_bounds__(kPartNT) void distill_stats_kernel(DistillArgs a, i
   if (w == 0.0f) return;
   int c0, c1;
   part_columns((int)a.V, P, &c0, &c1);
-  const float c2 = kLog2e / a.tau;
+  const float c2 = a.c2;
   Part<kPartNT, EK, VPT, false, false> part;
   part.open(a.z, row * a.ldz, c0, c1);
   float mx[1] = {part.top()};
   block_reduce<0>(mx, red);
-  const float m = safe_ref(mx[0]);
   float sm[2];
-  part.template sums<DUAL>(c2, m * c2, m * kLog2e, sm[0], sm[1]);
+  part.template sums<DUAL>(c2, safe_ref(mx[0]), sm[0], sm[1]);
   block_reduce<1>(sm, red);
   float* out = scratch + (row * ldp + blockIdx.x) * 4;
   if (threadIdx.x == 0) {
@@ -467,13 +469,13 @@ __global__ __launch_bounds__(kPartNT) void distill_stats_kernel(DistillArgs a, i
     z0s = fabsf(z) < INFINITY ? z : 0.0f;
   }
   float ts[1] = {0.0f};
-  for (int j = threadIdx.x; j < a.K; j += blockDim.x) ts[0] += __expf(sp.e[j] - tm[0]);
+  for (int j = threadIdx.x; j < a.K; j += blockDim.x) ts[0] += exp_of(sp.e[j], c2, tm[0]);
   block_reduce<1>(ts, red);
   const double c2e = (double)c2 * 0.6931471805599453;  // as the sums' exponentials have it
   const float lnT = logf(ts[0]), inv_t = !(ts[0] <= 0.0f) ? 1.0f / ts[0] : 0.0f;
   double l = 0.0;
   for (int j = threadIdx.x; j < a.K; j += blockDim.x) {
-    const float x = sp.e[j] - tm[0], p = sp.cls[j] >= 0 ? __expf(x) * inv_t : 0.0f;
+    const float x = (sp.e[j] - tm[0]) / a.tau, p = sp.cls[j] >= 0 ? exp_of(sp.e[j], c2, tm[0]) * inv_t : 0.0f;
     if (p != 0.0f) l += (double)p * ((double)(x - lnT) - ((double)sp.z[j] - (double)z0s) * c2e);
   }
 #pragma unroll
@@ -505,7 +507,7 @@ __global__ __launch_bounds__(kPartNT) void distill_grad_kernel(DistillArgs a, in
     if (t == 0 && blockIdx.x == 0) a.row_loss[row] = 0.0f;
     return;
   }
-  const float c2 = kLog2e / a.tau;
+  const float c2 = a.c2;
   Part<kPartNT, EK, VPT, false, false> part;
   if (a.dz) part.open(a.z, row * a.ldz, c0, c1);
   // the row's statistics, and the special classes: those of other
@@ -515,22 +517,22 @@ __global__ __launch_bounds__(kPartNT) void distill_grad_kernel(DistillArgs a, in
   if ((t & 63) < P) own = *reinterpret_cast<const f32x4_a4*>(in + (t & 63) * 4);
   // (a part without a class, and a lane without a part, has the maximum -inf and the factor 0: with 0 in the
   // maximum's place the factor would overflow far below zero, and 0 inf is NaN)
-  const float mx = wave_max(own[0]), m = safe_ref(mx), mc = m * c2, mc1 = m * kLog2e;
-  float S = wave_sum(own[1] * __builtin_amdgcn_exp2f(own[0] * c2 - mc));
-  float S1 = DUAL ? wave_sum(own[2] * __builtin_amdgcn_exp2f(own[0] * kLog2e - mc1)) : S;
+  const float mx = wave_max(own[0]), m = safe_ref(mx);
+  float S = wave_sum(own[1] * exp_of(own[0], c2, m));
+  float S1 = DUAL ? wave_sum(own[2] * exp_of(own[0], kLog2e, m)) : S;
   if (mx == -INFINITY) S = S1 = __builtin_nanf("");
   float tm[1] = {gather_special<EK>(a, tk, row, sp)};
   block_reduce<0>(tm, red);
   tm[0] = safe_ref(tm[0]);
   float ts[1] = {0.0f};
-  for (int j = t; j < a.K; j += blockDim.x) ts[0] += __expf(sp.e[j] - tm[0]);
+  for (int j = t; j < a.K; j += blockDim.x) ts[0] += exp_of(sp.e[j], c2, tm[0]);
   block_reduce<1>(ts, red);
   const bool some = !(ts[0] <= 0.0f), has = sp.cls[a.K] >= 0;
   const float soft_w = some ? (1.0f - a.alpha) * a.tau : 0.0f, hard_w = has ? a.alpha : 0.0f;
   const float inv_t = some ? 1.0f / ts[0] : 0.0f;
   float pr[1] = {0.0f};  // the sum of the probabilities: 1, or 0 without a teacher, or NaN
   for (int j = t; j < a.K; j += blockDim.x) {
-    const float p = sp.cls[j] >= 0 ? __expf(sp.e[j] - tm[0]) * inv_t : 0.0f;
+    const float p = sp.cls[j] >= 0 ? exp_of(sp.e[j], c2, tm[0]) * inv_t : 0.0f;
     pr[0] += p;
     sp.e[j] = soft_w * p;
   }
@@ -540,14 +542,14 @@ __global__ __launch_bounds__(kPartNT) void distill_grad_kernel(DistillArgs a, in
     const double l = __longlong_as_double((long long)((uint64_t)__float_as_uint(in[3]) |
                                                       (uint64_t)__float_as_uint(in[7]) << 32));
     // sum p (log p - (z - z0) / tau) + sum p (log sum exp(z / tau) - z0 / tau)
-    const double lse = ((double)mc + (double)log2f(S) - (double)in[15] * (double)c2) * 0.6931471805599453;
+    const double lse = (((double)m - (double)in[15]) * (double)c2 + (double)log2f(S)) * 0.6931471805599453;
     float rl = some ? (1.0f - a.alpha) * a.tau * a.tau * (float)(l + (double)pr[0] * lse) : 0.0f;
-    if (has) rl -= a.alpha * ((fmaf(in[11], kLog2e, -mc1) - log2f(S1)) * kLn2);
+    if (has) rl -= a.alpha * ((in[11] - m) - log2f(S1) * kLn2);
     a.row_loss[row] = rl;
   }
   if (!a.dz) return;
   const float k1 = w * hard_w / S1, k2 = w * soft_w / S + (DUAL ? 0.0f : k1);
-  write_gradient<EK, DUAL>(a, row, c0, c1, part, sp, c2, mc, mc1, k2, k1, w);
+  write_gradient<EK, DUAL>(a, row, c0, c1, part, sp, c2, m, k2, k1, w);
 }
 
 // loss = sum of w_r row_loss_r, f64 in a fixed order (one workgroup).
@@ -735,6 +737,7 @@ Status distill_launch(const TensorDesc* in, int ni, TensorDesc* out, int no, con
   if (c.dz) matrix_ld(*c.dz, true, &a.lddz);
   a.tau = c.tau;
   a.alpha = c.alpha;
+  a.c2 = (float)(1.4426950408889634 / (double)c.tau);
   int ek, tk;
   elem_kind(*c.z, &ek);
   elem_kind(*c.t, &tk);

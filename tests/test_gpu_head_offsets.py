@@ -8,11 +8,22 @@ import math
 import pytest
 import torch
 
+import head_ref as ref
 from test_gpu_head import DT, check, distill, student
 
 pytestmark = pytest.mark.gpu
 # the temperature at which exp(z / tau) is 2^z: no reference point is rounded
 LOG2E = 1.4426950408889634
+
+
+@pytest.fixture
+def below_normal(monkeypatch):
+    """Small temperatures bring exponentials below the smallest normal f32,
+    2^-126; the exponential instruction gives 0 there.  An element of the gradient
+    is then off by at most 2^-126 w ((1 - a) tau / S + a / S1) <= 2^-126: w <= 1/2, tau <= 2, and the sums S
+    and S1 are 1 or more."""
+    for t in ref.TINY:
+        monkeypatch.setitem(ref.TINY, t, ref.TINY[t] + 2.0 ** -126)
 
 
 def moved(r, v, k, dtype, shift, seed):
@@ -45,3 +56,48 @@ def test_parts_without_a_class(C, dev, v):
     ids[1] = torch.tensor([0, 2047, 7, 100])
     for scratch in (0, 64):
         check(distill(C, dev, z, t, ids, LOG2E, 0.0, scratch=scratch), z, t, ids, LOG2E, 0.0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shift,tau,alpha", [(-1000.0, 1.0, 0.0), (1000.0, 1.0, 0.5), (-1e4, 2.0, 0.5),
+                                             (-20.0, 0.05, 0.0), (-20.0, 0.05, 0.5), (3e4, 0.7, 0.25)])
+def test_moved_together(C, dev, below_normal, shift, tau, alpha, dtype):
+    """The bounds of logits around zero, whatever was added to all of them."""
+    for r, p, v in ((3, 64, 700), (2, 8, 50021), (2, 64, 131072)):
+        z, t, ids, labels = moved(r, v, 6, dtype, shift, v)
+        lab = labels if alpha else None
+        for scratch in (0, p):
+            check(distill(C, dev, z, t, ids, tau, alpha, lab, scratch=scratch), z, t, ids, tau, alpha, lab)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("v", [500, 9001, 50021, 140001])
+def test_masks_of_the_lowest_value(C, dev, v, dtype):
+    """Rows masked with the type's lowest finite value: whole (all classes are
+    then equally likely), but for a few classes, but for one part; a row of the highest."""
+    z, t, ids, labels = moved(4, v, 5, dtype, 0.0, v)
+    low = torch.finfo(z.dtype).min
+    few = z[1, ids[1].long()].clone()
+    z[0], z[1], z[3] = low, low, -low
+    z[1, ids[1].long()] = few
+    z[2, 300:] = low
+    ids[2] = torch.arange(5) * 50
+    labels[1], labels[2] = ids[1, 0], 7
+    for tau, alpha in ((1.0, 0.0), (0.5, 0.0), (2.0, 0.5)):
+        lab = labels if alpha else None
+        for scratch in (0, 8):
+            check(distill(C, dev, z, t, ids, tau, alpha, lab, scratch=scratch), z, t, ids, tau, alpha, lab)
+
+
+@pytest.mark.parametrize("v", [500, 50021])
+def test_teachers_far_from_zero(C, dev, below_normal, v):
+    """The teacher's logits moved together, alike, or masked with the lowest value."""
+    z, t, ids, _ = moved(5, v, 6, "f32", 0.0, v)
+    t[0] += 1000.0
+    t[1] -= 1e4
+    t[2] = -3.0e38
+    t[3, 2:] = torch.finfo(torch.float32).min
+    t[4] = 3.0e38
+    for tau in (1.0, 0.3, 2.0):
+        for scratch in (0, 8):
+            check(distill(C, dev, z, t, ids, tau, 0.0, scratch=scratch), z, t, ids, tau, 0.0)

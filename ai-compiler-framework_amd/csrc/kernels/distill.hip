@@ -288,14 +288,15 @@ __device__ __forceinline__ Special special_lds(int K) {
 }
 inline unsigned special_bytes(int K) { return (unsigned)((K + 4) & ~3) * 12; }
 
-// Fills cls, z, e of a row; the thread's largest teacher logit.
+// Fills cls, z, e of a row; the thread's largest teacher logit.  A term of weight 0
+// has no classes: it may be infinite, and 0 inf is NaN.
 template <int EK>
 __device__ __forceinline__ float gather_special(const DistillArgs& a, int tk, int64_t row, const Special& sp) {
   float tm = -INFINITY;
   const int V = (int)a.V;
   for (int j = threadIdx.x; j < sp.n; j += blockDim.x) {
     int id = -1;
-    if (j < a.K) id = a.ids[row * a.ldi + j];
+    if (j < a.K) id = a.alpha != 1.0f ? a.ids[row * a.ldi + j] : -1;
     else if (j == a.K && a.labels && a.alpha != 0.0f) id = a.labels[row];
     const bool ok = id >= 0 && id < V;
     sp.cls[j] = ok ? id : -1;

@@ -166,7 +166,8 @@ extern "C" {
  *     row loss = (1 - a) tau^2 KL(p || softmax(Z / tau)) + a CE(Z, label)
  *     loss [1] = sum_r w_r row_loss_r;   dlogits = d loss / d Z, in Z's type
  *   A class outside [0, V) is left out of its row; a row without any has no
- *   first term, one whose label is outside [0, V) no second.  The same class
+ *   first term, one whose label is outside [0, V) no second.  With a = 1 no row
+ *   has a first term, with a = 0 none a second, whatever they would be.  The same class
  *   twice counts with the sum of its probabilities.  A row of weight 0 is not
  *   read: its row loss and dlogits are 0.  A logit of -inf has probability 0;
  *   a row of nothing else gives NaN.  Outputs (loss, dlogits, row loss) or, for

@@ -101,3 +101,26 @@ def test_teachers_far_from_zero(C, dev, below_normal, v):
     for tau in (1.0, 0.3, 2.0):
         for scratch in (0, 8):
             check(distill(C, dev, z, t, ids, tau, 0.0, scratch=scratch), z, t, ids, tau, 0.0)
+
+
+@pytest.mark.parametrize("v", [300, 9001, 50021])
+def test_a_term_of_weight_0_is_left_out(C, dev, v):
+    """The labels' loss alone where the teacher's term is infinite or no number,
+    and the teacher's alone where the label's is."""
+    z, t, ids, labels = moved(4, v, 6, "f32", 0.0, v)
+    z[0, ids[0, 1].long()] = -math.inf
+    labels[0] = ids[0, 0]
+    zl, labels[1:] = z.clone(), ids[1:, 5] + 1
+    labels[labels == v] = 0
+    tn = t.clone()
+    tn[1, 2], tn[2] = math.nan, math.inf
+    zl[3, labels[3].long()] = -math.inf
+    ids[3, 5] = -1
+    ids[3][ids[3] == labels[3]] = -1
+    none = torch.full_like(ids, -1)  # (the definition without the teacher's term)
+    for scratch in (0, 8):
+        for tau in (1.0, 2.0):
+            check(distill(C, dev, z, tn, ids, tau, 1.0, labels, scratch=scratch), z, t, none, tau, 1.0, labels)
+            rest = slice(1, 4)
+            check(distill(C, dev, zl[rest], t[rest], ids[rest], tau, 0.0, labels[rest], scratch=scratch), zl[rest],
+                  t[rest], ids[rest], tau, 0.0)

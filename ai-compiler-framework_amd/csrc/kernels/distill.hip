@@ -585,7 +585,8 @@ bool distill_read(const TensorDesc* in, int ni, const TensorDesc* out, int no, c
     c.tau = field<float>(b, 0);
     c.alpha = field<float>(b, 4);
   }
-  if (!(c.tau > 0.0f && c.tau <= 3.0e38f) || !(c.alpha >= 0.0f && c.alpha <= 1.0f)) return false;
+  // tau^2 and log2(e) / tau stay within f32's range
+  if (!(c.tau >= 0x1p-60f && c.tau <= 0x1p60f) || !(c.alpha >= 0.0f && c.alpha <= 1.0f)) return false;
   c.z = in;
   c.t = in + 1;
   c.ids = in + 2;

@@ -161,7 +161,7 @@ extern "C" {
  * DISTILL_TOPK: logits Z [R, V] f32/f16/bf16, R >= 1, V <= 2^28; teacher logits
  *   T [R, K] f32/f16/bf16 and their classes I [R, K] i32, 1 <= K <= 1024; labels
  *   [R] i32 and row weights w [R] f32, each optional (without weights: 1/R).
- *   tau > 0 is the temperature, a in [0, 1] the weight of the labels' loss.
+ *   tau is the temperature, 2^-60 to 2^60, a in [0, 1] the weight of the labels' loss.
  *     p = softmax over the entries with 0 <= I < V of T / tau
  *     row loss = (1 - a) tau^2 KL(p || softmax(Z / tau)) + a CE(Z, label)
  *     loss [1] = sum_r w_r row_loss_r;   dlogits = d loss / d Z, in Z's type

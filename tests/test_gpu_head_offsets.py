@@ -124,3 +124,12 @@ def test_a_term_of_weight_0_is_left_out(C, dev, v):
             rest = slice(1, 4)
             check(distill(C, dev, zl[rest], t[rest], ids[rest], tau, 0.0, labels[rest], scratch=scratch), zl[rest],
                   t[rest], ids[rest], tau, 0.0)
+
+
+@pytest.mark.parametrize("tau", [2.0 ** -60, 2.0 ** -30, 2.0 ** 30, 2.0 ** 60])
+def test_temperatures_of_the_whole_range(C, dev, below_normal, tau):
+    """(the smallest ones: exponentials below 2^-126 again, times tau < 1; the largest ones have none)"""
+    for v in (500, 50021):
+        z, t, ids, labels = moved(2, v, 6, "f32", 0.0, v)
+        for scratch in (0, 8):
+            check(distill(C, dev, z, t, ids, tau, 0.5, labels, scratch=scratch), z, t, ids, tau, 0.5, labels)

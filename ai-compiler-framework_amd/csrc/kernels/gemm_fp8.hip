@@ -4,7 +4,9 @@
 //   C[m,n] = sum_b SA[m,b] SB[n,b] ( sum over k in block b of A[m,k] B[n,k] ) + bias[n]
 //
 // A [M, K] and B [N, K] are e4m3 or e5m2 each, K-contiguous; their scales are
-// by rows ([M, ceil(K/128)]) or by blocks ([ceil(M/128), ceil(K/128)]).
+// by rows ([M, ceil(K/128)]) or by blocks ([ceil(M/128), ceil(K/128)]).  SA SB is
+// taken first: one multiplication for a block's 4 results a lane, where scaling
+// each result twice would cost 3 more (39 and 49 cycles an MFMA, below).
 //
 // A K-step is one scale block, 128 bytes a row: its products start from zero,
 // and the four results a lane are added to the f32 accumulators with one
@@ -13,9 +15,15 @@
 // 16-bit outputs: one v_mfma_f32_16x16x128_f8f6f4 a block.  That instruction
 // (and every other 8-bit one) adds the products of 8 consecutive K after
 // aligning them to the largest, and keeps 13 bits below its exponent; the groups
-// of 8 are added in f32.  On normally distributed codes the result is off by
-// 1.5e-5 in the 2-norm, where an output of 16 bits is off by 2e-4 (f16) or 1.7e-3
-// (bf16) through its own rounding.
+// of 8 are added in f32.  So a result is off by up to 7 2^-13 of the sum of the
+// groups' largest products, whatever cancels behind them.  512 x 512 x 4096,
+// quantised values, error in the 2-norm relative to the result's, f16 and bf16
+// outputs (their rounding alone: 2.07e-4, 1.66e-3):
+//   normally distributed               2.08e-4  1.66e-3  (unrounded 1.5e-5)
+//   1% of A's channels 1000 x larger   2.19e-4  1.66e-3
+//   A log-normal, sigma 2              2.15e-4  1.65e-3
+//   pairs that cancel to some 2%       3.16e-4  1.68e-3
+// The last, and single results near 0, show it.  f32 outputs have f32 sums.
 // f32 outputs: the codes become bf16, which holds both 8-bit types exactly, and
 // four v_mfma_f32_16x16x32_bf16 make the block's products and f32 sums (off by
 // 1e-8), at half the rate.

@@ -154,9 +154,11 @@ extern "C" {
  *   C [M, N] f32/f16/bf16; the scales as QUANT_FP8 writes them, each by rows
  *   or by blocks, with any strides; the f8 types of A and B may differ.
  *     C[m,n] = sum_b SA[m,b] SB[n,b] (sum over k in block b of A[m,k] B[n,k]) + bias[n]
- *   in f32, rounded once; for C of 16 bits the products of 8 consecutive K are
- *   aligned to their largest and keep 13 bits below its exponent (the sum is off
- *   by some 1e-5 of its terms' magnitude).  K >= 1; M = 0 or N = 0 writes nothing.
+ *   in f32, SA SB first (where that product of two scales is no normal f32, bits or
+ *   the result are lost), rounded once.  For C of 16 bits the products of 8
+ *   consecutive K are aligned to their largest and keep 13 bits below its exponent:
+ *   some 1e-6 to 1e-5 of the terms' magnitudes, up to 7 2^-13 of each group's
+ *   largest; with f32 C all products and sums are f32.  K >= 1; M = 0 or N = 0 writes nothing.
  *
  * DISTILL_TOPK: logits Z [R, V] f32/f16/bf16, R >= 1, V <= 2^28; teacher logits
  *   T [R, K] f32/f16/bf16 and their classes I [R, K] i32, 1 <= K <= 1024; labels

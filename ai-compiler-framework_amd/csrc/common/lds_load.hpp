@@ -25,7 +25,7 @@ __device__ void raw_buffer_load_lds(i32x4_t rsrc, __attribute__((address_space(3
 // v_readfirstlane of the resource base right before the asm ended in a GPU
 // memory fault.)  PAD: the loads of a tile's first stages, which follow the
 // resource set-up; the K loop's loads (scalar offsets from SALU adds) keep
-// s_nop 0 for the M0 write, and a codegen test checks every asm load's wait
+// s_nop 0 for the M0 write, and codegen tests check every asm load's wait
 // states against the VALU writes before it.
 // The compiler does not know that it writes LDS, so it adds no vmcnt wait in
 // front of the LDS reads that follow it: it cannot prove that a transposing
@@ -75,7 +75,8 @@ __device__ __forceinline__ i32x4_t buffer_rsrc(const void* base, uint32_t bytes)
 }
 
 // Waits until at most N of the wave's vector-memory operations, and none of
-// its LDS operations, are in flight.
+// its LDS operations, are in flight.  (s_waitcnt immediate, gfx9 layout: vmcnt bits
+// 3:0 and 15:14, expcnt 6:4, left alone, lgkmcnt 11:8.)
 template <int N>
 __device__ __forceinline__ void wait_vm_lgkm0() {
   static_assert(N >= 0 && N < 64, "vmcnt is 6 bits");

@@ -761,8 +761,6 @@ constexpr bool nt_persistent(int BM, int BN, int WM, int WN) {
   return BM == 256 && BN == 256 && WM * WN == 8;
 }
 
-// s_waitcnt immediate for vmcnt(n), lgkmcnt(0), expcnt left alone (gfx9
-// layout: vmcnt bits 3:0 and 15:14, expcnt 6:4, lgkmcnt 11:8).
 // S: LDS stages.  Two for the large tiles (their K-step's MFMA work covers a
 // load's latency); small tiles, whose K-step is a few hundred cycles of MFMA
 // work, keep S - 1 K-steps of loads in flight.

@@ -366,8 +366,9 @@ __device__ __forceinline__ void write_zeros(const DistillArgs& a, int64_t row, i
 }
 
 // One workgroup a row: 4096 x 32000 bf16 101 us (5.2 TB/s, HBM), 1023 x 50021 f32
-// 96 (4.3: a CU holds one row at a time), 1 x 9000 bf16 10 (its chain of loads and
-// reductions, and the loss).
+// 98 (4.2: a CU holds one row at a time), 1 x 9000 bf16 10 (its chain of loads and
+// reductions, and the loss).  The loss alone, with its launch: 4096 x 32000 bf16 53
+// (both 106), 1023 x 50021 f32 57 (100).
 // Where the row takes at most 32 registers a thread, 8 waves fit a SIMD: a row's
 // chain of loads and reductions hides behind other rows'.
 template <int NT, int EK, int VPT, bool DUAL>
@@ -662,8 +663,8 @@ DistillArgs from_row(const DistillArgs& a, int tk, int64_t r, int64_t rows) {
 template <int EK, bool DUAL>
 Status distill_rows(const DistillArgs& a, int tk, float* scratch, int ldp, hipStream_t s) {
   // Few long rows share the chip: parts of 2048 columns or more, about two
-  // workgroups a CU.  A row a workgroup against this: 8 x 200000 bf16 34.3 us
-  // (15.2), 8 x 65536 15.4 (13.8), f32 20.2 (13.6), 48 x 131072 22.3 (21.3); the
+  // workgroups a CU.  A row a workgroup against this: 8 x 200000 bf16 37.9 us
+  // (17.1), 8 x 65536 19.4 (16.6), f32 22.2 (16.3), 48 x 131072 28.2 (24.9); the
   // other way 8 x 32000 f32 12.8 (15.1), 128 x 131072 f32 45.8 (51.3).
   const unsigned lds = special_bytes(a.K);
   int64_t P = (512 + a.R - 1) / a.R;

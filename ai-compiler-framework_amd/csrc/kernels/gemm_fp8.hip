@@ -302,12 +302,19 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_fp8_kernel(Fp8Gemm p) {
 // that no multiply-add waits for its MFMA.  A last, partial block goes through
 // registers with zeros behind K.
 // 8192 x 4096 x 4096 bf16 126-138 us (2.0-2.2 PFLOP/s; the library's 8-bit product
-// 2.8), 11008 x 4096 x 8192 f32 704 us (1.05; bf16 products 1.45).  Bound by the
-// matrix cores and the VALU beside them: an 8-bit MFMA alone issues every 35
-// cycles a SIMD, with the 5 multiply-adds of a block's results 39, with 8 (B's
-// scales by rows) 49; f32 outputs have 2 conversions and 2 multiply-adds beside
-// each bf16 MFMA (18 cycles alone, 24 with two).  Their 256 x 256 tiles would not
-// fit the LDS.  1 x 32000 x 4096 f32: 21-25 us, B at 5.2-6.1 TB/s.
+// 2.8): by its counters the matrix cores are busy 47% of the cycles (at 2.07 GHz),
+// the other VALU instructions, 5.5 an MFMA, take 33% at 4 cycles each, the waves wait
+// for loads, LDS or the barrier in 31% of their time, and 11% of the cycles a CU
+// has no wave (it takes two tiles one after the other, one workgroup at a time, so
+// each tile's first loads and its output stand alone).  Issue alone explains little of
+// it: an 8-bit MFMA issues every 35 cycles a SIMD, with the 5 multiply-adds of a
+// block's results every 39, with 8 (B's scales by rows) 49.
+// 11008 x 4096 x 8192 f32 700 us (1.05; bf16 products 1.45): MFMA busy 50% of the
+// cycles (at 1.83 GHz), the 4.3 other VALU instructions an MFMA 54%, so the two
+// hardly overlap.  Two of those are conversions, one more than needed: each
+// fragment is converted by the two waves that read it.  256 x 256 tiles would need
+// their f32 output staged in parts; they were not tried so.
+// 1 x 32000 x 4096 f32: 21-25 us, B at 5.2-6.1 TB/s.
 // ---------------------------------------------------------------------------
 template <int BM, int BN, int WM, int WN, int S, int AF, int BF, bool BROW, bool EXACT>
 __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_fp8_lds_kernel(Fp8Gemm p) {

@@ -195,7 +195,8 @@ extern "C" {
  *   a row of nothing else gives token -1 and log-probability -inf.  A third
  *   output, i32 [R, S] with S >= 8192, is scratch that lets several workgroups
  *   share a row where there are few long rows (used where S is even and its
- *   address a multiple of 8).
+ *   address a multiple of 8), as for DISTILL_TOPK: what it holds means nothing, and
+ *   calls that may run at the same time need scratch of their own.
  */
 
 /* GEPI epilogue kinds.  0..2 are the values core_v2/exec.py:223-252 packs;

@@ -29,7 +29,8 @@ HIPCC = str(ROCM / "bin" / "hipcc")
 
 HIP_SOURCES = ["kernels/optim.hip", "kernels/eltwise.hip", "kernels/reduce.hip", "kernels/gemm.hip",
                "kernels/gemm_edge.hip", "kernels/norm.hip", "kernels/diag.hip", "kernels/smallstep.hip",
-               "kernels/quant_fp8.hip", "kernels/gemm_fp8.hip", "kernels/distill.hip", "kernels/sample.hip"]
+               "kernels/quant_fp8.hip", "kernels/gemm_fp8.hip", "kernels/distill.hip", "kernels/sample.hip",
+               "kernels/linear_xent.hip", "kernels/grad_norm.hip"]
 CXX_SOURCES = ["registry/registry.cpp", "registry/register_all.cpp", "runtime/graph.cpp"]
 
 HIP_FLAGS = [

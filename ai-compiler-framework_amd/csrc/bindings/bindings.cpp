@@ -65,6 +65,8 @@ enum class OpKind : int {
   GemmFp8 = AICF_OP_GEMM_FP8,
   DistillTopk = AICF_OP_DISTILL_TOPK,
   SampleRow = AICF_OP_SAMPLE_ROW,
+  LinearXent = AICF_OP_LINEAR_XENT,
+  GradNorm = AICF_OP_GRAD_NORM,
 };
 
 std::string tensor_brief(const torch::Tensor& t) {
@@ -164,9 +166,13 @@ struct Call {
   }
 };
 
-// The appended ops from QuantFp8 on launch on the current device only.
-void check_device(int kind, const py::sequence& seq, const char* what) {
-  if (kind < AICF_OP_QUANT_FP8) return;
+// The appended ops from QuantFp8 on, and AdamW with the clip factor, launch on
+// the current device only.
+bool current_device_only(int kind, const Call& c) {
+  return kind >= AICF_OP_QUANT_FP8 ||
+         (kind == AICF_OP_ADAM_STEP && c.in.size() == 6 && c.in[4].dtype == AICF_DTYPE_I32);
+}
+void check_device(const py::sequence& seq, const char* what) {
   const int cur = c10::hip::getCurrentHIPStream().device_index();
   for (auto h : seq) {
     torch::Tensor t = py::cast<torch::Tensor>(h);
@@ -178,8 +184,10 @@ void check_device(int kind, const py::sequence& seq, const char* what) {
 void op_call_impl(int kind, const py::sequence& inputs, const py::sequence& outputs,
                   uint32_t schema_id, const py::bytes& attrs_bytes, uint64_t stream_u64) {
   Call c(inputs, outputs, schema_id, attrs_bytes, stream_u64);
-  check_device(kind, inputs, "inputs");
-  check_device(kind, outputs, "outputs");
+  if (current_device_only(kind, c)) {
+    check_device(inputs, "inputs");
+    check_device(outputs, "outputs");
+  }
   {
     std::lock_guard<std::mutex> lock(g_mu);
     if (g_trace_enabled) g_trace.emplace_back(aicf_opkind_name(kind));
@@ -197,8 +205,10 @@ void launch_by_id_impl(const std::string& kid, int kind, const py::sequence& inp
                        const py::sequence& outputs, uint32_t schema_id,
                        const py::bytes& attrs_bytes, uint64_t stream_u64) {
   Call c(inputs, outputs, schema_id, attrs_bytes, stream_u64);
-  check_device(kind, inputs, "inputs");
-  check_device(kind, outputs, "outputs");
+  if (current_device_only(kind, c)) {
+    check_device(inputs, "inputs");
+    check_device(outputs, "outputs");
+  }
   {
     std::lock_guard<std::mutex> lock(g_mu);
     if (g_trace_enabled)
@@ -266,6 +276,8 @@ PYBIND11_MODULE(_C, m) {
       .value("GemmFp8", OpKind::GemmFp8)
       .value("DistillTopk", OpKind::DistillTopk)
       .value("SampleRow", OpKind::SampleRow)
+      .value("LinearXent", OpKind::LinearXent)
+      .value("GradNorm", OpKind::GradNorm)
       .export_values();
 
   m.def(
@@ -378,6 +390,19 @@ PYBIND11_MODULE(_C, m) {
         py::arg("handle"));
 
   // introspection helpers (not in the reference binding)
+  // scratch of LinearXent in bytes (see aicf_hip.h)
+  m.def(
+      "linear_xent_scratch",
+      [](int64_t rows, int64_t classes, int64_t dim, py::object dtype, bool gradients, int64_t piece) -> int64_t {
+        const auto st = torch::python::detail::py_object_to_dtype(dtype);
+        const int d = st == at::kFloat ? AICF_DTYPE_F32 : st == at::kHalf ? AICF_DTYPE_F16
+                      : st == at::kBFloat16 ? AICF_DTYPE_BF16 : AICF_DTYPE_UNKNOWN;
+        const int64_t n = aicf_linear_xent_scratch(rows, classes, dim, d, gradients ? 1 : 0, piece);
+        if (n < 0) throw std::runtime_error("linear_xent_scratch: sizes or dtype out of range");
+        return n;
+      },
+      py::arg("rows"), py::arg("classes"), py::arg("dim"), py::arg("dtype"), py::arg("gradients") = true,
+      py::arg("piece") = (int64_t)0);
   m.def("registry_kernel_ids", [](int kind) {
     std::vector<std::string> ids;
     const int n = aicf_registry_count(kind);

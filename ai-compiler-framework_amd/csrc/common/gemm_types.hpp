@@ -16,7 +16,13 @@ enum InKind { IN_F32 = 0, IN_F16 = 1, IN_BF16 = 2 };
 enum OutKind { OUT_F32 = 0, OUT_F16 = 1, OUT_BF16 = 2 };
 // ACT_ADAMW (fp32 accumulators only): the tile is the gradient of a weight
 // matrix; the epilogue applies AdamW to that weight instead of storing it.
-enum Act { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2, ACT_DGELU = 3, ACT_ADAMW = 4 };
+// ACT_LX_*: the products of the linear cross-entropy (linear_xent.hip): logits
+// whose statistics are kept, logits that become their gradient, and products
+// with that gradient, finished or as f32 sums.
+enum Act {
+  ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2, ACT_DGELU = 3, ACT_ADAMW = 4,
+  ACT_LX_STATS = 5, ACT_LX_GRAD = 6, ACT_LX_OUT = 7, ACT_LX_SLAB = 8
+};
 
 // Optimizer state a fused weight-gradient GEMM updates in place ([M, N]
 // row-major like the output, leading dimension ldc).

@@ -75,6 +75,8 @@ enum class OpKind : int {
   GemmFp8 = AICF_OP_GEMM_FP8,
   DistillTopk = AICF_OP_DISTILL_TOPK,
   SampleRow = AICF_OP_SAMPLE_ROW,
+  LinearXent = AICF_OP_LINEAR_XENT,
+  GradNorm = AICF_OP_GRAD_NORM,
   _Count = AICF_OP_COUNT,
 };
 

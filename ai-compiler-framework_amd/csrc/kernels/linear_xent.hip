@@ -1,0 +1,898 @@
+// Softmax cross-entropy of a vocabulary head from its hidden rows and weights,
+// with the gradients of both; the logits are not kept.
+//
+//   z = X W^T [R, V] (f32 sums),  lse_r = log sum_v exp z_rv
+//   row loss_r = lse_r - z_{r, label},  loss = sum_r w_r row loss_r
+//   G = w_r (exp(z - lse) - onehot(label)),  dX = G W,  dW = G^T X
+//
+// The rows that count (a label, a weight other than 0) are gathered first, so
+// that the others cost nothing and nothing in them reaches a product; how many
+// they are only the device knows, and the products' grids cover all rows.
+//
+//   1. logits: tiles of the MFMA GEMM whose epilogue keeps, for each row and
+//      tile of classes, the maximum and the sum of exp(z - maximum); of the
+//      last `piece` classes also exp(z - tile maximum) itself, in the operands'
+//      type (a rounding of 2^-9 in bf16, 2^-12 in f16, as any operand of a
+//      product has; the sums are taken before it);
+//   2. the row's statistics are joined; the kept values become G in place,
+//      scaled to the type's range by a power of two that the products take out
+//      again (weights of 1/R would leave f16's range);
+//   3. dW and dX of those classes;
+//   4. the other pieces: logits once more, whose epilogue knows the row's
+//      statistics and writes G, then dW and dX as before.
+// So the scratch decides what is computed twice: 6 n V D operations where it
+// holds all classes (n rows that count), up to 8 n V D where it holds few.
+// dX is summed over the pieces, and over shares of the classes where its tiles
+// are fewer than the CUs, in f32 slabs that are joined in a fixed order.
+//
+// No counterpart in the reference.
+#include <algorithm>
+
+#include "../common/gemm_nt.hpp"
+#include "../common/head_util.hpp"
+
+namespace aicf::hip {
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// 2^((z - m) log2 e): the difference first, so that the exponent is off by
+// roundings of itself alone however far the logits lie from zero.
+__device__ __forceinline__ float exp_from(float z, float m) { return __builtin_amdgcn_exp2f((z - m) * kLog2e); }
+// A maximum over nothing but -inf is no reference: their exponentials are 0.
+__device__ __forceinline__ float safe_ref(float m) { return m == -INFINITY ? 0.0f : m; }
+// What a sum of exp(z - m) is multiplied by where the reference becomes `to`.
+__device__ __forceinline__ float rebase(float m, float to) { return m == -INFINITY ? 0.0f : exp_from(m, to); }
+
+// ---------------------------------------------------------------------------
+// The products' epilogues
+// ---------------------------------------------------------------------------
+template <int OUT, int ACT, int BM, int BN, int WM, int WN, int STAGE_BYTES, int MS>
+__device__ __forceinline__ void lx_epilogue(const NTParams& p, nt_acc_t<MS> (&acc)[BN / WN / MS][BM / WM / MS],
+                                            uint8_t* smem, int m0, int n0) {
+  constexpr int NW = WM * WN, NT = 64 * NW;
+  constexpr int WTM = BM / WM, WTN = BN / WN;
+  constexpr int TM = WTM / MS, TN = WTN / MS;
+  constexpr int G = MS == 32 ? 4 : 1;  // quads of columns a block (see nt_epilogue_staged)
+  constexpr int OB = OUT == OUT_F32 ? 4 : 2;
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));  // nothing of the epilogue is computed before the K loop
+  const int lane = tid & 63, wave = tid >> 6;
+  const int wm = wave / WN, wn = wave % WN;
+  const int fr = lane % MS, fh = lane / MS;
+  auto col_of = [&](int i, int g) -> int { return wn * WTN + i * MS + (MS == 32 ? 8 * g + 4 * fh : 4 * fh); };
+  auto row_of = [&](int j) -> int { return wm * WTM + j * MS + fr; };
+
+  if constexpr (ACT == ACT_LX_STATS) {
+    float* red_m = reinterpret_cast<float*>(smem);  // [WN][BM]
+    float* red_s = red_m + WN * BM;
+    static_assert(2 * WN * BM * 4 <= STAGE_BYTES, "the waves' statistics fit");
+    const int ncol = p.N - n0;
+    if (ncol < BN) {  // the last tile's columns without a class
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (col_of(i, g) + e >= ncol) {
+#pragma unroll
+              for (int j = 0; j < TM; ++j) acc[i][j][4 * g + e] = -INFINITY;
+            }
+    }
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+      float m = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int r = 0; r < 4 * G; ++r) m = fmaxf(m, acc[i][j][r]);
+      if constexpr (MS == 16) m = fmaxf(m, __shfl_xor(m, 16, 64));
+      m = fmaxf(m, __shfl_xor(m, 32, 64));
+      if (fh == 0) red_m[wn * BM + row_of(j)] = m;
+    }
+    // the label's logit: one lane of one tile has it
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+      const int m = m0 + row_of(j);
+      const int c = m < p.M ? p.lx.label[m] - p.lx.v0 - n0 : -1;
+      if (c >= 0 && c < BN) {
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+          for (int g = 0; g < G; ++g)
+            if ((c >> 2) == (col_of(i, g) >> 2)) {
+              const int e = c & 3;
+              p.lx.zlab[m] = e == 0 ? acc[i][j][4 * g] : e == 1 ? acc[i][j][4 * g + 1]
+                           : e == 2 ? acc[i][j][4 * g + 2] : acc[i][j][4 * g + 3];
+            }
+      }
+    }
+    __syncthreads();
+    const bool keep = n0 >= p.lx.keep_from;
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+      float m = red_m[row_of(j)];
+#pragma unroll
+      for (int w = 1; w < WN; ++w) m = fmaxf(m, red_m[w * BM + row_of(j)]);
+      m = safe_ref(m);
+      float s = 0.0f;
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int r = 0; r < 4 * G; ++r) {
+          const float e = exp_from(acc[i][j][r], m);
+          s += e;
+          acc[i][j][r] = e * p.lx.keep_scale;
+        }
+      if constexpr (MS == 16) s += __shfl_xor(s, 16, 64);
+      s += __shfl_xor(s, 32, 64);
+      if (fh == 0) red_s[wn * BM + row_of(j)] = s;
+    }
+    __syncthreads();
+    for (int t = tid; t < BM; t += NT) {
+      float m = red_m[t], s = red_s[t];
+#pragma unroll
+      for (int w = 1; w < WN; ++w) {
+        m = fmaxf(m, red_m[w * BM + t]);
+        s += red_s[w * BM + t];
+      }
+      p.lx.stats[(int64_t)((p.lx.v0 + n0) / BN) * p.lx.stats_ld + m0 + t] = make_float2(m, s);
+    }
+    if (!keep) return;
+    __syncthreads();
+  } else if constexpr (ACT == ACT_LX_GRAD) {
+    const int ncol = p.N - n0;
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+      const int m = m0 + row_of(j);
+      const bool in = m < p.M;
+      const float rm = in ? safe_ref(p.lx.row_max[m]) : 0.0f, f = in ? p.lx.row_f[m] : 0.0f;
+      const float w = in ? p.lx.row_w[m] : 0.0f;
+      const int c = in ? p.lx.label[m] - p.lx.v0 - n0 : -1;
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int col = col_of(i, g) + e;
+            float v = exp_from(acc[i][j][4 * g + e], rm) * f;
+            v = col == c ? v - w : v;
+            acc[i][j][4 * g + e] = col < ncol ? v : 0.0f;
+          }
+    }
+  } else if constexpr (ACT == ACT_LX_OUT) {
+    const float a = p.lx.alpha[0];
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+      for (int j = 0; j < TM; ++j)
+#pragma unroll
+        for (int r = 0; r < 4 * G; ++r) acc[i][j][r] *= a;
+  }
+
+  // Through LDS, so that whole rows are stored (as nt_epilogue_staged does).
+  constexpr int ROWB = BN * OB, CPR = ROWB / 16, CE = 16 / OB;
+  constexpr int ROWS_PASS = STAGE_BYTES / ROWB < BM ? STAGE_BYTES / ROWB : BM;
+  constexpr int NPASS = BM / ROWS_PASS, JP = TM / NPASS, WROWS = JP * MS;
+  static_assert(NPASS * ROWS_PASS == BM && JP * NPASS == TM, "pass split");
+  static_assert((CPR & (CPR - 1)) == 0 && (ROWS_PASS * CPR) % NT == 0, "chunk split");
+  typedef typename std::conditional<OB == 4, float, uint16_t>::type out_t;
+#pragma unroll
+  for (int pass = 0; pass < NPASS; ++pass) {
+#pragma unroll
+    for (int jj = 0; jj < JP; ++jj)
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          const nt_acc_t<MS>& a = acc[i][pass * JP + jj];
+          const int pr = wm * WROWS + jj * MS + fr, cb = col_of(i, g) * OB;
+          uint8_t* at = smem + pr * ROWB + (((cb / 16) ^ (pr & (CPR - 1))) * 16) + cb % 16;
+          if constexpr (OUT == OUT_F32) {
+            *reinterpret_cast<f32x4*>(at) = f32x4{a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]};
+          } else if constexpr (OUT == OUT_BF16) {
+            typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+            *reinterpret_cast<u32x2*>(at) =
+                u32x2{f32x2_to_bf16x2(a[4 * g], a[4 * g + 1]), f32x2_to_bf16x2(a[4 * g + 2], a[4 * g + 3])};
+          } else {
+            *reinterpret_cast<u16x4*>(at) = u16x4{f32_to_f16(a[4 * g]), f32_to_f16(a[4 * g + 1]),
+                                                  f32_to_f16(a[4 * g + 2]), f32_to_f16(a[4 * g + 3])};
+          }
+        }
+    __syncthreads();
+#pragma unroll 4
+    for (int k = 0; k < ROWS_PASS * CPR / NT; ++k) {
+      const int idx = tid + k * NT, pr = idx / CPR, c = idx % CPR;
+      const u16x8 x = *reinterpret_cast<const u16x8*>(smem + pr * ROWB + ((c ^ (pr & (CPR - 1))) * 16));
+      const int m = m0 + (pr / WROWS) * WTM + pass * WROWS + (pr % WROWS);
+      if (m >= p.M) continue;
+      if constexpr (ACT == ACT_LX_SLAB) {
+        const int n = n0 + c * CE;
+        if (n >= p.ldc) continue;  // (a slab's rows are whole 64s)
+        f32x4* q = reinterpret_cast<f32x4*>((float*)p.C + (int64_t)m * p.ldc + n);
+        f32x4 v = __builtin_bit_cast(f32x4, x);
+        if ((int)blockIdx.y < p.lx.add) v += *q;
+        *q = v;
+      } else if constexpr (ACT != ACT_LX_OUT) {  // G's rows hold whole tiles
+        out_t* q = (out_t*)p.C + (int64_t)m * p.ldc + (n0 - (ACT == ACT_LX_STATS ? p.lx.keep_from : 0)) + c * CE;
+        *reinterpret_cast<u16x8*>(q) = x;
+      } else {
+        const int n = n0 + c * CE;
+        const int64_t row = p.lx.row_map ? p.lx.row_map[m] : m;
+        out_t* q = (out_t*)p.C + row * p.ldc + n;
+        if (p.lx.vec && n + CE <= p.N) {
+          *reinterpret_cast<u16x8*>(q) = x;
+        } else {
+#pragma unroll
+          for (int e = 0; e < CE; ++e)
+            if (n + e < p.N) {
+              if constexpr (OUT == OUT_F32) q[e] = __builtin_bit_cast(f32x4, x)[e];
+              else q[e] = x[e];
+            }
+        }
+      }
+    }
+    if (pass + 1 < NPASS) __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Rows
+// ---------------------------------------------------------------------------
+// Scratch of a call, in this order; every array starts on 256 bytes.
+struct LxRows {
+  int32_t* head;    // [0] rows that count, [1] f32 alpha: what the products with G are multiplied by
+  int32_t* pos;     // [R] place of a row among those that count, -1: left out
+  int32_t* idx;     // [Rp] and back
+  int32_t* label;   // [Rp] of the rows that count, like all below
+  float* weight;    // as given
+  float* row_w;     // times 1 / alpha
+  float* zlab;
+  float* row_max;
+  float* row_f;     // row_w / sum of exp(z - row_max)
+  float* row_loss;
+  float2* stats;    // [tiles of classes][Rp]
+  void* xc;         // [Rp][Dp] rows of X, zeros behind D
+  float* slab;      // dX in f32, one for each share of the classes
+  void* wpad;       // [piece][Dp] rows of W, where W itself cannot be read in tiles
+  void* g;          // [Rp][piece]
+};
+
+// Which rows count, and the power of two that brings the largest weight to
+// 2^(top-1) .. 2^top.  One workgroup: a thread takes consecutive rows.
+__global__ __launch_bounds__(1024) void lx_rows_kernel(const int32_t* __restrict__ labels,
+                                                       const float* __restrict__ w, int R, int V, int top,
+                                                       LxRows s) {
+  __shared__ int cnt[17];
+  __shared__ float big[17];
+  const int per = (R + 1023) / 1024, r0 = threadIdx.x * per, r1 = r0 + per < R ? r0 + per : R;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  auto counts = [&](int r) {
+    const int c = labels[r];
+    return c >= 0 && c < V && (!w || w[r] != 0.0f);
+  };
+  int n = 0;
+  float most = 0.0f;
+  for (int r = r0; r < r1; ++r)
+    if (counts(r)) {
+      ++n;
+      if (w) most = fmaxf(most, fabsf(w[r]));
+    }
+  int before = n;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int o = __shfl_up(before, off, 64);
+    if (lane >= off) before += o;
+  }
+  most = wave_max(most);
+  if (lane == 63) cnt[wave] = before;
+  if (lane == 0) big[wave] = most;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int sum = 0;
+    float m = 0.0f;
+    for (int i = 0; i < 16; ++i) {
+      const int c = cnt[i];
+      cnt[i] = sum;
+      sum += c;
+      m = fmaxf(m, big[i]);
+    }
+    cnt[16] = sum;
+    big[16] = m;
+  }
+  __syncthreads();
+  const int total = cnt[16];
+  const float mean = total > 0 ? 1.0f / (float)total : 0.0f;
+  const float m = w ? big[16] : mean;
+  int e = 0;
+  if (m > 0.0f && m < INFINITY) frexpf(m, &e);  // m < 2^e
+  e = top - e;
+  e = e > 126 ? 126 : e < -126 ? -126 : e;
+  const float up = ldexpf(1.0f, e);
+  if (threadIdx.x == 0) {
+    s.head[0] = total;
+    s.head[1] = __float_as_int(ldexpf(1.0f, -e));
+  }
+  int at = cnt[wave] + before - n;
+  for (int r = r0; r < r1; ++r) {
+    const bool c = counts(r);
+    s.pos[r] = c ? at : -1;
+    if (c) {
+      const float wr = w ? w[r] : mean;
+      s.idx[at] = r;
+      s.label[at] = labels[r];
+      s.weight[at] = wr;
+      s.row_w[at] = wr * up;
+      ++at;
+    }
+  }
+}
+
+template <int ES>
+struct LxElem;
+template <>
+struct LxElem<2> {
+  typedef uint16_t T;
+  typedef u16x8 vec;
+  typedef u16x8_a2 loose;
+};
+template <>
+struct LxElem<4> {
+  typedef float T;
+  typedef f32x4 vec;
+  typedef f32x4_a4 loose;
+};
+
+// Rows copied onto 16-byte steps, zeros behind the D-th element to Dp (a
+// multiple of 64); pos: to row pos[r], and a row that is left out has its
+// gradient and loss cleared instead.  A wave a row.
+template <int ES>
+__global__ __launch_bounds__(256) void lx_copy_rows_kernel(const void* __restrict__ src, int64_t lds, void* dst,
+                                                           int D, int Dp, int rows, const int32_t* __restrict__ pos,
+                                                           void* dx, int64_t lddx, float* row_loss) {
+  typedef typename LxElem<ES>::T T;
+  typedef typename LxElem<ES>::vec vec;
+  typedef typename LxElem<ES>::loose loose;
+  constexpr int CE = 16 / ES;
+  const int lane = threadIdx.x & 63;
+  const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r >= rows) return;
+  const int to = pos ? pos[r] : r;
+  if (to >= 0) {
+    const T* a = (const T*)src + (int64_t)r * lds;
+    T* b = (T*)dst + (int64_t)to * Dp;
+    for (int c = lane * CE; c < Dp; c += 64 * CE) {
+      vec v;
+      if (c + CE <= D) {
+        v = *reinterpret_cast<const loose*>(a + c);
+      } else {
+#pragma unroll
+        for (int e = 0; e < CE; ++e) v[e] = c + e < D ? a[c + e] : T(0);
+      }
+      *reinterpret_cast<vec*>(b + c) = v;
+    }
+    return;
+  }
+  if (lane == 0) row_loss[r] = 0.0f;
+  if (!dx) return;
+  T* b = (T*)dx + (int64_t)r * lddx;
+  for (int c = lane * CE; c < D; c += 64 * CE) {
+    if (c + CE <= D) {
+      loose v;
+#pragma unroll
+      for (int e = 0; e < CE; ++e) v[e] = T(0);
+      *reinterpret_cast<loose*>(b + c) = v;
+    } else {
+      for (int e = 0; c + e < D; ++e) b[c + e] = T(0);
+    }
+  }
+}
+
+// The statistics of a row's tiles joined: 64 rows a workgroup, wave w takes
+// tiles w, w + 16, ...; the waves in order.
+__global__ __launch_bounds__(1024) void lx_stats_kernel(LxRows s, int tiles, int64_t ld,
+                                                        float* __restrict__ row_loss) {
+  __shared__ float2 red[16][64];
+  const int n = s.head[0], lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r = blockIdx.x * 64 + lane;
+  if (blockIdx.x * 64 >= n) return;
+  float m = -INFINITY, sum = 0.0f;
+  for (int t = wave; t < tiles; t += 16) {
+    const float2 v = s.stats[(int64_t)t * ld + r];  // (rows behind n: whatever is there, not used)
+    const float top = fmaxf(m, v.x), ref = safe_ref(top);
+    sum = sum * rebase(m, ref) + v.y * rebase(v.x, ref);
+    m = top;
+  }
+  red[wave][lane] = make_float2(m, sum);
+  __syncthreads();
+  if (wave > 0 || r >= n) return;
+  m = red[0][lane].x;
+#pragma unroll
+  for (int w = 1; w < 16; ++w) m = fmaxf(m, red[w][lane].x);
+  const float ref = safe_ref(m);
+  sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) sum += red[w][lane].y * rebase(red[w][lane].x, ref);
+  s.row_max[r] = m;
+  s.row_f[r] = s.row_w[r] / sum;
+  const float loss = logf(sum) + (ref - s.zlab[r]);
+  s.row_loss[r] = loss;
+  row_loss[s.idx[r]] = loss;
+}
+
+// loss = sum of weight * row loss, in f64 and a fixed order.
+__global__ __launch_bounds__(1024) void lx_loss_kernel(LxRows s, float* __restrict__ loss) {
+  __shared__ double red[16];
+  const int n = s.head[0];
+  double v = 0.0;
+  for (int r = threadIdx.x; r < n; r += 1024) v += (double)s.weight[r] * (double)s.row_loss[r];
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    v = red[0];
+    for (int i = 1; i < 16; ++i) v += red[i];
+    loss[0] = (float)v;
+  }
+}
+
+// The kept exp(z - tile maximum) of classes v0 .. v0 + cols become G in place.
+// A lane takes 16 bytes; a tile of BN classes has one factor a row.
+template <int EK, int BN>
+__global__ __launch_bounds__(256) void lx_scale_kernel(LxRows s, int64_t ldg, int width, int v0, int64_t stats_ld,
+                                                       float keep_scale) {
+  constexpr int ES = EK == EL_F32 ? 4 : 2, CE = 16 / ES;
+  typedef typename LxElem<ES>::T T;
+  typedef typename LxElem<ES>::vec vec;
+  const int n = s.head[0];
+  const int c = (blockIdx.x * 256 + threadIdx.x) * CE;
+  if (c >= width) return;
+  for (int r = blockIdx.y; r < n; r += gridDim.y) {
+    const float2 st = s.stats[(int64_t)((v0 + c) / BN) * stats_ld + r];
+    const float f = rebase(st.x, safe_ref(s.row_max[r])) * s.row_f[r] / keep_scale;
+    T* q = (T*)s.g + (int64_t)r * ldg + c;
+    vec x = *reinterpret_cast<const vec*>(q);
+    const int at = s.label[r] - v0 - c;
+    float v[CE];
+#pragma unroll
+    for (int e = 0; e < CE; ++e) {
+      if constexpr (EK == EL_F32) v[e] = x[e] * f;
+      else if constexpr (EK == EL_F16) v[e] = f16_to_f32(x[e]) * f;
+      else v[e] = bf16_to_f32(x[e]) * f;
+    }
+    if (at >= 0 && at < CE) {
+      const float w = s.row_w[r];
+#pragma unroll
+      for (int e = 0; e < CE; ++e) v[e] = e == at ? v[e] - w : v[e];
+    }
+#pragma unroll
+    for (int e = 0; e < CE; ++e) {
+      if constexpr (EK == EL_F32) x[e] = v[e];
+      else if constexpr (EK == EL_F16) x[e] = f32_to_f16(v[e]);
+      else x[e] = f32_to_bf16(v[e]);
+    }
+    *reinterpret_cast<vec*>(q) = x;
+  }
+}
+
+// dX from its slabs: alpha times their sum, in order, to the row it came from.
+template <int EK>
+__global__ __launch_bounds__(256) void lx_finish_kernel(LxRows s, int shares, int64_t stride, int64_t ld, int D,
+                                                        void* dx, int64_t lddx) {
+  const int n = s.head[0];
+  const float alpha = __int_as_float(s.head[1]);
+  const int c = (blockIdx.x * 256 + threadIdx.x) * 4;
+  if (c >= D) return;
+  for (int r = blockIdx.y; r < n; r += gridDim.y) {
+    f32x4 v = *reinterpret_cast<const f32x4*>(s.slab + (int64_t)r * ld + c);
+    for (int k = 1; k < shares; ++k) v += *reinterpret_cast<const f32x4*>(s.slab + k * stride + (int64_t)r * ld + c);
+    const int64_t at = (int64_t)s.idx[r] * lddx + c;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (c + e < D) {
+        const float x = v[e] * alpha;
+        if constexpr (EK == EL_F32) ((float*)dx)[at + e] = x;
+        else ((uint16_t*)dx)[at + e] = EK == EL_F16 ? f32_to_f16(x) : f32_to_bf16(x);
+      }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+int64_t up_to(int64_t n, int64_t step) { return (n + step - 1) / step * step; }
+
+// Tiles of a product of `rows` rows: 32, 64, 128 or 256 of them.
+int lx_tile_rows(int64_t rows, int64_t cols, bool f32) {
+  if (rows <= 32) return 32;
+  if (f32) return 128;
+  if (rows <= 64) return 64;
+  if (rows <= 128 || ((rows + 255) / 256) * ((cols + 255) / 256) < 192) return 128;
+  return 256;
+}
+// Columns of those tiles.
+int lx_tile_cols(int bm) { return bm == 256 ? 256 : 128; }
+
+struct LxCall {
+  const TensorDesc *x, *w, *labels, *rw, *loss, *dx, *dw, *row_loss, *scratch;
+  int ek;  // ElemKind of X and W
+  int64_t R, V, D, ldx, ldw, lddx, lddw;
+};
+
+struct LxPlan {
+  int64_t Rp, Dp, Vp, es;
+  int bm, bn;               // tiles of the logits
+  bool direct;              // W is read in place
+  int64_t piece;            // classes of a piece (a multiple of 256)
+  int bm_dx;                // tiles of dX
+  int64_t shares, k_share;  // of the classes of a piece
+  int64_t slab_rows;
+  int64_t stats_off, xc_off, slab_off, wpad_off, g_off, bytes;
+};
+
+constexpr int kRowArrays = 9;  // arrays of Rp 4-byte values behind the head
+
+// The plan of a call, with the largest piece of at most `piece` classes that
+// `bytes` of scratch hold (bytes < 0: any).  False: none fits.
+bool lx_plan(int64_t R, int64_t V, int64_t D, int64_t ldw, bool direct, bool f32, bool grad, int64_t piece,
+             int64_t bytes, LxPlan* pl) {
+  LxPlan p{};
+  p.es = f32 ? 4 : 2;
+  p.Rp = R > 0 ? up_to(R, 256) : 256;
+  p.Dp = up_to(D, 64);
+  p.Vp = up_to(V, 256);
+  p.direct = direct;
+  p.bm = lx_tile_rows(R, V, f32);
+  p.bn = lx_tile_cols(p.bm);
+  const int64_t lim = INT32_MAX;  // 32-bit offsets into an operand
+  const int64_t ldk = direct ? ldw : p.Dp;
+  if (p.Rp > lim / 2 || p.Dp * p.es * 256 >= lim || ldk * p.es * 256 >= lim || p.Vp > (int64_t)1 << 28) return false;
+  int64_t at = 256 + kRowArrays * p.Rp * 4;
+  p.stats_off = at;
+  at = up_to(at + p.Vp / p.bn * p.Rp * 8, 256);
+  p.xc_off = at;
+  at = up_to(at + p.Rp * p.Dp * p.es, 256);
+  p.slab_off = at;
+  p.bm_dx = lx_tile_rows(R, D, f32);
+  p.slab_rows = R > 0 ? up_to(R, p.bm_dx) : p.bm_dx;
+  if (grad) {
+    if (p.Rp * p.Dp * p.es >= lim) return false;
+    at = up_to(at + (p.Rp + 4096) * p.Dp * 4, 256);
+  }
+  p.wpad_off = at;
+  // a piece: its G (with gradients) and its rows of W (where they are copied)
+  const int64_t each = (grad ? p.Rp * p.es : 0) + (direct ? 0 : p.Dp * p.es);
+  int64_t most = piece > 0 && piece < p.Vp ? up_to(piece, 256) : p.Vp;
+  if (grad) {
+    most = std::min(most, (lim - 1) / (p.Rp * p.es) / 256 * 256);
+    most = std::min(most, (lim - 1) / (ldk * p.es) / 256 * 256);
+  }
+  if (bytes >= 0 && each > 0) most = std::min(most, (bytes - at - 256) / each / 256 * 256);
+  if (most < 256) return false;
+  p.piece = most;
+  p.g_off = up_to(at + (direct ? 0 : most * p.Dp * p.es), 256);
+  p.bytes = p.g_off + (grad ? p.Rp * most * p.es : 0) + 256;  // (the start is rounded up to 256 bytes)
+  if (bytes >= 0 && p.bytes > bytes) return false;
+  // dX: shares of the piece's classes while its tiles are fewer than what fills the chip
+  const int64_t tiles = p.slab_rows / p.bm_dx * up_to(D, lx_tile_cols(p.bm_dx)) / lx_tile_cols(p.bm_dx);
+  const int64_t want = p.bm_dx == 256 ? 256 : p.bm_dx == 128 ? 512 : 1024;
+  int64_t shares = want / std::max<int64_t>(tiles, 1);
+  shares = std::min(shares, most / 512);
+  shares = std::min(shares, (p.Rp + 4096) / p.slab_rows);
+  shares = std::max<int64_t>(shares, 1);
+  p.k_share = up_to((most + shares - 1) / shares, 64);
+  p.shares = shares;
+  if (pl) *pl = p;
+  return true;
+}
+
+template <int IN, int OUT, int ACT, int BM, int BN, int WM, int WN, bool AKC, bool BKC, int S>
+Status lx_gemm_as(const NTParams& q, int64_t rows, int64_t cols, int shares, hipStream_t s) {
+  NTParams p = q;
+  p.tiles_m = (int)((rows + BM - 1) / BM);
+  p.tiles_n = (int)((cols + BN - 1) / BN);
+  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+  if (tiles == 0) return Status::Ok;
+  if (tiles > INT32_MAX) return Status::InvalidArgument;
+  unsigned grid = (unsigned)tiles;
+  if constexpr (nt_persistent(BM, BN, WM, WN)) {
+    const int ncu = device_cu_count();
+    if (ncu > 0 && ncu % 8 == 0 && grid > (unsigned)ncu) grid = (unsigned)ncu;
+  }
+  gemm_nt_kernel<IN, OUT, ACT, BM, BN, WM, WN, AKC, BKC, S><<<dim3(grid, (unsigned)shares), 64 * WM * WN, 0, s>>>(p);
+  return launch_status("linear_xent");
+}
+
+// rows x cols of the product in tiles of bm rows.
+template <int IN, int OUT, int ACT, bool AKC, bool BKC>
+Status lx_gemm(const NTParams& p, int bm, int64_t rows, int64_t cols, int shares, hipStream_t s) {
+  if constexpr (IN != IN_F32) {
+    if (bm == 256) return lx_gemm_as<IN, OUT, ACT, 256, 256, 2, 4, AKC, BKC, 2>(p, rows, cols, shares, s);
+  }
+  if constexpr (AKC) {
+    if (bm == 32) return lx_gemm_as<IN, OUT, ACT, 32, 128, 1, 4, AKC, BKC, (IN == IN_F32 ? 2 : 4)>(p, rows, cols, shares, s);
+    if constexpr (IN != IN_F32) {
+      if (bm == 64) return lx_gemm_as<IN, OUT, ACT, 64, 128, 1, 4, AKC, BKC, 4>(p, rows, cols, shares, s);
+    }
+  }
+  return lx_gemm_as<IN, OUT, ACT, 128, 128, 2, 2, AKC, BKC, 2>(p, rows, cols, shares, s);
+}
+
+template <int IN, int EK>
+Status lx_run(const LxCall& c, const LxPlan& pl, hipStream_t s) {
+  constexpr int ES = IN == IN_F32 ? 4 : 2;
+  constexpr int OUT = IN == IN_F32 ? OUT_F32 : IN == IN_F16 ? OUT_F16 : OUT_BF16;
+  uint8_t* base = (uint8_t*)(((uintptr_t)c.scratch->data + 255) & ~(uintptr_t)255);
+  LxRows rw{};
+  rw.head = (int32_t*)base;
+  int32_t* arr = (int32_t*)(base + 256);
+  rw.pos = arr;
+  rw.idx = arr + pl.Rp;
+  rw.label = arr + 2 * pl.Rp;
+  rw.weight = (float*)arr + 3 * pl.Rp;
+  rw.row_w = (float*)arr + 4 * pl.Rp;
+  rw.zlab = (float*)arr + 5 * pl.Rp;
+  rw.row_max = (float*)arr + 6 * pl.Rp;
+  rw.row_f = (float*)arr + 7 * pl.Rp;
+  rw.row_loss = (float*)arr + 8 * pl.Rp;
+  rw.stats = (float2*)(base + pl.stats_off);
+  rw.xc = base + pl.xc_off;
+  rw.slab = (float*)(base + pl.slab_off);
+  rw.wpad = base + pl.wpad_off;
+  rw.g = base + pl.g_off;
+  const float* alpha = (const float*)(rw.head + 1);
+  const int R = (int)c.R, V = (int)c.V, D = (int)c.D, Dp = (int)pl.Dp;
+  // f16: exponentials of at most 2^14, G of at most 2^14 (2^13 times a weight's share, less one)
+  const int top = IN == IN_F16 ? 13 : 0;
+  const float keep_scale = IN == IN_F16 ? 16384.0f : 1.0f;
+  float* row_loss = (float*)c.row_loss->data;
+
+  lx_rows_kernel<<<1, 1024, 0, s>>>((const int32_t*)c.labels->data, c.rw ? (const float*)c.rw->data : nullptr, R, V,
+                                    top, rw);
+  if (R > 0)
+    lx_copy_rows_kernel<ES><<<(R + 3) / 4, 256, 0, s>>>(c.x->data, c.ldx, rw.xc, D, Dp, R, rw.pos,
+                                                        c.dx ? c.dx->data : nullptr, c.lddx, row_loss);
+  Status st = launch_status("linear_xent_rows");
+  if (st != Status::Ok) return st;
+
+  // W's rows of the classes v0 .. v0 + cols, in place or copied
+  auto weights = [&](NTParams& p, int64_t v0, int64_t cols) {
+    const uint8_t* w = (const uint8_t*)c.w->data + v0 * c.ldw * ES;
+    if (pl.direct) {
+      p.B = w;
+      p.ldb = c.ldw;
+    } else {
+      lx_copy_rows_kernel<ES><<<(unsigned)((cols + 3) / 4), 256, 0, s>>>(w, c.ldw, rw.wpad, D, Dp, (int)cols, nullptr,
+                                                                         nullptr, 0, nullptr);
+      p.B = rw.wpad;
+      p.ldb = Dp;
+    }
+  };
+  auto logits = [&](int64_t v0, int64_t cols) {
+    NTParams p{};
+    weights(p, v0, cols);
+    p.A = rw.xc;
+    p.lda = Dp;
+    p.C = rw.g;
+    p.ldc = pl.piece;
+    p.M = R;
+    p.N = (int)cols;
+    p.K = pl.direct ? D : Dp;
+    p.lx.n = rw.head;
+    p.lx.a_mn = (int)pl.Rp;
+    p.lx.b_mn = (int)cols;
+    p.lx.v0 = (int)v0;
+    p.lx.label = rw.label;
+    p.lx.zlab = rw.zlab;
+    p.lx.stats = rw.stats;
+    p.lx.stats_ld = pl.Rp;
+    p.lx.keep_scale = keep_scale;
+    p.lx.row_max = rw.row_max;
+    p.lx.row_f = rw.row_f;
+    p.lx.row_w = rw.row_w;
+    return p;
+  };
+  const bool grad = c.dx != nullptr;
+  const int64_t pieces = (c.V + pl.piece - 1) / pl.piece;
+  const int64_t last = (pieces - 1) * pl.piece;  // first class of the piece that is kept
+  auto stats = [&](int64_t v0, int64_t cols, int64_t keep) {
+    NTParams p = logits(v0, cols);
+    p.lx.keep_from = keep < 0 ? INT32_MAX : (int)keep;
+    return lx_gemm<IN, OUT, ACT_LX_STATS, true, true>(p, pl.bm, R, cols, 1, s);
+  };
+  if (pl.direct) {
+    st = stats(0, c.V, grad ? last : -1);
+    if (st != Status::Ok) return st;
+  } else {
+    for (int64_t v0 = 0; v0 < c.V; v0 += pl.piece) {
+      st = stats(v0, std::min(pl.piece, c.V - v0), grad && v0 == last ? 0 : -1);
+      if (st != Status::Ok) return st;
+    }
+  }
+  if (R > 0)
+    lx_stats_kernel<<<(R + 63) / 64, 1024, 0, s>>>(rw, (int)((c.V + pl.bn - 1) / pl.bn), pl.Rp, row_loss);
+  lx_loss_kernel<<<1, 1024, 0, s>>>(rw, (float*)c.loss->data);
+  st = launch_status("linear_xent_stats");
+  if (st != Status::Ok || !grad) return st;
+
+  const bool slabs = pieces > 1 || pl.shares > 1;
+  int64_t filled = 0;  // slabs that hold something
+  for (int64_t k = pieces - 1; k >= 0; --k) {
+    const int64_t v0 = k * pl.piece, cols = std::min(pl.piece, c.V - v0);
+    if (k == pieces - 1) {
+      if (R > 0) {
+        const int64_t width = up_to(cols, pl.bn);
+        const unsigned gx = (unsigned)((width + 256 * (16 / ES) - 1) / (256 * (16 / ES)));
+        const unsigned gy = (unsigned)std::min<int64_t>(R, 32768);
+        if (pl.bn == 256)
+          lx_scale_kernel<EK, 256><<<dim3(gx, gy), 256, 0, s>>>(rw, pl.piece, (int)width, (int)v0, pl.Rp, keep_scale);
+        else
+          lx_scale_kernel<EK, 128><<<dim3(gx, gy), 256, 0, s>>>(rw, pl.piece, (int)width, (int)v0, pl.Rp, keep_scale);
+      }
+    } else {
+      NTParams p = logits(v0, cols);
+      st = lx_gemm<IN, OUT, ACT_LX_GRAD, true, true>(p, pl.bm, R, cols, 1, s);
+      if (st != Status::Ok) return st;
+    }
+    if (c.dw) {
+      NTParams p{};
+      p.A = rw.g;
+      p.lda = pl.piece;
+      p.B = rw.xc;
+      p.ldb = Dp;
+      p.M = (int)cols;
+      p.N = D;
+      p.K = R;
+      p.ldc = c.lddw;
+      p.lx.n = rw.head;
+      p.lx.rows_are_k = 1;
+      p.lx.a_mn = (int)pl.piece;
+      p.lx.b_mn = Dp;
+      p.lx.alpha = alpha;
+      const bool f32 = dt(*c.dw) == DType::kF32;
+      const int ob = f32 ? 4 : 2;
+      p.C = (uint8_t*)c.dw->data + v0 * c.lddw * ob;
+      p.lx.vec = aligned(c.dw->data, 16) && c.lddw * ob % 16 == 0;
+      const int bm = IN == IN_F32 ? 128 : ((cols + 255) / 256) * ((c.D + 255) / 256) < 192 ? 128 : 256;
+      if (f32)
+        st = lx_gemm<IN, OUT_F32, ACT_LX_OUT, false, false>(p, bm, cols, D, 1, s);
+      else
+        st = lx_gemm<IN, OUT, ACT_LX_OUT, false, false>(p, bm, cols, D, 1, s);
+      if (st != Status::Ok) return st;
+    }
+    if (R > 0) {
+      NTParams p{};
+      // (a copy of the piece's rows is still there)
+      p.B = pl.direct ? (const uint8_t*)c.w->data + v0 * c.ldw * ES : (const uint8_t*)rw.wpad;
+      p.ldb = pl.direct ? c.ldw : Dp;
+      p.A = rw.g;
+      p.lda = pl.piece;
+      p.M = R;
+      p.N = D;
+      p.K = (int)cols;
+      p.lx.n = rw.head;
+      p.lx.a_mn = (int)pl.Rp;
+      p.lx.b_mn = pl.direct ? D : Dp;
+      if (!slabs) {
+        p.C = c.dx->data;
+        p.ldc = c.lddx;
+        p.lx.alpha = alpha;
+        p.lx.row_map = rw.idx;
+        p.lx.vec = aligned(c.dx->data, 16) && c.lddx * ES % 16 == 0;
+        st = lx_gemm<IN, OUT, ACT_LX_OUT, true, false>(p, pl.bm_dx, R, D, 1, s);
+      } else {
+        p.C = rw.slab;
+        p.ldc = Dp;
+        p.lx.add = (int)filled;
+        p.lx.k_split = (int)pl.k_share;
+        p.lx.split_stride = pl.slab_rows * Dp;
+        const int64_t used = (cols + pl.k_share - 1) / pl.k_share;  // (a short last piece has fewer shares)
+        filled = std::max(filled, used);
+        st = lx_gemm<IN, OUT_F32, ACT_LX_SLAB, true, false>(p, pl.bm_dx, R, D, (int)used, s);
+      }
+      if (st != Status::Ok) return st;
+    }
+  }
+  if (slabs && R > 0) {
+    const unsigned gx = (unsigned)((D + 1023) / 1024), gy = (unsigned)std::min<int64_t>(R, 32768);
+    lx_finish_kernel<EK><<<dim3(gx, gy), 256, 0, s>>>(rw, (int)filled, pl.slab_rows * Dp, Dp, D, c.dx->data,
+                                                      c.lddx);
+    return launch_status("linear_xent_finish");
+  }
+  return Status::Ok;
+}
+
+// X, W, labels [, weights] -> loss, row loss, scratch | loss, dX, row loss,
+// scratch | loss, dX, dW, row loss, scratch.
+bool lx_read(const TensorDesc* in, int ni, const TensorDesc* out, int no, LxCall* pc, LxPlan* pl) {
+  if (!in || !out || (ni != 3 && ni != 4) || no < 3 || no > 5) return false;
+  LxCall c{};
+  c.x = &in[0];
+  c.w = &in[1];
+  c.labels = &in[2];
+  c.rw = ni == 4 ? &in[3] : nullptr;
+  c.loss = &out[0];
+  c.dx = no >= 4 ? &out[1] : nullptr;
+  c.dw = no == 5 ? &out[2] : nullptr;
+  c.row_loss = &out[no - 2];
+  c.scratch = &out[no - 1];
+  int wk;
+  if (!elem_kind(*c.x, &c.ek) || !elem_kind(*c.w, &wk) || wk != c.ek) return false;
+  if (!matrix_ld(*c.x, false, &c.ldx) || !matrix_ld(*c.w, false, &c.ldw)) return false;
+  c.R = c.x->shape[0];
+  c.D = c.x->shape[1];
+  c.V = c.w->shape[0];
+  if (c.w->shape[1] != c.D || c.V < 1 || c.D < 1) return false;
+  if (!vector_of(*c.labels, DType::kI32, c.R)) return false;
+  if (c.rw && !vector_of(*c.rw, DType::kF32, c.R)) return false;
+  if (!vector_of(*c.loss, DType::kF32, 1) || !vector_of(*c.row_loss, DType::kF32, c.R)) return false;
+  if (dt(*c.scratch) != DType::kF32 || c.scratch->rank != 1 || (c.scratch->shape[0] > 1 && c.scratch->stride[0] != 1))
+    return false;
+  auto grad_of = [](const TensorDesc& g, const TensorDesc& of, int64_t* ld, bool f32_too) {
+    return matrix_ld(g, true, ld) && same_shape(g, of) && (dt(g) == dt(of) || (f32_too && dt(g) == DType::kF32));
+  };
+  if (c.dx && !grad_of(*c.dx, *c.x, &c.lddx, false)) return false;
+  if (c.dw && !grad_of(*c.dw, *c.w, &c.lddw, true)) return false;
+  if (any_overlap(in, ni, out, no)) return false;
+  const bool f32 = c.ek == EL_F32;
+  const int64_t es = f32 ? 4 : 2;
+  // tiles read W with 16-byte loads and whole K-steps
+  const bool direct = c.D % (128 / es) == 0 && aligned(c.w->data, 16) && c.ldw * es % 16 == 0 &&
+                      (c.V == 1 || c.ldw >= c.D) && c.ldw * es * 256 < INT32_MAX;
+  if (!lx_plan(c.R, c.V, c.D, c.ldw, direct, f32, c.dx != nullptr, 0, c.scratch->shape[0] * 4, pl)) return false;
+  if (pc) *pc = c;
+  return true;
+}
+
+bool lx_sup(const TensorDesc* in, int ni, const TensorDesc* out, int no, const void*) {
+  LxPlan pl;
+  return lx_read(in, ni, out, no, nullptr, &pl);
+}
+
+Status lx_launch(const TensorDesc* in, int ni, TensorDesc* out, int no, const void*, void*, size_t, void* stream) {
+  LxCall c;
+  LxPlan pl;
+  if (!lx_read(in, ni, out, no, &c, &pl)) return Status::InvalidArgument;
+  for (int k = 0; k < ni; ++k)
+    if (no_memory(in[k])) return Status::InvalidArgument;
+  for (int k = 0; k < no; ++k)
+    if (no_memory(out[k])) return Status::InvalidArgument;
+  hipStream_t s = as_stream(stream);
+  if (c.ek == EL_F32) return lx_run<IN_F32, EL_F32>(c, pl, s);
+  if (c.ek == EL_F16) return lx_run<IN_F16, EL_F16>(c, pl, s);
+  return lx_run<IN_BF16, EL_BF16>(c, pl, s);
+}
+
+size_t no_workspace(const TensorDesc*, int, const void*) { return 0; }
+
+}  // namespace
+
+KernelVariant make_linear_xent_variant() {
+  KernelVariant v;
+  v.name = "linear_xent";
+  v.launch = lx_launch;
+  v.supported = lx_sup;
+  v.query_workspace = no_workspace;
+  return v;
+}
+
+}  // namespace aicf::hip
+
+using namespace aicf::hip;
+
+extern "C" int64_t aicf_linear_xent_scratch(int64_t rows, int64_t classes, int64_t dim, int32_t dtype,
+                                            int32_t gradients, int64_t piece) {
+  if (rows < 0 || classes < 1 || dim < 1 ||
+      (dtype != AICF_DTYPE_F32 && dtype != AICF_DTYPE_F16 && dtype != AICF_DTYPE_BF16))
+    return -1;
+  const bool f32 = dtype == AICF_DTYPE_F32;
+  LxPlan p;
+  if (rows > INT32_MAX || classes > INT32_MAX || dim > INT32_MAX ||
+      !lx_plan(rows, classes, dim, dim, dim % (f32 ? 32 : 64) == 0, f32, gradients != 0, piece, -1, &p))
+    return -1;
+  return p.bytes;
+}

@@ -15,6 +15,7 @@
 // dispatcher spreads over all 8 XCDs.  Out-of-place Adam reads P and writes
 // Pout in the same pass instead of copying P first.
 #include "../common/adamw.hpp"
+#include "../common/head_util.hpp"
 #include "../common/hip_util.hpp"
 
 namespace aicf::hip {
@@ -339,6 +340,143 @@ Status adamw_launch(const TensorDesc* in, int ni, TensorDesc* out, int no, const
     adamw_scalar_kernel<<<blocks, 256, 0, s>>>(P, G, M, V, Po, Mo, Vo, Wb, done, n, a, step);
   }
   return launch_status("adamw_step_f32_v1");
+}
+
+// ---------------------------------------------------------------------------
+// AdamW on gradients that are scaled as they are read (no reference
+// counterpart): inputs (P, G, M, V, step i32, norm f32 [2]), norm[1] the clip
+// factor as grad_norm writes it; outputs as adamw_step_f32_v1.  g = factor G in
+// f32 (G f32, f16 or bf16), then adamw_elem: with f32 gradients the bits of
+// clipping them in place first, without the pass that rewrites them.
+// ---------------------------------------------------------------------------
+template <int GK>
+__device__ __forceinline__ f32x4 grad4(const void* G, int64_t i) {
+  if constexpr (GK == EL_F32) return __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(G) + i);
+  const u16x4 h = __builtin_nontemporal_load(reinterpret_cast<const u16x4*>(G) + i);
+  f32x4 v;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) v[c] = GK == EL_F16 ? f16_to_f32(h[c]) : bf16_to_f32(h[c]);
+  return v;
+}
+
+// VEC: every array's vectors of 4 lie on their own size; a workgroup takes 1024
+// elements, and lanes behind the last whole vector one element each.
+template <int GK, bool VEC>
+__global__ __launch_bounds__(256) void adamw_clip_kernel(const float* __restrict__ P, const void* __restrict__ G,
+                                                         const float* __restrict__ M, const float* __restrict__ V,
+                                                         float* __restrict__ Pout, float* __restrict__ Mout,
+                                                         float* __restrict__ Vout, uint16_t* __restrict__ Wb,
+                                                         int64_t n, AdamWArgs a, const int32_t* __restrict__ stepp,
+                                                         const float* __restrict__ norm) {
+  const int64_t n4 = VEC ? n / 4 : 0;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  f32x4 p, g, m, v;
+  if (i < n4) {  // the loads first: the counter and the corrections overlap them
+    p = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(P) + i);
+    g = grad4<GK>(G, i);
+    m = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(M) + i);
+    v = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(V) + i);
+  }
+  __shared__ float sh[3];
+  if (threadIdx.x < 64) {
+    const AdamWScalars t = adamw_scalars(stepp, a);
+    if (threadIdx.x == 0) {
+      sh[0] = t.step;
+      sh[1] = t.ibc2;
+      sh[2] = norm[1];
+    }
+  }
+  __syncthreads();
+  const AdamWScalars s{sh[0], sh[1]};
+  const float f = sh[2];
+  if (i < n4) {
+    u16x4 w;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      float pp = p[c], mm = m[c], vv = v[c], gg = g[c] * f;
+      asm("" : "+v"(gg));  // one rounding of its own, as a stored gradient has
+      adamw_elem(pp, gg, mm, vv, s, a);
+      p[c] = pp;
+      m[c] = mm;
+      v[c] = vv;
+      w[c] = f32_to_bf16(pp);
+    }
+    __builtin_nontemporal_store(p, reinterpret_cast<f32x4*>(Pout) + i);
+    __builtin_nontemporal_store(m, reinterpret_cast<f32x4*>(Mout) + i);
+    __builtin_nontemporal_store(v, reinterpret_cast<f32x4*>(Vout) + i);
+    if (Wb) __builtin_nontemporal_store(w, reinterpret_cast<u16x4*>(Wb) + i);
+    return;
+  }
+  const int64_t e = i - n4 + 4 * n4;
+  if (e >= n) return;
+  float pp = P[e], mm = M[e], vv = V[e], gg = elem_f32<GK>(G, e) * f;
+  asm("" : "+v"(gg));
+  adamw_elem(pp, gg, mm, vv, s, a);
+  Pout[e] = pp;
+  Mout[e] = mm;
+  Vout[e] = vv;
+  if (Wb) Wb[e] = f32_to_bf16(pp);
+}
+
+bool adamw_clip_supported(const TensorDesc* in, int ni, const TensorDesc* out, int no, const void*) {
+  if (!in || !out || ni != 6 || (no != 3 && no != 4)) return false;
+  const TensorDesc& P = in[0];
+  int gk;
+  if (!elem_kind(in[1], &gk) || !in[1].contiguous || in[1].rank < 1) return false;
+  for (int k : {0, 2, 3})
+    if (!f32_contig_anyrank(in[k]) || !same_shape(in[k], P)) return false;
+  for (int k = 0; k < 3; ++k)
+    if (!f32_contig_anyrank(out[k]) || !same_shape(out[k], P)) return false;
+  if (!same_shape(in[1], P) || !i32_scalar_contig(in[4]) || !vector_of(in[5], DType::kF32, 2)) return false;
+  if (no == 4 && (dt(out[3]) != DType::kBF16 || !out[3].contiguous || !same_shape(out[3], P))) return false;
+  // P, M and V in place or elsewhere; nothing else shared
+  const int own[4] = {0, 2, 3, -1};
+  for (int k = 0; k < no; ++k) {
+    for (int j = 0; j < ni; ++j)
+      if (views_overlap(out[k], in[j]) && !(j == own[k] && peq(out[k], in[j]))) return false;
+    for (int j = 0; j < k; ++j)
+      if (views_overlap(out[k], out[j])) return false;
+  }
+  return true;
+}
+
+Status adamw_clip_launch(const TensorDesc* in, int ni, TensorDesc* out, int no, const void* attr, void*, size_t,
+                         void* stream) {
+  if (!adamw_clip_supported(in, ni, out, no, attr)) return Status::InvalidArgument;
+  for (int k = 0; k < ni; ++k)
+    if (no_memory(in[k])) return Status::InvalidArgument;
+  for (int k = 0; k < no; ++k)
+    if (no_memory(out[k])) return Status::InvalidArgument;
+  const int64_t n = numel_of(in[0]);
+  if (n <= 0) return Status::Ok;
+  const AdamAttrs at = read_adam_attrs(attr);
+  const AdamWArgs a{at.lr, at.beta1, at.beta2, at.eps, at.wd, 1.0f - at.beta1, 1.0f - at.beta2,
+                    1.0f - at.lr * at.wd};
+  int gk;
+  elem_kind(in[1], &gk);
+  uint16_t* Wb = no == 4 ? (uint16_t*)out[3].data : nullptr;
+  const bool vec = all_aligned16({in[0].data, in[2].data, in[3].data, out[0].data, out[1].data, out[2].data}) &&
+                   aligned(in[1].data, gk == EL_F32 ? 16 : 8) && (!Wb || aligned(Wb, 8));
+  const int64_t lanes = vec ? n / 4 + n % 4 : n, blocks = (lanes + 255) / 256;
+  if (blocks > INT32_MAX) return Status::InvalidArgument;
+  hipStream_t s = as_stream(stream);
+#define ADAMW_CLIP(GK, VEC)                                                                                     \
+  adamw_clip_kernel<GK, VEC><<<(unsigned)blocks, 256, 0, s>>>(                                                  \
+      (const float*)in[0].data, in[1].data, (const float*)in[2].data, (const float*)in[3].data,                \
+      (float*)out[0].data, (float*)out[1].data, (float*)out[2].data, Wb, n, a, (const int32_t*)in[4].data,     \
+      (const float*)in[5].data)
+  if (gk == EL_F32) {
+    if (vec) ADAMW_CLIP(EL_F32, true);
+    else ADAMW_CLIP(EL_F32, false);
+  } else if (gk == EL_F16) {
+    if (vec) ADAMW_CLIP(EL_F16, true);
+    else ADAMW_CLIP(EL_F16, false);
+  } else {
+    if (vec) ADAMW_CLIP(EL_BF16, true);
+    else ADAMW_CLIP(EL_BF16, false);
+  }
+#undef ADAMW_CLIP
+  return launch_status("adamw_step_clip_v0");
 }
 
 size_t no_workspace(const TensorDesc*, int, const void*) { return 0; }
@@ -678,6 +816,9 @@ KernelVariant make_adam_step_f32_variant() {
 }
 KernelVariant make_adamw_step_f32_variant() {
   return make("adamw_step_f32_vec4", adamw_launch, adamw_supported, AICF_SCHEMA_ADAM);
+}
+KernelVariant make_adamw_step_clip_variant() {
+  return make("adamw_step_clip", adamw_clip_launch, adamw_clip_supported, AICF_SCHEMA_ADAM);
 }
 KernelVariant make_colsum_adamw_f32_variant() {
   return make("colsum_adamw_f32", colsum_adamw_launch, colsum_adamw_supported, AICF_SCHEMA_CADW);

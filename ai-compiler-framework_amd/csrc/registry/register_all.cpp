@@ -82,6 +82,10 @@ KernelVariant make_quant_fp8_variant();
 KernelVariant make_gemm_fp8_variant();
 KernelVariant make_distill_topk_variant();
 KernelVariant make_sample_row_variant();
+// linear_xent.hip, grad_norm.hip, optim.hip
+KernelVariant make_linear_xent_variant();
+KernelVariant make_grad_norm_variant();
+KernelVariant make_adamw_step_clip_variant();
 
 void register_all_kernels_into(KernelRegistry& R) {
   if (std::getenv("AICF_VERBOSE")) std::fprintf(stderr, "[aicf] register_all: gfx950 backend\n");
@@ -155,9 +159,11 @@ void register_all_kernels_into(KernelRegistry& R) {
 
   reg(OpKind::GradZero, make_grad_zero_variant(), 0, "grad_zero_v0");
 
-  // AdamStep: reference contract (6 inputs) and the AdamW variant (5 inputs)
+  // AdamStep: reference contract (6 inputs, the last two f32 scalars), the AdamW
+  // variant (5 inputs) and that with the clip factor (6, the fifth the i32 step)
   reg(OpKind::AdamStep, make_adamw_step_f32_variant(), 10, "adamw_step_f32_v1");
   reg(OpKind::AdamStep, make_adam_step_f32_variant(), 0, "adam_step_f32_v0");
+  reg(OpKind::AdamStep, make_adamw_step_clip_variant(), 0, "adamw_step_clip_v0");
 
   reg(OpKind::StepInc, make_step_inc_variant(), 0, "step_inc_v0");
   reg(OpKind::BiasCorr, make_biascorr_variant(), 0, "bias_corr_v0");
@@ -191,6 +197,8 @@ void register_all_kernels_into(KernelRegistry& R) {
   reg(OpKind::GemmFp8, make_gemm_fp8_variant(), 0, "gemm_fp8_mfma_v0");
   reg(OpKind::DistillTopk, make_distill_topk_variant(), 0, "distill_topk_v0");
   reg(OpKind::SampleRow, make_sample_row_variant(), 0, "sample_row_v0");
+  reg(OpKind::LinearXent, make_linear_xent_variant(), 0, "linear_xent_v0");
+  reg(OpKind::GradNorm, make_grad_norm_variant(), 0, "grad_norm_v0");
 }
 
 }  // namespace aicf::hip

@@ -167,6 +167,8 @@ const char* opkind_name(OpKind k) {
     case OpKind::GemmFp8: return "gemm_fp8";
     case OpKind::DistillTopk: return "distill_topk";
     case OpKind::SampleRow: return "sample_row";
+    case OpKind::LinearXent: return "linear_xent";
+    case OpKind::GradNorm: return "grad_norm";
     case OpKind::_Count: break;
   }
   return "unknown";

@@ -67,6 +67,7 @@ OPNAME_TO_KIND: Dict[str, int] = {
     "grad_group_adamw": int(_C.OpKind.GradGroup), "gemm_epilogue_bcopy": int(_C.OpKind.GemmEpilogue),
     "quant_fp8": int(_C.OpKind.QuantFp8), "gemm_fp8": int(_C.OpKind.GemmFp8),
     "distill_topk": int(_C.OpKind.DistillTopk), "sample_row": int(_C.OpKind.SampleRow),
+    "linear_xent": int(_C.OpKind.LinearXent), "grad_norm": int(_C.OpKind.GradNorm),
 }
 
 
@@ -88,6 +89,7 @@ SCHEMA_MSCS = _fourcc_le(b"MSCS")
 SCHEMA_CADW = _fourcc_le(b"CADW")
 SCHEMA_QFP8 = _fourcc_le(b"QFP8")
 SCHEMA_DTOP = _fourcc_le(b"DTOP")
+SCHEMA_GNRM = _fourcc_le(b"GNRM")
 SCHEMA_GEMM = int.from_bytes(b"GEMM", "big")
 SCHEMA_RSUM = int.from_bytes(b"RSUM", "big")
 
@@ -161,6 +163,8 @@ def pack_attrs(op: str, attrs: Dict[str, Any]) -> Tuple[int, bytes]:
         return SCHEMA_QFP8, struct.pack("<i", int(bool(a.get("pow2", False))))
     if op == "distill_topk":
         return SCHEMA_DTOP, struct.pack("<ff", float(a.get("temperature", 1.0)), float(a.get("label_weight", 0.0)))
+    if op == "grad_norm":
+        return SCHEMA_GNRM, struct.pack("<f", float(a.get("max_norm", float("inf"))))
     if op == "row_reduce":
         return SCHEMA_RRED, struct.pack("<i", 1 if str(a.get("op", "sum")) == "max" else 0)
     return 0, b""

@@ -7,7 +7,9 @@ compile-time rewrites of the reference pipeline:
     Save      -> copy_saved;  other ops map one to one
   and the ops this backend appends (GELU, softmax cross-entropy, fused MSE
   loss, AdamW with in-kernel bias correction, row softmax / reduce, the
-  vocabulary head's distillation loss and sampling), and Linear layers in
+  vocabulary head's distillation loss and sampling, the linear cross-entropy,
+  the gradient norm with clipping; an AdamW step with a sixth input, the
+  norm, scales its gradient by the clip factor), and Linear layers in
   8 bits (not in the reference):
     LinearFp8    x, W [, b] -> y, xq, xs, wq, ws [, xqT, xsT [, wqT, wsT]]
       quant_fp8 of x (rows) and of W (blocks; not with quant_w=False, for
@@ -62,7 +64,7 @@ _PRIMITIVES = {
     "adamw_step", "layernorm_fwd", "layernorm_bwd", "batchnorm_fwd", "batchnorm_bwd",
     "transpose", "gemm_adamw", "xent_head", "grad_group", "adamw_multi", "mse_colsum",
     "colsum_adamw", "grad_group_adamw", "gemm_epilogue_bcopy", "quant_fp8", "gemm_fp8",
-    "distill_topk", "sample_row",
+    "distill_topk", "sample_row", "linear_xent", "grad_norm",
 }
 
 _ALIASES = {"adamstep": "adam_step", "stepinc": "step_inc", "biascorr": "bias_corr",
@@ -71,7 +73,7 @@ _ALIASES = {"adamstep": "adam_step", "stepinc": "step_inc", "biascorr": "bias_co
             "mseloss": "mse_loss", "adamwstep": "adamw_step", "rowsoftmax": "row_softmax",
             "rowreduce": "row_reduce", "quantfp8": "quant_fp8", "gemmfp8": "gemm_fp8",
             "distilltopk": "distill_topk", "samplerow": "sample_row", "linearfp8": "linear_fp8",
-            "linearfp8bwd": "linear_fp8_bwd"}
+            "linearfp8bwd": "linear_fp8_bwd", "linearxent": "linear_xent", "gradnorm": "grad_norm"}
 
 
 EPILOGUE_KINDS = {"bias_relu": 0, "bias": 1, "relu": 2, "bias_gelu": 3, "gelu": 4, "dgelu": 5}
@@ -391,8 +393,8 @@ def pick_kernel_id(ir: IRGraph, it: Dict[str, Any]) -> Optional[str]:
         return "grad_zero_v0"
     if op == "adam_step":
         return "adam_step_f32_v0"
-    if op == "adamw_step":
-        return "adamw_step_f32_v1"
+    if op == "adamw_step":  # a sixth input is a grad_norm's, whose factor scales the gradient
+        return "adamw_step_clip_v0" if len(ins) == 6 else "adamw_step_f32_v1"
     if op == "gemm_adamw":
         return "gemm_adamw_bf16_v0"
     if op == "step_inc":
@@ -425,7 +427,7 @@ def pick_kernel_id(ir: IRGraph, it: Dict[str, Any]) -> Optional[str]:
         return "mse_colsum_v0"
     if op == "colsum_adamw":
         return "colsum_adamw_f32_v0"
-    if op in ("quant_fp8", "distill_topk", "sample_row"):
+    if op in ("quant_fp8", "distill_topk", "sample_row", "linear_xent", "grad_norm"):
         return f"{op}_v0"
     if op == "gemm_fp8":
         return "gemm_fp8_mfma_v0"
@@ -1241,11 +1243,14 @@ def compile_lowered(ir: IRGraph, *, fuse: bool = True, fuse_bias: bool = False,
     if nt_layout:
         policy = "all" if nt_layout is True else str(nt_layout)
         low = normalize_gemm_layout(ir, low, min_flops=nt_min_flops, policy=policy)
-    if fuse_optimizer:
+    # an update that a GEMM, a group or the tail applies would come before the
+    # norm of all gradients is known: with a grad_norm AdamW keeps its own launches
+    clipped = any(_kind(it) == "grad_norm" for it in low)
+    if fuse_optimizer and not clipped:
         low = fuse_optimizer_into_gemms(ir, low)
     if fuse_small:
-        low = fuse_small_step(ir, low, keep_values, adamw_into_group=fuse_small != "four")
-    if fuse_tail:
+        low = fuse_small_step(ir, low, keep_values, adamw_into_group=fuse_small != "four" and not clipped)
+    if fuse_tail and not clipped:
         low = fuse_step_tail(ir, low)
     return apply_kernel_selection(ir, low)
 

@@ -12,6 +12,10 @@
   8 bits: logits, a token drawn a row, the distillation loss from a teacher's
   top logits, both layers' gradients, AdamW on fp32 master weights.
 
+* build_mlp_lm: a 2-layer bf16 model with a vocabulary head trained by softmax
+  cross-entropy whose logits are not kept, the gradients clipped by their
+  global norm, AdamW on fp32 master weights with bf16 copies for the products.
+
 All return (ir, lowered, plan) ready for PlannedExecutor, plus helpers to
 initialise inputs/parameters from a seed.
 """
@@ -23,6 +27,8 @@ from typing import Dict, List, Optional, Tuple
 
 import numpy as np
 import torch
+
+from aicf_cuda import _C
 
 from .executor import ExecOptions, PlannedExecutor
 from .ir import IRGraph
@@ -287,6 +293,66 @@ def init_mlp_distill(B: int, din: int, dh: int, V: int, K: int, seed: int = 0, d
            "min_p": torch.from_numpy((0.01 * (rows % 5)).astype(np.float32))}
     params = {"1.W": torch.from_numpy(kaiming_uniform(r, dh, din)), "1.b": torch.zeros(dh),
               "2.W": torch.from_numpy(kaiming_uniform(r, V, dh)), "2.b": torch.zeros(V)}
+    return {k: v.to(device) for k, v in ins.items()}, {k: v.to(device) for k, v in params.items()}
+
+
+# ============================================================ language-model MLP
+LM_INPUTS = {"x", "t"}
+
+
+def build_mlp_lm(B: int, din: int, dh: int, V: int, *, max_norm: float = 1.0, clip_in_place: bool = False,
+                 piece: int = 0, lr: float = 1e-3, beta1: float = 0.9, beta2: float = 0.999, eps: float = 1e-8,
+                 weight_decay: float = 0.0, fuse_small=False, device: str = "cuda:0"):
+    """x [B, din] bf16 -> Linear -> GELU -> linear cross-entropy with the labels
+    t [B] (i32; outside [0, V): the row does not count), mean over the rows that
+    count.  The gradients' norm over all tensors scales them by at most
+    max_norm / norm: as AdamW reads them or, clip_in_place, before.  `norm` [2]
+    holds the norm and the factor.  piece: classes whose gradient of the logits
+    is held at a time (0: all)."""
+    ir = IRGraph(name=f"mlp_lm_{B}x{din}x{dh}x{V}")
+    nv = lambda n, s, dt=F32: ir.new_value(name=n, shape=s, dtype=dt, device=device)  # noqa: E731
+    x, t = nv("x", (B, din), BF16), nv("t", (B,), I32)
+    W1, b1, W2 = nv("1.W", (dh, din)), nv("1.b", (dh,)), nv("2.W", (V, dh))
+    W1b, W2b = nv("1.Wb", (dh, din), BF16), nv("2.Wb", (V, dh), BF16)
+    z, h = nv("z1", (B, dh), BF16), nv("h1", (B, dh), BF16)
+    loss, row_loss = nv("loss", (1,)), nv("row_loss", (B,))
+    dh_, dz, dx = nv("d_h1", (B, dh), BF16), nv("d_z1", (B, dh), BF16), nv("d_x", (B, din), BF16)
+    dW1, db1, dW2 = (nv(f"d_{p.name}", p.shape) for p in (W1, b1, W2))
+    ws = nv("xent.ws", (_C.linear_xent_scratch(B, V, dh, torch.bfloat16, True, piece) // 4,))
+    norm, norm_ws = nv("norm", (2,)), nv("norm.ws", (2048,))
+    step = nv("opt.step", (), I32)
+    lin = {"bias": True, "layout": "y = x @ W^T + b"}
+    ir.emit(op="Linear", inputs=[x, W1b, b1], outputs=[z], attrs=lin)
+    ir.emit(op="Gelu", inputs=[z], outputs=[h], attrs={"save_preact": True})
+    ir.emit(op="LinearXent", inputs=[h, W2b, t], outputs=[loss, dh_, dW2, row_loss, ws])
+    ir.emit(op="GeluBwd", inputs=[dh_, z], outputs=[dz])
+    ir.emit(op="LinearBwd", inputs=[x, W1b, dz], outputs=[dx, dW1, db1], attrs=dict(lin, need_dx=False))
+    grads = [dW1, db1, dW2]
+    ir.emit(op="GradNorm", inputs=grads, outputs=[norm, norm_ws] + (grads if clip_in_place else []),
+            attrs={"max_norm": max_norm})
+    ir.emit(op="StepInc", inputs=[step], outputs=[step])
+    hp = {"lr": lr, "beta1": beta1, "beta2": beta2, "eps": eps, "weight_decay": weight_decay}
+    for p, g, shadow in ((W1, dW1, [W1b]), (b1, db1, []), (W2, dW2, [W2b])):
+        m, v = nv(f"opt.m.{p.name}", p.shape), nv(f"opt.v.{p.name}", p.shape)
+        ir.emit(op="AdamWStep", inputs=[p, g, m, v, step] + ([] if clip_in_place else [norm]),
+                outputs=[p, m, v] + shadow, attrs=hp)
+    lowered = compile_lowered(ir, fuse_bias=True, fuse_small=fuse_small)
+    plan = build_binding_plan(ir, opts=PlanOptions(input_names=set(LM_INPUTS),
+                                                   param_names={p.name for p in (W1, b1, W2, W1b, W2b)}))
+    return ir, lowered, plan
+
+
+def init_mlp_lm(B: int, din: int, dh: int, V: int, seed: int = 0, device: str = "cuda:0"):
+    """Synthetic rows, labels for all but every fourth of them; Kaiming-uniform
+    weights and their bf16 copies, zero biases.  (inputs, params)."""
+    r = np.random.default_rng(seed)
+    t = r.integers(0, V, B).astype(np.int32)
+    t[3::4] = -1
+    ins = {"x": torch.from_numpy(r.standard_normal((B, din)).astype(np.float32)).to(torch.bfloat16),
+           "t": torch.from_numpy(t)}
+    params = {"1.W": torch.from_numpy(kaiming_uniform(r, dh, din)), "1.b": torch.zeros(dh),
+              "2.W": torch.from_numpy(kaiming_uniform(r, V, dh))}
+    params.update({f"{k}.Wb": params[f"{k}.W"].to(torch.bfloat16) for k in "12"})
     return {k: v.to(device) for k, v in ins.items()}, {k: v.to(device) for k, v in params.items()}
 
 

@@ -96,7 +96,11 @@ extern "C" {
                                     logits, forward and backward (schema DTOP; see below) */
 #define AICF_OP_SAMPLE_ROW 33    /* logits, u, temperature, top_k, top_p, min_p -> token [, log-probability
                                     [, scratch]]: one draw a row from given random numbers (see below) */
-#define AICF_OP_COUNT 34
+#define AICF_OP_LINEAR_XENT 34   /* X, W, labels [, row weights] -> loss, [dX, [dW,]] row loss, scratch: softmax
+                                    cross-entropy of a vocabulary head, the logits not kept (see below) */
+#define AICF_OP_GRAD_NORM 35     /* G_1 .. G_T -> norm [2], scratch [, clipped G_1 .. G_T]: global gradient norm
+                                    and clipping (schema GNRM; see below) */
+#define AICF_OP_COUNT 36
 
 /*
  * Attribute schema ids (numeric ABI).  The reference mixes big-endian fourccs
@@ -131,6 +135,8 @@ extern "C" {
 
 #define AICF_SCHEMA_QFP8 0x38504651u /* appended: b"QFP8" little-endian, <i> flags: bit 0 = scales are powers of two */
 #define AICF_SCHEMA_DTOP 0x504F5444u /* appended: b"DTOP" little-endian, <ff> temperature, weight of the labels' loss */
+
+#define AICF_SCHEMA_GNRM 0x4D524E47u /* appended: b"GNRM" little-endian, <f> largest norm (>= 0; infinity: no clipping) */
 
 /*
  * The 8-bit and vocabulary-head ops (appended kinds 30..33, no counterpart in
@@ -197,6 +203,42 @@ extern "C" {
  *   share a row where there are few long rows (used where S is even and its
  *   address a multiple of 8), as for DISTILL_TOPK: what it holds means nothing, and
  *   calls that may run at the same time need scratch of their own.
+ *
+ * LINEAR_XENT: X [R, D], W [V, D], one of f32/f16/bf16, R >= 0, V >= 1, D >= 1;
+ *   labels [R] i32; row weights w [R] f32 (optional).  A row counts if its label
+ *   is in [0, V) and its weight is not 0; without weights each row that counts
+ *   has 1 / (rows that count).
+ *     z = X W^T,  row loss_r = log sum_v exp z_rv - z_{r, label},  loss [1] = sum_r w_r row loss_r
+ *     G = w_r (softmax(z) - onehot(label)),  dX [R, D] = G W,  dW [V, D] = G^T X
+ *   A row that does not count is not read: its row loss and its row of dX are 0.
+ *   A logit of -inf has probability 0; a row of nothing else, or with a NaN or
+ *   +inf, has a NaN loss.  Outputs (loss, row loss [R], scratch), (loss, dX, row
+ *   loss, scratch) or (loss, dX, dW, row loss, scratch); dX in X's type, dW in
+ *   W's or f32.  Products and sums are f32; with 16-bit operands G is rounded to
+ *   their type (as the operand of a product), so a f32 dW holds sums of such.
+ *   scratch [n] f32: 4 n >= aicf_linear_xent_scratch(...) bytes for some piece.
+ *   With gradients it holds G of a piece of the classes (16 bits a value for
+ *   16-bit operands); the largest piece that fits is taken, and what the other
+ *   classes' logits cost is computed twice.  Views of W whose rows are not on
+ *   16-byte steps, or D not a multiple of 64 (f32: 32), need scratch for a copy
+ *   of a piece's rows.  Refused: R D (rounded up to 256 and 64) of 2^31 bytes or
+ *   more with gradients, V > 2^28, scratch too small for 256 classes.  What
+ *   scratch holds means nothing; calls that may run at the same time (two
+ *   streams, two graphs) need scratch of their own.
+ *
+ * GRAD_NORM: T >= 1 row-major tensors of rank 0..4, f32/f16/bf16 in any mixture,
+ *   2^42 elements in all at most -> norm [2] f32 and scratch [n] f32 on an 8-byte
+ *   step, n >= 2048 ceil(T / 96).
+ *     norm[0] = sqrt(sum of all squares),  norm[1] = min(1, max_norm / (norm[0] + 1e-6))
+ *   in f64, each rounded once.  With T further outputs, of the tensors' shapes
+ *   and types: G' = norm[1] G, each the tensor itself or memory of its own.  A
+ *   NaN makes norm and factor (so every G') NaN; an infinite norm the factor 0.
+ *   What scratch holds means nothing, and is for one call at a time.
+ *
+ * ADAM_STEP with inputs (P, G, M, V, step i32, norm [2] f32), norm[1] the factor
+ *   as GRAD_NORM writes it: AdamW (schema ADAM with weight decay) on norm[1] G
+ *   instead of G, G f32/f16/bf16; outputs (P, M, V [, bf16 P]), in place or apart.
+ *   With f32 G the results are those of clipping G first, then AdamW, bit for bit.
  */
 
 /* GEPI epilogue kinds.  0..2 are the values core_v2/exec.py:223-252 packs;
@@ -261,6 +303,16 @@ int32_t aicf_dispatch_by_id_v0(int32_t kind, const char* kernel_id,
                                const aicf_tensor_desc* inputs, int32_t num_inputs,
                                aicf_tensor_desc* outputs, int32_t num_outputs,
                                const aicf_attr_blob* attrs, void* stream);
+
+/*
+ * Bytes of scratch of a LINEAR_XENT call over contiguous X [rows, dim] and W
+ * [classes, dim] of `dtype` (AICF_DTYPE_F32/F16/BF16), with gradients or without,
+ * that handles `piece` classes at a time (<= 0: as many as possible, at most all).
+ * Scratch tensors may be larger.  -1 for sizes or a type that the op refuses.
+ * No counterpart in the reference.
+ */
+int64_t aicf_linear_xent_scratch(int64_t rows, int64_t classes, int64_t dim, int32_t dtype, int32_t gradients,
+                                 int64_t piece);
 
 /* Replaces registry/register_all.hpp:8 (aicf_cuda_register_all_kernels).
  * Idempotent: registration happens once per process. */

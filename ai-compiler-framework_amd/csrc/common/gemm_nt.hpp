@@ -49,24 +49,28 @@ struct LxArgs {
   const int32_t* n;      // rows that count: M, or K with rows_are_k
   int rows_are_k;
   int a_mn, b_mn;        // extents of A's and B's rows (M/N-contiguous: columns) in memory
-  int k_split;           // K of a share; workgroups of blockIdx.y = s take share s
-  int64_t split_stride;  // elements of C from share to share
+  // dX: K is divided into shares (chosen on the device: how many rows count is
+  // known there alone).  ACT_LX_SLAB: share s writes slab s of C; ACT_LX_OUT with
+  // `shares` runs where there is one, and SLAB with `direct` where there are more.
+  const int32_t* shares;
+  int direct;
+  int k_piece;           // K that the shares divide
+  int k_before;          // K of the piece whose sums the slabs hold (0: none), to be added to
   // ACT_LX_STATS, ACT_LX_GRAD: logits
   int v0;                // class of column 0
   const int32_t* label;  // class of each row
   float* zlab;           // logit of that class
   float2* stats;         // [tiles_n][stats_ld]: maximum and sum over a tile's classes
   int64_t stats_ld;
-  int keep_from;         // columns from here on go to C as exp(z - tile maximum) * keep_scale
-  float keep_scale;
+  int keep_from;         // columns from here on go to C as exp(z - tile maximum)
   const float* row_max;  // ACT_LX_GRAD: C = exp(z - row_max) row_f - (class == label) row_w
   const float* row_f;
   const float* row_w;
   // ACT_LX_OUT: C[row_map ? row_map[m] : m] = acc * *alpha
   const float* alpha;
   const int32_t* row_map;
-  int vec;               // C's rows lie on 16-byte steps
-  int add;               // ACT_LX_SLAB: C = acc, shares below this one: C + acc (rows on 16-byte steps)
+  int vec;               // C's rows lie on 16-byte steps (a slab's always do)
+  int add;               // (ACT_LX_SLAB, set by the kernel: this share's slab holds sums)
 };
 
 struct NTParams {
@@ -540,6 +544,10 @@ __device__ __forceinline__ void nt_operand_init(NTOperand<KC, BMN, NW, ES>& o, c
   }
 }
 
+// K of a share: whole K-steps of every type.
+__host__ __device__ __forceinline__ int lx_share_k(int k, int shares) {
+  return ((k + shares - 1) / shares + 63) / 64 * 64;
+}
 // The epilogues of ACT_LX_* (linear_xent.hip).
 template <int OUT, int ACT, int BM, int BN, int WM, int WN, int STAGE_BYTES, int MS>
 __device__ void lx_epilogue(const NTParams& p, nt_acc_t<MS> (&acc)[BN / WN / MS][BM / WM / MS], uint8_t* smem,
@@ -581,13 +589,15 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_nt_kernel(NTParams p) {
       p.M = rows;
       p.tiles_m = (rows + BM - 1) / BM;
     }
-    if (p.lx.k_split) {  // A K-contiguous, B N-contiguous
-      const int k0 = blockIdx.y * p.lx.k_split;
-      p.K = p.K - k0 < p.lx.k_split ? p.K - k0 : p.lx.k_split;
-      p.A = (const uint8_t*)p.A + (int64_t)k0 * ES;
-      p.B = (const uint8_t*)p.B + (int64_t)k0 * p.ldb * ES;
-      p.C = (uint8_t*)p.C + blockIdx.y * p.lx.split_stride * (OUT == OUT_F32 ? 4 : 2);
+    if constexpr (ACT == ACT_LX_OUT) {
+      if (p.lx.shares && p.lx.shares[0] != 1) return;
     }
+  }
+  int shares = 1, k_share = 0;
+  if constexpr (ACT == ACT_LX_SLAB) {
+    shares = p.lx.shares[0];
+    if (p.lx.direct && shares == 1) return;
+    k_share = lx_share_k(p.lx.k_piece, shares);
   }
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -792,12 +802,25 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_nt_kernel(NTParams p) {
   // the global stores of a tile's epilogue drain while the next tile's loads
   // and MFMAs run.  With a grid that is a multiple of 8, tile % 8 is the
   // workgroup's XCD, as the remap in tile_coords_of assumes.
-  const int total_tiles = p.tiles_m * p.tiles_n;
-  constexpr bool PERSIST = nt_persistent(BM, BN, WM, WN);
+  int total_tiles = p.tiles_m * p.tiles_n;
+  constexpr bool PERSIST = nt_persistent(BM, BN, WM, WN) || ACT == ACT_LX_SLAB;
+  const int tiles_of_share = total_tiles;
+  NTParams q = p;  // ACT_LX_SLAB: of the tile's share
+  if constexpr (ACT == ACT_LX_SLAB) total_tiles *= shares;
   for (int tile = blockIdx.x; tile < total_tiles; tile += gridDim.x) {
   {
-    int tm_i, tn_i;
-    tile_coords_of(tile, p.tiles_m, p.tiles_n, tm_i, tn_i);
+    int tm_i, tn_i, in_share = tile;
+    if constexpr (ACT == ACT_LX_SLAB) {  // (A K-contiguous, B N-contiguous)
+      const int share = tile / tiles_of_share, k0 = share * k_share;
+      if (k0 >= p.K) continue;  // a short piece has fewer shares
+      in_share = tile - share * tiles_of_share;
+      q.K = p.K - k0 < k_share ? p.K - k0 : k_share;
+      q.A = (const uint8_t*)p.A + (int64_t)k0 * ES;
+      q.B = (const uint8_t*)p.B + (int64_t)k0 * p.ldb * ES;
+      q.C = (float*)p.C + (int64_t)share * (p.tiles_m * BM) * p.ldc;  // (slabs of whole tiles)
+      q.lx.add = k0 < p.lx.k_before;
+    }
+    tile_coords_of<LX>(in_share, p.tiles_m, p.tiles_n, tm_i, tn_i);
     m0 = tm_i * BM;
     n0 = tn_i * BN;
     if constexpr (ACT != ACT_ADAMW && !LX) {
@@ -808,8 +831,8 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_nt_kernel(NTParams p) {
       n0 = n0 < p.N - BN ? n0 : p.N - BN;
     }
   }
-  nt_operand_init<AKC, BM, NW, ES, MS, LX>(opa, p.A, p.lda, m0, p.K, lane, wave, p.lx.a_mn);
-  nt_operand_init<BKC, BN, NW, ES, MS, LX>(opb, p.B, p.ldb, n0, p.K, lane, wave, p.lx.b_mn);
+  nt_operand_init<AKC, BM, NW, ES, MS, LX>(opa, q.A, p.lda, m0, q.K, lane, wave, p.lx.a_mn);
+  nt_operand_init<BKC, BN, NW, ES, MS, LX>(opb, q.B, p.ldb, n0, q.K, lane, wave, p.lx.b_mn);
 #pragma unroll
   for (int i = 0; i < TN; ++i)
 #pragma unroll
@@ -817,8 +840,8 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_nt_kernel(NTParams p) {
 #pragma unroll
       for (int r = 0; r < (MS == 16 ? 4 : 16); ++r) acc[i][j][r] = 0.0f;
 
-  int nk = p.K / (128 / ES);
-  if constexpr (LX) nk = p.K > 0 ? (p.K + 128 / ES - 1) / (128 / ES) : 1;
+  int nk = q.K / (128 / ES);
+  if constexpr (LX) nk = q.K > 0 ? (q.K + 128 / ES - 1) / (128 / ES) : 1;
   constexpr int L1 = NVM / 2;  // with four sub-steps: loads in the first of the two
   // Wait until at most n K-steps of this wave's loads are in flight (and its
   // fragment reads are done); n < S - 1.
@@ -921,7 +944,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_nt_kernel(NTParams p) {
 
   __syncthreads();  // every wave is done reading the last stage
   if constexpr (LX)
-    lx_epilogue<OUT, ACT, BM, BN, WM, WN, 2 * STAGE, MS>(p, acc, smem, m0, n0);
+    lx_epilogue<OUT, ACT, BM, BN, WM, WN, 2 * STAGE, MS>(q, acc, smem, m0, n0);
   else
     nt_epilogue_staged<OUT, ACT, BM, BN, WM, WN, 2 * STAGE, MS>(p, acc, smem, m0, n0);
   if constexpr (!PERSIST) break;  // one tile per workgroup: no loop-carried registers

@@ -173,11 +173,16 @@ __device__ __forceinline__ floatx4 mfma16(const uint16_t* a, const uint16_t* b, 
 // Grouped raster: workgroup w of XCD x (dispatch order w*8+x) gets
 // tile (tm, tn) so that each XCD sweeps a contiguous run of tiles and
 // GROUP_M consecutive tile rows share B columns in its L2.
+// ANY: also where 8 does not divide the tiles; the first total % 8 XCDs get one more.
+template <bool ANY = false>
 __device__ __forceinline__ void tile_coords_of(int id, int tiles_m, int tiles_n, int& tm, int& tn) {
   const int total = tiles_m * tiles_n;
   // XCD-aware remap: hardware id i runs on XCD (i % 8); give every XCD a
   // contiguous range of logical ids.
-  if ((total & 7) == 0) {
+  if constexpr (ANY) {
+    const int x = id & 7, more = total & 7;
+    id = x * (total >> 3) + (x < more ? x : more) + (id >> 3);
+  } else if ((total & 7) == 0) {
     const int per = total >> 3;
     id = (id & 7) * per + (id >> 3);
   }

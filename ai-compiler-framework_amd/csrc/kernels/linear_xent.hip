@@ -40,6 +40,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 // 2^((z - m) log2 e): the difference first, so that the exponent is off by
 // roundings of itself alone however far the logits lie from zero.
 __device__ __forceinline__ float exp_from(float z, float m) { return __builtin_amdgcn_exp2f((z - m) * kLog2e); }
+// f16: the kept exponentials are at most 2^14, so that they lose bits only below 2^-28 of their tile's largest.
+constexpr float kKeepScale = 16384.0f;
 // A maximum over nothing but -inf is no reference: their exponentials are 0.
 __device__ __forceinline__ float safe_ref(float m) { return m == -INFINITY ? 0.0f : m; }
 // What a sum of exp(z - m) is multiplied by where the reference becomes `to`.
@@ -64,72 +66,70 @@ __device__ __forceinline__ void lx_epilogue(const NTParams& p, nt_acc_t<MS> (&ac
   auto col_of = [&](int i, int g) -> int { return wn * WTN + i * MS + (MS == 32 ? 8 * g + 4 * fh : 4 * fh); };
   auto row_of = [&](int j) -> int { return wm * WTM + j * MS + fr; };
 
+  const int ncol = p.N - n0;  // classes (columns) of the tile
+  // Accumulators are read where they are used and never written: changed in
+  // place, the 256 of a lane of the four-wave tiles went through a second set.
+  auto value = [&](auto TAIL, int i, int j, int r) -> float {
+    if constexpr (decltype(TAIL)::value)
+      return col_of(i, r >> 2) + (r & 3) < ncol ? acc[i][j][r] : -INFINITY;
+    return acc[i][j][r];
+  };
+
   if constexpr (ACT == ACT_LX_STATS) {
     float* red_m = reinterpret_cast<float*>(smem);  // [WN][BM]
     float* red_s = red_m + WN * BM;
     static_assert(2 * WN * BM * 4 <= STAGE_BYTES, "the waves' statistics fit");
-    const int ncol = p.N - n0;
-    if (ncol < BN) {  // the last tile's columns without a class
+    auto maxima = [&](auto TAIL) {
 #pragma unroll
-      for (int i = 0; i < TN; ++i)
+      for (int j = 0; j < TM; ++j) {
+        float m = -INFINITY;
 #pragma unroll
-        for (int g = 0; g < G; ++g)
+        for (int i = 0; i < TN; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (col_of(i, g) + e >= ncol) {
+          for (int r = 0; r < 4 * G; ++r) m = fmaxf(m, value(TAIL, i, j, r));
+        if constexpr (MS == 16) m = fmaxf(m, __shfl_xor(m, 16, 64));
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
+        if (fh == 0) red_m[wn * BM + row_of(j)] = m;
+      }
+    };
+    auto sums = [&](auto TAIL) {
 #pragma unroll
-              for (int j = 0; j < TM; ++j) acc[i][j][4 * g + e] = -INFINITY;
-            }
-    }
+      for (int j = 0; j < TM; ++j) {
+        float m = red_m[row_of(j)];
 #pragma unroll
-    for (int j = 0; j < TM; ++j) {
-      float m = -INFINITY;
+        for (int w = 1; w < WN; ++w) m = fmaxf(m, red_m[w * BM + row_of(j)]);
+        m = safe_ref(m);
+        float s = 0.0f;
 #pragma unroll
-      for (int i = 0; i < TN; ++i)
+        for (int i = 0; i < TN; ++i)
 #pragma unroll
-        for (int r = 0; r < 4 * G; ++r) m = fmaxf(m, acc[i][j][r]);
-      if constexpr (MS == 16) m = fmaxf(m, __shfl_xor(m, 16, 64));
-      m = fmaxf(m, __shfl_xor(m, 32, 64));
-      if (fh == 0) red_m[wn * BM + row_of(j)] = m;
-    }
+          for (int r = 0; r < 4 * G; ++r) s += exp_from(value(TAIL, i, j, r), m);
+        if constexpr (MS == 16) s += __shfl_xor(s, 16, 64);
+        s += __shfl_xor(s, 32, 64);
+        if (fh == 0) red_s[wn * BM + row_of(j)] = s;
+      }
+    };
+    const bool tail = ncol < BN;
+    if (tail) maxima(std::true_type{});
+    else maxima(std::false_type{});
     // the label's logit: one lane of one tile has it
 #pragma unroll
     for (int j = 0; j < TM; ++j) {
       const int m = m0 + row_of(j);
-      const int c = m < p.M ? p.lx.label[m] - p.lx.v0 - n0 : -1;
-      if (c >= 0 && c < BN) {
+      const int c = (m < p.M ? p.lx.label[m] - p.lx.v0 - n0 : -1) - wn * WTN;
+      if (c >= 0 && c < WTN && ((c >> 2) & (64 / MS - 1)) == fh) {
+        float z = 0.0f;
 #pragma unroll
         for (int i = 0; i < TN; ++i)
 #pragma unroll
-          for (int g = 0; g < G; ++g)
-            if ((c >> 2) == (col_of(i, g) >> 2)) {
-              const int e = c & 3;
-              p.lx.zlab[m] = e == 0 ? acc[i][j][4 * g] : e == 1 ? acc[i][j][4 * g + 1]
-                           : e == 2 ? acc[i][j][4 * g + 2] : acc[i][j][4 * g + 3];
-            }
+          for (int r = 0; r < 4 * G; ++r)
+            z = c == i * MS + (MS == 32 ? 8 * (r >> 2) : 0) + 4 * fh + (r & 3) ? acc[i][j][r] : z;
+        p.lx.zlab[m] = z;
       }
     }
     __syncthreads();
-    const bool keep = n0 >= p.lx.keep_from;
-#pragma unroll
-    for (int j = 0; j < TM; ++j) {
-      float m = red_m[row_of(j)];
-#pragma unroll
-      for (int w = 1; w < WN; ++w) m = fmaxf(m, red_m[w * BM + row_of(j)]);
-      m = safe_ref(m);
-      float s = 0.0f;
-#pragma unroll
-      for (int i = 0; i < TN; ++i)
-#pragma unroll
-        for (int r = 0; r < 4 * G; ++r) {
-          const float e = exp_from(acc[i][j][r], m);
-          s += e;
-          acc[i][j][r] = e * p.lx.keep_scale;
-        }
-      if constexpr (MS == 16) s += __shfl_xor(s, 16, 64);
-      s += __shfl_xor(s, 32, 64);
-      if (fh == 0) red_s[wn * BM + row_of(j)] = s;
-    }
+    if (tail) sums(std::true_type{});
+    else sums(std::false_type{});
     __syncthreads();
     for (int t = tid; t < BM; t += NT) {
       float m = red_m[t], s = red_s[t];
@@ -140,40 +140,55 @@ __device__ __forceinline__ void lx_epilogue(const NTParams& p, nt_acc_t<MS> (&ac
       }
       p.lx.stats[(int64_t)((p.lx.v0 + n0) / BN) * p.lx.stats_ld + m0 + t] = make_float2(m, s);
     }
-    if (!keep) return;
-    __syncthreads();
-  } else if constexpr (ACT == ACT_LX_GRAD) {
-    const int ncol = p.N - n0;
-#pragma unroll
-    for (int j = 0; j < TM; ++j) {
-      const int m = m0 + row_of(j);
-      const bool in = m < p.M;
-      const float rm = in ? safe_ref(p.lx.row_max[m]) : 0.0f, f = in ? p.lx.row_f[m] : 0.0f;
-      const float w = in ? p.lx.row_w[m] : 0.0f;
-      const int c = in ? p.lx.label[m] - p.lx.v0 - n0 : -1;
-#pragma unroll
-      for (int i = 0; i < TN; ++i)
-#pragma unroll
-        for (int g = 0; g < G; ++g)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int col = col_of(i, g) + e;
-            float v = exp_from(acc[i][j][4 * g + e], rm) * f;
-            v = col == c ? v - w : v;
-            acc[i][j][4 * g + e] = col < ncol ? v : 0.0f;
-          }
-    }
-  } else if constexpr (ACT == ACT_LX_OUT) {
-    const float a = p.lx.alpha[0];
-#pragma unroll
-    for (int i = 0; i < TN; ++i)
-#pragma unroll
-      for (int j = 0; j < TM; ++j)
-#pragma unroll
-        for (int r = 0; r < 4 * G; ++r) acc[i][j][r] *= a;
+    if (n0 < p.lx.keep_from) return;
   }
 
   // Through LDS, so that whole rows are stored (as nt_epilogue_staged does).
+  // A pass' four columns of a lane, v[4], from the row's constants c.
+  struct RowConst {
+    float a, f, w;  // reference or factor; G: factor and weight
+    int col;        // G: the label's column
+  };
+  auto row_const = [&](int j) -> RowConst {
+    RowConst c{0.0f, 0.0f, 0.0f, -1};
+    const int m = m0 + row_of(j);
+    if constexpr (ACT == ACT_LX_STATS) {
+      const float* red_m = reinterpret_cast<const float*>(smem);
+      c.a = red_m[row_of(j)];
+#pragma unroll
+      for (int w = 1; w < WN; ++w) c.a = fmaxf(c.a, red_m[w * BM + row_of(j)]);
+      c.a = safe_ref(c.a);
+    } else if constexpr (ACT == ACT_LX_GRAD) {
+      if (m < p.M) {
+        c.a = safe_ref(p.lx.row_max[m]);
+        c.f = p.lx.row_f[m];
+        c.w = p.lx.row_w[m];
+        c.col = p.lx.label[m] - p.lx.v0 - n0;
+      }
+    } else if constexpr (ACT == ACT_LX_OUT) {
+      c.a = p.lx.alpha[0];
+    }
+    return c;
+  };
+  auto result = [&](const RowConst& c, int i, int j, int g, int e) -> float {
+    const float z = acc[i][j][4 * g + e];
+    const int col = col_of(i, g) + e;
+    if constexpr (ACT == ACT_LX_STATS) {
+      const float v = exp_from(col < ncol ? z : -INFINITY, c.a);
+      return OUT == OUT_F16 ? v * kKeepScale : v;
+    } else if constexpr (ACT == ACT_LX_GRAD) {
+      const float v = exp_from(z, c.a) * c.f;
+      return col < ncol ? (col == c.col ? v - c.w : v) : 0.0f;
+    } else if constexpr (ACT == ACT_LX_OUT) {
+      return z * c.a;
+    } else {
+      return z;
+    }
+  };
+  RowConst rc[TM];
+#pragma unroll
+  for (int j = 0; j < TM; ++j) rc[j] = row_const(j);
+  if constexpr (ACT == ACT_LX_STATS) __syncthreads();  // the maxima are read: the stage is free
   constexpr int ROWB = BN * OB, CPR = ROWB / 16, CE = 16 / OB;
   constexpr int ROWS_PASS = STAGE_BYTES / ROWB < BM ? STAGE_BYTES / ROWB : BM;
   constexpr int NPASS = BM / ROWS_PASS, JP = TM / NPASS, WROWS = JP * MS;
@@ -188,18 +203,19 @@ __device__ __forceinline__ void lx_epilogue(const NTParams& p, nt_acc_t<MS> (&ac
       for (int i = 0; i < TN; ++i)
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-          const nt_acc_t<MS>& a = acc[i][pass * JP + jj];
+          const int j = pass * JP + jj;
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = result(rc[j], i, j, g, e);
           const int pr = wm * WROWS + jj * MS + fr, cb = col_of(i, g) * OB;
           uint8_t* at = smem + pr * ROWB + (((cb / 16) ^ (pr & (CPR - 1))) * 16) + cb % 16;
           if constexpr (OUT == OUT_F32) {
-            *reinterpret_cast<f32x4*>(at) = f32x4{a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]};
+            *reinterpret_cast<f32x4*>(at) = f32x4{v[0], v[1], v[2], v[3]};
           } else if constexpr (OUT == OUT_BF16) {
             typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-            *reinterpret_cast<u32x2*>(at) =
-                u32x2{f32x2_to_bf16x2(a[4 * g], a[4 * g + 1]), f32x2_to_bf16x2(a[4 * g + 2], a[4 * g + 3])};
+            *reinterpret_cast<u32x2*>(at) = u32x2{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3])};
           } else {
-            *reinterpret_cast<u16x4*>(at) = u16x4{f32_to_f16(a[4 * g]), f32_to_f16(a[4 * g + 1]),
-                                                  f32_to_f16(a[4 * g + 2]), f32_to_f16(a[4 * g + 3])};
+            *reinterpret_cast<u16x4*>(at) = u16x4{f32_to_f16(v[0]), f32_to_f16(v[1]), f32_to_f16(v[2]), f32_to_f16(v[3])};
           }
         }
     __syncthreads();
@@ -214,7 +230,7 @@ __device__ __forceinline__ void lx_epilogue(const NTParams& p, nt_acc_t<MS> (&ac
         if (n >= p.ldc) continue;  // (a slab's rows are whole 64s)
         f32x4* q = reinterpret_cast<f32x4*>((float*)p.C + (int64_t)m * p.ldc + n);
         f32x4 v = __builtin_bit_cast(f32x4, x);
-        if ((int)blockIdx.y < p.lx.add) v += *q;
+        if (p.lx.add) v += *q;
         *q = v;
       } else if constexpr (ACT != ACT_LX_OUT) {  // G's rows hold whole tiles
         out_t* q = (out_t*)p.C + (int64_t)m * p.ldc + (n0 - (ACT == ACT_LX_STATS ? p.lx.keep_from : 0)) + c * CE;
@@ -244,12 +260,13 @@ __device__ __forceinline__ void lx_epilogue(const NTParams& p, nt_acc_t<MS> (&ac
 // ---------------------------------------------------------------------------
 // Scratch of a call, in this order; every array starts on 256 bytes.
 struct LxRows {
-  int32_t* head;    // [0] rows that count, [1] f32 alpha: what the products with G are multiplied by
+  int32_t* head;    // [0] rows that count; f32 [1] what the products with G are multiplied by, [2] its inverse,
+                    // [3] 1 / rows that count; [4] shares of dX's K
   int32_t* pos;     // [R] place of a row among those that count, -1: left out
   int32_t* idx;     // [Rp] and back
   int32_t* label;   // [Rp] of the rows that count, like all below
   float* weight;    // as given
-  float* row_w;     // times 1 / alpha
+  float* row_w;     // times head[2]
   float* zlab;
   float* row_max;
   float* row_f;     // row_w / sum of exp(z - row_max)
@@ -260,76 +277,6 @@ struct LxRows {
   void* wpad;       // [piece][Dp] rows of W, where W itself cannot be read in tiles
   void* g;          // [Rp][piece]
 };
-
-// Which rows count, and the power of two that brings the largest weight to
-// 2^(top-1) .. 2^top.  One workgroup: a thread takes consecutive rows.
-__global__ __launch_bounds__(1024) void lx_rows_kernel(const int32_t* __restrict__ labels,
-                                                       const float* __restrict__ w, int R, int V, int top,
-                                                       LxRows s) {
-  __shared__ int cnt[17];
-  __shared__ float big[17];
-  const int per = (R + 1023) / 1024, r0 = threadIdx.x * per, r1 = r0 + per < R ? r0 + per : R;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  auto counts = [&](int r) {
-    const int c = labels[r];
-    return c >= 0 && c < V && (!w || w[r] != 0.0f);
-  };
-  int n = 0;
-  float most = 0.0f;
-  for (int r = r0; r < r1; ++r)
-    if (counts(r)) {
-      ++n;
-      if (w) most = fmaxf(most, fabsf(w[r]));
-    }
-  int before = n;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int o = __shfl_up(before, off, 64);
-    if (lane >= off) before += o;
-  }
-  most = wave_max(most);
-  if (lane == 63) cnt[wave] = before;
-  if (lane == 0) big[wave] = most;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    int sum = 0;
-    float m = 0.0f;
-    for (int i = 0; i < 16; ++i) {
-      const int c = cnt[i];
-      cnt[i] = sum;
-      sum += c;
-      m = fmaxf(m, big[i]);
-    }
-    cnt[16] = sum;
-    big[16] = m;
-  }
-  __syncthreads();
-  const int total = cnt[16];
-  const float mean = total > 0 ? 1.0f / (float)total : 0.0f;
-  const float m = w ? big[16] : mean;
-  int e = 0;
-  if (m > 0.0f && m < INFINITY) frexpf(m, &e);  // m < 2^e
-  e = top - e;
-  e = e > 126 ? 126 : e < -126 ? -126 : e;
-  const float up = ldexpf(1.0f, e);
-  if (threadIdx.x == 0) {
-    s.head[0] = total;
-    s.head[1] = __float_as_int(ldexpf(1.0f, -e));
-  }
-  int at = cnt[wave] + before - n;
-  for (int r = r0; r < r1; ++r) {
-    const bool c = counts(r);
-    s.pos[r] = c ? at : -1;
-    if (c) {
-      const float wr = w ? w[r] : mean;
-      s.idx[at] = r;
-      s.label[at] = labels[r];
-      s.weight[at] = wr;
-      s.row_w[at] = wr * up;
-      ++at;
-    }
-  }
-}
 
 template <int ES>
 struct LxElem;
@@ -346,81 +293,235 @@ struct LxElem<4> {
   typedef f32x4_a4 loose;
 };
 
-// Rows copied onto 16-byte steps, zeros behind the D-th element to Dp (a
-// multiple of 64); pos: to row pos[r], and a row that is left out has its
-// gradient and loss cleared instead.  A wave a row.
+struct LxCopy {
+  const void* src;
+  void* dst;   // [.][Dp], 16-byte steps
+  void* dx;    // nullptr: none
+  float* row_loss;
+  int64_t lds, lddx;
+  int D, Dp;
+};
+
+// Row r of src (D elements) to row `to` of dst, zeros behind them to Dp; to < 0:
+// a row that is left out, whose gradient and loss are cleared instead.  By a wave.
 template <int ES>
-__global__ __launch_bounds__(256) void lx_copy_rows_kernel(const void* __restrict__ src, int64_t lds, void* dst,
-                                                           int D, int Dp, int rows, const int32_t* __restrict__ pos,
-                                                           void* dx, int64_t lddx, float* row_loss) {
+__device__ __forceinline__ void lx_copy_row(const LxCopy& c, int64_t r, int to, int lane) {
   typedef typename LxElem<ES>::T T;
   typedef typename LxElem<ES>::vec vec;
   typedef typename LxElem<ES>::loose loose;
   constexpr int CE = 16 / ES;
-  const int lane = threadIdx.x & 63;
-  const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (r >= rows) return;
-  const int to = pos ? pos[r] : r;
   if (to >= 0) {
-    const T* a = (const T*)src + (int64_t)r * lds;
-    T* b = (T*)dst + (int64_t)to * Dp;
-    for (int c = lane * CE; c < Dp; c += 64 * CE) {
+    const T* a = (const T*)c.src + r * c.lds;
+    T* b = (T*)c.dst + (int64_t)to * c.Dp;
+    for (int i = lane * CE; i < c.Dp; i += 64 * CE) {
       vec v;
-      if (c + CE <= D) {
-        v = *reinterpret_cast<const loose*>(a + c);
+      if (i + CE <= c.D) {
+        v = *reinterpret_cast<const loose*>(a + i);
       } else {
 #pragma unroll
-        for (int e = 0; e < CE; ++e) v[e] = c + e < D ? a[c + e] : T(0);
+        for (int e = 0; e < CE; ++e) v[e] = i + e < c.D ? a[i + e] : T(0);
       }
-      *reinterpret_cast<vec*>(b + c) = v;
+      *reinterpret_cast<vec*>(b + i) = v;
     }
     return;
   }
-  if (lane == 0) row_loss[r] = 0.0f;
-  if (!dx) return;
-  T* b = (T*)dx + (int64_t)r * lddx;
-  for (int c = lane * CE; c < D; c += 64 * CE) {
-    if (c + CE <= D) {
+  if (lane == 0) c.row_loss[r] = 0.0f;
+  if (!c.dx) return;
+  T* b = (T*)c.dx + r * c.lddx;
+  for (int i = lane * CE; i < c.D; i += 64 * CE) {
+    if (i + CE <= c.D) {
       loose v;
 #pragma unroll
       for (int e = 0; e < CE; ++e) v[e] = T(0);
-      *reinterpret_cast<loose*>(b + c) = v;
+      *reinterpret_cast<loose*>(b + i) = v;
     } else {
-      for (int e = 0; c + e < D; ++e) b[c + e] = T(0);
+      for (int e = 0; i + e < c.D; ++e) b[i + e] = T(0);
     }
   }
 }
 
+// Rows of X to their places, or (without pos) rows of W onto 16-byte steps.
+template <int ES>
+__global__ __launch_bounds__(256) void lx_copy_rows_kernel(LxCopy c, int rows, const int32_t* __restrict__ pos) {
+  const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r < rows) lx_copy_row<ES>(c, r, pos ? pos[r] : r, threadIdx.x & 63);
+}
+
+// How dX's tiles are shared out: tiles of bm rows, tiles_n in a row of them,
+// `slots` workgroups run at once, K-steps of a piece, rows that a slab may have.
+struct LxShares {
+  int bm, tiles_n, slots, k_piece, slab_rows;
+};
+
+// Which rows count, the power of two that brings the largest weight to
+// 2^(top-1) .. 2^top, and how many shares dX's K is divided into.  One
+// workgroup: 16 rows a thread at a time.
+// COPY (at most 64 rows): also what lx_copy_rows_kernel does.
+template <int ES, bool COPY>
+__global__ __launch_bounds__(1024) void lx_rows_kernel(const int32_t* __restrict__ labels,
+                                                       const float* __restrict__ w, int R, int V, int top, LxRows s,
+                                                       LxShares sh, LxCopy cp) {
+  constexpr int PER = COPY ? 1 : 16;
+  __shared__ int cnt[PER * 16 + 1];
+  __shared__ float big[16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float most = 0.0f;
+  int total = 0;
+  for (int base = 0; base < R; base += PER * 1024) {
+    int label[PER];
+    uint64_t in[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int r = base + k * 1024 + threadIdx.x;
+      label[k] = r < R ? labels[r] : -1;
+      const float wr = r < R && w ? w[r] : 1.0f;
+      const bool c = label[k] >= 0 && label[k] < V && wr != 0.0f;
+      if (c) most = fmaxf(most, fabsf(wr));
+      in[k] = __ballot(c);
+      if (lane == 0) cnt[k * 16 + wave] = __popcll(in[k]);
+    }
+    __syncthreads();
+    if (wave == 0) {  // places of the groups of 64 rows, in the rows' order
+      int before[(PER * 16 + 63) / 64], sum = 0;
+      constexpr int EACH = (PER * 16 + 63) / 64;
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        const int at = lane * EACH + i;
+        before[i] = sum;
+        sum += at < PER * 16 ? cnt[at] : 0;
+      }
+      int up = sum;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const int o = __shfl_up(up, off, 64);
+        if (lane >= off) up += o;
+      }
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        const int at = lane * EACH + i;
+        if (at < PER * 16) cnt[at] = total + up - sum + before[i];
+      }
+      if (lane == 63) cnt[PER * 16] = total + up;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int r = base + k * 1024 + threadIdx.x;
+      if (r >= R) continue;
+      const bool c = in[k] >> lane & 1;
+      const int at = cnt[k * 16 + wave] + __popcll(in[k] & ((1ull << lane) - 1));
+      s.pos[r] = c ? at : -1;
+      if (c) {
+        s.idx[at] = r;
+        s.label[at] = label[k];
+        if (w) s.weight[at] = w[r];
+      }
+    }
+    total = cnt[PER * 16];
+    __syncthreads();
+  }
+  most = wave_max(most);
+  if (lane == 0) big[wave] = most;
+  __syncthreads();
+  if (wave == 0) {
+    float m = big[lane & 15];
+    m = wave_max(m);
+    const float mean = total > 0 ? 1.0f / (float)total : 0.0f;
+    if (!w) m = mean;
+    int e = 0;
+    if (m > 0.0f && m < INFINITY) frexpf(m, &e);  // m < 2^e
+    e = top - e;
+    e = e > 126 ? 126 : e < -126 ? -126 : e;
+    // Shares: rounds of the workgroups that run at once, times a share's K-steps
+    // and some 8 for a tile's first loads and its end; a share's sums are
+    // written and read once more (1/32 of a step a tile when all CUs do it).
+    const int tiles = (total + sh.bm - 1) / sh.bm * sh.tiles_n, k = lane + 1;
+    const int steps = (sh.k_piece + 63) / 64;
+    float cost = INFINITY;
+    if (k == 1 || (steps / k >= 8 && (int64_t)k * ((total + sh.bm - 1) / sh.bm * sh.bm) <= sh.slab_rows &&
+                   tiles * k <= 4 * sh.slots))
+      cost = (float)((tiles * k + sh.slots - 1) / sh.slots) * (float)((steps + k - 1) / k + 8) +
+             (k > 1 ? 4.0f + (float)(tiles * k) * (8.0f / 256.0f) : 0.0f);
+    int best = k;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+      const float oc = __shfl_xor(cost, off, 64);
+      const int ok = __shfl_xor(best, off, 64);
+      if (oc < cost || (oc == cost && ok < best)) {
+        cost = oc;
+        best = ok;
+      }
+    }
+    if (lane == 0) {
+      s.head[0] = total;
+      s.head[1] = __float_as_int(ldexpf(1.0f, -e));
+      s.head[2] = __float_as_int(ldexpf(1.0f, e));
+      s.head[3] = __float_as_int(mean);
+      s.head[4] = best;
+    }
+  }
+  if constexpr (COPY) {
+    __syncthreads();
+    for (int r = wave; r < R; r += 16) lx_copy_row<ES>(cp, r, s.pos[r], lane);
+  }
+}
+
 // The statistics of a row's tiles joined: 64 rows a workgroup, wave w takes
-// tiles w, w + 16, ...; the waves in order.
-__global__ __launch_bounds__(1024) void lx_stats_kernel(LxRows s, int tiles, int64_t ld,
-                                                        float* __restrict__ row_loss) {
+// tiles w, w + 16, ..., eight loads in flight; the waves in order.  loss (at
+// most 64 rows, one workgroup): their weighted sum too.
+__global__ __launch_bounds__(1024) void lx_stats_kernel(LxRows s, int tiles, int64_t ld, bool weights,
+                                                        float* __restrict__ row_loss, float* __restrict__ loss) {
   __shared__ float2 red[16][64];
   const int n = s.head[0], lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int r = blockIdx.x * 64 + lane;
-  if (blockIdx.x * 64 >= n) return;
+  if (blockIdx.x * 64 >= n) {
+    if (loss && threadIdx.x == 0) loss[0] = 0.0f;
+    return;
+  }
   float m = -INFINITY, sum = 0.0f;
-  for (int t = wave; t < tiles; t += 16) {
-    const float2 v = s.stats[(int64_t)t * ld + r];  // (rows behind n: whatever is there, not used)
-    const float top = fmaxf(m, v.x), ref = safe_ref(top);
-    sum = sum * rebase(m, ref) + v.y * rebase(v.x, ref);
+  for (int t0 = wave; t0 < tiles; t0 += 16 * 8) {
+    float2 v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int t = t0 + u * 16;  // (rows behind n: whatever is there, not used)
+      v[u] = t < tiles ? s.stats[(int64_t)t * ld + r] : make_float2(-INFINITY, 0.0f);
+    }
+    float top = m;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) top = fmaxf(top, v[u].x);
+    const float ref = safe_ref(top);
+    sum *= rebase(m, ref);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) sum += v[u].y * rebase(v[u].x, ref);
     m = top;
   }
   red[wave][lane] = make_float2(m, sum);
   __syncthreads();
-  if (wave > 0 || r >= n) return;
-  m = red[0][lane].x;
+  if (wave > 0) return;
+  float part = 0.0f, weight = 0.0f;
+  if (r < n) {
+    m = red[0][lane].x;
 #pragma unroll
-  for (int w = 1; w < 16; ++w) m = fmaxf(m, red[w][lane].x);
-  const float ref = safe_ref(m);
-  sum = 0.0f;
+    for (int w = 1; w < 16; ++w) m = fmaxf(m, red[w][lane].x);
+    const float ref = safe_ref(m);
+    sum = 0.0f;
 #pragma unroll
-  for (int w = 0; w < 16; ++w) sum += red[w][lane].y * rebase(red[w][lane].x, ref);
-  s.row_max[r] = m;
-  s.row_f[r] = s.row_w[r] / sum;
-  const float loss = logf(sum) + (ref - s.zlab[r]);
-  s.row_loss[r] = loss;
-  row_loss[s.idx[r]] = loss;
+    for (int w = 0; w < 16; ++w) sum += red[w][lane].y * rebase(red[w][lane].x, ref);
+    weight = weights ? s.weight[r] : __int_as_float(s.head[3]);
+    const float up = weight * __int_as_float(s.head[2]);
+    s.row_max[r] = m;
+    s.row_w[r] = up;
+    s.row_f[r] = up / sum;
+    part = logf(sum) + (ref - s.zlab[r]);
+    s.row_loss[r] = part;
+    if (!weights) s.weight[r] = weight;
+    row_loss[s.idx[r]] = part;
+  }
+  if (!loss) return;
+  double v = (double)weight * (double)part;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  if (lane == 0) loss[0] = (float)v;
 }
 
 // loss = sum of weight * row loss, in f64 and a fixed order.
@@ -443,8 +544,8 @@ __global__ __launch_bounds__(1024) void lx_loss_kernel(LxRows s, float* __restri
 // The kept exp(z - tile maximum) of classes v0 .. v0 + cols become G in place.
 // A lane takes 16 bytes; a tile of BN classes has one factor a row.
 template <int EK, int BN>
-__global__ __launch_bounds__(256) void lx_scale_kernel(LxRows s, int64_t ldg, int width, int v0, int64_t stats_ld,
-                                                       float keep_scale) {
+__global__ __launch_bounds__(256) void lx_scale_kernel(LxRows s, int64_t ldg, int width, int v0,
+                                                       int64_t stats_ld) {
   constexpr int ES = EK == EL_F32 ? 4 : 2, CE = 16 / ES;
   typedef typename LxElem<ES>::T T;
   typedef typename LxElem<ES>::vec vec;
@@ -453,7 +554,7 @@ __global__ __launch_bounds__(256) void lx_scale_kernel(LxRows s, int64_t ldg, in
   if (c >= width) return;
   for (int r = blockIdx.y; r < n; r += gridDim.y) {
     const float2 st = s.stats[(int64_t)((v0 + c) / BN) * stats_ld + r];
-    const float f = rebase(st.x, safe_ref(s.row_max[r])) * s.row_f[r] / keep_scale;
+    const float f = rebase(st.x, safe_ref(s.row_max[r])) * s.row_f[r] * (EK == EL_F16 ? 1.0f / kKeepScale : 1.0f);
     T* q = (T*)s.g + (int64_t)r * ldg + c;
     vec x = *reinterpret_cast<const vec*>(q);
     const int at = s.label[r] - v0 - c;
@@ -479,17 +580,29 @@ __global__ __launch_bounds__(256) void lx_scale_kernel(LxRows s, int64_t ldg, in
   }
 }
 
-// dX from its slabs: alpha times their sum, in order, to the row it came from.
+// dX from its slabs: head[1] times their sum, in order, to the row it came from.
 template <int EK>
-__global__ __launch_bounds__(256) void lx_finish_kernel(LxRows s, int shares, int64_t stride, int64_t ld, int D,
+__global__ __launch_bounds__(256) void lx_finish_kernel(LxRows s, int direct, int k_piece, int bm, int64_t ld, int D,
                                                         void* dx, int64_t lddx) {
-  const int n = s.head[0];
+  const int n = s.head[0], shares = s.head[4];
+  if (direct && shares == 1) return;  // (stored by the product itself)
+  const int k_share = lx_share_k(k_piece, shares), slabs = (k_piece + k_share - 1) / k_share;
+  const int64_t stride = (int64_t)((n + bm - 1) / bm * bm) * ld;
   const float alpha = __int_as_float(s.head[1]);
   const int c = (blockIdx.x * 256 + threadIdx.x) * 4;
   if (c >= D) return;
   for (int r = blockIdx.y; r < n; r += gridDim.y) {
-    f32x4 v = *reinterpret_cast<const f32x4*>(s.slab + (int64_t)r * ld + c);
-    for (int k = 1; k < shares; ++k) v += *reinterpret_cast<const f32x4*>(s.slab + k * stride + (int64_t)r * ld + c);
+    const float* q = s.slab + (int64_t)r * ld + c;
+    f32x4 v{0.0f, 0.0f, 0.0f, 0.0f};
+    int k = 0;
+    for (; k + 8 <= slabs; k += 8) {
+      f32x4 x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) x[u] = *reinterpret_cast<const f32x4*>(q + (k + u) * stride);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v += x[u];
+    }
+    for (; k < slabs; ++k) v += *reinterpret_cast<const f32x4*>(q + k * stride);
     const int64_t at = (int64_t)s.idx[r] * lddx + c;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -506,16 +619,19 @@ __global__ __launch_bounds__(256) void lx_finish_kernel(LxRows s, int shares, in
 // ---------------------------------------------------------------------------
 int64_t up_to(int64_t n, int64_t step) { return (n + step - 1) / step * step; }
 
-// Tiles of a product of `rows` rows: 32, 64, 128 or 256 of them.
+// Rows of a product's tiles.  16-bit: 256 (256 x 256) where those fill three
+// quarters of the CUs, else 128, for few rows 64 or 32.  f32 is bound by its
+// MFMAs, so by the CU with most tiles: 64 x 64 unless 128 x 128 give it no more.
 int lx_tile_rows(int64_t rows, int64_t cols, bool f32) {
   if (rows <= 32) return 32;
-  if (f32) return 128;
+  auto tiles = [&](int64_t n) { return ((rows + n - 1) / n) * ((cols + n - 1) / n); };
+  if (f32) return (tiles(64) + 255) / 256 < 4 * ((tiles(128) + 255) / 256) ? 64 : 128;
   if (rows <= 64) return 64;
-  if (rows <= 128 || ((rows + 255) / 256) * ((cols + 255) / 256) < 192) return 128;
-  return 256;
+  return rows <= 128 || tiles(256) < 192 ? 128 : 256;
 }
-// Columns of those tiles.
-int lx_tile_cols(int bm) { return bm == 256 ? 256 : 128; }
+// Their columns, and how many of them run on the chip at once (by LDS).
+int lx_tile_cols(int bm, bool f32) { return bm == 256 ? 256 : bm == 64 && f32 ? 64 : 128; }
+int lx_slots(int bm, bool f32) { return 256 * (f32 ? (bm == 128 ? 2 : 4) : bm == 128 || bm == 32 ? 2 : 1); }
 
 struct LxCall {
   const TensorDesc *x, *w, *labels, *rw, *loss, *dx, *dw, *row_loss, *scratch;
@@ -529,8 +645,7 @@ struct LxPlan {
   bool direct;              // W is read in place
   int64_t piece;            // classes of a piece (a multiple of 256)
   int bm_dx;                // tiles of dX
-  int64_t shares, k_share;  // of the classes of a piece
-  int64_t slab_rows;
+  int64_t slab_rows;        // of all its slabs together
   int64_t stats_off, xc_off, slab_off, wpad_off, g_off, bytes;
 };
 
@@ -547,7 +662,7 @@ bool lx_plan(int64_t R, int64_t V, int64_t D, int64_t ldw, bool direct, bool f32
   p.Vp = up_to(V, 256);
   p.direct = direct;
   p.bm = lx_tile_rows(R, V, f32);
-  p.bn = lx_tile_cols(p.bm);
+  p.bn = lx_tile_cols(p.bm, f32);
   const int64_t lim = INT32_MAX;  // 32-bit offsets into an operand
   const int64_t ldk = direct ? ldw : p.Dp;
   if (p.Rp > lim / 2 || p.Dp * p.es * 256 >= lim || ldk * p.es * 256 >= lim || p.Vp > (int64_t)1 << 28) return false;
@@ -558,10 +673,10 @@ bool lx_plan(int64_t R, int64_t V, int64_t D, int64_t ldw, bool direct, bool f32
   at = up_to(at + p.Rp * p.Dp * p.es, 256);
   p.slab_off = at;
   p.bm_dx = lx_tile_rows(R, D, f32);
-  p.slab_rows = R > 0 ? up_to(R, p.bm_dx) : p.bm_dx;
+  p.slab_rows = p.Rp + 4096;
   if (grad) {
     if (p.Rp * p.Dp * p.es >= lim) return false;
-    at = up_to(at + (p.Rp + 4096) * p.Dp * 4, 256);
+    at = up_to(at + p.slab_rows * p.Dp * 4, 256);
   }
   p.wpad_off = at;
   // a piece: its G (with gradients) and its rows of W (where they are copied)
@@ -577,21 +692,19 @@ bool lx_plan(int64_t R, int64_t V, int64_t D, int64_t ldw, bool direct, bool f32
   p.g_off = up_to(at + (direct ? 0 : most * p.Dp * p.es), 256);
   p.bytes = p.g_off + (grad ? p.Rp * most * p.es : 0) + 256;  // (the start is rounded up to 256 bytes)
   if (bytes >= 0 && p.bytes > bytes) return false;
-  // dX: shares of the piece's classes while its tiles are fewer than what fills the chip
-  const int64_t tiles = p.slab_rows / p.bm_dx * up_to(D, lx_tile_cols(p.bm_dx)) / lx_tile_cols(p.bm_dx);
-  const int64_t want = p.bm_dx == 256 ? 256 : p.bm_dx == 128 ? 512 : 1024;
-  int64_t shares = want / std::max<int64_t>(tiles, 1);
-  shares = std::min(shares, most / 512);
-  shares = std::min(shares, (p.Rp + 4096) / p.slab_rows);
-  shares = std::max<int64_t>(shares, 1);
-  p.k_share = up_to((most + shares - 1) / shares, 64);
-  p.shares = shares;
+  if (grad && bytes > p.bytes) {  // what is left: more slabs, behind everything else
+    const int64_t room = (bytes - p.g_off - p.Rp * most * p.es - 256) / (p.Dp * 4);
+    if (room > p.slab_rows) {
+      p.slab_rows = std::min<int64_t>(room, 8 * p.Rp + 4096);
+      p.slab_off = p.g_off + p.Rp * most * p.es;
+    }
+  }
   if (pl) *pl = p;
   return true;
 }
 
 template <int IN, int OUT, int ACT, int BM, int BN, int WM, int WN, bool AKC, bool BKC, int S>
-Status lx_gemm_as(const NTParams& q, int64_t rows, int64_t cols, int shares, hipStream_t s) {
+Status lx_gemm_as(const NTParams& q, int64_t rows, int64_t cols, hipStream_t s) {
   NTParams p = q;
   p.tiles_m = (int)((rows + BM - 1) / BM);
   p.tiles_n = (int)((cols + BN - 1) / BN);
@@ -599,27 +712,37 @@ Status lx_gemm_as(const NTParams& q, int64_t rows, int64_t cols, int shares, hip
   if (tiles == 0) return Status::Ok;
   if (tiles > INT32_MAX) return Status::InvalidArgument;
   unsigned grid = (unsigned)tiles;
-  if constexpr (nt_persistent(BM, BN, WM, WN)) {
+  if constexpr (ACT == ACT_LX_SLAB) {
+    grid = (unsigned)lx_slots(BM, IN == IN_F32);  // they loop over the tiles' shares
+  } else if constexpr (nt_persistent(BM, BN, WM, WN)) {
     const int ncu = device_cu_count();
     if (ncu > 0 && ncu % 8 == 0 && grid > (unsigned)ncu) grid = (unsigned)ncu;
   }
-  gemm_nt_kernel<IN, OUT, ACT, BM, BN, WM, WN, AKC, BKC, S><<<dim3(grid, (unsigned)shares), 64 * WM * WN, 0, s>>>(p);
+  gemm_nt_kernel<IN, OUT, ACT, BM, BN, WM, WN, AKC, BKC, S><<<grid, 64 * WM * WN, 0, s>>>(p);
   return launch_status("linear_xent");
 }
 
 // rows x cols of the product in tiles of bm rows.
 template <int IN, int OUT, int ACT, bool AKC, bool BKC>
-Status lx_gemm(const NTParams& p, int bm, int64_t rows, int64_t cols, int shares, hipStream_t s) {
-  if constexpr (IN != IN_F32) {
-    if (bm == 256) return lx_gemm_as<IN, OUT, ACT, 256, 256, 2, 4, AKC, BKC, 2>(p, rows, cols, shares, s);
-  }
-  if constexpr (AKC) {
-    if (bm == 32) return lx_gemm_as<IN, OUT, ACT, 32, 128, 1, 4, AKC, BKC, (IN == IN_F32 ? 2 : 4)>(p, rows, cols, shares, s);
-    if constexpr (IN != IN_F32) {
-      if (bm == 64) return lx_gemm_as<IN, OUT, ACT, 64, 128, 1, 4, AKC, BKC, 4>(p, rows, cols, shares, s);
+Status lx_gemm(const NTParams& p, int bm, int64_t rows, int64_t cols, hipStream_t s) {
+  if constexpr (IN == IN_F32) {
+    if constexpr (AKC) {
+      if (bm == 32) return lx_gemm_as<IN, OUT, ACT, 32, 128, 1, 4, AKC, BKC, 2>(p, rows, cols, s);
+    }
+    if (bm == 64) return lx_gemm_as<IN, OUT, ACT, 64, 64, 2, 2, AKC, BKC, 2>(p, rows, cols, s);
+  } else {
+    // Both operands K-contiguous (logits) and long K: four waves of 128 x 128, which read half the LDS bytes a
+    // product (8192 x 32000 x 4096 bf16 1719 -> 1656 us, 4096 x 32000 x 4096 897 -> 868; x 1024 300, 327).
+    if constexpr (AKC && BKC) {
+      if (bm == 256 && p.K >= 2048) return lx_gemm_as<IN, OUT, ACT, 256, 256, 2, 2, AKC, BKC, 2>(p, rows, cols, s);
+    }
+    if (bm == 256) return lx_gemm_as<IN, OUT, ACT, 256, 256, 2, 4, AKC, BKC, 2>(p, rows, cols, s);
+    if constexpr (AKC) {
+      if (bm == 32) return lx_gemm_as<IN, OUT, ACT, 32, 128, 1, 4, AKC, BKC, 4>(p, rows, cols, s);
+      if (bm == 64) return lx_gemm_as<IN, OUT, ACT, 64, 128, 1, 4, AKC, BKC, 4>(p, rows, cols, s);
     }
   }
-  return lx_gemm_as<IN, OUT, ACT, 128, 128, 2, 2, AKC, BKC, 2>(p, rows, cols, shares, s);
+  return lx_gemm_as<IN, OUT, ACT, 128, 128, 2, 2, AKC, BKC, 2>(p, rows, cols, s);
 }
 
 template <int IN, int EK>
@@ -646,16 +769,22 @@ Status lx_run(const LxCall& c, const LxPlan& pl, hipStream_t s) {
   rw.g = base + pl.g_off;
   const float* alpha = (const float*)(rw.head + 1);
   const int R = (int)c.R, V = (int)c.V, D = (int)c.D, Dp = (int)pl.Dp;
-  // f16: exponentials of at most 2^14, G of at most 2^14 (2^13 times a weight's share, less one)
-  const int top = IN == IN_F16 ? 13 : 0;
-  const float keep_scale = IN == IN_F16 ? 16384.0f : 1.0f;
+  const int top = IN == IN_F16 ? 13 : 0;  // G of at most 2^13 in f16
   float* row_loss = (float*)c.row_loss->data;
 
-  lx_rows_kernel<<<1, 1024, 0, s>>>((const int32_t*)c.labels->data, c.rw ? (const float*)c.rw->data : nullptr, R, V,
-                                    top, rw);
-  if (R > 0)
-    lx_copy_rows_kernel<ES><<<(R + 3) / 4, 256, 0, s>>>(c.x->data, c.ldx, rw.xc, D, Dp, R, rw.pos,
-                                                        c.dx ? c.dx->data : nullptr, c.lddx, row_loss);
+  const bool grad = c.dx != nullptr;
+  const int tn_dx = lx_tile_cols(pl.bm_dx, IN == IN_F32);
+  const LxShares sh{pl.bm_dx, grad ? (D + tn_dx - 1) / tn_dx : 0, lx_slots(pl.bm_dx, IN == IN_F32),
+                    (int)std::min(pl.piece, c.V), (int)std::min<int64_t>(pl.slab_rows, INT32_MAX)};
+  const LxCopy cx{c.x->data, rw.xc, grad ? c.dx->data : nullptr, row_loss, c.ldx, c.lddx, D, Dp};
+  const int32_t* labels = (const int32_t*)c.labels->data;
+  const float* weight = c.rw ? (const float*)c.rw->data : nullptr;
+  if (R <= 64) {
+    lx_rows_kernel<ES, true><<<1, 1024, 0, s>>>(labels, weight, R, V, top, rw, sh, cx);
+  } else {
+    lx_rows_kernel<ES, false><<<1, 1024, 0, s>>>(labels, weight, R, V, top, rw, sh, cx);
+    lx_copy_rows_kernel<ES><<<(R + 3) / 4, 256, 0, s>>>(cx, R, rw.pos);
+  }
   Status st = launch_status("linear_xent_rows");
   if (st != Status::Ok) return st;
 
@@ -666,8 +795,8 @@ Status lx_run(const LxCall& c, const LxPlan& pl, hipStream_t s) {
       p.B = w;
       p.ldb = c.ldw;
     } else {
-      lx_copy_rows_kernel<ES><<<(unsigned)((cols + 3) / 4), 256, 0, s>>>(w, c.ldw, rw.wpad, D, Dp, (int)cols, nullptr,
-                                                                         nullptr, 0, nullptr);
+      lx_copy_rows_kernel<ES><<<(unsigned)((cols + 3) / 4), 256, 0, s>>>(
+          LxCopy{w, rw.wpad, nullptr, nullptr, c.ldw, 0, D, Dp}, (int)cols, nullptr);
       p.B = rw.wpad;
       p.ldb = Dp;
     }
@@ -690,19 +819,17 @@ Status lx_run(const LxCall& c, const LxPlan& pl, hipStream_t s) {
     p.lx.zlab = rw.zlab;
     p.lx.stats = rw.stats;
     p.lx.stats_ld = pl.Rp;
-    p.lx.keep_scale = keep_scale;
     p.lx.row_max = rw.row_max;
     p.lx.row_f = rw.row_f;
     p.lx.row_w = rw.row_w;
     return p;
   };
-  const bool grad = c.dx != nullptr;
   const int64_t pieces = (c.V + pl.piece - 1) / pl.piece;
   const int64_t last = (pieces - 1) * pl.piece;  // first class of the piece that is kept
   auto stats = [&](int64_t v0, int64_t cols, int64_t keep) {
     NTParams p = logits(v0, cols);
     p.lx.keep_from = keep < 0 ? INT32_MAX : (int)keep;
-    return lx_gemm<IN, OUT, ACT_LX_STATS, true, true>(p, pl.bm, R, cols, 1, s);
+    return lx_gemm<IN, OUT, ACT_LX_STATS, true, true>(p, pl.bm, R, cols, s);
   };
   if (pl.direct) {
     st = stats(0, c.V, grad ? last : -1);
@@ -713,14 +840,14 @@ Status lx_run(const LxCall& c, const LxPlan& pl, hipStream_t s) {
       if (st != Status::Ok) return st;
     }
   }
-  if (R > 0)
-    lx_stats_kernel<<<(R + 63) / 64, 1024, 0, s>>>(rw, (int)((c.V + pl.bn - 1) / pl.bn), pl.Rp, row_loss);
-  lx_loss_kernel<<<1, 1024, 0, s>>>(rw, (float*)c.loss->data);
+  float* loss = (float*)c.loss->data;
+  lx_stats_kernel<<<R > 0 ? (R + 63) / 64 : 1, 1024, 0, s>>>(rw, (int)((c.V + pl.bn - 1) / pl.bn), pl.Rp, weight != nullptr,
+                                                             row_loss, R <= 64 ? loss : nullptr);
+  if (R > 64) lx_loss_kernel<<<1, 1024, 0, s>>>(rw, loss);
   st = launch_status("linear_xent_stats");
   if (st != Status::Ok || !grad) return st;
 
-  const bool slabs = pieces > 1 || pl.shares > 1;
-  int64_t filled = 0;  // slabs that hold something
+  const bool direct = pieces == 1;  // dX needs no slab unless its K is shared
   for (int64_t k = pieces - 1; k >= 0; --k) {
     const int64_t v0 = k * pl.piece, cols = std::min(pl.piece, c.V - v0);
     if (k == pieces - 1) {
@@ -728,14 +855,16 @@ Status lx_run(const LxCall& c, const LxPlan& pl, hipStream_t s) {
         const int64_t width = up_to(cols, pl.bn);
         const unsigned gx = (unsigned)((width + 256 * (16 / ES) - 1) / (256 * (16 / ES)));
         const unsigned gy = (unsigned)std::min<int64_t>(R, 32768);
-        if (pl.bn == 256)
-          lx_scale_kernel<EK, 256><<<dim3(gx, gy), 256, 0, s>>>(rw, pl.piece, (int)width, (int)v0, pl.Rp, keep_scale);
+        if (pl.bn == 64)
+          lx_scale_kernel<EK, 64><<<dim3(gx, gy), 256, 0, s>>>(rw, pl.piece, (int)width, (int)v0, pl.Rp);
+        else if (pl.bn == 256)
+          lx_scale_kernel<EK, 256><<<dim3(gx, gy), 256, 0, s>>>(rw, pl.piece, (int)width, (int)v0, pl.Rp);
         else
-          lx_scale_kernel<EK, 128><<<dim3(gx, gy), 256, 0, s>>>(rw, pl.piece, (int)width, (int)v0, pl.Rp, keep_scale);
+          lx_scale_kernel<EK, 128><<<dim3(gx, gy), 256, 0, s>>>(rw, pl.piece, (int)width, (int)v0, pl.Rp);
       }
     } else {
       NTParams p = logits(v0, cols);
-      st = lx_gemm<IN, OUT, ACT_LX_GRAD, true, true>(p, pl.bm, R, cols, 1, s);
+      st = lx_gemm<IN, OUT, ACT_LX_GRAD, true, true>(p, pl.bm, R, cols, s);
       if (st != Status::Ok) return st;
     }
     if (c.dw) {
@@ -757,11 +886,11 @@ Status lx_run(const LxCall& c, const LxPlan& pl, hipStream_t s) {
       const int ob = f32 ? 4 : 2;
       p.C = (uint8_t*)c.dw->data + v0 * c.lddw * ob;
       p.lx.vec = aligned(c.dw->data, 16) && c.lddw * ob % 16 == 0;
-      const int bm = IN == IN_F32 ? 128 : ((cols + 255) / 256) * ((c.D + 255) / 256) < 192 ? 128 : 256;
+      const int bm = lx_tile_rows(std::max<int64_t>(cols, 129), c.D, IN == IN_F32);
       if (f32)
-        st = lx_gemm<IN, OUT_F32, ACT_LX_OUT, false, false>(p, bm, cols, D, 1, s);
+        st = lx_gemm<IN, OUT_F32, ACT_LX_OUT, false, false>(p, bm, cols, D, s);
       else
-        st = lx_gemm<IN, OUT, ACT_LX_OUT, false, false>(p, bm, cols, D, 1, s);
+        st = lx_gemm<IN, OUT, ACT_LX_OUT, false, false>(p, bm, cols, D, s);
       if (st != Status::Ok) return st;
     }
     if (R > 0) {
@@ -777,30 +906,28 @@ Status lx_run(const LxCall& c, const LxPlan& pl, hipStream_t s) {
       p.lx.n = rw.head;
       p.lx.a_mn = (int)pl.Rp;
       p.lx.b_mn = pl.direct ? D : Dp;
-      if (!slabs) {
+      p.lx.shares = rw.head + 4;
+      if (direct) {
         p.C = c.dx->data;
         p.ldc = c.lddx;
         p.lx.alpha = alpha;
         p.lx.row_map = rw.idx;
         p.lx.vec = aligned(c.dx->data, 16) && c.lddx * ES % 16 == 0;
-        st = lx_gemm<IN, OUT, ACT_LX_OUT, true, false>(p, pl.bm_dx, R, D, 1, s);
-      } else {
-        p.C = rw.slab;
-        p.ldc = Dp;
-        p.lx.add = (int)filled;
-        p.lx.k_split = (int)pl.k_share;
-        p.lx.split_stride = pl.slab_rows * Dp;
-        const int64_t used = (cols + pl.k_share - 1) / pl.k_share;  // (a short last piece has fewer shares)
-        filled = std::max(filled, used);
-        st = lx_gemm<IN, OUT_F32, ACT_LX_SLAB, true, false>(p, pl.bm_dx, R, D, (int)used, s);
+        st = lx_gemm<IN, OUT, ACT_LX_OUT, true, false>(p, pl.bm_dx, R, D, s);
+        if (st != Status::Ok) return st;
       }
+      p.C = rw.slab;
+      p.ldc = Dp;
+      p.lx.direct = direct;
+      p.lx.k_piece = sh.k_piece;
+      p.lx.k_before = k == pieces - 1 ? 0 : k == pieces - 2 ? (int)(c.V - last) : sh.k_piece;
+      st = lx_gemm<IN, OUT_F32, ACT_LX_SLAB, true, false>(p, pl.bm_dx, R, D, s);
       if (st != Status::Ok) return st;
     }
   }
-  if (slabs && R > 0) {
+  if (R > 0) {
     const unsigned gx = (unsigned)((D + 1023) / 1024), gy = (unsigned)std::min<int64_t>(R, 32768);
-    lx_finish_kernel<EK><<<dim3(gx, gy), 256, 0, s>>>(rw, (int)filled, pl.slab_rows * Dp, Dp, D, c.dx->data,
-                                                      c.lddx);
+    lx_finish_kernel<EK><<<dim3(gx, gy), 256, 0, s>>>(rw, direct, sh.k_piece, pl.bm_dx, Dp, D, c.dx->data, c.lddx);
     return launch_status("linear_xent_finish");
   }
   return Status::Ok;

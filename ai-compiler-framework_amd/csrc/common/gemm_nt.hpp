@@ -50,10 +50,11 @@ struct LxArgs {
   int rows_are_k;
   int a_mn, b_mn;        // extents of A's and B's rows (M/N-contiguous: columns) in memory
   // dX: K is divided into shares (chosen on the device: how many rows count is
-  // known there alone).  ACT_LX_SLAB: share s writes slab s of C; ACT_LX_OUT with
-  // `shares` runs where there is one, and SLAB with `direct` where there are more.
+  // known there alone).  ACT_LX_SLAB: share s writes slab s of C; the only one,
+  // with `direct`, writes `direct` itself as ACT_LX_OUT does C.
   const int32_t* shares;
-  int direct;
+  void* direct;
+  int64_t ld_direct;
   int k_piece;           // K that the shares divide
   int k_before;          // K of the piece whose sums the slabs hold (0: none), to be added to
   // ACT_LX_STATS, ACT_LX_GRAD: logits
@@ -589,14 +590,10 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_nt_kernel(NTParams p) {
       p.M = rows;
       p.tiles_m = (rows + BM - 1) / BM;
     }
-    if constexpr (ACT == ACT_LX_OUT) {
-      if (p.lx.shares && p.lx.shares[0] != 1) return;
-    }
   }
   int shares = 1, k_share = 0;
   if constexpr (ACT == ACT_LX_SLAB) {
     shares = p.lx.shares[0];
-    if (p.lx.direct && shares == 1) return;
     k_share = lx_share_k(p.lx.k_piece, shares);
   }
 
@@ -943,7 +940,16 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_nt_kernel(NTParams p) {
   substep(NoRd{}, z, z, 1, nullptr, 0, 0, 0, 0);
 
   __syncthreads();  // every wave is done reading the last stage
-  if constexpr (LX)
+  if constexpr (ACT == ACT_LX_SLAB) {
+    if (shares == 1 && q.lx.direct) {
+      q.C = q.lx.direct;
+      q.ldc = q.lx.ld_direct;
+      lx_epilogue<OUT, ACT_LX_OUT, BM, BN, WM, WN, 2 * STAGE, MS>(q, acc, smem, m0, n0);
+    } else {
+      q.ldc = p.ldc;
+      lx_epilogue<OUT_F32, ACT, BM, BN, WM, WN, 2 * STAGE, MS>(q, acc, smem, m0, n0);
+    }
+  } else if constexpr (LX)
     lx_epilogue<OUT, ACT, BM, BN, WM, WN, 2 * STAGE, MS>(q, acc, smem, m0, n0);
   else
     nt_epilogue_staged<OUT, ACT, BM, BN, WM, WN, 2 * STAGE, MS>(p, acc, smem, m0, n0);

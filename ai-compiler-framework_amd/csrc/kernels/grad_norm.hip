@@ -7,9 +7,10 @@
 //
 // One pass reads every gradient once (bound by memory: 2 operations an
 // element), a second workgroup-sized launch joins the partial sums, and the
-// clipping reads and writes once more; in place with factor 1 it touches
-// nothing.  A launch takes kTable tensors by value, so nothing is copied to the
-// device and the call can be captured.  Squares and sums are f64: exact squares
+// clipping reads and writes once more (the other way round, so that it begins
+// with what the last-level cache still holds); in place with factor 1 it touches
+// nothing.  A launch takes a table of tensors by value, so nothing is copied to
+// the device and the call can be captured.  Squares and sums are f64: exact squares
 // of any f32, no overflow or underflow where the norm itself has none, and the
 // same bits whatever scale the gradients are at; the loads bound the pass all
 // the same.  Every sum has a fixed order.
@@ -25,29 +26,40 @@ namespace aicf::hip {
 
 namespace {
 
-constexpr int kTable = 96;      // tensors a launch (2.8 KB of kernel arguments)
-constexpr int kItem = 4096;     // elements of a workgroup's step: 16 a lane
-constexpr int kBlocks = 1024;   // workgroups a launch at most: partial sums of a call are kBlocks a launch
+constexpr int kScratchTensors = 96;  // partial sums of a call: kBlocks for each 96 tensors
+constexpr int kBlocks = 1024;        // workgroups a launch at most
+// Tensors a launch: 3.6 and 3.9 KB of kernel arguments.
+constexpr int kNormTable = 256, kClipTable = 176;
 
+// A workgroup's step, an item, is kRow H 16-bit elements of a tensor (f32: half
+// as many, but kRow at least), 8 a lane and load, all loaded at once.  H = 4, or
+// 1 where that left workgroups without an item.
+constexpr int kThreads = 512, kRow = 8 * kThreads;
+__host__ __device__ __forceinline__ int item_of(int kind, int H) { return kRow * (kind == EL_F32 ? (H + 1) / 2 : H); }
+
+template <int N, bool OUT>
 struct NormTable {
-  const void* g[kTable];
-  void* out[kTable];
-  int64_t n[kTable];
-  int32_t start[kTable + 1];  // items before a tensor
-  uint8_t kind[kTable];
+  const void* g[N];
+  void* out[OUT ? N : 1];
+  int32_t start[N + 1];  // items before a tensor
+  uint16_t last[N];      // elements of its last item - 1, and its type << 14
   int count;
-};
 
-// The tensor that item belongs to.
-__device__ __forceinline__ int tensor_of(const NormTable& t, int item) {
-  int lo = 0, hi = t.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (t.start[mid] <= item) lo = mid;
-    else hi = mid - 1;
+  __device__ __forceinline__ int kind(int k) const { return last[k] >> 14; }
+  __device__ __forceinline__ int64_t numel(int k, int per) const {
+    return (int64_t)(start[k + 1] - start[k] - 1) * per + (last[k] & 0x3fff) + 1;
   }
-  return lo;
-}
+  // The tensor that item i belongs to.
+  __device__ __forceinline__ int tensor_of(int i) const {
+    int lo = 0, hi = count - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (start[mid] <= i) lo = mid;
+      else hi = mid - 1;
+    }
+    return lo;
+  }
+};
 
 __device__ __forceinline__ double block_sum_f64(double v, double* red) {
 #pragma unroll
@@ -60,29 +72,32 @@ __device__ __forceinline__ double block_sum_f64(double v, double* red) {
   return v;
 }
 
-template <int EK>
+template <int EK, int H>
 __device__ __forceinline__ void squares(const void* g, int64_t at, int64_t n, double (&acc)[2]) {
-  float v[2][8];
-  load8<EK>(v[0], g, at + threadIdx.x * 8, n - threadIdx.x * 8);
-  load8<EK>(v[1], g, at + 2048 + threadIdx.x * 8, n - 2048 - threadIdx.x * 8);
+  float v[H][8];
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
+  for (int h = 0; h < H; ++h) load8<EK>(v[h], g, at + h * kRow + threadIdx.x * 8, n - h * kRow - threadIdx.x * 8);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[h] = fma((double)v[h][e], (double)v[h][e], acc[h]);
+  for (int h = 0; h < H; ++h)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[h & 1] = fma((double)v[h][e], (double)v[h][e], acc[h & 1]);
 }
 
 // Workgroup b takes items b per .. (b + 1) per - 1.
-__global__ __launch_bounds__(256) void norm_part_kernel(NormTable t, int per, double* __restrict__ partial) {
-  __shared__ double red[4];
+template <int H>
+__global__ __launch_bounds__(kThreads) void norm_part_kernel(NormTable<kNormTable, false> t, int per,
+                                                             double* __restrict__ partial) {
+  __shared__ double red[kThreads / 64];
   const int first = blockIdx.x * per, last = first + per < t.start[t.count] ? first + per : t.start[t.count];
   double acc[2] = {0.0, 0.0};
-  int k = first < last ? tensor_of(t, first) : 0;
+  int k = first < last ? t.tensor_of(first) : 0;
   for (int i = first; i < last; ++i) {
     while (i >= t.start[k + 1]) ++k;
-    const int64_t at = (int64_t)(i - t.start[k]) * kItem, n = t.n[k] - at;
-    if (t.kind[k] == EL_F32) squares<EL_F32>(t.g[k], at, n, acc);
-    else if (t.kind[k] == EL_F16) squares<EL_F16>(t.g[k], at, n, acc);
-    else squares<EL_BF16>(t.g[k], at, n, acc);
+    const int item = item_of(t.kind(k), H);
+    const int64_t at = (int64_t)(i - t.start[k]) * item, n = t.numel(k, item) - at;
+    if (t.kind(k) == EL_F32) squares<EL_F32, (H + 1) / 2>(t.g[k], at, n, acc);
+    else if (t.kind(k) == EL_F16) squares<EL_F16, H>(t.g[k], at, n, acc);
+    else squares<EL_BF16, H>(t.g[k], at, n, acc);
   }
   const double v = block_sum_f64(acc[0] + acc[1], red);
   if (threadIdx.x == 0) partial[blockIdx.x] = v;
@@ -101,14 +116,14 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(const double* __restric
   }
 }
 
-template <int EK>
+template <int EK, int H>
 __device__ __forceinline__ void scaled(const void* g, void* out, int64_t at, int64_t n, float f) {
-  float v[2][8];
-  load8<EK>(v[0], g, at + threadIdx.x * 8, n - threadIdx.x * 8);
-  load8<EK>(v[1], g, at + 2048 + threadIdx.x * 8, n - 2048 - threadIdx.x * 8);
+  float v[H][8];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int64_t i = at + h * 2048 + threadIdx.x * 8, left = n - h * 2048 - threadIdx.x * 8;
+  for (int h = 0; h < H; ++h) load8<EK>(v[h], g, at + h * kRow + threadIdx.x * 8, n - h * kRow - threadIdx.x * 8);
+#pragma unroll
+  for (int h = 0; h < H; ++h) {
+    const int64_t i = at + h * kRow + threadIdx.x * 8, left = n - h * kRow - threadIdx.x * 8;
     if constexpr (EK == EL_F32) {
       float* q = (float*)out + i;
       if (left >= 8) {
@@ -135,17 +150,21 @@ __device__ __forceinline__ void scaled(const void* g, void* out, int64_t at, int
   }
 }
 
-__global__ __launch_bounds__(256) void norm_clip_kernel(NormTable t, int per, const float* __restrict__ norm) {
+template <int H>
+__global__ __launch_bounds__(kThreads) void norm_clip_kernel(NormTable<kClipTable, true> t, int per,
+                                                             const float* __restrict__ norm) {
   const float f = norm[1];
-  const int first = blockIdx.x * per, last = first + per < t.start[t.count] ? first + per : t.start[t.count];
-  int k = first < last ? tensor_of(t, first) : 0;
+  const int first = (gridDim.x - 1 - blockIdx.x) * per;
+  const int last = first + per < t.start[t.count] ? first + per : t.start[t.count];
+  int k = first < last ? t.tensor_of(first) : 0;
   for (int i = first; i < last; ++i) {
     while (i >= t.start[k + 1]) ++k;
     if (f == 1.0f && t.g[k] == t.out[k]) continue;
-    const int64_t at = (int64_t)(i - t.start[k]) * kItem, n = t.n[k] - at;
-    if (t.kind[k] == EL_F32) scaled<EL_F32>(t.g[k], t.out[k], at, n, f);
-    else if (t.kind[k] == EL_F16) scaled<EL_F16>(t.g[k], t.out[k], at, n, f);
-    else scaled<EL_BF16>(t.g[k], t.out[k], at, n, f);
+    const int item = item_of(t.kind(k), H);
+    const int64_t at = (int64_t)(i - t.start[k]) * item, n = t.numel(k, item) - at;
+    if (t.kind(k) == EL_F32) scaled<EL_F32, (H + 1) / 2>(t.g[k], t.out[k], at, n, f);
+    else if (t.kind(k) == EL_F16) scaled<EL_F16, H>(t.g[k], t.out[k], at, n, f);
+    else scaled<EL_BF16, H>(t.g[k], t.out[k], at, n, f);
   }
 }
 
@@ -169,7 +188,7 @@ bool row_major(const TensorDesc& t) {
   return true;
 }
 
-int64_t norm_scratch(int T) { return (int64_t)2 * kBlocks * ((T + kTable - 1) / kTable); }
+int64_t norm_scratch(int T) { return (int64_t)2 * kBlocks * ((T + kScratchTensors - 1) / kScratchTensors); }
 
 bool norm_sup(const TensorDesc* in, int ni, const TensorDesc* out, int no, const void* attr) {
   float max_norm;
@@ -227,36 +246,42 @@ Status norm_launch(const TensorDesc* in, int ni, TensorDesc* out, int no, const 
   hipStream_t s = as_stream(stream);
   float* norm = (float*)out[0].data;
   double* partial = (double*)out[1].data;
-  // launches of kTable tensors each: f(table, items of a workgroup, workgroups)
-  auto tables = [&](auto f) {
-    NormTable t;
-    for (int k0 = 0; k0 < ni; k0 += kTable) {
-      t.count = 0;
-      t.start[0] = 0;
-      for (int k = k0; k < ni && k < k0 + kTable; ++k) {
-        const int64_t n = numel_of(in[k]);
-        if (n == 0) continue;
-        int ek;
-        elem_kind(in[k], &ek);
-        t.g[t.count] = in[k].data;
-        t.out[t.count] = no > 2 ? out[2 + k].data : nullptr;
-        t.n[t.count] = n;
-        t.kind[t.count] = (uint8_t)ek;
-        t.start[t.count + 1] = t.start[t.count] + (int32_t)((n + kItem - 1) / kItem);
-        ++t.count;
-      }
-      const int items = t.start[t.count], per = (items + kBlocks - 1) / kBlocks;
-      if (items > 0) f(t, per, (unsigned)((items + per - 1) / per));
+  int64_t bytes = 0;
+  for (int k = 0; k < ni; ++k) bytes += numel_of(in[k]) * (dt(in[k]) == DType::kF32 ? 4 : 2);
+  const int h = bytes >= (int64_t)8 * kRow * kBlocks ? 4 : 1;
+  // tensors k0 .. in a table: f(table, items of a workgroup, workgroups)
+  auto table = [&](auto t, int N, int k0, auto f) {
+    t.count = 0;
+    t.start[0] = 0;
+    for (int k = k0; k < ni && k < k0 + N; ++k) {
+      const int64_t n = numel_of(in[k]);
+      if (n == 0) continue;
+      int ek;
+      elem_kind(in[k], &ek);
+      const int64_t item = item_of(ek, h);
+      t.g[t.count] = in[k].data;
+      if (N == kClipTable) t.out[t.count] = out[2 + k].data;
+      t.last[t.count] = (uint16_t)((n - 1) % item | ek << 14);
+      t.start[t.count + 1] = t.start[t.count] + (int32_t)((n + item - 1) / item);
+      ++t.count;
     }
+    const int items = t.start[t.count], per = (items + kBlocks - 1) / kBlocks;
+    if (items > 0) f(t, per, (unsigned)((items + per - 1) / per));
   };
   int parts = 0;
-  tables([&](const NormTable& t, int per, unsigned blocks) {
-    norm_part_kernel<<<blocks, 256, 0, s>>>(t, per, partial + parts);
-    parts += (int)blocks;
-  });
+  for (int k0 = 0; k0 < ni; k0 += kNormTable)
+    table(NormTable<kNormTable, false>(), kNormTable, k0, [&](const auto& t, int per, unsigned blocks) {
+      if (h == 4) norm_part_kernel<4><<<blocks, kThreads, 0, s>>>(t, per, partial + parts);
+      else norm_part_kernel<1><<<blocks, kThreads, 0, s>>>(t, per, partial + parts);
+      parts += (int)blocks;
+    });
   norm_join_kernel<<<1, 1024, 0, s>>>(partial, parts, max_norm, norm);
   if (no > 2)
-    tables([&](const NormTable& t, int per, unsigned blocks) { norm_clip_kernel<<<blocks, 256, 0, s>>>(t, per, norm); });
+    for (int k0 = (ni - 1) / kClipTable * kClipTable; k0 >= 0; k0 -= kClipTable)
+      table(NormTable<kClipTable, true>(), kClipTable, k0, [&](const auto& t, int per, unsigned blocks) {
+        if (h == 4) norm_clip_kernel<4><<<blocks, kThreads, 0, s>>>(t, per, norm);
+        else norm_clip_kernel<1><<<blocks, kThreads, 0, s>>>(t, per, norm);
+      });
   return launch_status("grad_norm");
 }
 

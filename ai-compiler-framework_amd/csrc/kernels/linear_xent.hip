@@ -10,18 +10,21 @@
 // they are only the device knows, and the products' grids cover all rows.
 //
 //   1. logits: tiles of the MFMA GEMM whose epilogue keeps, for each row and
-//      tile of classes, the maximum and the sum of exp(z - maximum); of the
-//      last `piece` classes also exp(z - tile maximum) itself, in the operands'
-//      type (a rounding of 2^-9 in bf16, 2^-12 in f16, as any operand of a
-//      product has; the sums are taken before it);
+//      tile of classes, the maximum and the sum of exp(z - maximum); of some
+//      classes also exp(z - tile maximum) itself (f32, or f16 for operands of
+//      16 bits: 2^-12 against the 2^-9 of a bf16 G; the sums are taken before
+//      the rounding): of the last `piece` in scratch, of the first `held` in the
+//      memory of dW's other rows, which are written later;
 //   2. the row's statistics are joined; the kept values become G in place,
 //      scaled to the type's range by a power of two that the products take out
 //      again (weights of 1/R would leave f16's range);
 //   3. dW and dX of those classes;
 //   4. the other pieces: logits once more, whose epilogue knows the row's
 //      statistics and writes G, then dW and dX as before.
-// So the scratch decides what is computed twice: 6 n V D operations where it
-// holds all classes (n rows that count), up to 8 n V D where it holds few.
+// So the memory decides what is computed twice: 6 n V D operations where it
+// holds all classes (n rows that count), up to 8 n V D where it holds few.  At
+// 8192 x 131072 x 4096 bf16 and 1.5 GiB scratch holds 58% of the classes and dW
+// 33%: 20.7 ms; with the 42% behind scratch alone kept it took 23.0.
 // dX is summed over the pieces, and over shares of the classes where its tiles
 // are fewer than the CUs, in f32 slabs that are joined in a fixed order.
 //
@@ -40,7 +43,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // 2^((z - m) log2 e): the difference first, so that the exponent is off by
 // roundings of itself alone however far the logits lie from zero.
 __device__ __forceinline__ float exp_from(float z, float m) { return __builtin_amdgcn_exp2f((z - m) * kLog2e); }
-// f16: the kept exponentials are at most 2^14, so that they lose bits only below 2^-28 of their tile's largest.
+// The exponentials kept in f16 are at most 2^14, so that they lose bits only below 2^-28 of their tile's largest.
 constexpr float kKeepScale = 16384.0f;
 // A maximum over nothing but -inf is no reference: their exponentials are 0.
 __device__ __forceinline__ float safe_ref(float m) { return m == -INFINITY ? 0.0f : m; }
@@ -175,7 +178,7 @@ __device__ __forceinline__ void lx_epilogue(const NTParams& p, nt_acc_t<MS> (&ac
     const int col = col_of(i, g) + e;
     if constexpr (ACT == ACT_LX_STATS) {
       const float v = exp_from(col < ncol ? z : -INFINITY, c.a);
-      return OUT == OUT_F16 ? v * kKeepScale : v;
+      return OUT == OUT_F32 ? v : v * kKeepScale;
     } else if constexpr (ACT == ACT_LX_GRAD) {
       const float v = exp_from(z, c.a) * c.f;
       return col < ncol ? (col == c.col ? v - c.w : v) : 0.0f;
@@ -211,7 +214,7 @@ __device__ __forceinline__ void lx_epilogue(const NTParams& p, nt_acc_t<MS> (&ac
           uint8_t* at = smem + pr * ROWB + (((cb / 16) ^ (pr & (CPR - 1))) * 16) + cb % 16;
           if constexpr (OUT == OUT_F32) {
             *reinterpret_cast<f32x4*>(at) = f32x4{v[0], v[1], v[2], v[3]};
-          } else if constexpr (OUT == OUT_BF16) {
+          } else if constexpr (OUT == OUT_BF16 && ACT != ACT_LX_STATS) {
             typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
             *reinterpret_cast<u32x2*>(at) = u32x2{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3])};
           } else {
@@ -262,9 +265,8 @@ __device__ __forceinline__ void lx_epilogue(const NTParams& p, nt_acc_t<MS> (&ac
 struct LxRows {
   int32_t* head;    // [0] rows that count; f32 [1] what the products with G are multiplied by, [2] its inverse,
                     // [3] 1 / rows that count; [4] shares of dX's K
-  int32_t* pos;     // [R] place of a row among those that count, -1: left out
-  int32_t* idx;     // [Rp] and back
-  int32_t* label;   // [Rp] of the rows that count, like all below
+  int32_t* idx;     // [Rp] rows that count, in their order
+  int32_t* label;   // [Rp] theirs, like all below
   float* weight;    // as given
   float* row_w;     // times head[2]
   float* zlab;
@@ -302,49 +304,48 @@ struct LxCopy {
   int D, Dp;
 };
 
-// Row r of src (D elements) to row `to` of dst, zeros behind them to Dp; to < 0:
-// a row that is left out, whose gradient and loss are cleared instead.  By a wave.
+// 16 bytes from element i of row r of src (D elements), zeros behind them.
 template <int ES>
-__device__ __forceinline__ void lx_copy_row(const LxCopy& c, int64_t r, int to, int lane) {
+__device__ __forceinline__ typename LxElem<ES>::vec lx_load_part(const LxCopy& c, int64_t r, int i) {
   typedef typename LxElem<ES>::T T;
-  typedef typename LxElem<ES>::vec vec;
-  typedef typename LxElem<ES>::loose loose;
-  constexpr int CE = 16 / ES;
-  if (to >= 0) {
-    const T* a = (const T*)c.src + r * c.lds;
-    T* b = (T*)c.dst + (int64_t)to * c.Dp;
-    for (int i = lane * CE; i < c.Dp; i += 64 * CE) {
-      vec v;
-      if (i + CE <= c.D) {
-        v = *reinterpret_cast<const loose*>(a + i);
-      } else {
+  const T* a = (const T*)c.src + r * c.lds;
+  if (i + 16 / ES <= c.D) return *reinterpret_cast<const typename LxElem<ES>::loose*>(a + i);
+  typename LxElem<ES>::vec v;
 #pragma unroll
-        for (int e = 0; e < CE; ++e) v[e] = i + e < c.D ? a[i + e] : T(0);
-      }
-      *reinterpret_cast<vec*>(b + i) = v;
-    }
+  for (int e = 0; e < 16 / ES; ++e) v[e] = i + e < c.D ? a[i + e] : T(0);
+  return v;
+}
+
+// They go to row `to` of dst; to < 0: a row that is left out, whose gradient and
+// loss are cleared.
+template <int ES>
+__device__ __forceinline__ void lx_store_part(const LxCopy& c, int64_t r, int to, int i,
+                                              const typename LxElem<ES>::vec& v) {
+  typedef typename LxElem<ES>::T T;
+  if (to >= 0) {
+    if (i < c.Dp) *reinterpret_cast<typename LxElem<ES>::vec*>((T*)c.dst + (int64_t)to * c.Dp + i) = v;
     return;
   }
-  if (lane == 0) c.row_loss[r] = 0.0f;
+  if (i == 0) c.row_loss[r] = 0.0f;
   if (!c.dx) return;
   T* b = (T*)c.dx + r * c.lddx;
-  for (int i = lane * CE; i < c.D; i += 64 * CE) {
-    if (i + CE <= c.D) {
-      loose v;
+  if (i + 16 / ES <= c.D) {
+    typename LxElem<ES>::loose z;
 #pragma unroll
-      for (int e = 0; e < CE; ++e) v[e] = T(0);
-      *reinterpret_cast<loose*>(b + i) = v;
-    } else {
-      for (int e = 0; i + e < c.D; ++e) b[i + e] = T(0);
-    }
+    for (int e = 0; e < 16 / ES; ++e) z[e] = T(0);
+    *reinterpret_cast<typename LxElem<ES>::loose*>(b + i) = z;
+  } else {
+    for (int e = 0; i + e < c.D; ++e) b[i + e] = T(0);
   }
 }
 
-// Rows of X to their places, or (without pos) rows of W onto 16-byte steps.
+// Rows of W onto 16-byte steps.
 template <int ES>
-__global__ __launch_bounds__(256) void lx_copy_rows_kernel(LxCopy c, int rows, const int32_t* __restrict__ pos) {
+__global__ __launch_bounds__(256) void lx_copy_rows_kernel(LxCopy c, int rows) {
   const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (r < rows) lx_copy_row<ES>(c, r, pos ? pos[r] : r, threadIdx.x & 63);
+  if (r >= rows) return;
+  for (int i = (threadIdx.x & 63) * (16 / ES); i < c.Dp; i += 64 * (16 / ES))
+    lx_store_part<ES>(c, r, r, i, lx_load_part<ES>(c, r, i));
 }
 
 // How dX's tiles are shared out: tiles of bm rows, tiles_n in a row of them,
@@ -354,14 +355,21 @@ struct LxShares {
 };
 
 // Which rows count, the power of two that brings the largest weight to
-// 2^(top-1) .. 2^top, and how many shares dX's K is divided into.  One
-// workgroup: 16 rows a thread at a time.
-// COPY (at most 64 rows): also what lx_copy_rows_kernel does.
-template <int ES, bool COPY>
+// 2^(top-1) .. 2^top, how many shares dX's K is divided into; and the rows of X
+// to their places.  Every workgroup counts all rows (16 a thread at a time: 32
+// KB of labels and weights at 4096 rows, from L2) and copies kCopyRows of them
+// at most; the first one writes what the others computed too.  64 rows of 2048
+// f16 take 8 us (counted and copied by one workgroup 14.5), 3072 of 4096 rows of
+// 4096 bf16 22 (in two launches 23 and what lies between them).
+constexpr int kCopyRows = 256;
+template <int ES>
 __global__ __launch_bounds__(1024) void lx_rows_kernel(const int32_t* __restrict__ labels,
                                                        const float* __restrict__ w, int R, int V, int top, LxRows s,
-                                                       LxShares sh, LxCopy cp) {
-  constexpr int PER = COPY ? 1 : 16;
+                                                       LxShares sh, LxCopy cp, int per) {
+  constexpr int PER = 16;
+  __shared__ int place[kCopyRows];
+  const bool first = blockIdx.x == 0;
+  const int r0 = blockIdx.x * per;
   __shared__ int cnt[PER * 16 + 1];
   __shared__ float big[16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -410,8 +418,8 @@ __global__ __launch_bounds__(1024) void lx_rows_kernel(const int32_t* __restrict
       if (r >= R) continue;
       const bool c = in[k] >> lane & 1;
       const int at = cnt[k * 16 + wave] + __popcll(in[k] & ((1ull << lane) - 1));
-      s.pos[r] = c ? at : -1;
-      if (c) {
+      if (r >= r0 && r < r0 + per) place[r - r0] = c ? at : -1;
+      if (first && c) {
         s.idx[at] = r;
         s.label[at] = label[k];
         if (w) s.weight[at] = w[r];
@@ -420,10 +428,12 @@ __global__ __launch_bounds__(1024) void lx_rows_kernel(const int32_t* __restrict
     total = cnt[PER * 16];
     __syncthreads();
   }
-  most = wave_max(most);
-  if (lane == 0) big[wave] = most;
-  __syncthreads();
-  if (wave == 0) {
+  if (first) {
+    most = wave_max(most);
+    if (lane == 0) big[wave] = most;
+    __syncthreads();
+  }
+  if (first && wave == 0) {
     float m = big[lane & 15];
     m = wave_max(m);
     const float mean = total > 0 ? 1.0f / (float)total : 0.0f;
@@ -460,9 +470,22 @@ __global__ __launch_bounds__(1024) void lx_rows_kernel(const int32_t* __restrict
       s.head[4] = best;
     }
   }
-  if constexpr (COPY) {
-    __syncthreads();
-    for (int r = wave; r < R; r += 16) lx_copy_row<ES>(cp, r, s.pos[r], lane);
+  constexpr int SEG = 64 * (16 / ES);  // (place[]: behind the last chunk's barrier)
+  const int segs = (cp.Dp + SEG - 1) / SEG, rows = R - r0 < per ? R - r0 : per;
+  for (int t0 = wave; t0 < rows * segs; t0 += 64) {  // four loads in flight
+    typename LxElem<ES>::vec v[4];
+    int to[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int t = t0 + 16 * u, k = t / segs;
+      to[u] = t < rows * segs ? place[k] : -1;
+      if (to[u] >= 0) v[u] = lx_load_part<ES>(cp, r0 + k, (t - k * segs) * SEG + lane * (16 / ES));
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int t = t0 + 16 * u, k = t / segs;
+      if (t < rows * segs) lx_store_part<ES>(cp, r0 + k, to[u], (t - k * segs) * SEG + lane * (16 / ES), v[u]);
+    }
   }
 }
 
@@ -544,7 +567,7 @@ __global__ __launch_bounds__(1024) void lx_loss_kernel(LxRows s, float* __restri
 // The kept exp(z - tile maximum) of classes v0 .. v0 + cols become G in place.
 // A lane takes 16 bytes; a tile of BN classes has one factor a row.
 template <int EK, int BN>
-__global__ __launch_bounds__(256) void lx_scale_kernel(LxRows s, int64_t ldg, int width, int v0,
+__global__ __launch_bounds__(256) void lx_scale_kernel(LxRows s, void* g, int64_t ldg, int width, int v0,
                                                        int64_t stats_ld) {
   constexpr int ES = EK == EL_F32 ? 4 : 2, CE = 16 / ES;
   typedef typename LxElem<ES>::T T;
@@ -554,21 +577,20 @@ __global__ __launch_bounds__(256) void lx_scale_kernel(LxRows s, int64_t ldg, in
   if (c >= width) return;
   for (int r = blockIdx.y; r < n; r += gridDim.y) {
     const float2 st = s.stats[(int64_t)((v0 + c) / BN) * stats_ld + r];
-    const float f = rebase(st.x, safe_ref(s.row_max[r])) * s.row_f[r] * (EK == EL_F16 ? 1.0f / kKeepScale : 1.0f);
-    T* q = (T*)s.g + (int64_t)r * ldg + c;
+    const float f = rebase(st.x, safe_ref(s.row_max[r])) * s.row_f[r] * (EK == EL_F32 ? 1.0f : 1.0f / kKeepScale);
+    T* q = (T*)g + (int64_t)r * ldg + c;
     vec x = *reinterpret_cast<const vec*>(q);
     const int at = s.label[r] - v0 - c;
     float v[CE];
 #pragma unroll
     for (int e = 0; e < CE; ++e) {
       if constexpr (EK == EL_F32) v[e] = x[e] * f;
-      else if constexpr (EK == EL_F16) v[e] = f16_to_f32(x[e]) * f;
-      else v[e] = bf16_to_f32(x[e]) * f;
+      else v[e] = f16_to_f32(x[e]) * f;
     }
-    if (at >= 0 && at < CE) {
-      const float w = s.row_w[r];
+    if (at >= 0 && at < CE) {  // from the logit: a rounded exponential less 1 has few bits left where the row is sure
+      const float g = exp_from(s.zlab[r], safe_ref(s.row_max[r])) * s.row_f[r] - s.row_w[r];
 #pragma unroll
-      for (int e = 0; e < CE; ++e) v[e] = e == at ? v[e] - w : v[e];
+      for (int e = 0; e < CE; ++e) v[e] = e == at ? g : v[e];
     }
 #pragma unroll
     for (int e = 0; e < CE; ++e) {
@@ -644,12 +666,13 @@ struct LxPlan {
   int bm, bn;               // tiles of the logits
   bool direct;              // W is read in place
   int64_t piece;            // classes of a piece (a multiple of 256)
+  int64_t held;             // classes whose G is held in dW first (a multiple of 256)
   int bm_dx;                // tiles of dX
   int64_t slab_rows;        // of all its slabs together
   int64_t stats_off, xc_off, slab_off, wpad_off, g_off, bytes;
 };
 
-constexpr int kRowArrays = 9;  // arrays of Rp 4-byte values behind the head
+constexpr int kRowArrays = 8;  // arrays of Rp 4-byte values behind the head
 
 // The plan of a call, with the largest piece of at most `piece` classes that
 // `bytes` of scratch hold (bytes < 0: any).  False: none fits.
@@ -703,6 +726,16 @@ bool lx_plan(int64_t R, int64_t V, int64_t D, int64_t ldw, bool direct, bool f32
   return true;
 }
 
+// Classes [0, held) whose G fits in dW's rows [held, V), where scratch does not hold all.
+int64_t lx_held(const LxCall& c, const LxPlan& pl) {
+  if (!c.dw || pl.piece >= pl.Vp || (c.V > 1 && c.lddw != c.D)) return 0;
+  const int64_t ob = dt(*c.dw) == DType::kF32 ? 4 : 2, lim = INT32_MAX - 1;
+  int64_t n = std::min(pl.Vp - pl.piece, (c.V * c.D * ob - 256) / (pl.Rp * pl.es + c.D * ob));
+  n = std::min({n, lim / (pl.Rp * pl.es), lim / ((pl.direct ? c.ldw : pl.Dp) * pl.es)});
+  if (!pl.direct) n = std::min(n, pl.piece);  // (room for the copy of W's rows)
+  return n > 0 ? n / 256 * 256 : 0;
+}
+
 template <int IN, int OUT, int ACT, int BM, int BN, int WM, int WN, bool AKC, bool BKC, int S>
 Status lx_gemm_as(const NTParams& q, int64_t rows, int64_t cols, hipStream_t s) {
   NTParams p = q;
@@ -753,15 +786,14 @@ Status lx_run(const LxCall& c, const LxPlan& pl, hipStream_t s) {
   LxRows rw{};
   rw.head = (int32_t*)base;
   int32_t* arr = (int32_t*)(base + 256);
-  rw.pos = arr;
-  rw.idx = arr + pl.Rp;
-  rw.label = arr + 2 * pl.Rp;
-  rw.weight = (float*)arr + 3 * pl.Rp;
-  rw.row_w = (float*)arr + 4 * pl.Rp;
-  rw.zlab = (float*)arr + 5 * pl.Rp;
-  rw.row_max = (float*)arr + 6 * pl.Rp;
-  rw.row_f = (float*)arr + 7 * pl.Rp;
-  rw.row_loss = (float*)arr + 8 * pl.Rp;
+  rw.idx = arr;
+  rw.label = arr + pl.Rp;
+  rw.weight = (float*)arr + 2 * pl.Rp;
+  rw.row_w = (float*)arr + 3 * pl.Rp;
+  rw.zlab = (float*)arr + 4 * pl.Rp;
+  rw.row_max = (float*)arr + 5 * pl.Rp;
+  rw.row_f = (float*)arr + 6 * pl.Rp;
+  rw.row_loss = (float*)arr + 7 * pl.Rp;
   rw.stats = (float2*)(base + pl.stats_off);
   rw.xc = base + pl.xc_off;
   rw.slab = (float*)(base + pl.slab_off);
@@ -775,39 +807,43 @@ Status lx_run(const LxCall& c, const LxPlan& pl, hipStream_t s) {
   const bool grad = c.dx != nullptr;
   const int tn_dx = lx_tile_cols(pl.bm_dx, IN == IN_F32);
   const LxShares sh{pl.bm_dx, grad ? (D + tn_dx - 1) / tn_dx : 0, lx_slots(pl.bm_dx, IN == IN_F32),
-                    (int)std::min(pl.piece, c.V), (int)std::min<int64_t>(pl.slab_rows, INT32_MAX)};
+                    (int)std::max(pl.held, std::min(pl.piece, c.V)), (int)std::min<int64_t>(pl.slab_rows, INT32_MAX)};
   const LxCopy cx{c.x->data, rw.xc, grad ? c.dx->data : nullptr, row_loss, c.ldx, c.lddx, D, Dp};
   const int32_t* labels = (const int32_t*)c.labels->data;
   const float* weight = c.rw ? (const float*)c.rw->data : nullptr;
-  if (R <= 64) {
-    lx_rows_kernel<ES, true><<<1, 1024, 0, s>>>(labels, weight, R, V, top, rw, sh, cx);
-  } else {
-    lx_rows_kernel<ES, false><<<1, 1024, 0, s>>>(labels, weight, R, V, top, rw, sh, cx);
-    lx_copy_rows_kernel<ES><<<(R + 3) / 4, 256, 0, s>>>(cx, R, rw.pos);
-  }
+  const int per = std::max(1, std::min((R + 255) / 256, kCopyRows));
+  lx_rows_kernel<ES><<<R > 0 ? (R + per - 1) / per : 1, 1024, 0, s>>>(labels, weight, R, V, top, rw, sh, cx, per);
   Status st = launch_status("linear_xent_rows");
   if (st != Status::Ok) return st;
 
-  // W's rows of the classes v0 .. v0 + cols, in place or copied
+  // W's rows of the classes v0 .. v0 + cols, in place or copied (unless the copy is there)
+  int64_t copied = -1;
   auto weights = [&](NTParams& p, int64_t v0, int64_t cols) {
     const uint8_t* w = (const uint8_t*)c.w->data + v0 * c.ldw * ES;
     if (pl.direct) {
       p.B = w;
       p.ldb = c.ldw;
     } else {
-      lx_copy_rows_kernel<ES><<<(unsigned)((cols + 3) / 4), 256, 0, s>>>(
-          LxCopy{w, rw.wpad, nullptr, nullptr, c.ldw, 0, D, Dp}, (int)cols, nullptr);
+      if (copied != v0)
+        lx_copy_rows_kernel<ES><<<(unsigned)((cols + 3) / 4), 256, 0, s>>>(
+            LxCopy{w, rw.wpad, nullptr, nullptr, c.ldw, 0, D, Dp}, (int)cols);
+      copied = v0;
       p.B = rw.wpad;
       p.ldb = Dp;
     }
   };
-  auto logits = [&](int64_t v0, int64_t cols) {
+  struct Part {  // classes v0 .. v0 + cols and their G
+    int64_t v0, cols;
+    void* g;
+    int64_t ldg;
+  };
+  auto logits = [&](int64_t v0, int64_t cols, const Part& keep) {
     NTParams p{};
     weights(p, v0, cols);
     p.A = rw.xc;
     p.lda = Dp;
-    p.C = rw.g;
-    p.ldc = pl.piece;
+    p.C = keep.g;
+    p.ldc = keep.ldg;
     p.M = R;
     p.N = (int)cols;
     p.K = pl.direct ? D : Dp;
@@ -824,19 +860,33 @@ Status lx_run(const LxCall& c, const LxPlan& pl, hipStream_t s) {
     p.lx.row_w = rw.row_w;
     return p;
   };
-  const int64_t pieces = (c.V + pl.piece - 1) / pl.piece;
-  const int64_t last = (pieces - 1) * pl.piece;  // first class of the piece that is kept
-  auto stats = [&](int64_t v0, int64_t cols, int64_t keep) {
-    NTParams p = logits(v0, cols);
-    p.lx.keep_from = keep < 0 ? INT32_MAX : (int)keep;
+  // The parts in the order in which their G is used: dW's rows hold the first one's
+  // until then; the last classes' is in scratch, which the others take after it.
+  const int64_t last = grad ? std::max<int64_t>(pl.Vp - pl.piece, 0) : c.V;
+  const int kept = grad ? (pl.held > 0 ? 2 : 1) : 0;
+  const int64_t step = std::min(pl.piece, c.V), parts = kept + (last - pl.held + step - 1) / step;
+  auto part = [&](int64_t k) -> Part {
+    if (k == kept - 1) return {last, c.V - last, rw.g, pl.piece};
+    if (k < kept) {
+      const uintptr_t at = (uintptr_t)c.dw->data + pl.held * D * (dt(*c.dw) == DType::kF32 ? 4 : 2);
+      return {0, pl.held, (void*)((at + 255) & ~(uintptr_t)255), pl.held};
+    }
+    const int64_t v0 = pl.held + (k - kept) * step;
+    return {v0, std::min(step, last - v0), rw.g, pl.piece};
+  };
+  auto stats = [&](const Part& q, int64_t cols, int64_t keep_from) {
+    NTParams p = logits(q.v0, cols, q);
+    p.lx.keep_from = (int)keep_from;
     return lx_gemm<IN, OUT, ACT_LX_STATS, true, true>(p, pl.bm, R, cols, s);
   };
-  if (pl.direct) {
-    st = stats(0, c.V, grad ? last : -1);
+  if (pl.direct) {  // W read in place: all classes behind the held ones at once
+    if (pl.held > 0 && (st = stats(part(0), pl.held, 0)) != Status::Ok) return st;
+    st = stats({pl.held, 0, rw.g, pl.piece}, c.V - pl.held, last - pl.held);
     if (st != Status::Ok) return st;
   } else {
-    for (int64_t v0 = 0; v0 < c.V; v0 += pl.piece) {
-      st = stats(v0, std::min(pl.piece, c.V - v0), grad && v0 == last ? 0 : -1);
+    for (int64_t k = 0; k < parts; ++k) {
+      const Part q = part(k);
+      st = stats(q, q.cols, k < kept ? 0 : INT32_MAX);
       if (st != Status::Ok) return st;
     }
   }
@@ -847,30 +897,32 @@ Status lx_run(const LxCall& c, const LxPlan& pl, hipStream_t s) {
   st = launch_status("linear_xent_stats");
   if (st != Status::Ok || !grad) return st;
 
-  const bool direct = pieces == 1;  // dX needs no slab unless its K is shared
-  for (int64_t k = pieces - 1; k >= 0; --k) {
-    const int64_t v0 = k * pl.piece, cols = std::min(pl.piece, c.V - v0);
-    if (k == pieces - 1) {
+  const bool direct = parts == 1;  // dX needs no slab unless its K is shared
+  int64_t k_before = 0;
+  for (int64_t k = 0; k < parts; ++k) {
+    const Part q = part(k);
+    const int64_t v0 = q.v0, cols = q.cols;
+    if (k < kept) {
       if (R > 0) {
         const int64_t width = up_to(cols, pl.bn);
         const unsigned gx = (unsigned)((width + 256 * (16 / ES) - 1) / (256 * (16 / ES)));
         const unsigned gy = (unsigned)std::min<int64_t>(R, 32768);
         if (pl.bn == 64)
-          lx_scale_kernel<EK, 64><<<dim3(gx, gy), 256, 0, s>>>(rw, pl.piece, (int)width, (int)v0, pl.Rp);
+          lx_scale_kernel<EK, 64><<<dim3(gx, gy), 256, 0, s>>>(rw, q.g, q.ldg, (int)width, (int)v0, pl.Rp);
         else if (pl.bn == 256)
-          lx_scale_kernel<EK, 256><<<dim3(gx, gy), 256, 0, s>>>(rw, pl.piece, (int)width, (int)v0, pl.Rp);
+          lx_scale_kernel<EK, 256><<<dim3(gx, gy), 256, 0, s>>>(rw, q.g, q.ldg, (int)width, (int)v0, pl.Rp);
         else
-          lx_scale_kernel<EK, 128><<<dim3(gx, gy), 256, 0, s>>>(rw, pl.piece, (int)width, (int)v0, pl.Rp);
+          lx_scale_kernel<EK, 128><<<dim3(gx, gy), 256, 0, s>>>(rw, q.g, q.ldg, (int)width, (int)v0, pl.Rp);
       }
     } else {
-      NTParams p = logits(v0, cols);
+      NTParams p = logits(v0, cols, q);
       st = lx_gemm<IN, OUT, ACT_LX_GRAD, true, true>(p, pl.bm, R, cols, s);
       if (st != Status::Ok) return st;
     }
     if (c.dw) {
       NTParams p{};
-      p.A = rw.g;
-      p.lda = pl.piece;
+      p.A = q.g;
+      p.lda = q.ldg;
       p.B = rw.xc;
       p.ldb = Dp;
       p.M = (int)cols;
@@ -879,7 +931,7 @@ Status lx_run(const LxCall& c, const LxPlan& pl, hipStream_t s) {
       p.ldc = c.lddw;
       p.lx.n = rw.head;
       p.lx.rows_are_k = 1;
-      p.lx.a_mn = (int)pl.piece;
+      p.lx.a_mn = (int)q.ldg;
       p.lx.b_mn = Dp;
       p.lx.alpha = alpha;
       const bool f32 = dt(*c.dw) == DType::kF32;
@@ -895,11 +947,9 @@ Status lx_run(const LxCall& c, const LxPlan& pl, hipStream_t s) {
     }
     if (R > 0) {
       NTParams p{};
-      // (a copy of the piece's rows is still there)
-      p.B = pl.direct ? (const uint8_t*)c.w->data + v0 * c.ldw * ES : (const uint8_t*)rw.wpad;
-      p.ldb = pl.direct ? c.ldw : Dp;
-      p.A = rw.g;
-      p.lda = pl.piece;
+      weights(p, v0, cols);
+      p.A = q.g;
+      p.lda = q.ldg;
       p.M = R;
       p.N = D;
       p.K = (int)cols;
@@ -908,20 +958,18 @@ Status lx_run(const LxCall& c, const LxPlan& pl, hipStream_t s) {
       p.lx.b_mn = pl.direct ? D : Dp;
       p.lx.shares = rw.head + 4;
       if (direct) {
-        p.C = c.dx->data;
-        p.ldc = c.lddx;
+        p.lx.direct = c.dx->data;
+        p.lx.ld_direct = c.lddx;
         p.lx.alpha = alpha;
         p.lx.row_map = rw.idx;
         p.lx.vec = aligned(c.dx->data, 16) && c.lddx * ES % 16 == 0;
-        st = lx_gemm<IN, OUT, ACT_LX_OUT, true, false>(p, pl.bm_dx, R, D, s);
-        if (st != Status::Ok) return st;
       }
       p.C = rw.slab;
       p.ldc = Dp;
-      p.lx.direct = direct;
       p.lx.k_piece = sh.k_piece;
-      p.lx.k_before = k == pieces - 1 ? 0 : k == pieces - 2 ? (int)(c.V - last) : sh.k_piece;
-      st = lx_gemm<IN, OUT_F32, ACT_LX_SLAB, true, false>(p, pl.bm_dx, R, D, s);
+      p.lx.k_before = (int)k_before;
+      k_before = std::max(k_before, cols);
+      st = lx_gemm<IN, OUT, ACT_LX_SLAB, true, false>(p, pl.bm_dx, R, D, s);
       if (st != Status::Ok) return st;
     }
   }
@@ -971,6 +1019,7 @@ bool lx_read(const TensorDesc* in, int ni, const TensorDesc* out, int no, LxCall
   const bool direct = c.D % (128 / es) == 0 && aligned(c.w->data, 16) && c.ldw * es % 16 == 0 &&
                       (c.V == 1 || c.ldw >= c.D) && c.ldw * es * 256 < INT32_MAX;
   if (!lx_plan(c.R, c.V, c.D, c.ldw, direct, f32, c.dx != nullptr, 0, c.scratch->shape[0] * 4, pl)) return false;
+  pl->held = lx_held(c, *pl);
   if (pc) *pc = c;
   return true;
 }

@@ -298,3 +298,16 @@ def test_other_device_and_types_are_refused(C, dev):
         C.op_call(C.OpKind.LinearXent, [x.to(dev), w.to(dev), labels.to(dev)], outs[:2] + [outs[2][:64]])
     with pytest.raises(RuntimeError):
         C.op_call(C.OpKind.LinearXent, [x, w.to(dev), labels.to(dev)], outs)
+
+
+@pytest.mark.parametrize("dtype,dw_type", [("bf16", None), ("f16", None), ("f32", None), ("bf16", torch.float32)])
+@pytest.mark.parametrize("r,v,d,piece", [(200, 4099, 128, 512), (250, 3001, 512, 256), (256, 6000, 1024, 1536),
+                                         (129, 5003, 200, 768), (500, 9001, 320, 256), (1, 2000, 64, 256)])
+def test_gradient_held_in_dw(C, dev, r, v, d, piece, dtype, dw_type):
+    """Few classes in scratch, and dW with room for more until its rows are written: some, half or all of the others,
+    behind W in place and behind copies of its rows."""
+    x, w, labels, g = problem(r, v, d, dtype, r + piece)
+    rw = torch.rand(r, generator=g) + 0.1
+    rw[r // 2] = 0.0
+    check(call(C, dev, x, w, labels, rw, piece=piece, dw_type=dw_type), x, w, labels, rw)
+    check(call(C, dev, x, w, labels, rw, piece=piece, dw_type=dw_type, w_pad=8, w_off=3), x, w, labels, rw)

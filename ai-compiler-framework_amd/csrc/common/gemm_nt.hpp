@@ -64,9 +64,9 @@ struct LxArgs {
   float2* stats;         // [tiles_n][stats_ld]: maximum and sum over a tile's classes
   int64_t stats_ld;
   int keep_from;         // columns from here on go to C as exp(z - tile maximum)
-  const float* row_max;  // ACT_LX_GRAD: C = exp(z - row_max) row_f - (class == label) row_w
+  const float* row_max;  // ACT_LX_GRAD: C = exp(z - row_max) row_f, row_g at the label
   const float* row_f;
-  const float* row_w;
+  const float* row_g;
   // ACT_LX_OUT: C[row_map ? row_map[m] : m] = acc * *alpha
   const float* alpha;
   const int32_t* row_map;

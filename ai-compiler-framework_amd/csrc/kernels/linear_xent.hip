@@ -16,8 +16,8 @@
 //      the rounding): of the last `piece` in scratch, of the first `held` in the
 //      memory of dW's other rows, which are written later;
 //   2. the row's statistics are joined; the kept values become G in place,
-//      scaled to the type's range by a power of two that the products take out
-//      again (weights of 1/R would leave f16's range);
+//      scaled by what makes the largest weight 1 (f16: 2^13), which the products
+//      take out again (weights of 1/R would leave f16's range);
 //   3. dW and dX of those classes;
 //   4. the other pieces: logits once more, whose epilogue knows the row's
 //      statistics and writes G, then dW and dX as before.
@@ -149,7 +149,7 @@ __device__ __forceinline__ void lx_epilogue(const NTParams& p, nt_acc_t<MS> (&ac
   // Through LDS, so that whole rows are stored (as nt_epilogue_staged does).
   // A pass' four columns of a lane, v[4], from the row's constants c.
   struct RowConst {
-    float a, f, w;  // reference or factor; G: factor and weight
+    float a, f, w;  // reference or factor; G: factor and the label's value
     int col;        // G: the label's column
   };
   auto row_const = [&](int j) -> RowConst {
@@ -165,7 +165,7 @@ __device__ __forceinline__ void lx_epilogue(const NTParams& p, nt_acc_t<MS> (&ac
       if (m < p.M) {
         c.a = safe_ref(p.lx.row_max[m]);
         c.f = p.lx.row_f[m];
-        c.w = p.lx.row_w[m];
+        c.w = p.lx.row_g[m];
         c.col = p.lx.label[m] - p.lx.v0 - n0;
       }
     } else if constexpr (ACT == ACT_LX_OUT) {
@@ -181,7 +181,7 @@ __device__ __forceinline__ void lx_epilogue(const NTParams& p, nt_acc_t<MS> (&ac
       return OUT == OUT_F32 ? v : v * kKeepScale;
     } else if constexpr (ACT == ACT_LX_GRAD) {
       const float v = exp_from(z, c.a) * c.f;
-      return col < ncol ? (col == c.col ? v - c.w : v) : 0.0f;
+      return col < ncol ? (col == c.col ? c.w : v) : 0.0f;
     } else if constexpr (ACT == ACT_LX_OUT) {
       return z * c.a;
     } else {
@@ -268,10 +268,10 @@ struct LxRows {
   int32_t* idx;     // [Rp] rows that count, in their order
   int32_t* label;   // [Rp] theirs, like all below
   float* weight;    // as given
-  float* row_w;     // times head[2]
+  float* row_g;     // G of the label, from its f32 logit
   float* zlab;
   float* row_max;
-  float* row_f;     // row_w / sum of exp(z - row_max)
+  float* row_f;     // weight head[2] / sum of exp(z - row_max)
   float* row_loss;
   float2* stats;    // [tiles of classes][Rp]
   void* xc;         // [Rp][Dp] rows of X, zeros behind D
@@ -354,8 +354,7 @@ struct LxShares {
   int bm, tiles_n, slots, k_piece, slab_rows;
 };
 
-// Which rows count, the power of two that brings the largest weight to
-// 2^(top-1) .. 2^top, how many shares dX's K is divided into; and the rows of X
+// Which rows count, the factor that makes the largest weight 2^top, how many shares dX's K is divided into; and the rows of X
 // to their places.  Every workgroup counts all rows (16 a thread at a time: 32
 // KB of labels and weights at 4096 rows, from L2) and copies kCopyRows of them
 // at most; the first one writes what the others computed too.  64 rows of 2048
@@ -438,10 +437,18 @@ __global__ __launch_bounds__(1024) void lx_rows_kernel(const int32_t* __restrict
     m = wave_max(m);
     const float mean = total > 0 ? 1.0f / (float)total : 0.0f;
     if (!w) m = mean;
-    int e = 0;
-    if (m > 0.0f && m < INFINITY) frexpf(m, &e);  // m < 2^e
-    e = top - e;
-    e = e > 126 ? 126 : e < -126 ? -126 : e;
+    // 2^top / m, so that the largest weight (all of them, in a mean) has no
+    // rounding in G, which all products with its row would share; a power of
+    // two where the quotient is no normal number.
+    float up = ldexpf(1.0f / m, top), down = ldexpf(m, -top);
+    if (!(m > 0x1p-100f && m < 0x1p100f)) {
+      int e = 0;
+      if (m > 0.0f && m < INFINITY) frexpf(m, &e);  // m < 2^e
+      e = top - e;
+      e = e > 126 ? 126 : e < -126 ? -126 : e;
+      up = ldexpf(1.0f, e);
+      down = ldexpf(1.0f, -e);
+    }
     // Shares: rounds of the workgroups that run at once, times a share's K-steps
     // and some 8 for a tile's first loads and its end; a share's sums are
     // written and read once more (1/32 of a step a tile when all CUs do it).
@@ -464,8 +471,8 @@ __global__ __launch_bounds__(1024) void lx_rows_kernel(const int32_t* __restrict
     }
     if (lane == 0) {
       s.head[0] = total;
-      s.head[1] = __float_as_int(ldexpf(1.0f, -e));
-      s.head[2] = __float_as_int(ldexpf(1.0f, e));
+      s.head[1] = __float_as_int(down);
+      s.head[2] = __float_as_int(up);
       s.head[3] = __float_as_int(mean);
       s.head[4] = best;
     }
@@ -533,8 +540,8 @@ __global__ __launch_bounds__(1024) void lx_stats_kernel(LxRows s, int tiles, int
     weight = weights ? s.weight[r] : __int_as_float(s.head[3]);
     const float up = weight * __int_as_float(s.head[2]);
     s.row_max[r] = m;
-    s.row_w[r] = up;
     s.row_f[r] = up / sum;
+    s.row_g[r] = exp_from(s.zlab[r], ref) * (up / sum) - up;
     part = logf(sum) + (ref - s.zlab[r]);
     s.row_loss[r] = part;
     if (!weights) s.weight[r] = weight;
@@ -587,8 +594,8 @@ __global__ __launch_bounds__(256) void lx_scale_kernel(LxRows s, void* g, int64_
       if constexpr (EK == EL_F32) v[e] = x[e] * f;
       else v[e] = f16_to_f32(x[e]) * f;
     }
-    if (at >= 0 && at < CE) {  // from the logit: a rounded exponential less 1 has few bits left where the row is sure
-      const float g = exp_from(s.zlab[r], safe_ref(s.row_max[r])) * s.row_f[r] - s.row_w[r];
+    if (at >= 0 && at < CE) {  // (a rounded exponential less 1 has few bits left where the row is sure)
+      const float g = s.row_g[r];
 #pragma unroll
       for (int e = 0; e < CE; ++e) v[e] = e == at ? g : v[e];
     }
@@ -602,10 +609,213 @@ __global__ __launch_bounds__(256) void lx_scale_kernel(LxRows s, void* g, int64_
   }
 }
 
+template <int EK>
+__device__ __forceinline__ uint16_t to_elem(float v) { return EK == EL_F16 ? f32_to_f16(v) : f32_to_bf16(v); }
+// What rounding G's value g to the operands' type takes from it.
+template <int EK>
+__device__ __forceinline__ float g_rest(float g) {
+  if constexpr (EK == EL_F32) return 0.0f;
+  return g - (EK == EL_F16 ? f16_to_f32(to_elem<EK>(g)) : bf16_to_f32(to_elem<EK>(g)));
+}
+
+// dW of few rows (16-bit operands): bound by its stores.  The general product's
+// tiles wait for their loads, for LDS and for the queue of the tile before; here
+// a wave keeps X's 32 KB rows x 32 CB columns in registers, four waves read the
+// next 64 classes of G while they store 64 rows of dW, and no result goes
+// through LDS: X's columns are dealt to a pair of 16 x 16 blocks four by four,
+// so that a lane holds eight neighbours.  64 x 32003 x 2048 f16 39.6 -> 28.8 us
+// (131 MB written; stores alone take 23), 128 x 32000 x 4096 bf16 77.6 -> 59.0,
+// 256 105.7 -> 86.2.
+// To 128 rows (KB <= 4), what the rounding of G took from a label's value is
+// added as products of their own, in the blocks that have labels: in a sum of so
+// few rows it is most of the error, and it does not average out.
+struct LxDw {
+  const uint16_t* g;  // [Rp][ldg]
+  const uint16_t* x;  // [Rp][Dp]
+  void* dw;
+  const int32_t* n;   // rows that count; head[1] behind it
+  const int32_t* label;
+  const float* row_g;
+  int v0;             // class of G's column 0
+  int64_t ldg, lddw;
+  int Dp, D, classes;
+  int per;            // blocks of 64 classes of a workgroup
+};
+
+template <int IN, int OUT, int KB, int CB>
+__global__ __launch_bounds__(256, 2) void lx_dw_kernel(LxDw a) {
+  constexpr int TILE = 32 * KB * 128;  // [32 KB rows][64 columns]
+  __shared__ __align__(16) uint8_t smem[2 * TILE];
+  __shared__ int lab[32 * KB];        // column of G, -1 behind the last row
+  __shared__ uint16_t rest[32 * KB];  // row_g less its rounding, in the operands' type
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int n = a.n[0];
+  const float alpha = __int_as_float(a.n[1]);
+  const int g16 = lane >> 4, i16 = lane & 15;
+  // rows below n of 64 columns from src on, zeros elsewhere (behind `cols` columns too)
+  auto fetch = [&](const uint16_t* src, int64_t ld, int cols, u16x8 (&v)[KB]) {
+#pragma unroll
+    for (int j = 0; j < KB; ++j) {
+      const int k = (tid >> 3) + 32 * j, c = (tid & 7) * 8;
+      v[j] = k < n && c < cols ? *reinterpret_cast<const u16x8*>(src + k * ld + c) : u16x8{};
+    }
+  };
+  auto put = [&](uint8_t* tile, const u16x8 (&v)[KB]) {
+#pragma unroll
+    for (int j = 0; j < KB; ++j) {
+      const int k = (tid >> 3) + 32 * j;
+      *reinterpret_cast<u16x8*>(tile + k * 128 + (((tid & 7) ^ nt_mn_swizzle<16, 2, 8>(k)) * 16)) = v[j];
+    }
+  };
+  // K-rows 8 g16 .. + 7 of a step, eight bytes of each of four lanes a row
+  const int row = 8 * g16 + (i16 >> 2), swz = nt_mn_swizzle<16, 2, 8>(row);
+  typedef short v4i16 __attribute__((ext_vector_type(4)));
+  auto frag = [&](const uint8_t* tile, int kb, int chunk, int half) -> u16x8 {
+    const uint8_t* at = tile + (kb * 32 + row) * 128 + ((chunk ^ swz) * 16) + 8 * half;
+    const v4i16 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4i16*)at);
+    const v4i16 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4i16*)(at + 4 * 128));
+    u16x8 f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f[e] = (uint16_t)lo[e];
+      f[e + 4] = (uint16_t)hi[e];
+    }
+    return f;
+  };
+
+  constexpr bool REST = KB <= 4;
+  if (REST && tid < 32 * KB) {
+    lab[tid] = tid < n ? a.label[tid] - a.v0 : -1;
+    rest[tid] = tid < n ? to_elem<IN == IN_F16 ? EL_F16 : EL_BF16>(g_rest<IN == IN_F16 ? EL_F16 : EL_BF16>(a.row_g[tid])) : 0;
+  }
+  const int col0 = blockIdx.x * 128 * CB;                // of the workgroup
+  const int blocks = (a.classes + 63) / 64, first = blockIdx.y * a.per;
+  const int last = first + a.per < blocks ? first + a.per : blocks;
+  u16x8 next[KB];
+  fetch(a.g + first * 64, a.ldg, 64, next);
+  u16x8 fx[CB][2][KB];
+#pragma unroll
+  for (int t = 0; t < 2 * CB; ++t) {  // 64 columns each: CB / 2 of them a wave's
+    u16x8 v[KB];
+    fetch(a.x + col0 + t * 64, a.Dp, a.Dp - col0 - t * 64, v);
+    uint8_t* tile = smem + (t & 1) * TILE;
+    put(tile, v);
+    __syncthreads();
+    if (t / (CB / 2) == wave) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb) fx[t % (CB / 2) * 2 + q][h][kb] = frag(tile, kb, 4 * q + (i16 & 3), h);
+    }
+  }
+  __syncthreads();
+  for (int b = first; b < last; ++b) {
+    const uint8_t* tile = smem + (b & 1) * TILE;
+    put(smem + (b & 1) * TILE, next);
+    __syncthreads();  // (the other tile's readers are behind the barrier before)
+    if (b + 1 < last) fetch(a.g + (b + 1) * 64, a.ldg, 64, next);
+    bool has = false;  // a label among the block's classes
+    for (int k = lane; REST && k < 32 * KB; k += 64) has |= lab[k] >= b * 64 && lab[k] < b * 64 + 64;
+    has = __any(has);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      u16x8 fg[KB];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) fg[kb] = frag(tile, kb, 2 * j + ((i16 >> 1) & 1), i16 & 1);
+      const int v = b * 64 + j * 16 + i16;
+      u16x8 fr[REST ? KB : 1];
+      if constexpr (REST) if (has) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int k = kb * 32 + 8 * g16 + e;
+            fr[kb][e] = lab[k] == v ? rest[k] : 0;
+          }
+      }
+#pragma unroll
+      for (int p = 0; p < CB; ++p) {
+        floatx4 acc[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          acc[h] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+            acc[h] = mfma16<IN>(reinterpret_cast<const uint16_t*>(&fx[p][h][kb]),
+                                reinterpret_cast<const uint16_t*>(&fg[kb]), acc[h]);
+          if constexpr (REST) if (has) {
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+              acc[h] = mfma16<IN>(reinterpret_cast<const uint16_t*>(&fx[p][h][kb]),
+                                  reinterpret_cast<const uint16_t*>(&fr[kb]), acc[h]);
+          }
+        }
+        const int c = col0 + wave * 32 * CB + p * 32 + 8 * g16;
+        if (v >= a.classes || c >= a.D) continue;
+        float o[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = acc[e >> 2][e & 3] * alpha;
+        if constexpr (OUT == OUT_F32) {
+          float* q = (float*)a.dw + v * a.lddw + c;
+          if (c + 8 <= a.D) {
+            reinterpret_cast<f32x4_a4*>(q)[0] = f32x4_a4{o[0], o[1], o[2], o[3]};
+            reinterpret_cast<f32x4_a4*>(q)[1] = f32x4_a4{o[4], o[5], o[6], o[7]};
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (c + e < a.D) q[e] = o[e];
+          }
+        } else {
+          uint16_t* q = (uint16_t*)a.dw + v * a.lddw + c;
+          u16x8_a2 r;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) r[e] = OUT == OUT_F16 ? f32_to_f16(o[e]) : f32_to_bf16(o[e]);
+          if (c + 8 <= a.D) {
+            *reinterpret_cast<u16x8_a2*>(q) = r;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (c + e < a.D) q[e] = r[e];
+          }
+        }
+      }
+    }
+  }
+}
+
+// Columns of a workgroup and blocks of 64 classes that each has, for R <= 256 rows.
+constexpr int kFewRows = 128;
+int lx_dw_cols(int64_t R) { return R <= kFewRows ? 512 : 256; }
+int lx_dw_blocks(int64_t R, int64_t classes, int64_t D) {
+  const int64_t gx = (D + lx_dw_cols(R) - 1) / lx_dw_cols(R), blocks = (classes + 63) / 64;
+  const int64_t share = std::max<int64_t>(1, 512 / gx);  // two workgroups run on a CU
+  return (int)((blocks + share - 1) / share);
+}
+// 16-bit operands: always to 128 rows; to 256 where each workgroup has three
+// blocks or more, over which X's loads are spread (10007 x 2048 21.6 us against
+// the product's 25.8, but 16384 x 1024 19.0 against 17.4).
+bool lx_dw_fits(int64_t R, int64_t classes, int64_t D) {
+  return R <= kFewRows || (R <= 256 && lx_dw_blocks(R, classes, D) >= 3);
+}
+
+template <int IN, int OUT>
+Status lx_dw(LxDw a, int64_t R, hipStream_t s) {
+  const int cols = lx_dw_cols(R), blocks = (a.classes + 63) / 64;
+  a.per = lx_dw_blocks(R, a.classes, a.D);
+  const dim3 grid((a.D + cols - 1) / cols, (blocks + a.per - 1) / a.per);
+  if (R <= kFewRows / 2) lx_dw_kernel<IN, OUT, 2, 4><<<grid, 256, 0, s>>>(a);
+  else if (R <= kFewRows) lx_dw_kernel<IN, OUT, 4, 4><<<grid, 256, 0, s>>>(a);
+  else lx_dw_kernel<IN, OUT, 8, 2><<<grid, 256, 0, s>>>(a);
+  return launch_status("linear_xent_dw");
+}
+
 // dX from its slabs: head[1] times their sum, in order, to the row it came from.
+// rest: and what the rounding of G took from the label's value, from W's row.
 template <int EK>
 __global__ __launch_bounds__(256) void lx_finish_kernel(LxRows s, int direct, int k_piece, int bm, int64_t ld, int D,
-                                                        void* dx, int64_t lddx) {
+                                                        void* dx, int64_t lddx, const void* rest, int64_t ldw) {
   const int n = s.head[0], shares = s.head[4];
   if (direct && shares == 1) return;  // (stored by the product itself)
   const int k_share = lx_share_k(k_piece, shares), slabs = (k_piece + k_share - 1) / k_share;
@@ -626,10 +836,14 @@ __global__ __launch_bounds__(256) void lx_finish_kernel(LxRows s, int direct, in
     }
     for (; k < slabs; ++k) v += *reinterpret_cast<const f32x4*>(q + k * stride);
     const int64_t at = (int64_t)s.idx[r] * lddx + c;
+    const float g = rest ? g_rest<EK>(s.row_g[r]) : 0.0f;
+    const int64_t w_at = (int64_t)s.label[r] * ldw + c;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (c + e < D) {
-        const float x = v[e] * alpha;
+        float x = v[e];
+        if (rest) x = fmaf(g, elem_f32<EK>(rest, w_at + e), x);
+        x *= alpha;
         if constexpr (EK == EL_F32) ((float*)dx)[at + e] = x;
         else ((uint16_t*)dx)[at + e] = EK == EL_F16 ? f32_to_f16(x) : f32_to_bf16(x);
       }
@@ -789,7 +1003,7 @@ Status lx_run(const LxCall& c, const LxPlan& pl, hipStream_t s) {
   rw.idx = arr;
   rw.label = arr + pl.Rp;
   rw.weight = (float*)arr + 2 * pl.Rp;
-  rw.row_w = (float*)arr + 3 * pl.Rp;
+  rw.row_g = (float*)arr + 3 * pl.Rp;
   rw.zlab = (float*)arr + 4 * pl.Rp;
   rw.row_max = (float*)arr + 5 * pl.Rp;
   rw.row_f = (float*)arr + 6 * pl.Rp;
@@ -857,7 +1071,7 @@ Status lx_run(const LxCall& c, const LxPlan& pl, hipStream_t s) {
     p.lx.stats_ld = pl.Rp;
     p.lx.row_max = rw.row_max;
     p.lx.row_f = rw.row_f;
-    p.lx.row_w = rw.row_w;
+    p.lx.row_g = rw.row_g;
     return p;
   };
   // The parts in the order in which their G is used: dW's rows hold the first one's
@@ -897,7 +1111,9 @@ Status lx_run(const LxCall& c, const LxPlan& pl, hipStream_t s) {
   st = launch_status("linear_xent_stats");
   if (st != Status::Ok || !grad) return st;
 
-  const bool direct = parts == 1;  // dX needs no slab unless its K is shared
+  // Few rows of 16 bits: their labels' values of G count in full (lx_dw_kernel, lx_finish_kernel).
+  const bool few = IN != IN_F32 && R <= kFewRows;
+  const bool direct = parts == 1 && !few;  // dX needs no slab unless its K is shared
   int64_t k_before = 0;
   for (int64_t k = 0; k < parts; ++k) {
     const Part q = part(k);
@@ -939,7 +1155,17 @@ Status lx_run(const LxCall& c, const LxPlan& pl, hipStream_t s) {
       p.C = (uint8_t*)c.dw->data + v0 * c.lddw * ob;
       p.lx.vec = aligned(c.dw->data, 16) && c.lddw * ob % 16 == 0;
       const int bm = lx_tile_rows(std::max<int64_t>(cols, 129), c.D, IN == IN_F32);
-      if (f32)
+      const bool dw_few = IN != IN_F32 && lx_dw_fits(R, cols, D);
+      if constexpr (IN != IN_F32) {
+        if (dw_few) {
+          const LxDw a{(const uint16_t*)q.g, (const uint16_t*)rw.xc, p.C, rw.head, rw.label, rw.row_g,
+                       (int)v0, q.ldg, c.lddw, Dp, D, (int)cols, 0};
+          st = f32 ? lx_dw<IN, OUT_F32>(a, R, s) : lx_dw<IN, OUT>(a, R, s);
+        }
+      }
+      if (dw_few)
+        ;
+      else if (f32)
         st = lx_gemm<IN, OUT_F32, ACT_LX_OUT, false, false>(p, bm, cols, D, s);
       else
         st = lx_gemm<IN, OUT, ACT_LX_OUT, false, false>(p, bm, cols, D, s);
@@ -975,7 +1201,8 @@ Status lx_run(const LxCall& c, const LxPlan& pl, hipStream_t s) {
   }
   if (R > 0) {
     const unsigned gx = (unsigned)((D + 1023) / 1024), gy = (unsigned)std::min<int64_t>(R, 32768);
-    lx_finish_kernel<EK><<<dim3(gx, gy), 256, 0, s>>>(rw, direct, sh.k_piece, pl.bm_dx, Dp, D, c.dx->data, c.lddx);
+    lx_finish_kernel<EK><<<dim3(gx, gy), 256, 0, s>>>(rw, direct, sh.k_piece, pl.bm_dx, Dp, D, c.dx->data, c.lddx,
+                                                      few ? c.w->data : nullptr, c.ldw);
     return launch_status("linear_xent_finish");
   }
   return Status::Ok;

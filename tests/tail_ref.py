@@ -45,12 +45,15 @@ def linear_xent(x, w, labels, rw=None, piece=None):
     bl = torch.zeros_like(rl)
     bl[i] = (2 * most + rel_sum + 8 * U * (lse.abs() + zl.abs() + (top - zl).abs() + 4))[:, 0]
     # G in the operands' type: the numerator is rounded, then G itself; one more rounding each of the products
-    # in f32.  f16: steps of 2^-25 of what is scaled to at most 2^14 (numerators) and 2^13 (largest weight).
+    # in f32.  Numerators of 16-bit operands are kept in f16, scaled to at most 2^14: half steps of 2^-25 below the
+    # normal numbers, 2^-39 of their tile's largest, which is at most the row's.  f16: G too, scaled to 2^13.
     h = HALF_STEP[dt]
     ge = wi.abs() * pe + h * (wi.abs() * (p + pe)) + h * (g.abs() + wi.abs() * pe) + 4 * U * wi.abs() * (p + 1)
     if dt == torch.float16:
         big = wr.abs().max() if len(i) else 0.0
-        ge = ge + 2.0 ** -39 * wi.abs() + 2.0 ** -36 * big
+        ge = ge + 2.0 ** -36 * big
+    if dt != torch.float32:
+        ge = ge + 2.0 ** -39 * wi.abs()
     e = wi.abs() * 2.0 ** -120  # (exponentials below the normal numbers are zero)
     ge = ge + e
     bx = torch.zeros_like(x)

@@ -311,3 +311,62 @@ def test_gradient_held_in_dw(C, dev, r, v, d, piece, dtype, dw_type):
     rw[r // 2] = 0.0
     check(call(C, dev, x, w, labels, rw, piece=piece, dw_type=dw_type), x, w, labels, rw)
     check(call(C, dev, x, w, labels, rw, piece=piece, dw_type=dw_type, w_pad=8, w_off=3), x, w, labels, rw)
+
+
+@pytest.mark.parametrize("dtype,dw_type", [("bf16", None), ("f16", None), ("f16", torch.float32)])
+@pytest.mark.parametrize("r,v,d,pad", [(1, 63, 8, 0), (3, 65, 520, 0), (31, 1000, 1024, 8), (64, 4100, 1032, 0),
+                                       (65, 129, 504, 16), (128, 2050, 1536, 0), (129, 13000, 1000, 0),
+                                       (256, 24600, 512, 0), (200, 17001, 776, 24)])
+def test_few_rows(C, dev, r, v, d, pad, dtype, dw_type):
+    """Up to 256 rows: dW by blocks of 64 classes, columns and classes that end inside a block."""
+    x, w, labels, g = problem(r, v, d, dtype, r + d)
+    rw = torch.rand(r, generator=g) + 0.1
+    labels[r // 2] = v - 1
+    if r > 4:
+        labels[r - 1], rw[0] = -1, 0.0
+    check(call(C, dev, x, w, labels, rw, pad=pad, dw_type=dw_type), x, w, labels, rw)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("r,v,d", [(1, 700, 64), (5, 3001, 136), (64, 2000, 256), (100, 5000, 72), (128, 4096, 128)])
+def test_few_rows_keep_the_labels_values(C, dev, r, v, d, dtype):
+    """To 128 rows the label's value of G counts with the bits of f32: a row of dW with one label is off by its own
+    rounding, by that of the other rows' probabilities (twice half a step) and by f32's, here 2^-16 in all."""
+    x, w, labels, g = problem(r, v, d, dtype, r + v)
+    w = w / 4  # (no row is sure of another class)
+    labels = torch.randperm(v, generator=g)[:r].to(torch.int32)
+    rw = torch.rand(r, generator=g) + 0.3
+    got = call(C, dev, x, w, labels, rw)
+    _, dx, dw, _, _, _, _, _ = ref.linear_xent(x, w, labels, rw)
+    p = torch.softmax(x.double() @ w.double().t(), 1) * rw.double()[:, None]
+    at = labels.long()
+    p[torch.arange(r), at] = 0.0
+    h = ref.HALF_STEP[x.dtype]
+    slack = 2.0 ** -16 * (rw.double()[:, None] * x.double().abs()) + 2.0 ** -36 * x.double().abs().sum(0)
+    bound = h * dw[at].abs() + 3 * h * (p[:, at].t() @ x.double().abs()) + slack + ref.TINY[x.dtype]
+    assert ((got[2].double()[at] - dw[at]).abs() <= bound).all()
+    slack = 2.0 ** -16 * (rw.double()[:, None] * w.double()[at].abs()) + 2.0 ** -36 * w.double().abs().sum(0)
+    bound = h * dx.abs() + 3 * h * (p @ w.double().abs()) + slack + ref.TINY[x.dtype]
+    assert ((got[1].double() - dx).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_equal_weights_are_not_rounded(C, dev, dtype):
+    """The mean over any number of rows: 1 / rows is in no product, so dW of a label keeps all but the rounding of
+    the probabilities."""
+    for r in (3, 131, 700):
+        x, w, labels, g = problem(r, 2003, 64, dtype, r)
+        w = w / 64  # probabilities of about 1 / 2003
+        labels = torch.randperm(2003, generator=g)[:r].to(torch.int32)
+        for rw in (None, torch.full((r,), 1.0 / r)):
+            got = call(C, dev, x, w, labels, rw)
+            _, _, dw, _, _, _, _, _ = ref.linear_xent(x, w, labels, rw)
+            p = torch.softmax(x.double() @ w.double().t(), 1)
+            at, h = labels.long(), ref.HALF_STEP[x.dtype]
+            own = p[torch.arange(r), at]
+            # label: 1 - p lies in [1/2, 1], off by at most a quarter of a step of 1 and at most by p itself
+            far = torch.minimum(torch.full_like(own, h / 2), own)[:, None] * x.double().abs()
+            p[torch.arange(r), at] = 0.0
+            far = far + 3 * h * (p[:, at].t() @ x.double().abs()) + 2.0 ** -16 * x.double().abs()
+            bound = h * dw[at].abs() + far / r + ref.TINY[x.dtype] + 2.0 ** -36 / r * x.double().abs().sum(0)
+            assert ((got[2].double()[at] - dw[at]).abs() <= bound * (1 + h)).all()

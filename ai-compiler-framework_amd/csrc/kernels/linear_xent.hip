@@ -355,17 +355,16 @@ struct LxShares {
 };
 
 // Which rows count, the factor that makes the largest weight 2^top, how many shares dX's K is divided into; and the rows of X
-// to their places.  Every workgroup counts all rows (16 a thread at a time: 32
+// to their places.  Every workgroup counts all rows (PER a thread at a time: 32
 // KB of labels and weights at 4096 rows, from L2) and copies kCopyRows of them
 // at most; the first one writes what the others computed too.  64 rows of 2048
-// f16 take 8 us (counted and copied by one workgroup 14.5), 3072 of 4096 rows of
-// 4096 bf16 22 (in two launches 23 and what lies between them).
+// f16 take 5 us (counted and copied by one workgroup 14.5), 3072 of 4096 rows of
+// 4096 bf16 18 (in two launches 23 and what lies between them).
 constexpr int kCopyRows = 256;
-template <int ES>
+template <int ES, int PER>
 __global__ __launch_bounds__(1024) void lx_rows_kernel(const int32_t* __restrict__ labels,
                                                        const float* __restrict__ w, int R, int V, int top, LxRows s,
                                                        LxShares sh, LxCopy cp, int per) {
-  constexpr int PER = 16;
   __shared__ int place[kCopyRows];
   const bool first = blockIdx.x == 0;
   const int r0 = blockIdx.x * per;
@@ -1026,7 +1025,9 @@ Status lx_run(const LxCall& c, const LxPlan& pl, hipStream_t s) {
   const int32_t* labels = (const int32_t*)c.labels->data;
   const float* weight = c.rw ? (const float*)c.rw->data : nullptr;
   const int per = std::max(1, std::min((R + 255) / 256, kCopyRows));
-  lx_rows_kernel<ES><<<R > 0 ? (R + per - 1) / per : 1, 1024, 0, s>>>(labels, weight, R, V, top, rw, sh, cx, per);
+  const unsigned groups = R > 0 ? (R + per - 1) / per : 1;
+  if (R <= 1024) lx_rows_kernel<ES, 1><<<groups, 1024, 0, s>>>(labels, weight, R, V, top, rw, sh, cx, per);
+  else lx_rows_kernel<ES, 4><<<groups, 1024, 0, s>>>(labels, weight, R, V, top, rw, sh, cx, per);
   Status st = launch_status("linear_xent_rows");
   if (st != Status::Ok) return st;
 

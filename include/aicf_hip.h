@@ -215,11 +215,13 @@ extern "C" {
  *   +inf, has a NaN loss.  Outputs (loss, row loss [R], scratch), (loss, dX, row
  *   loss, scratch) or (loss, dX, dW, row loss, scratch); dX in X's type, dW in
  *   W's or f32.  Products and sums are f32; with 16-bit operands G is rounded to
- *   their type (as the operand of a product), so a f32 dW holds sums of such.
+ *   their type (as the operand of a product), so a f32 dW holds sums of such; to
+ *   128 rows the labels' values of G count in f32.
  *   scratch [n] f32: 4 n >= aicf_linear_xent_scratch(...) bytes for some piece.
  *   With gradients it holds G of a piece of the classes (16 bits a value for
  *   16-bit operands); the largest piece that fits is taken, and what the other
- *   classes' logits cost is computed twice.  Views of W whose rows are not on
+ *   classes' logits cost is computed twice, less those whose G a contiguous dW
+ *   has room for: until the call is done dW's memory holds other values.  Views of W whose rows are not on
  *   16-byte steps, or D not a multiple of 64 (f32: 32), need scratch for a copy
  *   of a piece's rows.  Refused: R D (rounded up to 256 and 64) of 2^31 bytes or
  *   more with gradients, V > 2^28, scratch too small for 256 classes.  What

@@ -611,17 +611,27 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_nt_kernel(NTParams p) {
   // places by itself.
   constexpr bool ASM_LDS = !(AKC && BKC);
   constexpr int NVM = opa.BLOCKS + opb.BLOCKS;  // loads per wave and K-step
-  auto load_one = [&](int kt, int stage, int u, auto PAD) {
+  // ACT_LX_*, K-contiguous: the K-step that K does not fill is taken first, as
+  // K-step nk of 1 .. nk, with B's chunks behind K sent out of bounds (16 bytes
+  // divide a row; A has zeros there).
+  int k_shift = 0, k_out = 0;
+  if constexpr (LX && AKC && BKC) {
+    static_assert(NW % 2 == 0, "a wave's blocks have one parity");
+    const int rest = p.K * ES % 128, c = (lane & 7) ^ ((4 * (wave & 1) + (lane >> 4)) & 7);
+    k_shift = rest > 0 ? 1 : 0;
+    k_out = rest > 0 && c * 16 >= rest ? (int)0x80000000 : 0;
+  }
+  auto load_one = [&](int kt, int stage, int u, auto PAD, int out = 0) {
     uint8_t* base = smem + stage * STAGE;
     const bool is_a = u < opa.BLOCKS;
     uint8_t* dst = is_a ? base + (wave_s + u * NW) * 1024 : base + A_BYTES + (wave_s + (u - opa.BLOCKS) * NW) * 1024;
     const i32x4_t rsrc = is_a ? opa.rsrc : opb.rsrc;
     const int voff = is_a ? opa.voff[u] : opb.voff[u - opa.BLOCKS];
-    const int soff = kt * (is_a ? opa.soff_step : opb.soff_step);
+    const int soff = (kt - k_shift) * (is_a ? opa.soff_step : opb.soff_step);
     if constexpr (ASM_LDS)
       asm_buffer_load_lds<decltype(PAD)::value>(rsrc, (uint32_t)(uintptr_t)dst, voff, soff);
     else
-      raw_buffer_load_lds(rsrc, (__attribute__((address_space(3))) unsigned*)dst, 16, voff, soff, 0, 0);
+      raw_buffer_load_lds(rsrc, (__attribute__((address_space(3))) unsigned*)dst, 16, voff | out, soff, 0, 0);
   };
   auto issue_loads = [&](int kt, int stage) {
 #pragma unroll
@@ -853,7 +863,12 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_nt_kernel(NTParams p) {
     }
     __builtin_amdgcn_s_waitcnt(0);
   };
-  issue_loads(0, 0);
+  if constexpr (LX && AKC && BKC) {
+#pragma unroll
+    for (int u = 0; u < NVM; ++u) load_one(k_shift * nk, 0, u, std::false_type{}, u < opa.BLOCKS ? 0 : k_out);
+  } else {
+    issue_loads(0, 0);
+  }
   if constexpr (S > 2) {
     // K-steps 1 .. S - 2 go out before the first wait
     for (int q = 1; q < S - 1 && q < nk; ++q) issue_loads(q, q);

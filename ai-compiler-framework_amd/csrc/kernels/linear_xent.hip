@@ -1250,8 +1250,8 @@ bool lx_read(const TensorDesc* in, int ni, const TensorDesc* out, int no, LxCall
   if (any_overlap(in, ni, out, no)) return false;
   const bool f32 = c.ek == EL_F32;
   const int64_t es = f32 ? 4 : 2;
-  // tiles read W with 16-byte loads and whole K-steps
-  const bool direct = c.D % (128 / es) == 0 && aligned(c.w->data, 16) && c.ldw * es % 16 == 0 &&
+  // tiles read W with 16-byte loads
+  const bool direct = c.D * es % 16 == 0 && aligned(c.w->data, 16) && c.ldw * es % 16 == 0 &&
                       (c.V == 1 || c.ldw >= c.D) && c.ldw * es * 256 < INT32_MAX;
   if (!lx_plan(c.R, c.V, c.D, c.ldw, direct, f32, c.dx != nullptr, 0, c.scratch->shape[0] * 4, pl)) return false;
   pl->held = lx_held(c, *pl);
@@ -1303,7 +1303,7 @@ extern "C" int64_t aicf_linear_xent_scratch(int64_t rows, int64_t classes, int64
   const bool f32 = dtype == AICF_DTYPE_F32;
   LxPlan p;
   if (rows > INT32_MAX || classes > INT32_MAX || dim > INT32_MAX ||
-      !lx_plan(rows, classes, dim, dim, dim % (f32 ? 32 : 64) == 0, f32, gradients != 0, piece, -1, &p))
+      !lx_plan(rows, classes, dim, dim, dim * (f32 ? 4 : 2) % 16 == 0, f32, gradients != 0, piece, -1, &p))
     return -1;
   return p.bytes;
 }

@@ -221,10 +221,10 @@ extern "C" {
  *   With gradients it holds G of a piece of the classes (16 bits a value for
  *   16-bit operands); the largest piece that fits is taken, and what the other
  *   classes' logits cost is computed twice, less those whose G a contiguous dW
- *   has room for: until the call is done dW's memory holds other values.  Views of W whose rows are not on
- *   16-byte steps, or D not a multiple of 64 (f32: 32), need scratch for a copy
- *   of a piece's rows.  Refused: R D (rounded up to 256 and 64) of 2^31 bytes or
- *   more with gradients, V > 2^28, scratch too small for 256 classes.  What
+ *   has room for: until the call is done dW's memory holds other values.  Where
+ *   W's rows are not whole 16-byte steps on 16-byte steps, scratch also holds a
+ *   copy of a piece's rows.  Refused: R D (rounded up to 256 and 64) of 2^31
+ *   bytes or more with gradients, V > 2^28, scratch too small for 256 classes.  What
  *   scratch holds means nothing; calls that may run at the same time (two
  *   streams, two graphs) need scratch of their own.
  *

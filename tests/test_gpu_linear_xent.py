@@ -370,3 +370,27 @@ def test_equal_weights_are_not_rounded(C, dev, dtype):
             far = far + 3 * h * (p[:, at].t() @ x.double().abs()) + 2.0 ** -16 * x.double().abs()
             bound = h * dw[at].abs() + far / r + ref.TINY[x.dtype] + 2.0 ** -36 / r * x.double().abs().sum(0)
             assert ((got[2].double()[at] - dw[at]).abs() <= bound * (1 + h)).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("r,v,d", [(3, 700, 8), (20, 1000, 40), (60, 900, 72), (100, 3000, 136), (300, 2600, 200),
+                                   (600, 25000, 72), (1025, 13001, 264), (4096, 4096, 104), (2000, 9001, 2056)])
+def test_rows_of_w_that_end_inside_a_k_step(C, dev, r, v, d, dtype):
+    """W read in place: what lies behind a row is the next one, here with infinities where no other row may see them
+    (classes of probability 0)."""
+    x, w, labels, g = problem(r, v, d, dtype, r + d)
+    x[:, 0] = x[:, 0].abs() + 0.5
+    dead = torch.arange(1, v, 7)
+    w[dead, 0] = -math.inf
+    w[dead, 1:] = 0.0
+    labels[(labels.long() % 7) == 1] -= 1
+    loss, rl = call(C, dev, x, w, labels, outs="loss")[0::3]
+    ws, xs, alive = w.clone(), x, torch.ones(v, dtype=torch.bool)
+    alive[dead] = False
+    at = torch.cumsum(alive, 0) - 1  # the same classes without the dead ones
+    want, _, _, wl, bt, _, _, bl = ref.linear_xent(xs, ws[alive], at[labels.long()].to(torch.int32))
+    assert ((rl.double() - wl).abs() <= bl).all()
+    assert abs(float(loss) - float(want)) <= bt
+    w[dead] = 0.0
+    w[dead, 0] = -4.0
+    check(call(C, dev, x, w, labels, outs="all"), x, w, labels)

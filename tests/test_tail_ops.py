@@ -61,7 +61,8 @@ def test_scratch(lib):
     assert scratch(lib, 512, 32000, 1024, grad=0) < scratch(lib, 512, 32000, 1024, piece=256)
     assert scratch(lib, 512, 32000, 1024, piece=10 ** 9) == whole
     # rows of W that tiles cannot read in place are copied, a piece at a time
-    assert scratch(lib, 512, 32000, 1000, grad=0, piece=256) - scratch(lib, 512, 32000, 1024, grad=0) == 256 * 1024 * 2
+    assert scratch(lib, 512, 32000, 1001, grad=0, piece=256) - scratch(lib, 512, 32000, 1024, grad=0) == 256 * 1024 * 2
+    assert scratch(lib, 512, 32000, 1000, grad=0, piece=256) == scratch(lib, 512, 32000, 1024, grad=0)  # (1000: in place)
     for bad in ((-1, 10, 10), (1, 0, 10), (1, 10, 0), (1, 2 ** 28 + 1, 64), (2 ** 31, 10, 10), (1, 10, 2 ** 23),
                 (2 ** 20, 1000, 1024)):
         assert scratch(lib, *bad) == -1

@@ -339,13 +339,17 @@ __device__ __forceinline__ void lx_store_part(const LxCopy& c, int64_t r, int to
   }
 }
 
-// Rows of W onto 16-byte steps.
+// Rows of W onto 16-byte steps, or (with pos) rows of X to their places.
 template <int ES>
-__global__ __launch_bounds__(256) void lx_copy_rows_kernel(LxCopy c, int rows) {
+__global__ __launch_bounds__(256) void lx_copy_rows_kernel(LxCopy c, int rows, const int32_t* __restrict__ pos) {
   const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (r >= rows) return;
-  for (int i = (threadIdx.x & 63) * (16 / ES); i < c.Dp; i += 64 * (16 / ES))
-    lx_store_part<ES>(c, r, r, i, lx_load_part<ES>(c, r, i));
+  const int to = pos ? pos[r] : r;
+  for (int i = (threadIdx.x & 63) * (16 / ES); i < c.Dp; i += 64 * (16 / ES)) {
+    typename LxElem<ES>::vec v{};
+    if (to >= 0) v = lx_load_part<ES>(c, r, i);
+    lx_store_part<ES>(c, r, to, i, v);
+  }
 }
 
 // How dX's tiles are shared out: tiles of bm rows, tiles_n in a row of them,
@@ -360,11 +364,15 @@ struct LxShares {
 // at most; the first one writes what the others computed too.  64 rows of 2048
 // f16 take 5 us (counted and copied by one workgroup 14.5), 3072 of 4096 rows of
 // 4096 bf16 18 (in two launches 23 and what lies between them).
-constexpr int kCopyRows = 256;
+// Above kCountedByAll rows the counting, which grows with their square, is done by
+// one workgroup that leaves the places in pos, and the copy by another launch
+// (262144 rows of 64 bf16 522 -> 192 us; 65536 44 either way).
+constexpr int kCountedByAll = 32768, kCopyRows = kCountedByAll / 256;
 template <int ES, int PER>
 __global__ __launch_bounds__(1024) void lx_rows_kernel(const int32_t* __restrict__ labels,
                                                        const float* __restrict__ w, int R, int V, int top, LxRows s,
-                                                       LxShares sh, LxCopy cp, int per) {
+                                                       LxShares sh, LxCopy cp, int per,
+                                                       int32_t* __restrict__ pos) {
   __shared__ int place[kCopyRows];
   const bool first = blockIdx.x == 0;
   const int r0 = blockIdx.x * per;
@@ -417,6 +425,7 @@ __global__ __launch_bounds__(1024) void lx_rows_kernel(const int32_t* __restrict
       const bool c = in[k] >> lane & 1;
       const int at = cnt[k * 16 + wave] + __popcll(in[k] & ((1ull << lane) - 1));
       if (r >= r0 && r < r0 + per) place[r - r0] = c ? at : -1;
+      if (pos) pos[r] = c ? at : -1;
       if (first && c) {
         s.idx[at] = r;
         s.label[at] = label[k];
@@ -1031,10 +1040,16 @@ Status lx_run(const LxCall& c, const LxPlan& pl, hipStream_t s) {
   const LxCopy cx{c.x->data, rw.xc, grad ? c.dx->data : nullptr, row_loss, c.ldx, c.lddx, D, Dp};
   const int32_t* labels = (const int32_t*)c.labels->data;
   const float* weight = c.rw ? (const float*)c.rw->data : nullptr;
-  const int per = std::max(1, std::min((R + 255) / 256, kCopyRows));
-  const unsigned groups = R > 0 ? (R + per - 1) / per : 1;
-  if (R <= 1024) lx_rows_kernel<ES, 1><<<groups, 1024, 0, s>>>(labels, weight, R, V, top, rw, sh, cx, per);
-  else lx_rows_kernel<ES, 4><<<groups, 1024, 0, s>>>(labels, weight, R, V, top, rw, sh, cx, per);
+  if (R <= kCountedByAll) {
+    const int per = std::max(1, (R + 255) / 256);
+    const unsigned groups = R > 0 ? (R + per - 1) / per : 1;
+    if (R <= 1024) lx_rows_kernel<ES, 1><<<groups, 1024, 0, s>>>(labels, weight, R, V, top, rw, sh, cx, per, nullptr);
+    else lx_rows_kernel<ES, 4><<<groups, 1024, 0, s>>>(labels, weight, R, V, top, rw, sh, cx, per, nullptr);
+  } else {
+    int32_t* pos = (int32_t*)rw.row_loss;  // (written by lx_stats_kernel)
+    lx_rows_kernel<ES, 16><<<1, 1024, 0, s>>>(labels, weight, R, V, top, rw, sh, cx, 0, pos);
+    lx_copy_rows_kernel<ES><<<(R + 3) / 4, 256, 0, s>>>(cx, R, pos);
+  }
   Status st = launch_status("linear_xent_rows");
   if (st != Status::Ok) return st;
 
@@ -1048,7 +1063,7 @@ Status lx_run(const LxCall& c, const LxPlan& pl, hipStream_t s) {
     } else {
       if (copied != v0)
         lx_copy_rows_kernel<ES><<<(unsigned)((cols + 3) / 4), 256, 0, s>>>(
-            LxCopy{w, rw.wpad, nullptr, nullptr, c.ldw, 0, D, Dp}, (int)cols);
+            LxCopy{w, rw.wpad, nullptr, nullptr, c.ldw, 0, D, Dp}, (int)cols, nullptr);
       copied = v0;
       p.B = rw.wpad;
       p.ldb = Dp;

@@ -394,3 +394,14 @@ def test_rows_of_w_that_end_inside_a_k_step(C, dev, r, v, d, dtype):
     w[dead] = 0.0
     w[dead, 0] = -4.0
     check(call(C, dev, x, w, labels, outs="all"), x, w, labels)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("r", [32768, 32769, 70001])
+def test_many_rows(C, dev, r, dtype):
+    """Rows counted by every workgroup, and above 32768 by one."""
+    x, w, labels, g = problem(r, 300, 64, dtype, r)
+    rw = torch.rand(r, generator=g) + 0.1
+    rw[::5] = 0.0
+    labels[2::3], labels[r - 1] = -1, 299
+    check(call(C, dev, x, w, labels, rw), x, w, labels, rw)

@@ -12,7 +12,7 @@
 //   1. logits: tiles of the MFMA GEMM whose epilogue keeps, for each row and
 //      tile of classes, the maximum and the sum of exp(z - maximum); of some
 //      classes also exp(z - tile maximum) itself (f32, or f16 for operands of
-//      16 bits: 2^-12 against the 2^-9 of a bf16 G; the sums are taken before
+//      16 bits: 2^-11 against the 2^-8 of a bf16 G; the sums are taken before
 //      the rounding): of the last `piece` in scratch, of the first `held` in the
 //      memory of dW's other rows, which are written later;
 //   2. the row's statistics are joined; the kept values become G in place,
@@ -362,8 +362,8 @@ struct LxShares {
 // to their places.  Every workgroup counts all rows (PER a thread at a time: 32
 // KB of labels and weights at 4096 rows, from L2) and copies kCopyRows of them
 // at most; the first one writes what the others computed too.  64 rows of 2048
-// f16 take 5 us (counted and copied by one workgroup 14.5), 3072 of 4096 rows of
-// 4096 bf16 18 (in two launches 23 and what lies between them).
+// f16 take 5 us (counted and copied by one workgroup 14.5), three quarters of 4096
+// rows of 4096 bf16 18 (in two launches 23 and what lies between them).
 // Above kCountedByAll rows the counting, which grows with their square, is done by
 // one workgroup that leaves the places in pos, and the copy by another launch
 // (262144 rows of 64 bf16 522 -> 192 us; 65536 44 either way).

@@ -405,3 +405,13 @@ def test_many_rows(C, dev, r, dtype):
     rw[::5] = 0.0
     labels[2::3], labels[r - 1] = -1, 299
     check(call(C, dev, x, w, labels, rw), x, w, labels, rw)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("scale", [2.0 ** -105, 2.0 ** -95, -2.0 ** -20, 2.0 ** 90, -2.0 ** 101])
+def test_weights_of_any_scale(C, dev, scale, dtype):
+    """On both sides of where the largest weight is divided out."""
+    for r in (30, 150):
+        x, w, labels, g = problem(r, 600, 64, dtype, r)
+        rw = (torch.rand(r, generator=g) + 0.5) * scale
+        check(call(C, dev, x, w, labels, rw), x, w, labels, rw)

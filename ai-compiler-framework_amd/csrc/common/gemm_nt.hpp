@@ -7,6 +7,7 @@
 
 #include "gemm_types.hpp"
 #include "lds_load.hpp"
+#include "linear_xent_plan.hpp"
 
 namespace aicf::hip {
 
@@ -545,10 +546,6 @@ __device__ __forceinline__ void nt_operand_init(NTOperand<KC, BMN, NW, ES>& o, c
   }
 }
 
-// K of a share: whole K-steps of every type.
-__host__ __device__ __forceinline__ int lx_share_k(int k, int shares) {
-  return ((k + shares - 1) / shares + 63) / 64 * 64;
-}
 // The epilogues of ACT_LX_* (linear_xent.hip).
 template <int OUT, int ACT, int BM, int BN, int WM, int WN, int STAGE_BYTES, int MS>
 __device__ void lx_epilogue(const NTParams& p, nt_acc_t<MS> (&acc)[BN / WN / MS][BM / WM / MS], uint8_t* smem,

@@ -833,7 +833,7 @@ __global__ __launch_bounds__(256) void lx_finish_kernel(LxRows s, int direct, in
                                                         void* dx, int64_t lddx, const void* rest, int64_t ldw) {
   const int n = s.head[0], shares = s.head[4];
   if (direct && shares == 1) return;  // (stored by the product itself)
-  const int k_share = lx_share_k(k_piece, shares), slabs = (k_piece + k_share - 1) / k_share;
+  const int k_share = lx_share_k(k_piece, shares), slabs = lx_slabs(k_piece, k_share);
   const int64_t stride = (int64_t)((n + bm - 1) / bm * bm) * ld;
   const float alpha = __int_as_float(s.head[1]);
   const int c = (blockIdx.x * 256 + threadIdx.x) * 4;
@@ -868,102 +868,11 @@ __global__ __launch_bounds__(256) void lx_finish_kernel(LxRows s, int direct, in
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-int64_t up_to(int64_t n, int64_t step) { return (n + step - 1) / step * step; }
-
-// Rows of a product's tiles.  16-bit: 256 (256 x 256) where those fill three
-// quarters of the CUs, else 128, for few rows 64 or 32.  f32 is bound by its
-// MFMAs, so by the CU with most tiles: 64 x 64 unless 128 x 128 give it no more.
-int lx_tile_rows(int64_t rows, int64_t cols, bool f32) {
-  if (rows <= 32) return 32;
-  auto tiles = [&](int64_t n) { return ((rows + n - 1) / n) * ((cols + n - 1) / n); };
-  if (f32) return (tiles(64) + 255) / 256 < 4 * ((tiles(128) + 255) / 256) ? 64 : 128;
-  if (rows <= 64) return 64;
-  return rows <= 128 || tiles(256) < 192 ? 128 : 256;
-}
-// Their columns, and how many of them run on the chip at once (by LDS).
-int lx_tile_cols(int bm, bool f32) { return bm == 256 ? 256 : bm == 64 && f32 ? 64 : 128; }
-int lx_slots(int bm, bool f32) { return 256 * (f32 ? (bm == 128 ? 2 : 4) : bm == 128 || bm == 32 ? 2 : 1); }
-
 struct LxCall {
   const TensorDesc *x, *w, *labels, *rw, *loss, *dx, *dw, *row_loss, *scratch;
   int ek;  // ElemKind of X and W
   int64_t R, V, D, ldx, ldw, lddx, lddw;
 };
-
-struct LxPlan {
-  int64_t Rp, Dp, Vp, es;
-  int bm, bn;               // tiles of the logits
-  bool direct;              // W is read in place
-  int64_t piece;            // classes of a piece (a multiple of 256)
-  int64_t held;             // classes whose G is held in dW first (a multiple of 256)
-  int bm_dx;                // tiles of dX
-  int64_t slab_rows;        // of all its slabs together
-  int64_t stats_off, xc_off, slab_off, wpad_off, g_off, bytes;
-};
-
-constexpr int kRowArrays = 8;  // arrays of Rp 4-byte values behind the head
-
-// The plan of a call, with the largest piece of at most `piece` classes that
-// `bytes` of scratch hold (bytes < 0: any).  False: none fits.
-bool lx_plan(int64_t R, int64_t V, int64_t D, int64_t ldw, bool direct, bool f32, bool grad, int64_t piece,
-             int64_t bytes, LxPlan* pl) {
-  LxPlan p{};
-  p.es = f32 ? 4 : 2;
-  p.Rp = R > 0 ? up_to(R, 256) : 256;
-  p.Dp = up_to(D, 64);
-  p.Vp = up_to(V, 256);
-  p.direct = direct;
-  p.bm = lx_tile_rows(R, V, f32);
-  p.bn = lx_tile_cols(p.bm, f32);
-  const int64_t lim = INT32_MAX;  // 32-bit offsets into an operand
-  const int64_t ldk = direct ? ldw : p.Dp;
-  if (p.Rp > lim / 2 || p.Dp * p.es * 256 >= lim || ldk * p.es * 256 >= lim || p.Vp > (int64_t)1 << 28) return false;
-  int64_t at = 256 + kRowArrays * p.Rp * 4;
-  p.stats_off = at;
-  at = up_to(at + p.Vp / p.bn * p.Rp * 8, 256);
-  p.xc_off = at;
-  at = up_to(at + p.Rp * p.Dp * p.es, 256);
-  p.slab_off = at;
-  p.bm_dx = lx_tile_rows(R, D, f32);
-  p.slab_rows = p.Rp + 4096;
-  if (grad) {
-    if (p.Rp * p.Dp * p.es >= lim) return false;
-    at = up_to(at + p.slab_rows * p.Dp * 4, 256);
-  }
-  p.wpad_off = at;
-  // a piece: its G (with gradients) and its rows of W (where they are copied)
-  const int64_t each = (grad ? p.Rp * p.es : 0) + (direct ? 0 : p.Dp * p.es);
-  int64_t most = piece > 0 && piece < p.Vp ? up_to(piece, 256) : p.Vp;
-  if (grad) {
-    most = std::min(most, (lim - 1) / (p.Rp * p.es) / 256 * 256);
-    most = std::min(most, (lim - 1) / (ldk * p.es) / 256 * 256);
-  }
-  if (bytes >= 0 && each > 0) most = std::min(most, (bytes - at - 256) / each / 256 * 256);
-  if (most < 256) return false;
-  p.piece = most;
-  p.g_off = up_to(at + (direct ? 0 : most * p.Dp * p.es), 256);
-  p.bytes = p.g_off + (grad ? p.Rp * most * p.es : 0) + 256;  // (the start is rounded up to 256 bytes)
-  if (bytes >= 0 && p.bytes > bytes) return false;
-  if (grad && bytes > p.bytes) {  // what is left: more slabs, behind everything else
-    const int64_t room = (bytes - p.g_off - p.Rp * most * p.es - 256) / (p.Dp * 4);
-    if (room > p.slab_rows) {
-      p.slab_rows = std::min<int64_t>(room, 8 * p.Rp + 4096);
-      p.slab_off = p.g_off + p.Rp * most * p.es;
-    }
-  }
-  if (pl) *pl = p;
-  return true;
-}
-
-// Classes [0, held) whose G fits in dW's rows [held, V), where scratch does not hold all.
-int64_t lx_held(const LxCall& c, const LxPlan& pl) {
-  if (!c.dw || pl.piece >= pl.Vp || (c.V > 1 && c.lddw != c.D)) return 0;
-  const int64_t ob = dt(*c.dw) == DType::kF32 ? 4 : 2, lim = INT32_MAX - 1;
-  int64_t n = std::min(pl.Vp - pl.piece, (c.V * c.D * ob - 256) / (pl.Rp * pl.es + c.D * ob));
-  n = std::min({n, lim / (pl.Rp * pl.es), lim / ((pl.direct ? c.ldw : pl.Dp) * pl.es)});
-  if (!pl.direct) n = std::min(n, pl.piece);  // (room for the copy of W's rows)
-  return n > 0 ? n / 256 * 256 : 0;
-}
 
 template <int IN, int OUT, int ACT, int BM, int BN, int WM, int WN, bool AKC, bool BKC, int S>
 Status lx_gemm_as(const NTParams& q, int64_t rows, int64_t cols, hipStream_t s) {
@@ -1035,8 +944,9 @@ Status lx_run(const LxCall& c, const LxPlan& pl, hipStream_t s) {
 
   const bool grad = c.dx != nullptr;
   const int tn_dx = lx_tile_cols(pl.bm_dx, IN == IN_F32);
+  const LxParts pt = lx_parts(pl, c.V, grad);
   const LxShares sh{pl.bm_dx, grad ? (D + tn_dx - 1) / tn_dx : 0, lx_slots(pl.bm_dx, IN == IN_F32),
-                    (int)std::max(pl.held, std::min(pl.piece, c.V)), (int)std::min<int64_t>(pl.slab_rows, INT32_MAX)};
+                    (int)pt.longest(), (int)std::min<int64_t>(pl.slab_rows, INT32_MAX)};
   const LxCopy cx{c.x->data, rw.xc, grad ? c.dx->data : nullptr, row_loss, c.ldx, c.lddx, D, Dp};
   const int32_t* labels = (const int32_t*)c.labels->data;
   const float* weight = c.rw ? (const float*)c.rw->data : nullptr;
@@ -1097,19 +1007,13 @@ Status lx_run(const LxCall& c, const LxPlan& pl, hipStream_t s) {
     p.lx.row_g = rw.row_g;
     return p;
   };
-  // The parts in the order in which their G is used: dW's rows hold the first one's
-  // until then; the last classes' is in scratch, which the others take after it.
-  const int64_t last = grad ? std::max<int64_t>(pl.Vp - pl.piece, 0) : c.V;
-  const int kept = grad ? (pl.held > 0 ? 2 : 1) : 0;
-  const int64_t step = std::min(pl.piece, c.V), parts = kept + (last - pl.held + step - 1) / step;
+  const int64_t last = pt.last, parts = pt.count;
+  const int kept = pt.kept;
   auto part = [&](int64_t k) -> Part {
-    if (k == kept - 1) return {last, c.V - last, rw.g, pl.piece};
-    if (k < kept) {
-      const uintptr_t at = (uintptr_t)c.dw->data + pl.held * D * (dt(*c.dw) == DType::kF32 ? 4 : 2);
-      return {0, pl.held, (void*)((at + 255) & ~(uintptr_t)255), pl.held};
-    }
-    const int64_t v0 = pl.held + (k - kept) * step;
-    return {v0, std::min(step, last - v0), rw.g, pl.piece};
+    const LxPart q = pt.at(k);
+    if (k >= kept - 1) return {q.v0, q.cols, rw.g, pl.piece};
+    const uintptr_t at = (uintptr_t)c.dw->data + pl.held * D * (dt(*c.dw) == DType::kF32 ? 4 : 2);
+    return {q.v0, q.cols, (void*)((at + 255) & ~(uintptr_t)255), pl.held};
   };
   auto stats = [&](const Part& q, int64_t cols, int64_t keep_from) {
     NTParams p = logits(q.v0, cols, q);
@@ -1143,7 +1047,7 @@ Status lx_run(const LxCall& c, const LxPlan& pl, hipStream_t s) {
     const int64_t v0 = q.v0, cols = q.cols;
     if (k < kept) {
       if (R > 0) {
-        const int64_t width = up_to(cols, pl.bn);
+        const int64_t width = lx_up_to(cols, pl.bn);
         const unsigned gx = (unsigned)((width + 256 * (16 / ES) - 1) / (256 * (16 / ES)));
         const unsigned gy = (unsigned)std::min<int64_t>(R, 32768);
         if (pl.bn == 64)
@@ -1269,7 +1173,7 @@ bool lx_read(const TensorDesc* in, int ni, const TensorDesc* out, int no, LxCall
   const bool direct = c.D * es % 16 == 0 && aligned(c.w->data, 16) && c.ldw * es % 16 == 0 &&
                       (c.V == 1 || c.ldw >= c.D) && c.ldw * es * 256 < INT32_MAX;
   if (!lx_plan(c.R, c.V, c.D, c.ldw, direct, f32, c.dx != nullptr, 0, c.scratch->shape[0] * 4, pl)) return false;
-  pl->held = lx_held(c, *pl);
+  if (c.dw && (c.V == 1 || c.lddw == c.D)) pl->held = lx_held(*pl, c.V, c.D, c.ldw, dt(*c.dw) == DType::kF32 ? 4 : 2);
   if (pc) *pc = c;
   return true;
 }

@@ -495,7 +495,8 @@ def fuse_optimizer_into_gemms(ir: IRGraph, lowered: Lowered) -> Lowered:
     have stored (the dispatcher splits K for both alike)."""
     kind = lambda it: str(it.get("op", "")).strip().lower()  # noqa: E731
     ad = [i for i, it in enumerate(lowered) if kind(it) == "adamw_step"]
-    if len(ad) != 1 or len(lowered[ad[0]]["outputs"]) != 4:
+    # (with the clip factor, a sixth input, the update waits for the norm of all gradients)
+    if len(ad) != 1 or len(lowered[ad[0]]["inputs"]) != 5 or len(lowered[ad[0]]["outputs"]) != 4:
         return lowered
     adam = lowered[ad[0]]
     P, G, M, V, step = (int(x) for x in adam["inputs"])
@@ -654,6 +655,8 @@ def fuse_step_tail(ir: IRGraph, lowered: Lowered) -> Lowered:
     dY = int(low[im]["outputs"][0])
     step = int(low[iss]["inputs"][0])
     adam = low[ia]
+    if len(adam["inputs"]) != 5:  # (colsum_adamw has no clip factor)
+        return lowered
     if int(adam["inputs"][4]) != step or int(low[iss]["outputs"][0]) != step or not im < iss < ia:
         return lowered
     sY = ir.values[dY].shape

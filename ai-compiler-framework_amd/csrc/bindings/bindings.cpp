@@ -403,6 +403,17 @@ PYBIND11_MODULE(_C, m) {
       },
       py::arg("rows"), py::arg("classes"), py::arg("dim"), py::arg("dtype"), py::arg("gradients") = true,
       py::arg("piece") = (int64_t)0);
+  // ... for this W, wherever its rows lie
+  m.def(
+      "linear_xent_scratch",
+      [](int64_t rows, const torch::Tensor& w, bool gradients, int64_t piece) -> int64_t {
+        TORCH_CHECK(w.dim() >= 0 && w.dim() <= AICF_MAX_RANK, "w: rank out of range. got: ", tensor_brief(w));
+        const aicf_tensor_desc d = to_desc(w);
+        const int64_t n = aicf_linear_xent_scratch_for(rows, &d, gradients ? 1 : 0, piece);
+        if (n < 0) throw std::runtime_error("linear_xent_scratch: sizes, strides or dtype out of range");
+        return n;
+      },
+      py::arg("rows"), py::arg("w"), py::arg("gradients") = true, py::arg("piece") = (int64_t)0);
   m.def("registry_kernel_ids", [](int kind) {
     std::vector<std::string> ids;
     const int n = aicf_registry_count(kind);

@@ -1135,6 +1135,13 @@ Status lx_run(const LxCall& c, const LxPlan& pl, hipStream_t s) {
   return Status::Ok;
 }
 
+// Whether tiles read W with 16-byte loads.
+bool lx_in_place(const TensorDesc& w, int64_t ldw, int64_t es) {
+  const int64_t V = w.shape[0], D = w.shape[1];
+  return D * es % 16 == 0 && aligned(w.data, 16) && ldw * es % 16 == 0 && (V == 1 || ldw >= D) &&
+         ldw < INT32_MAX / (256 * es);
+}
+
 // X, W, labels [, weights] -> loss, row loss, scratch | loss, dX, row loss,
 // scratch | loss, dX, dW, row loss, scratch.
 bool lx_read(const TensorDesc* in, int ni, const TensorDesc* out, int no, LxCall* pc, LxPlan* pl) {
@@ -1167,11 +1174,7 @@ bool lx_read(const TensorDesc* in, int ni, const TensorDesc* out, int no, LxCall
   if (c.dx && !grad_of(*c.dx, *c.x, &c.lddx, false)) return false;
   if (c.dw && !grad_of(*c.dw, *c.w, &c.lddw, true)) return false;
   if (any_overlap(in, ni, out, no)) return false;
-  const bool f32 = c.ek == EL_F32;
-  const int64_t es = f32 ? 4 : 2;
-  // tiles read W with 16-byte loads
-  const bool direct = c.D * es % 16 == 0 && aligned(c.w->data, 16) && c.ldw * es % 16 == 0 &&
-                      (c.V == 1 || c.ldw >= c.D) && c.ldw * es * 256 < INT32_MAX;
+  const bool f32 = c.ek == EL_F32, direct = lx_in_place(*c.w, c.ldw, f32 ? 4 : 2);
   if (!lx_plan(c.R, c.V, c.D, c.ldw, direct, f32, c.dx != nullptr, 0, c.scratch->shape[0] * 4, pl)) return false;
   if (c.dw && (c.V == 1 || c.lddw == c.D)) pl->held = lx_held(*pl, c.V, c.D, c.ldw, dt(*c.dw) == DType::kF32 ? 4 : 2);
   if (pc) *pc = c;
@@ -1224,5 +1227,18 @@ extern "C" int64_t aicf_linear_xent_scratch(int64_t rows, int64_t classes, int64
   if (rows > INT32_MAX || classes > INT32_MAX || dim > INT32_MAX ||
       !lx_plan(rows, classes, dim, dim, dim * (f32 ? 4 : 2) % 16 == 0, f32, gradients != 0, piece, -1, &p))
     return -1;
+  return p.bytes;
+}
+
+extern "C" int64_t aicf_linear_xent_scratch_for(int64_t rows, const aicf_tensor_desc* w, int32_t gradients,
+                                                int64_t piece) {
+  int ek;
+  int64_t ldw;
+  if (!w || !elem_kind(*w, &ek) || !matrix_ld(*w, false, &ldw)) return -1;
+  const int64_t V = w->shape[0], D = w->shape[1];
+  if (rows < 0 || V < 1 || D < 1 || rows > INT32_MAX || V > INT32_MAX || D > INT32_MAX) return -1;
+  const bool f32 = ek == EL_F32;
+  LxPlan p;
+  if (!lx_plan(rows, V, D, ldw, lx_in_place(*w, ldw, f32 ? 4 : 2), f32, gradients != 0, piece, -1, &p)) return -1;
   return p.bytes;
 }

@@ -54,6 +54,8 @@ SIGNATURES = {
                                                     ctypes.c_float, ctypes.c_void_p]),
     "aicf_linear_xent_scratch": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32,
                                                   ctypes.c_int32, ctypes.c_int64]),
+    "aicf_linear_xent_scratch_for": (ctypes.c_int64, [ctypes.c_int64, ctypes.POINTER(TensorDesc), ctypes.c_int32,
+                                                      ctypes.c_int64]),
     "aicf_registry_count": (ctypes.c_int32, [ctypes.c_int32]),
     "aicf_registry_kernel_id": (ctypes.c_char_p, [ctypes.c_int32, ctypes.c_int32]),
     "aicf_registry_priority": (ctypes.c_int32, [ctypes.c_int32, ctypes.c_int32]),

@@ -217,7 +217,7 @@ extern "C" {
  *   W's or f32.  Products and sums are f32; with 16-bit operands G is rounded to
  *   their type (as the operand of a product), so a f32 dW holds sums of such; to
  *   128 rows the labels' values of G count in f32.
- *   scratch [n] f32: 4 n >= aicf_linear_xent_scratch(...) bytes for some piece.
+ *   scratch [n] f32: 4 n >= aicf_linear_xent_scratch_for(R, W, ...) bytes for some piece.
  *   With gradients it holds G of a piece of the classes (16 bits a value for
  *   16-bit operands); the largest piece that fits is taken, and what the other
  *   classes' logits cost is computed twice, less those whose G a contiguous dW
@@ -307,12 +307,16 @@ int32_t aicf_dispatch_by_id_v0(int32_t kind, const char* kernel_id,
                                const aicf_attr_blob* attrs, void* stream);
 
 /*
- * Bytes of scratch of a LINEAR_XENT call over contiguous X [rows, dim] and W
- * [classes, dim] of `dtype` (AICF_DTYPE_F32/F16/BF16), with gradients or without,
- * that handles `piece` classes at a time (<= 0: as many as possible, at most all).
- * Scratch tensors may be larger.  -1 for sizes or a type that the op refuses.
+ * Bytes of scratch of a LINEAR_XENT call over X of `rows` rows and this W, with
+ * gradients or without, that handles `piece` classes at a time (<= 0: as many as
+ * possible, at most all).  Scratch tensors may be larger.  -1 for sizes or a type
+ * that the op refuses.  W's address and strides count: off 16-byte steps its rows
+ * are copied, a piece at a time.  aicf_linear_xent_scratch: the same for a
+ * contiguous W [classes, dim] of `dtype` (AICF_DTYPE_F32/F16/BF16) that starts on
+ * 16 bytes, as an allocation does and a view into one may not.
  * No counterpart in the reference.
  */
+int64_t aicf_linear_xent_scratch_for(int64_t rows, const aicf_tensor_desc* w, int32_t gradients, int64_t piece);
 int64_t aicf_linear_xent_scratch(int64_t rows, int64_t classes, int64_t dim, int32_t dtype, int32_t gradients,
                                  int64_t piece);
 

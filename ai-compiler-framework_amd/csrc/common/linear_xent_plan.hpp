@@ -42,6 +42,12 @@ struct LxPlan {
 
 constexpr int kRowArrays = 8;  // arrays of Rp 4-byte values behind the head
 
+// Work-items of a launch lie below 2^32, and all but the logits' 256 x 256 tiles
+// of eight waves, which loop over their tiles, have a workgroup of 256 for each.
+constexpr int64_t kRowsEnd = (int64_t)1 << 26;  // a wave copies a row (of X, and of W)
+inline bool lx_tiles_loop(int bm, bool f32, int64_t K) { return bm == 256 && !f32 && K < 2048; }
+inline int64_t lx_most_tiles(bool loop) { return loop ? INT32_MAX - 1024 : ((int64_t)1 << 24) - 1; }
+
 // The plan of a call, with the largest piece of at most `piece` classes that
 // `bytes` of scratch hold (bytes < 0: any).  False: none fits.
 inline bool lx_plan(int64_t R, int64_t V, int64_t D, int64_t ldw, bool direct, bool f32, bool grad, int64_t piece,
@@ -57,6 +63,10 @@ inline bool lx_plan(int64_t R, int64_t V, int64_t D, int64_t ldw, bool direct, b
   const int64_t lim = INT32_MAX;  // 32-bit offsets into an operand
   const int64_t ldk = direct ? ldw : p.Dp;
   if (p.Rp > lim / 2 || p.Dp * p.es * 256 >= lim || ldk * p.es * 256 >= lim || p.Vp > (int64_t)1 << 28) return false;
+  // classes of a launch of the logits: all where W is read in place, else a piece
+  const int64_t tile_rows = (std::max<int64_t>(R, 1) + p.bm - 1) / p.bm;
+  const int64_t in_launch = lx_most_tiles(lx_tiles_loop(p.bm, f32, direct ? D : p.Dp)) / tile_rows * p.bn;
+  if (p.Rp >= kRowsEnd || (direct && p.Vp > in_launch)) return false;
   int64_t at = 256 + kRowArrays * p.Rp * 4;
   p.stats_off = at;
   at = lx_up_to(at + p.Vp / p.bn * p.Rp * 8, 256);
@@ -77,6 +87,7 @@ inline bool lx_plan(int64_t R, int64_t V, int64_t D, int64_t ldw, bool direct, b
     most = std::min(most, (lim - 1) / (p.Rp * p.es) / 256 * 256);
     most = std::min(most, (lim - 1) / (ldk * p.es) / 256 * 256);
   }
+  if (!direct) most = std::min({most, in_launch / 256 * 256, kRowsEnd - 256});
   if (bytes >= 0 && each > 0) most = std::min(most, (bytes - at - 256) / each / 256 * 256);
   if (most < 256) return false;
   p.piece = most;

@@ -905,7 +905,7 @@ Status lx_gemm(const NTParams& p, int bm, int64_t rows, int64_t cols, hipStream_
     // Both operands K-contiguous (logits) and long K: four waves of 128 x 128, which read half the LDS bytes a
     // product (8192 x 32000 x 4096 bf16 1719 -> 1656 us, 4096 x 32000 x 4096 897 -> 868; x 1024 300, 327).
     if constexpr (AKC && BKC) {
-      if (bm == 256 && p.K >= 2048) return lx_gemm_as<IN, OUT, ACT, 256, 256, 2, 2, AKC, BKC, 2>(p, rows, cols, s);
+      if (bm == 256 && !lx_tiles_loop(bm, false, p.K)) return lx_gemm_as<IN, OUT, ACT, 256, 256, 2, 2, AKC, BKC, 2>(p, rows, cols, s);
     }
     if (bm == 256) return lx_gemm_as<IN, OUT, ACT, 256, 256, 2, 4, AKC, BKC, 2>(p, rows, cols, s);
     if constexpr (AKC) {

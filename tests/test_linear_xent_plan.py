@@ -21,7 +21,7 @@ extern "C" int64_t plan(int64_t R, int64_t V, int64_t D, int64_t ldw, int direct
   if (ob > 0) p.held = lx_held(p, V, D, ldw, ob);
   const LxParts q = lx_parts(p, V, grad);
   const int64_t o[] = {p.Rp, p.Dp, p.piece, p.held, p.slab_rows, p.stats_off, p.xc_off, p.slab_off, p.wpad_off,
-                       p.g_off, p.bytes, p.bn, p.bm_dx, q.longest(), q.kept};
+                       p.g_off, p.bytes, p.bn, p.bm_dx, q.longest(), q.kept, p.bm};
   std::copy(o, o + sizeof o / 8, out);
   for (int64_t k = 0; k < q.count && k < most; ++k) {
     v0[k] = q.at(k).v0;
@@ -33,7 +33,7 @@ extern "C" int share_k(int k, int shares) { return lx_share_k(k, shares); }
 extern "C" int slabs(int k, int share) { return lx_slabs(k, share); }
 """
 NAMES = ("Rp", "Dp", "piece", "held", "slab_rows", "stats_off", "xc_off", "slab_off", "wpad_off", "g_off", "bytes",
-         "bn", "bm_dx", "longest", "kept")
+         "bn", "bm_dx", "longest", "kept", "bm")
 MOST = 4096
 
 
@@ -52,14 +52,14 @@ def lib(tmp_path_factory):
 
 
 def plan(lib, r, v, d, f32=False, grad=True, piece=0, ob=0, direct=None, ldw=None, scratch=-1):
-    """(the plan's numbers, its parts [(first class, classes)]), or None."""
+    """(the plan's numbers, its first parts [(first class, classes)]), or None."""
     if direct is None:
         direct = d * (4 if f32 else 2) % 16 == 0
     out, v0, cols = (ctypes.c_int64 * len(NAMES))(), (ctypes.c_int64 * MOST)(), (ctypes.c_int64 * MOST)()
     n = lib.plan(r, v, d, ldw or d, direct, f32, grad, piece, scratch, ob, out, v0, cols, MOST)
     if n < 0:
         return None
-    assert n <= MOST
+    n = min(n, MOST)
     return dict(zip(NAMES, out)), list(zip(v0[:n], cols[:n]))
 
 
@@ -131,3 +131,42 @@ def test_any_sizes(lib):
             check(lib, r, v, d, f32, grad, 4 if f32 and ob else ob, *more)
         seen += len(got[1]) > 1
     assert seen > 3000
+
+
+def test_launches_stay_below_2_32_work_items(lib):
+    """The largest calls: copies of rows (a wave each) and the logits' tiles, 256 threads each unless workgroups of
+    512 loop over them; what would need more is refused, or done in smaller pieces."""
+    def launches(r, v, d, f32):
+        """Work-items of the copies and tiles of the logits' launch, or None where the call is refused."""
+        got = plan(lib, r, v, d, f32, grad=False)
+        if got is None:
+            return None
+        p, parts = got
+        direct = d * (4 if f32 else 2) % 16 == 0
+        cols = v if direct else max(c for _, c in parts)
+        copies = max(r, 0 if direct else cols)
+        return -(-copies // 4) * 256, -(-r // p["bm"]) * -(-cols // p["bn"]), p["bm"]
+
+    rng = random.Random(3)
+    taken = refused = 0
+    for _ in range(4000):
+        r, v, d = (int(2 ** rng.uniform(0, top)) for top in (30, 28, 12))
+        d = max(1, d // 8 * 8) if rng.random() < 0.7 else d
+        f32 = rng.random() < 0.5
+        got = launches(r, v, d, f32)
+        if got is None:
+            refused += 1
+            assert r >= 2 ** 26 - 256 or r * v > 2 ** 35
+            continue
+        copies, tiles, bm = got
+        looped = bm == 256 and not f32 and (d if d * 2 % 16 == 0 else -(-d // 64) * 64) < 2048
+        assert copies < 2 ** 32 and tiles < (2 ** 31 - 1024 if looped else 2 ** 24)
+        taken += 1
+    assert taken > 1000 and refused > 100
+    assert launches(1, 2 ** 28, 64, False) and launches(2 ** 26 - 256, 1000, 64, False)
+    assert launches(2 ** 26, 1000, 64, False) is None
+    for f32, d, r, v, ok in ((True, 64, 2 ** 18, 2 ** 17, True), (True, 64, 2 ** 20, 2 ** 20, False),
+                             (False, 4096, 2 ** 20, 2 ** 19, True), (False, 4096, 2 ** 20, 2 ** 20, False),
+                             (False, 1024, 2 ** 20, 2 ** 20, True), (False, 1024, 2 ** 24, 2 ** 24, False),
+                             (True, 65, 2 ** 20, 2 ** 20, True)):  # (rows of W copied: by pieces)
+        assert (launches(r, v, d, f32) is not None) == ok, (f32, d, r, v)

@@ -14,6 +14,8 @@
 // loop, so the whole array is covered by one wave of workgroups that the
 // dispatcher spreads over all 8 XCDs.  Out-of-place Adam reads P and writes
 // Pout in the same pass instead of copying P first.
+#include <algorithm>
+
 #include "../common/adamw.hpp"
 #include "../common/head_util.hpp"
 #include "../common/hip_util.hpp"
@@ -457,25 +459,29 @@ Status adamw_clip_launch(const TensorDesc* in, int ni, TensorDesc* out, int no, 
   uint16_t* Wb = no == 4 ? (uint16_t*)out[3].data : nullptr;
   const bool vec = all_aligned16({in[0].data, in[2].data, in[3].data, out[0].data, out[1].data, out[2].data}) &&
                    aligned(in[1].data, gk == EL_F32 ? 16 : 8) && (!Wb || aligned(Wb, 8));
-  const int64_t lanes = vec ? n / 4 + n % 4 : n, blocks = (lanes + 255) / 256;
-  if (blocks > INT32_MAX) return Status::InvalidArgument;
   hipStream_t s = as_stream(stream);
+  constexpr int64_t kLaunch = (int64_t)1 << 31;  // elements of a launch, whose work-items lie below 2^32
+  for (int64_t i = 0; i < n; i += kLaunch) {
+    const int64_t m = std::min(kLaunch, n - i), lanes = vec ? m / 4 + m % 4 : m;
+    const unsigned blocks = (unsigned)((lanes + 255) / 256);
 #define ADAMW_CLIP(GK, VEC)                                                                                     \
-  adamw_clip_kernel<GK, VEC><<<(unsigned)blocks, 256, 0, s>>>(                                                  \
-      (const float*)in[0].data, in[1].data, (const float*)in[2].data, (const float*)in[3].data,                \
-      (float*)out[0].data, (float*)out[1].data, (float*)out[2].data, Wb, n, a, (const int32_t*)in[4].data,     \
-      (const float*)in[5].data)
-  if (gk == EL_F32) {
-    if (vec) ADAMW_CLIP(EL_F32, true);
-    else ADAMW_CLIP(EL_F32, false);
-  } else if (gk == EL_F16) {
-    if (vec) ADAMW_CLIP(EL_F16, true);
-    else ADAMW_CLIP(EL_F16, false);
-  } else {
-    if (vec) ADAMW_CLIP(EL_BF16, true);
-    else ADAMW_CLIP(EL_BF16, false);
-  }
+  adamw_clip_kernel<GK, VEC><<<blocks, 256, 0, s>>>(                                                            \
+      (const float*)in[0].data + i, (const uint8_t*)in[1].data + i * (GK == EL_F32 ? 4 : 2),                   \
+      (const float*)in[2].data + i, (const float*)in[3].data + i, (float*)out[0].data + i,                     \
+      (float*)out[1].data + i, (float*)out[2].data + i, Wb ? Wb + i : nullptr, m, a,                           \
+      (const int32_t*)in[4].data, (const float*)in[5].data)
+    if (gk == EL_F32) {
+      if (vec) ADAMW_CLIP(EL_F32, true);
+      else ADAMW_CLIP(EL_F32, false);
+    } else if (gk == EL_F16) {
+      if (vec) ADAMW_CLIP(EL_F16, true);
+      else ADAMW_CLIP(EL_F16, false);
+    } else {
+      if (vec) ADAMW_CLIP(EL_BF16, true);
+      else ADAMW_CLIP(EL_BF16, false);
+    }
 #undef ADAMW_CLIP
+  }
   return launch_status("adamw_step_clip_v0");
 }
 

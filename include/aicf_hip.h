@@ -216,7 +216,10 @@ extern "C" {
  *   loss, scratch) or (loss, dX, dW, row loss, scratch); dX in X's type, dW in
  *   W's or f32.  Products and sums are f32; with 16-bit operands G is rounded to
  *   their type (as the operand of a product), so a f32 dW holds sums of such; to
- *   128 rows the labels' values of G count in f32.
+ *   128 rows the labels' values of G count in f32.  G has one scale for all rows;
+ *   in f16, where the largest weight becomes 2^13, its steps are 2^-37 of that
+ *   weight or more, and in dX the probabilities of rows whose weights are 2^-14 of
+ *   it and less have few bits, or none.
  *   scratch [n] f32: 4 n >= aicf_linear_xent_scratch_for(R, W, ...) bytes for some piece.
  *   With gradients it holds G of a piece of the classes (16 bits a value for
  *   16-bit operands); the largest piece that fits is taken, and what the other

@@ -353,7 +353,8 @@ __global__ __launch_bounds__(256) void lx_copy_rows_kernel(LxCopy c, int rows, c
 }
 
 // How dX's tiles are shared out: tiles of bm rows, tiles_n in a row of them,
-// `slots` workgroups run at once, K-steps of a piece, rows that a slab may have.
+// `slots` workgroups run at once, K (the classes of the longest part), rows that
+// all slabs together may have.
 struct LxShares {
   int bm, tiles_n, slots, k_piece, slab_rows;
 };

@@ -233,9 +233,9 @@ extern "C" {
  *   scratch holds means nothing; calls that may run at the same time (two
  *   streams, two graphs) need scratch of their own.
  *
- * GRAD_NORM: T >= 1 row-major tensors of rank 0..4, f32/f16/bf16 in any mixture,
- *   2^42 elements in all at most -> norm [2] f32 and scratch [n] f32 on an 8-byte
- *   step, n >= 2048 ceil(T / 96).
+ * GRAD_NORM: 1 <= T <= 65536 row-major tensors of rank 0..4, f32/f16/bf16 in any
+ *   mixture, 2^42 elements in all at most -> norm [2] f32 and scratch [n] f32 on an
+ *   8-byte step, n >= 2048 ceil(T / 96).
  *     norm[0] = sqrt(sum of all squares),  norm[1] = min(1, max_norm / (norm[0] + 1e-6))
  *   in f64, each rounded once.  With T further outputs, of the tensors' shapes
  *   and types: G' = norm[1] G, each the tensor itself or memory of its own.  A

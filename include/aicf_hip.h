@@ -227,7 +227,7 @@ extern "C" {
  *   has room for: until the call is done dW's memory holds other values.  Where
  *   W's rows are not whole 16-byte steps on 16-byte steps, scratch also holds a
  *   copy of a piece's rows.  Refused: R D (rounded up to 256 and 64) of 2^31
- *   bytes or more with gradients, V > 2^28, R >= 2^26, scratch too small for 256
+ *   bytes or more with gradients, V > 2^28, R > 2^26 - 256, scratch too small for 256
  *   classes, and W in place with more tiles than a launch has workgroups (R V of
  *   2^36 or more in f32; 2^40 in 16 bits where D >= 2048, else 2^47).  What
  *   scratch holds means nothing; calls that may run at the same time (two
